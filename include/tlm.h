@@ -52,6 +52,7 @@ typedef struct tlm_ctx tlm_ctx;
 typedef struct tlm_linear tlm_linear;
 typedef struct tlm_attn tlm_attn;
 typedef struct tlm_model tlm_model;
+typedef struct tlm_paged tlm_paged;
 
 /* ---------------------------------------------------------------- context */
 int tlm_abi_version(void);
@@ -159,6 +160,71 @@ int tlm_attn_reset(tlm_attn* attn);
 /* Cache rows [0, count) as fp32 [count][kv_heads*head_dim] (host). */
 int tlm_attn_read_cache(tlm_attn* attn, int count, float* k_out, float* v_out);
 
+/* ------------------------------------------------------- paged attention
+ * TSLAttention's step (tsl/TSLAttention.ts:19-449: RoPE, KV append, causal
+ * softmax attention with grouped KV heads and an optional sliding window) for
+ * many sequences at once, whose keys and values lie in pages of a shared pool.
+ * The reference keeps one sequence in one cache; the pages have no counterpart
+ * there.  A handle holds a model's head shapes and RoPE table; the pools, the
+ * page tables and the batch belong to the caller, so one handle serves every
+ * layer. */
+typedef struct tlm_paged_desc {
+  int32_t heads, kv_heads, head_dim, max_tokens; /* head_dim 32, 64, 96 or 128; heads / kv_heads at most 16;
+                                                    max_tokens: positions a sequence can have */
+  int32_t rotary_dim;       /* 0 disables RoPE */
+  int32_t sliding_window;   /* 0 = full causal */
+  int32_t kv_fmt;           /* TLM_FMT_F16 or TLM_FMT_F32 */
+  int32_t page_tokens;      /* a power of two from 32 to 1024 */
+  const float* inv_freq;    /* host, rotary_dim/2 entries (ropeParameters) */
+  double attention_factor;  /* ropeParameters().attentionFactor */
+  double attn_scale;        /* <= 0 selects 1/sqrt(head_dim) */
+} tlm_paged_desc;
+
+/* One step's rows.  Sequence s has `tokens` rows, of which the first counts[s]
+ * are there (counts NULL: all), at the positions starts[s], starts[s] + 1, ...
+ * A sequence with starts[s] < 0 or counts[s] < 1 is idle.  Rows that are not
+ * there are neither read nor written: what the outputs hold for them stays.
+ * Position p lies in page tables[s][p / page_tokens]; only the entries of
+ * pages that hold a position in use are read (a window's earlier pages may be
+ * given back, their entries anything).  Sequences may share pages that they
+ * read; a position that two of them append to gets either's row.
+ * All pointers are device memory; the struct itself is the host's and is read
+ * during the call. */
+typedef struct tlm_paged_batch {
+  void* k_pages;            /* pools of num_pages * kv_heads * page_tokens * head_dim kv_fmt elements, 16-byte */
+  void* v_pages;            /* aligned, in the order that tlm_paged_locate tells */
+  const int32_t* tables;    /* [seqs][table_width] */
+  const int32_t* starts;    /* [seqs] */
+  const int32_t* counts;    /* [seqs] or NULL */
+  int32_t num_pages, table_width, seqs, tokens;
+} tlm_paged_batch;
+
+int tlm_paged_create(tlm_ctx* ctx, const tlm_paged_desc* desc, tlm_paged** out);
+void tlm_paged_destroy(tlm_paged* paged);
+/* qkv: fp32 [seqs][tokens][(heads + 2 kv_heads) * head_dim] (Q|K|V, bias
+ * included, pre-RoPE).  The rotated K and the V rows go to their pages; q, when
+ * not NULL: fp32 [seqs][tokens][heads * head_dim], the rotated queries, apart
+ * from qkv.  Any number of tokens.  Enqueue only. */
+int tlm_op_paged_append(tlm_paged* paged, const tlm_paged_batch* batch, const float* qkv, float* q);
+/* Attention of every row over positions [max(0, pos - W + 1), pos] of its
+ * sequence, which the pages hold (append first).  q: fp32 [seqs][tokens]
+ * [heads * head_dim], rotated; out: the same shape in out_fmt, TLM_FMT_F16 or
+ * TLM_FMT_F32, apart from q.  Scores and the weighted sum to 32 bits: an fp16
+ * cache's products take q (relative to its row's largest element) and the
+ * probabilities as pairs of fp16 values.  What masked positions hold does not
+ * matter; attended K and V are finite.  Enqueue only. */
+int tlm_op_paged_attention(tlm_paged* paged, const tlm_paged_batch* batch, const float* q, int out_fmt, void* out);
+/* Waits for the stream and tells of what the calls since the last status met on
+ * the device: TLM_ERR_RANGE where counts[s] was above `tokens`, a row's position
+ * beyond max_tokens or its table (such rows were left out), or a table entry in
+ * use was no page of the pool (its rows were not appended, its positions not
+ * attended to; a row with no position left is zero). */
+int tlm_paged_status(tlm_paged* paged);
+/* Where element `dim` of `position` lies: its index in a K and in a V pool, from
+ * a host copy of the sequence's table.  Host only: needs no device. */
+int tlm_paged_locate(const tlm_paged_desc* desc, int32_t num_pages, const int32_t* table, int32_t table_width,
+                     int32_t position, int32_t kv_head, int32_t dim, int64_t* k_index, int64_t* v_index);
+
 /* ------------------------------------------------------------------ logits
  * TSLLogits chunk layers + greedy sampler (tsl/TSLLogits.ts:40-69, :201-274):
  * logits = head x; token = argmax, ties to the lower id.  logits may be NULL. */
@@ -171,6 +237,31 @@ int tlm_op_argmax(tlm_ctx* ctx, const float* logits, int n, int32_t* token);
  * take part; missing slots are (0, LOWEST_FLOAT).  1 <= k <= 16; device
  * tokens[k], scores[k].  Enqueue only. */
 int tlm_op_topk(tlm_ctx* ctx, const float* logits, int n, int k, double softcap, int32_t* tokens, float* scores);
+/* Verification of drafted tokens, for many sequences at once: which of a
+ * sequence's drafts the target's distribution lets stand, and the token after
+ * them.  No counterpart in the reference (it samples one token at a time,
+ * TSLLogits.ts:336-383); without drafts (tokens = 1) it is that sampling over
+ * the whole vocabulary.
+ * logits: fp32 [seqs][tokens][vocab]; of sequence s the first counts[s] rows
+ * (NULL: tokens; < 1: idle, its results stay as they are) are there, row j
+ * following the drafts 0 .. j - 1, so it has counts[s] - 1 drafts.
+ * drafts: [seqs][tokens - 1]; draft_logits: fp32 [seqs][tokens - 1][vocab], what
+ * they were drawn from, or NULL: drafted for certain (a lookup, a greedy model).
+ * uniforms: fp32 [seqs][tokens] in [0, 1).  With p_j and q_j the softmax of
+ * logits / temperature, draft x_j stands where uniforms[s][j] q_j(x_j) < p_j(x_j)
+ * (q_j(x_j) = 1 without draft_logits); at the first that does not, the lowest
+ * token whose running sum of max(p_j - q_j, 0) passes uniforms[s][tokens - 1] of
+ * the whole is drawn (of p_j where nothing is left), after the last draft from
+ * p_j; sums in 64 bits.  temperature 0: a draft stands where it is the row's
+ * argmax (ties to the lower id), which the row gives otherwise; draft_logits and
+ * uniforms are not read.  Temperatures up to 1e-6 count as 1e-6 (math.ts:527-547).
+ * Entries at or below LOWEST_FLOAT (-inf, NaN included) never take part; a draft
+ * outside the vocabulary never stands; a row without entries gives -1.
+ * accepted: [seqs] drafts that stand; out_tokens: [seqs][tokens] those, the token
+ * after them, then -1.  tokens <= 64.  Enqueue only. */
+int tlm_op_verify_drafts(tlm_ctx* ctx, const float* logits, const float* draft_logits, const int32_t* drafts,
+                         const int32_t* counts, const float* uniforms, int32_t seqs, int32_t tokens, int32_t vocab,
+                         double temperature, int32_t* accepted, int32_t* out_tokens);
 
 /* ------------------------------------------------------------------- model */
 typedef struct tlm_model_desc {

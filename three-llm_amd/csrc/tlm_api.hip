@@ -1,4 +1,5 @@
 // C ABI (include/tlm.h) over the gfx950 kernels of tlm_kernels.hip.
+#include <float.h>
 #include <math.h>
 #include <stdarg.h>
 #include <stdio.h>
@@ -6,6 +7,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <exception>
 #include <map>
 #include <mutex>
 #include <string>
@@ -13,6 +15,7 @@
 
 #include "../../include/tlm.h"
 #include "tlm_kernels.h"
+#include "tlm_paged.h"
 
 using namespace tlm;
 
@@ -146,6 +149,27 @@ struct tlm_attn {
   float* pacc = nullptr;
   float* pml = nullptr;
   float* zero_bias = nullptr;  // stands in for an absent QKV bias
+};
+
+struct tlm_paged {
+  tlm_ctx* ctx = nullptr;
+  tlm_paged_desc d{};
+  float scale = 1.f;
+  float* rope_cos = nullptr;
+  float* rope_sin = nullptr;
+  int* status = nullptr;  // kPagedStatus* bits since the last tlm_paged_status
+};
+
+// The device of a context, current for a call's launches; the caller's after it.
+struct DeviceScope {
+  int before = -1;
+  explicit DeviceScope(int device) {
+    int d = -1;
+    if (hipGetDevice(&d) == hipSuccess && d != device && hipSetDevice(device) == hipSuccess) before = d;
+  }
+  ~DeviceScope() {
+    if (before >= 0) hipSetDevice(before);
+  }
 };
 
 struct Layer {
@@ -1113,6 +1137,180 @@ int tlm_attn_read_cache(tlm_attn* A, int count, float* k_out, float* v_out) {
   return TLM_OK;
 }
 
+// -------------------------------------------------------- paged attention --
+
+static int paged_check(const tlm_paged_desc* d) {
+  if (d->heads <= 0 || d->kv_heads <= 0 || d->heads % d->kv_heads != 0)
+    return fail(TLM_ERR_INVALID, "TLMPaged: heads %d must be a multiple of kv heads %d", d->heads, d->kv_heads);
+  if (d->heads / d->kv_heads > 16) return fail(TLM_ERR_INVALID, "TLMPaged: more than 16 query heads per kv head");
+  if (d->heads > 1024) return fail(TLM_ERR_INVALID, "TLMPaged: more than 1024 heads");
+  if (d->head_dim != 32 && d->head_dim != 64 && d->head_dim != 96 && d->head_dim != 128)
+    return fail(TLM_ERR_INVALID, "TLMPaged: head_dim %d is not 32, 64, 96 or 128", d->head_dim);
+  if (d->rotary_dim < 0 || d->rotary_dim > d->head_dim || d->rotary_dim % 2 != 0)
+    return fail(TLM_ERR_INVALID, "TLMPaged: invalid rotary dimension %d", d->rotary_dim);
+  if (d->rotary_dim > 0 && !d->inv_freq) return fail(TLM_ERR_INVALID, "TLMPaged: missing inv_freq");
+  if (d->sliding_window < 0) return fail(TLM_ERR_INVALID, "TLMPaged: negative sliding window");
+  if (d->kv_fmt != TLM_FMT_F16 && d->kv_fmt != TLM_FMT_F32)
+    return fail(TLM_ERR_INVALID, "TLMPaged: cache format %d is not fp16 or fp32", d->kv_fmt);
+  if (d->page_tokens < 32 || d->page_tokens > 1024 || (d->page_tokens & (d->page_tokens - 1)))
+    return fail(TLM_ERR_INVALID, "TLMPaged: page of %d tokens is not a power of two from 32 to 1024", d->page_tokens);
+  if (d->max_tokens <= 0 || d->max_tokens > (1 << 30))
+    return fail(TLM_ERR_INVALID, "TLMPaged: max_tokens %d outside [1, 2^30]", d->max_tokens);
+  return TLM_OK;
+}
+
+static int page_shift(const tlm_paged_desc& d) { return __builtin_ctz((unsigned)d.page_tokens); }
+
+int tlm_paged_create(tlm_ctx* ctx, const tlm_paged_desc* desc, tlm_paged** out) {
+  if (!ctx || !desc || !out) return fail(TLM_ERR_INVALID, "TLMPaged: null argument");
+  if (const int rc = paged_check(desc)) return rc;
+  const DeviceScope on(ctx->device);
+  std::vector<float> cs, sn;
+  tlm_paged* P = nullptr;
+  try {
+    P = new tlm_paged();
+    if (desc->rotary_dim > 0)
+      rope_tables(desc->max_tokens, desc->rotary_dim, desc->inv_freq, desc->attention_factor, cs, sn);
+  } catch (const std::exception&) {
+    delete P;
+    return fail(TLM_ERR_OOM, "TLMPaged: no host memory for %d positions", desc->max_tokens);
+  }
+  P->ctx = ctx;
+  P->d = *desc;
+  P->d.inv_freq = nullptr;  // the caller's
+  P->scale = (float)(desc->attn_scale > 0 ? desc->attn_scale : 1.0 / sqrt((double)desc->head_dim));
+  hipError_t e = hipMalloc(&P->status, sizeof(int));
+  if (e == hipSuccess) e = hipMemset(P->status, 0, sizeof(int));
+  const size_t bytes = cs.size() * sizeof(float);
+  if (e == hipSuccess && bytes) e = hipMalloc(&P->rope_cos, bytes);
+  if (e == hipSuccess && bytes) e = hipMalloc(&P->rope_sin, bytes);
+  if (e == hipSuccess && bytes) e = hipMemcpy(P->rope_cos, cs.data(), bytes, hipMemcpyHostToDevice);
+  if (e == hipSuccess && bytes) e = hipMemcpy(P->rope_sin, sn.data(), bytes, hipMemcpyHostToDevice);
+  if (e == hipSuccess) e = hipStreamSynchronize(nullptr);  // the fill is on another stream than the context's
+  if (e != hipSuccess) {
+    tlm_paged_destroy(P);
+    return fail(e == hipErrorOutOfMemory ? TLM_ERR_OOM : TLM_ERR_HIP, "TLMPaged: setup failed: %s",
+                hipGetErrorString(e));
+  }
+  *out = P;
+  return TLM_OK;
+}
+
+void tlm_paged_destroy(tlm_paged* P) {
+  if (!P) return;
+  const DeviceScope on(P->ctx->device);
+  hipStreamSynchronize(P->ctx->stream);
+  hipFree(P->rope_cos);
+  hipFree(P->rope_sin);
+  hipFree(P->status);
+  delete P;
+}
+
+static int paged_args(const tlm_paged* P, const tlm_paged_batch* b, PagedArgs& a) {
+  if (!P || !b) return fail(TLM_ERR_INVALID, "TLMPaged: null argument");
+  if (!b->k_pages || !b->v_pages || !b->tables || !b->starts)
+    return fail(TLM_ERR_INVALID, "TLMPaged: the batch lacks a pool, the tables or the starts");
+  if (b->num_pages < 1 || b->table_width < 1 || b->seqs < 1 || b->tokens < 1)
+    return fail(TLM_ERR_INVALID, "TLMPaged: %d pages, tables of %d, %d sequences of %d rows", b->num_pages,
+                b->table_width, b->seqs, b->tokens);
+  if ((int64_t)b->seqs * b->tokens > (1 << 20))
+    return fail(TLM_ERR_RANGE, "TLMPaged: %d sequences of %d rows are more than 2^20 rows", b->seqs, b->tokens);
+  if ((reinterpret_cast<uintptr_t>(b->k_pages) | reinterpret_cast<uintptr_t>(b->v_pages)) % 16)
+    return fail(TLM_ERR_INVALID, "TLMPaged: a pool is not 16-byte aligned");
+  memset(&a, 0, sizeof a);
+  a.kc = b->k_pages;
+  a.vc = b->v_pages;
+  a.tables = b->tables;
+  a.starts = b->starts;
+  a.counts = b->counts;
+  a.rope_cos = P->rope_cos;
+  a.rope_sin = P->rope_sin;
+  a.status = P->status;
+  a.num_pages = b->num_pages;
+  a.width = b->table_width;
+  a.page_shift = page_shift(P->d);
+  a.seqs = b->seqs;
+  a.tokens = b->tokens;
+  a.limit = paged_limit(P->d.max_tokens, b->table_width, a.page_shift);
+  a.Hq = P->d.heads;
+  a.Hkv = P->d.kv_heads;
+  a.D = P->d.head_dim;
+  a.G = P->d.heads / P->d.kv_heads;
+  a.rd = P->d.rotary_dim;
+  a.window = P->d.sliding_window;
+  a.scale = P->scale;
+  return TLM_OK;
+}
+
+int tlm_op_paged_append(tlm_paged* P, const tlm_paged_batch* b, const float* qkv, float* q) {
+  PagedArgs a;
+  if (const int rc = paged_args(P, b, a)) return rc;
+  if (!qkv) return fail(TLM_ERR_INVALID, "TLMPaged: null argument");
+  const size_t rows = (size_t)a.seqs * a.tokens;
+  if (q && overlap(qkv, rows * (a.Hq + 2 * a.Hkv) * a.D, q, rows * a.Hq * a.D))
+    return fail(TLM_ERR_INVALID, "TLMPaged: the rotated queries overlap qkv");
+  a.x = qkv;
+  a.q = q;
+  const DeviceScope on(P->ctx->device);
+  if (!launch_paged_append(P->d.kv_fmt == TLM_FMT_F32, a, P->ctx->stream))
+    return fail(TLM_ERR_STATE, "TLMPaged: no append kernel for this shape");
+  CHECK_LAUNCH("TLMPaged");
+  return TLM_OK;
+}
+
+int tlm_op_paged_attention(tlm_paged* P, const tlm_paged_batch* b, const float* q, int out_fmt, void* out) {
+  PagedArgs a;
+  if (const int rc = paged_args(P, b, a)) return rc;
+  if (!q || !out) return fail(TLM_ERR_INVALID, "TLMPaged: null argument");
+  if (out_fmt != TLM_FMT_F16 && out_fmt != TLM_FMT_F32)
+    return fail(TLM_ERR_INVALID, "TLMPaged: output format %d is not fp16 or fp32", out_fmt);
+  const size_t n = (size_t)a.seqs * a.tokens * a.Hq * a.D;  // a multiple of 32
+  if (overlap(q, n, static_cast<const float*>(out), out_fmt == TLM_FMT_F32 ? n : n / 2))
+    return fail(TLM_ERR_INVALID, "TLMPaged: out overlaps q");
+  a.x = q;
+  a.out = out;
+  a.out_f32 = out_fmt == TLM_FMT_F32;
+  const DeviceScope on(P->ctx->device);
+  if (!launch_paged_attention(P->d.kv_fmt == TLM_FMT_F32, a, P->ctx->stream))
+    return fail(TLM_ERR_STATE, "TLMPaged: no attention kernel for this shape");
+  CHECK_LAUNCH("TLMPaged");
+  return TLM_OK;
+}
+
+int tlm_paged_status(tlm_paged* P) {
+  if (!P) return fail(TLM_ERR_INVALID, "TLMPaged: null argument");
+  const DeviceScope on(P->ctx->device);
+  int bits = 0;
+  HIP_TRY(hipStreamSynchronize(P->ctx->stream));
+  HIP_TRY(hipMemcpy(&bits, P->status, sizeof bits, hipMemcpyDeviceToHost));
+  if (!bits) return TLM_OK;
+  const int zero = 0;
+  HIP_TRY(hipMemcpy(P->status, &zero, sizeof zero, hipMemcpyHostToDevice));
+  return fail(TLM_ERR_RANGE, "TLMPaged: %s%s%s", bits & kPagedStatusRows ? "rows beyond the batch or the positions were left out" : "",
+              bits == (kPagedStatusRows | kPagedStatusPage) ? "; " : "",
+              bits & kPagedStatusPage ? "a table entry in use is no page of the pool" : "");
+}
+
+int tlm_paged_locate(const tlm_paged_desc* d, int32_t num_pages, const int32_t* table, int32_t table_width,
+                     int32_t position, int32_t kv_head, int32_t dim, int64_t* k_index, int64_t* v_index) {
+  if (!d || !table || !k_index || !v_index) return fail(TLM_ERR_INVALID, "TLMPaged: null argument");
+  if (const int rc = paged_check(d)) return rc;
+  if (num_pages < 1 || table_width < 1 || kv_head < 0 || kv_head >= d->kv_heads || dim < 0 || dim >= d->head_dim)
+    return fail(TLM_ERR_INVALID, "TLMPaged: no kv head %d or dim %d", kv_head, dim);
+  const int shift = page_shift(*d), limit = paged_limit(d->max_tokens, table_width, shift);
+  if (position < 0 || position >= limit)
+    return fail(TLM_ERR_RANGE, "TLMPaged: position %d outside [0, %d)", position, limit);
+  const int page = paged_page(table, position, shift, num_pages);
+  if (page < 0)
+    return fail(TLM_ERR_RANGE, "TLMPaged: entry %d of position %d is none of %d pages", table[position >> shift],
+                position, num_pages);
+  const int E = d->kv_fmt == TLM_FMT_F32 ? 4 : 8, token = position & (d->page_tokens - 1);
+  const size_t head = paged_head_at(page, kv_head, d->kv_heads, shift, d->head_dim);
+  *k_index = (int64_t)(head + paged_k_at(token, dim, d->head_dim, E));
+  *v_index = (int64_t)(head + paged_v_at(token, dim, d->head_dim, E));
+  return TLM_OK;
+}
+
 // ------------------------------------------------------------------- logits --
 
 // LM head grid: every block resident at once (two 8-wave blocks per CU) with
@@ -1175,6 +1373,41 @@ int tlm_op_topk(tlm_ctx* ctx, const float* logits, int n, int k, double softcap,
   if (!launch_topk(logits, n, k, (float)(softcap > 0 ? softcap : 0), topk_work(ctx), scores, tokens, ctx->stream))
     return fail(TLM_ERR_INVALID, "TLMLogitSampler: %d logits exceed the candidate workspace", n);
   CHECK_LAUNCH("TLMLogitSampler");
+  return TLM_OK;
+}
+
+int tlm_op_verify_drafts(tlm_ctx* ctx, const float* logits, const float* draft_logits, const int32_t* drafts,
+                         const int32_t* counts, const float* uniforms, int32_t seqs, int32_t tokens, int32_t vocab,
+                         double temperature, int32_t* accepted, int32_t* out_tokens) {
+  if (!ctx || !logits || !accepted || !out_tokens || seqs < 1 || tokens < 1 || vocab < 1)
+    return fail(TLM_ERR_INVALID, "TLMVerify: invalid argument");
+  if (tokens > kVerifyMaxTokens)
+    return fail(TLM_ERR_INVALID, "TLMVerify: %d rows per sequence, at most %d", tokens, kVerifyMaxTokens);
+  if (tokens > 1 && !drafts) return fail(TLM_ERR_INVALID, "TLMVerify: %d rows without drafts", tokens);
+  if (!(temperature >= 0) || temperature > DBL_MAX)
+    return fail(TLM_ERR_INVALID, "TLMVerify: temperature %g", temperature);
+  if (temperature > 0 && !uniforms) return fail(TLM_ERR_INVALID, "TLMVerify: no random numbers");
+  if ((int64_t)seqs * tokens > (1 << 20))
+    return fail(TLM_ERR_RANGE, "TLMVerify: %d sequences of %d rows are more than 2^20 rows", seqs, tokens);
+  VerifyArgs a;
+  memset(&a, 0, sizeof a);
+  a.logits = logits;
+  a.draft_logits = draft_logits;
+  a.drafts = drafts;
+  a.counts = counts;
+  a.uniforms = uniforms;
+  a.accepted = accepted;
+  a.ids = out_tokens;
+  a.seqs = seqs;
+  a.tokens = tokens;
+  a.vocab = vocab;
+  a.inv_temp = temperature > 0 ? 1.0 / std::max(temperature, 1e-6) : 0.0;
+  verify_plan(a, ctx->cus, kPartFloats * sizeof(float));
+  const DeviceScope on(ctx->device);
+  std::lock_guard<std::mutex> lock(ctx->part_mu);
+  a.work = ctx->part;
+  launch_verify(a, ctx->stream);
+  CHECK_LAUNCH("TLMVerify");
   return TLM_OK;
 }
 

@@ -468,4 +468,45 @@ void launch_rope_kv(const RopeKvArgs& a, hipStream_t st);
 bool launch_prefill_attention(const PrefillAttnArgs& a, hipStream_t st);
 void launch_rows_to_f16(const float* x, size_t n, uint16_t* y, hipStream_t st);
 
+// Paged caches (tlm_paged.h) and the verification of drafted tokens.
+constexpr int kPagedStatusRows = 1;  // bits of a handle's status word: rows left out,
+constexpr int kPagedStatusPage = 2;  // a table entry that is no page of the pool
+struct PagedArgs {
+  const float* x;      // append: [seqs][tokens][(Hq + 2 Hkv) D] q|k|v; attention: [seqs][tokens][Hq D] q
+  float* q;            // append: rotated queries [seqs][tokens][Hq D], or null
+  void* out;           // attention: [seqs][tokens][Hq D], fp16 or fp32
+  void* kc;            // pools [num_pages][Hkv][page tokens x D]
+  void* vc;
+  const int32_t* tables;  // [seqs][width]
+  const int32_t* starts;  // [seqs]: position of a sequence's first row; < 0: idle
+  const int32_t* counts;  // [seqs]: its rows, or null for `tokens` each
+  const float* rope_cos;  // [max_tokens][rd / 2]
+  const float* rope_sin;
+  int* status;            // or'ed with kPagedStatus*
+  int num_pages, width, page_shift, seqs, tokens, limit;
+  int Hq, Hkv, D, G, rd, window;
+  int out_f32;
+  float scale;
+};
+bool launch_paged_append(bool kv_f32, const PagedArgs& a, hipStream_t st);
+bool launch_paged_attention(bool kv_f32, const PagedArgs& a, hipStream_t st);
+
+struct VerifyArgs {
+  const float* logits;        // [seqs][tokens][vocab]
+  const float* draft_logits;  // [seqs][tokens - 1][vocab], or null: the drafts are certain
+  const int32_t* drafts;      // [seqs][tokens - 1]
+  const int32_t* counts;      // [seqs], or null: tokens each
+  const float* uniforms;      // [seqs][tokens]
+  int32_t* accepted;          // [seqs]
+  int32_t* ids;               // [seqs][tokens]
+  int seqs, tokens, vocab;
+  double inv_temp;            // 0: greedy
+  int chunks, chunk;          // of the vocabulary
+  void* work;
+};
+constexpr int kVerifyMaxTokens = 64;
+// chunk and chunks, for at most `most` bytes of work
+void verify_plan(VerifyArgs& a, int cus, size_t most);
+void launch_verify(const VerifyArgs& a, hipStream_t st);
+
 }  // namespace tlm

@@ -29,6 +29,8 @@ EXPORTS = [
     "tlm_op_linear", "tlm_op_linear_rows", "tlm_rows_plan", "tlm_op_rmsnorm", "tlm_op_silu_mul", "tlm_op_gated_mlp", "tlm_attn_create", "tlm_attn_destroy",
     "tlm_op_attention", "tlm_op_attention_rows", "tlm_op_attention_rows_noalloc", "tlm_attn_reset", "tlm_attn_read_cache", "tlm_op_logits", "tlm_op_argmax",
     "tlm_op_topk", "tlm_read_candidates",
+    "tlm_paged_create", "tlm_paged_destroy", "tlm_op_paged_append", "tlm_op_paged_attention", "tlm_paged_status",
+    "tlm_paged_locate", "tlm_op_verify_drafts",
     "tlm_model_create", "tlm_model_destroy", "tlm_model_upload", "tlm_model_finalize", "tlm_model_set_prefill",
     "tlm_compute_token",
     "tlm_prefill", "tlm_read_logits", "tlm_read_token", "tlm_decode_greedy", "tlm_reset_cache", "tlm_kv_write",
@@ -49,6 +51,20 @@ class AttnDesc(ctypes.Structure):
                 ("max_tokens", ctypes.c_int32), ("rotary_dim", ctypes.c_int32), ("sliding_window", ctypes.c_int32),
                 ("kv_fmt", ctypes.c_int32), ("reserved", ctypes.c_int32), ("inv_freq", ctypes.POINTER(ctypes.c_float)),
                 ("attention_factor", ctypes.c_double), ("attn_scale", ctypes.c_double)]
+
+
+class PagedDesc(ctypes.Structure):
+    _fields_ = [("heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("max_tokens", ctypes.c_int32), ("rotary_dim", ctypes.c_int32), ("sliding_window", ctypes.c_int32),
+                ("kv_fmt", ctypes.c_int32), ("page_tokens", ctypes.c_int32),
+                ("inv_freq", ctypes.POINTER(ctypes.c_float)), ("attention_factor", ctypes.c_double),
+                ("attn_scale", ctypes.c_double)]
+
+
+class PagedBatch(ctypes.Structure):
+    _fields_ = [("k_pages", ctypes.c_void_p), ("v_pages", ctypes.c_void_p), ("tables", ctypes.c_void_p),
+                ("starts", ctypes.c_void_p), ("counts", ctypes.c_void_p), ("num_pages", ctypes.c_int32),
+                ("table_width", ctypes.c_int32), ("seqs", ctypes.c_int32), ("tokens", ctypes.c_int32)]
 
 
 class ModelDesc(ctypes.Structure):
@@ -114,6 +130,14 @@ def lib():
             "tlm_op_logits": ([VP, VP, VP, VP], ctypes.c_int),
             "tlm_op_argmax": ([VP, VP, ctypes.c_int, VP], ctypes.c_int),
             "tlm_op_topk": ([VP, VP, ctypes.c_int, ctypes.c_int, dbl, VP, VP], ctypes.c_int),
+            "tlm_paged_create": ([VP, ctypes.POINTER(PagedDesc), ctypes.POINTER(VP)], ctypes.c_int),
+            "tlm_paged_destroy": ([VP], None),
+            "tlm_op_paged_append": ([VP, ctypes.POINTER(PagedBatch), VP, VP], ctypes.c_int),
+            "tlm_op_paged_attention": ([VP, ctypes.POINTER(PagedBatch), VP, ctypes.c_int, VP], ctypes.c_int),
+            "tlm_paged_status": ([VP], ctypes.c_int),
+            "tlm_paged_locate": ([ctypes.POINTER(PagedDesc), i32, VP, i32, i32, i32, i32,
+                                  ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_int64)], ctypes.c_int),
+            "tlm_op_verify_drafts": ([VP, VP, VP, VP, VP, VP, i32, i32, i32, dbl, VP, VP], ctypes.c_int),
             "tlm_read_candidates": ([VP, ctypes.c_int, dbl, VP, VP], ctypes.c_int),
             "tlm_model_create": ([VP, ctypes.POINTER(ModelDesc), ctypes.POINTER(VP)], ctypes.c_int),
             "tlm_model_destroy": ([VP], None),
@@ -358,6 +382,76 @@ class Attention:
             self.ptr = None
 
 
+def paged_desc(heads, kv_heads, head_dim, max_tokens, page_tokens=64, inv_freq=None, rotary_dim=None,
+               attention_factor=1.0, sliding_window=0, kv_fmt=FMT_F16, attn_scale=0.0) -> PagedDesc:
+    """The head shapes, RoPE frequencies (inv_freq None: no RoPE) and page size of a paged cache."""
+    rd = 0 if inv_freq is None else head_dim if rotary_dim is None else rotary_dim
+    inv = np.ascontiguousarray(inv_freq if inv_freq is not None else np.zeros(1), np.float32)
+    if rd > 2 * inv.size:
+        raise ValueError(f"paged_desc: {inv.size} frequencies for {rd} rotary dims")
+    d = PagedDesc(heads, kv_heads, head_dim, max_tokens, rd, sliding_window, kv_fmt, page_tokens,
+                  inv.ctypes.data_as(ctypes.POINTER(ctypes.c_float)), attention_factor, attn_scale)
+    d.keep = inv
+    return d
+
+
+def paged_locate(desc: PagedDesc, num_pages: int, table, position: int, kv_head: int, dim: int):
+    """(index in a K pool, index in a V pool) of one element, from a host table (no device)."""
+    t = np.ascontiguousarray(table, np.int32).reshape(-1)
+    k, v = ctypes.c_int64(), ctypes.c_int64()
+    check(lib().tlm_paged_locate(ctypes.byref(desc), num_pages, _ptr(t), t.size, position, kv_head, dim,
+                                 ctypes.byref(k), ctypes.byref(v)))
+    return k.value, v.value
+
+
+def _addr(b):
+    return None if b is None else b.ptr
+
+
+class Paged:
+    """Attention over paged caches for many sequences at once: the head shapes and the RoPE table of a model.  Pools,
+    page tables and batches are the caller's device buffers."""
+
+    def __init__(self, ctx: Context, heads, kv_heads, head_dim, max_tokens, page_tokens=64, **options):
+        self.ctx = ctx
+        self.desc = paged_desc(heads, kv_heads, head_dim, max_tokens, page_tokens, **options)
+        p = VP()
+        check(lib().tlm_paged_create(ctx.ptr, ctypes.byref(self.desc), ctypes.byref(p)))
+        self.ptr = p
+
+    def page_bytes(self) -> int:
+        """Bytes of one page in the K pool, and again in the V pool."""
+        d = self.desc
+        return d.kv_heads * d.page_tokens * d.head_dim * (4 if d.kv_fmt == FMT_F32 else 2)
+
+    def batch(self, k_pages: Buffer, v_pages: Buffer, num_pages: int, tables: Buffer, table_width: int, starts: Buffer,
+              seqs: int, tokens: int = 1, counts: Optional[Buffer] = None) -> PagedBatch:
+        """One step's rows: tables int32 [seqs][table_width], starts (and counts) int32 [seqs]."""
+        b = PagedBatch(k_pages.ptr, v_pages.ptr, tables.ptr, starts.ptr, _addr(counts), num_pages, table_width, seqs,
+                       tokens)
+        b.keep = (k_pages, v_pages, tables, starts, counts)
+        return b
+
+    def append(self, batch: PagedBatch, qkv: Buffer, q: Optional[Buffer] = None) -> Optional[Buffer]:
+        """qkv fp32 [seqs][tokens][(H+2Hkv)D]: K and V to their pages, the rotated queries to q fp32 [..][H D]."""
+        check(lib().tlm_op_paged_append(self.ptr, ctypes.byref(batch), qkv.ptr, _addr(q)))
+        return q
+
+    def attention(self, batch: PagedBatch, q: Buffer, out: Buffer, out_fmt: int = FMT_F16) -> Buffer:
+        """Rotated queries fp32 [seqs][tokens][H D] over the pages -> out in out_fmt."""
+        check(lib().tlm_op_paged_attention(self.ptr, ctypes.byref(batch), q.ptr, out_fmt, out.ptr))
+        return out
+
+    def status(self):
+        """Waits; raises where a call since the last status met a row or a page out of range."""
+        check(lib().tlm_paged_status(self.ptr))
+
+    def close(self):
+        if self.ptr:
+            lib().tlm_paged_destroy(self.ptr)
+            self.ptr = None
+
+
 def rmsnorm(ctx: Context, x: Buffer, w: Optional[Buffer], n: int, eps: float, offset: bool, y: Buffer) -> Buffer:
     check(lib().tlm_op_rmsnorm(ctx.ptr, x.ptr, w.ptr if w else None, n, eps, int(offset), y.ptr))
     return y
@@ -391,6 +485,16 @@ def topk(ctx: Context, logits_buf: Buffer, n: int, k: int, softcap: float = 0.0)
     tok.free()
     sc.free()
     return [(int(a), float(b)) for a, b in zip(t, v)]
+
+
+def verify_drafts(ctx: Context, logits_buf: Buffer, seqs: int, tokens: int, vocab: int, accepted: Buffer,
+                  out_tokens: Buffer, drafts: Optional[Buffer] = None, draft_logits: Optional[Buffer] = None,
+                  counts: Optional[Buffer] = None, uniforms: Optional[Buffer] = None, temperature: float = 1.0):
+    """Which drafts stand and the token after them (tlm_op_verify_drafts); (accepted, out_tokens)."""
+    check(lib().tlm_op_verify_drafts(ctx.ptr, logits_buf.ptr, _addr(draft_logits), _addr(drafts), _addr(counts),
+                                     _addr(uniforms), seqs, tokens, vocab, float(temperature), accepted.ptr,
+                                     out_tokens.ptr))
+    return accepted, out_tokens
 
 
 # ------------------------------------------------------------------ model --
