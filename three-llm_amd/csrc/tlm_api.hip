@@ -1271,7 +1271,10 @@ int tlm_op_paged_attention(tlm_paged* P, const tlm_paged_batch* b, const float* 
   a.out = out;
   a.out_f32 = out_fmt == TLM_FMT_F32;
   const DeviceScope on(P->ctx->device);
-  if (!launch_paged_attention(P->d.kv_fmt == TLM_FMT_F32, a, P->ctx->stream))
+  // the chunks' results live in the context's buffer from one launch to the next
+  std::lock_guard<std::mutex> lock(P->ctx->part_mu);
+  a.part = P->ctx->part;
+  if (!launch_paged_attention(P->d.kv_fmt == TLM_FMT_F32, a, P->ctx->cus, kPartFloats, P->ctx->stream))
     return fail(TLM_ERR_STATE, "TLMPaged: no attention kernel for this shape");
   CHECK_LAUNCH("TLMPaged");
   return TLM_OK;

@@ -487,9 +487,13 @@ struct PagedArgs {
   int Hq, Hkv, D, G, rd, window;
   int out_f32;
   float scale;
+  // attention: how the sequences' position tiles are shared out (launch_paged_attention)
+  float* part;
+  int units, chunks, chunk_min, plan_shift;
 };
 bool launch_paged_append(bool kv_f32, const PagedArgs& a, hipStream_t st);
-bool launch_paged_attention(bool kv_f32, const PagedArgs& a, hipStream_t st);
+// part_floats: what a.part holds
+bool launch_paged_attention(bool kv_f32, const PagedArgs& a, int cus, size_t part_floats, hipStream_t st);
 
 struct VerifyArgs {
   const float* logits;        // [seqs][tokens][vocab]

@@ -2,7 +2,10 @@
 // rotated and appended to its pages (tlm_op_paged_append), and their attention
 // over those pages (tlm_op_paged_attention).
 #include <float.h>
+#include <limits.h>
 #include <math.h>
+
+#include <algorithm>
 
 #include "tlm_device.h"
 #include "tlm_paged.h"
@@ -51,62 +54,506 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedArgs a) {
   }
 }
 
-// One block per row and query head, 256 positions at a time: scores, their
-// softmax carried with a running maximum, the weighted sum of the values.
+typedef _Float16 ph8_t __attribute__((ext_vector_type(8)));
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // a row from any 4-byte address
+
+// Attention of the rows of a step.  A kv head's rows r = j G + g (token j, head g
+// of its group) are the columns of 16-column matrix-core tiles, so that K and V
+// are read once for all of them; a block holds NT of those tiles (`a.groups` row
+// groups of 16 NT cover tokens x G).  Its W waves take the position tiles of one
+// chunk of the sequence in turn:
+//   * scores S^T (positions x rows) = K Q^T, K the A operand, q the B operand;
+//   * softmax with a running maximum and sum per row, base 2;
+//   * O^T (dims x rows) += V^T P^T, V^T the A operand, P^T from the score registers.
+// The pages hold K and V in operand order (tlm_paged.h), so a tile's operands are
+// loaded straight into registers, 1 KB in a row per wave and instruction.
+// fp16 caches: 32 positions a tile, v_mfma_f32_16x16x32_f16 with q and P as hi +
+// lo pairs (x = hi + lo to 2^-22 of the row's largest q, resp. of 1; K and V are
+// exact).  fp32 caches: 16 positions a tile, v_mfma_f32_16x16x4_f32.
 template <typename KT>
-__global__ __launch_bounds__(256) void paged_attention_kernel(PagedArgs a) {
-  constexpr int E = 16 / sizeof(KT);
-  __shared__ float q[128], p[256], red[8];
-  const int h = blockIdx.x % a.Hq, row = blockIdx.x / a.Hq, s = row / a.tokens, j = row % a.tokens;
-  const int start = a.starts[s], tid = threadIdx.x, D = a.D, hk = h / a.G;
+struct PagedTile {
+  static constexpr int SUB = 4 / sizeof(KT);  // 16-position score tiles
+  static constexpr int TS = 16 * SUB;         // positions
+  static constexpr int SHIFT = SUB == 2 ? 5 : 4;
+};
+
+// A sequence's part in a call: its rows and the position tiles that they attend to.
+struct SeqWork {
+  int start, rows, first, tiles;
+};
+template <int SHIFT>
+__device__ __forceinline__ SeqWork seq_work(const PagedArgs& a, int s, bool* bad) {
+  SeqWork w;
+  w.start = a.starts[s];
+  w.rows = paged_rows(w.start, a.counts ? a.counts[s] : a.tokens, a.tokens, a.limit, bad);
+  const int first = a.window > 0 ? max(0, w.start - a.window + 1) : 0;
+  w.first = first >> SHIFT;
+  w.tiles = w.rows > 0 ? ((w.start + w.rows - 1) >> SHIFT) - w.first + 1 : 0;
+  return w;
+}
+
+// Chunks of equal size over sequences of unequal length: c tiles a chunk, such
+// that all sequences together have at most a.chunks more chunks than sequences.
+// Every wave works it out for itself from the starts (which only the device
+// knows): the sum of the tiles, then a running sum of the sequences' chunks up to
+// the one that `found` accepts (excl: chunks of the sequences before, n: its own).
+// slot: records of partial results before it (sequences of one chunk have none).
+struct SeqChunks {
+  SeqWork w;
+  int s, n, chunk, slot;  // chunk: which of the sequence's (plan_chunk)
   bool bad;
-  const int rows = paged_rows(start, a.counts ? a.counts[s] : a.tokens, a.tokens, a.limit, &bad);
-  if (bad && j == 0 && h == 0 && tid == 0) paged_flag(a.status, kPagedStatusRows);
-  if (j >= rows) return;
-  const int pos = start + j, first = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-  const int* table = a.tables + (size_t)s * a.width;
-  if (tid < D) q[tid] = a.x[((size_t)row * a.Hq + h) * D + tid] * a.scale;
-  float M = -FLT_MAX, L = 0.f, acc = 0.f;
-  for (int t0 = first; t0 <= pos; t0 += 256) {
-    __syncthreads();
-    const int t = t0 + tid;
-    float sc = -INFINITY;
-    if (t <= pos) {
-      const int page = paged_page(table, t, a.page_shift, a.num_pages);
-      if (page < 0) {
-        paged_flag(a.status, kPagedStatusPage);
-      } else {
-        const KT* k = static_cast<const KT*>(a.kc) + paged_head_at(page, hk, a.Hkv, a.page_shift, D);
-        sc = 0.f;
-        for (int d = 0; d < D; d++)
-          sc = fmaf(q[d], kv_load<KT>(k + paged_k_at(t & ((1 << a.page_shift) - 1), d, D, E)), sc);
+};
+template <int SHIFT, typename Found>
+__device__ __forceinline__ bool plan(const PagedArgs& a, SeqChunks& r, Found found) {
+  const int lane = threadIdx.x & 63;
+  bool bad = false;
+  SeqWork w = lane < a.seqs ? seq_work<SHIFT>(a, lane, &bad) : SeqWork{0, 0, 0, 0};
+  int total = (w.tiles + (1 << a.plan_shift) - 1) >> a.plan_shift;
+  for (int s = lane + 64; s < a.seqs; s += 64) {
+    bool b;
+    total += (seq_work<SHIFT>(a, s, &b).tiles + (1 << a.plan_shift) - 1) >> a.plan_shift;
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) total += __shfl_xor(total, o);
+  const int c = max(a.chunk_min, ((total + a.chunks - 1) / a.chunks) << a.plan_shift);
+  int before = 0, slots = 0;
+  for (int s0 = 0; s0 < a.seqs; s0 += 64) {
+    if (s0) w = s0 + lane < a.seqs ? seq_work<SHIFT>(a, s0 + lane, &bad) : SeqWork{0, 0, 0, 0};
+    const int n = (w.tiles + c - 1) / c, m = n > 1 ? n : 0;
+    int incl = n, sincl = m;
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+      const int x = __shfl_up(incl, o), y = __shfl_up(sincl, o);
+      if (lane >= o) incl += x, sincl += y;
+    }
+    const int excl = before + incl - n;
+    const unsigned long long hit = __ballot(found(s0 + lane, excl, n));
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      r.s = s0 + l;
+      r.w.start = __builtin_amdgcn_readlane(w.start, l);
+      r.w.rows = __builtin_amdgcn_readlane(w.rows, l);
+      r.w.first = __builtin_amdgcn_readlane(w.first, l);
+      r.w.tiles = __builtin_amdgcn_readlane(w.tiles, l);
+      r.n = __builtin_amdgcn_readlane(n, l);
+      r.chunk = __builtin_amdgcn_readlane(excl, l);  // chunks before the sequence
+      r.slot = slots + __builtin_amdgcn_readlane(sincl - m, l);
+      r.bad = __builtin_amdgcn_readlane((int)bad, l);
+      return true;
+    }
+    before += __builtin_amdgcn_readlane(incl, 63);
+    slots += __builtin_amdgcn_readlane(sincl, 63);
+  }
+  return false;
+}
+
+// Partial results: per slot, unit (kv head and row group) and row the unscaled
+// output, then per row (maximum in base 2, sum).
+__device__ __forceinline__ float* part_row(const PagedArgs& a, int slot, int unit, int row, int rows, int DT) {
+  return a.part + (((size_t)slot * a.units + unit) * rows + row) * (DT + 2);
+}
+
+template <typename KT, int DT, int NT, int W>
+__global__ __launch_bounds__(64 * W) void paged_attention_kernel(PagedArgs a) {
+  using T = PagedTile<KT>;
+  constexpr int SUB = T::SUB, TS = T::TS, NF = DT / 16;  // 1 KB operand pieces of a tile's K, of its V
+  constexpr bool F16 = sizeof(KT) == 2, QREG = NT == 1;
+  constexpr int RS = DT + 2;  // floats of a row's record: maximum, sum, output
+  constexpr int QB = QREG ? 0 : NT * NF * 64 * 4, MB = W * 16 * RS;  // floats
+  __shared__ __align__(16) float lds[QB > MB ? QB : MB];
+  const int unit = blockIdx.x % a.units, hk = unit % a.Hkv, r0 = unit / a.Hkv * 16 * NT;
+  const int g = blockIdx.x / a.units;
+  SeqChunks sc;
+  if (!plan<T::SHIFT>(a, sc, [&](int, int excl, int n) { return excl <= g && g < excl + n; })) return;
+  const int ci = g - sc.chunk, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  if (sc.bad && ci == 0 && unit == 0 && tid == 0) paged_flag(a.status, kPagedStatusRows);
+  const int R = sc.w.rows * a.G;  // rows of the kv head
+  if (r0 >= R) return;
+  const int i16 = lane & 15, qd = lane >> 4;
+  // positions that some row of the block attends to, and that all do
+  const int ja = r0 / a.G, jb = (min(r0 + 16 * NT, R) - 1) / a.G, start = sc.w.start;
+  const int lo_any = a.window > 0 ? max(0, start + ja - a.window + 1) : 0, hi_any = start + jb;
+  const int lo_all = a.window > 0 ? max(0, start + jb - a.window + 1) : 0, hi_all = start + ja;
+  const int per = (sc.w.tiles + sc.n - 1) / sc.n;
+  const int t0 = max(sc.w.first + ci * per, lo_any >> T::SHIFT);
+  const int t1 = min(min(sc.w.first + (ci + 1) * per, sc.w.first + sc.w.tiles), (hi_any >> T::SHIFT) + 1);
+  const int32_t* const table = a.tables + (size_t)sc.s * a.width;
+  const int tpp = a.page_shift - T::SHIFT;  // log2 of the tiles of a page
+
+  // this lane's rows (a column of each tile): their positions' bounds, q scaled by
+  // a power of two per row to at most 1
+  int lo[NT], hi[NT];
+  float mult[NT];
+  u32x4 qreg[QREG ? NF : 1];
+  u32x4* const qlds = reinterpret_cast<u32x4*>(lds);  // [NT][NF][64]
+  const float qscale = a.scale * 1.4426950408889634f;  // log2 e: the softmax runs in base 2
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++) {
+    const int r = r0 + 16 * nt + i16, rc = min(r, R - 1), j = rc / a.G, pos = start + j;
+    lo[nt] = a.window > 0 ? pos - a.window + 1 : 0;
+    hi[nt] = pos;
+    const float* q = a.x + (((size_t)sc.s * a.tokens + j) * a.Hq + hk * a.G + rc % a.G) * DT;
+    f32x4 x[NF];
+#pragma unroll
+    for (int f = 0; f < NF; f++)  // fp16: dims 32 (f / 2) + 8 qd + 4 (f % 2) ..; fp32: 16 f + 4 qd ..
+      x[f] = *(const TLM_GLOBAL f32x4u*)(q + (F16 ? 32 * (f / 2) + 8 * qd + 4 * (f & 1) : 16 * f + 4 * qd));
+    float m = 0.f;
+#pragma unroll
+    for (int f = 0; f < NF; f++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) m = fmaxf(m, fabsf(x[f][e]));
+    m = fmaxf(m, lane_swap16(m));
+    m = fmaxf(m, lane_swap32(m));
+    const int ex = max(-120, min(120, __builtin_amdgcn_frexp_expf(m)));
+    mult[nt] = ldexpf(qscale, ex);
+#pragma unroll
+    for (int f = 0; f < NF; f++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) x[f][e] = r < R ? ldexpf(x[f][e], -ex) : 0.f;
+    if (F16) {
+#pragma unroll
+      for (int jj = 0; jj < NF / 2; jj++) {
+        ph8_t h, l;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const float v = x[2 * jj + e / 4][e & 3];
+          h[e] = (_Float16)v;
+          l[e] = (_Float16)(v - (float)h[e]);
+        }
+        const u32x4 hb = __builtin_bit_cast(u32x4, h), lb = __builtin_bit_cast(u32x4, l);
+        if (QREG) qreg[QREG ? 2 * jj : 0] = hb, qreg[QREG ? 2 * jj + 1 : 0] = lb;
+        else if (w == nt % W) qlds[(nt * NF + 2 * jj) * 64 + lane] = hb, qlds[(nt * NF + 2 * jj + 1) * 64 + lane] = lb;
+      }
+    } else {
+#pragma unroll
+      for (int f = 0; f < NF; f++) {
+        if (QREG) qreg[QREG ? f : 0] = __builtin_bit_cast(u32x4, x[f]);
+        else if (w == nt % W) qlds[(nt * NF + f) * 64 + lane] = __builtin_bit_cast(u32x4, x[f]);
       }
     }
-    const float wm = wave_max(sc);
-    if ((tid & 63) == 0) red[tid >> 6] = wm;
-    __syncthreads();
-    const float m = fmaxf(M, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-    const float corr = __expf(M - m), e = __expf(sc - m);
-    p[tid] = e;
-    const float ws = wave_sum(e);
-    if ((tid & 63) == 0) red[4 + (tid >> 6)] = ws;
-    __syncthreads();
-    L = L * corr + (red[4] + red[5] + red[6] + red[7]);
-    M = m;
-    acc *= corr;
-    if (tid < D)
-      for (int i = 0; i < min(256, pos + 1 - t0); i++) {
-        const int page = paged_page(table, t0 + i, a.page_shift, a.num_pages);
-        if (page < 0) continue;
-        const KT* v = static_cast<const KT*>(a.vc) + paged_head_at(page, hk, a.Hkv, a.page_shift, D);
-        acc = fmaf(p[i], kv_load<KT>(v + paged_v_at((t0 + i) & ((1 << a.page_shift) - 1), tid, D, E)), acc);
-      }
   }
-  if (tid >= D) return;
-  const float y = L == 0.f ? 0.f : acc / L;  // 0: no position has a page
-  const size_t at = ((size_t)row * a.Hq + h) * D + tid;
+  if (!QREG) lds_barrier();
+
+  f32x4 o[NT][NF];
+  float mrun[NT], lrun[NT];  // running maximum, this lane's share of the sum
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++) {
+    mrun[nt] = -FLT_MAX;
+    lrun[nt] = 0.f;
+#pragma unroll
+    for (int f = 0; f < NF; f++) o[nt][f] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  }
+
+  struct Tile {
+    u32x4 k[NF], v[NF];
+  };
+  auto load = [&](u32x4* x, const void* pool, int t, int page) {
+    const size_t at = paged_head_at(max(page, 0), hk, a.Hkv, a.page_shift, DT) +
+                      (size_t)(t & ((1 << tpp) - 1)) * (TS * DT) + lane * (16 / sizeof(KT));
+    const TLM_GLOBAL u32x4* p = gl(reinterpret_cast<const u32x4*>(static_cast<const KT*>(pool) + at));
+#pragma unroll
+    for (int f = 0; f < NF; f++) x[f] = p[64 * f];
+  };
+  // V with positions outside [first, last] taken out (0 times what they hold may be NaN)
+  auto keep = [&](const u32x4& v, int p, int first, int last) {
+    u32x4 y;
+#pragma unroll
+    for (int d = 0; d < 4; d++) {
+      if (F16) {  // dword d: positions 16 (d / 2) + 4 qd + 2 (d % 2) + {0, 1}
+        const int x = p + 16 * (d / 2) + 4 * qd + 2 * (d & 1);
+        y[d] = v[d] & ((x >= first && x <= last ? 0xFFFFu : 0u) | (x + 1 >= first && x + 1 <= last ? 0xFFFF0000u : 0u));
+      } else {
+        const int x = p + 4 * qd + d;
+        y[d] = x >= first && x <= last ? v[d] : 0u;
+      }
+    }
+    return y;
+  };
+  // tile t; k_read() and v_read() run once x.k and x.v have been read
+  auto process = [&](Tile& x, int t, auto k_read, auto v_read) {
+    if (!QREG) asm volatile("" ::: "memory");  // q is read again, not kept in registers that o needs
+    const int p = t << T::SHIFT;
+    const bool edge = p < lo_all || p + TS - 1 > hi_all;  // some row does not see all of it (wave-uniform)
+    bool apart = false;
+    if (edge) {
+      // only a value that is not finite could reach a row that masks its position
+      unsigned nf = 0;
+#pragma unroll
+      for (int f = 0; f < NF; f++) {
+        x.v[f] = keep(x.v[f], p, lo_any, hi_any);
+#pragma unroll
+        for (int d = 0; d < 4; d++)
+          nf |= F16 ? ((x.v[f][d] & 0x7C007C00u) + 0x04000400u) & 0x80008000u
+                    : ((x.v[f][d] & 0x7F800000u) + 0x00800000u) & 0x80000000u;
+      }
+      apart = ja != jb && __ballot(nf != 0) != 0;
+    }
+    u32x4 ph[NT], pl[F16 ? NT : 1];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+      f32x4 acc[2] = {(f32x4){0.f, 0.f, 0.f, 0.f}, (f32x4){0.f, 0.f, 0.f, 0.f}};
+      if (F16) {
+#pragma unroll
+        for (int jj = 0; jj < NF / 2; jj++) {
+          const ph8_t qh = __builtin_bit_cast(ph8_t, QREG ? qreg[QREG ? 2 * jj : 0] : qlds[(nt * NF + 2 * jj) * 64 + lane]);
+          const ph8_t ql = __builtin_bit_cast(ph8_t, QREG ? qreg[QREG ? 2 * jj + 1 : 0] : qlds[(nt * NF + 2 * jj + 1) * 64 + lane]);
+#pragma unroll
+          for (int st = 0; st < SUB; st++) {
+            const ph8_t k = __builtin_bit_cast(ph8_t, x.k[st * (NF / SUB) + jj]);
+            acc[st] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh, acc[st], 0, 0, 0);
+            acc[st] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql, acc[st], 0, 0, 0);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int f = 0; f < NF; f++) {
+          const f32x4 q = __builtin_bit_cast(f32x4, QREG ? qreg[QREG ? f : 0] : qlds[(nt * NF + f) * 64 + lane]);
+          const f32x4 k = __builtin_bit_cast(f32x4, x.k[f]);
+#pragma unroll
+          for (int e = 0; e < 4; e++) acc[e & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[e], q[e], acc[e & 1], 0, 0, 0);
+        }
+        acc[0] += acc[1];
+      }
+      // lane (row i16, qd): positions p + 16 st + 4 qd + e
+      float sv[4 * SUB];
+#pragma unroll
+      for (int st = 0; st < SUB; st++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) sv[4 * st + e] = acc[st][e] * mult[nt];
+      if (edge) {
+#pragma unroll
+        for (int i = 0; i < 4 * SUB; i++) {
+          const int y = p + 16 * (i / 4) + 4 * qd + (i & 3);
+          if (y < lo[nt] || y > hi[nt]) sv[i] = -INFINITY;
+        }
+      }
+      float mx = sv[0];
+#pragma unroll
+      for (int i = 1; i < 4 * SUB; i++) mx = fmaxf(mx, sv[i]);
+      mx = fmaxf(mx, lane_swap16(mx));
+      mx = fmaxf(mx, lane_swap32(mx));
+      const float mn = fmaxf(mrun[nt], mx);  // finite: it starts at -FLT_MAX
+      const float corr = __builtin_amdgcn_exp2f(mrun[nt] - mn);
+      float ps = 0.f;
+      if (F16) {
+        ph8_t h, l;
+#pragma unroll
+        for (int i = 0; i < 4 * SUB; i++) {
+          const float v = __builtin_amdgcn_exp2f(sv[i] - mn);
+          ps += v;
+          h[i % 8] = (_Float16)v;
+          l[i % 8] = (_Float16)(v - (float)h[i % 8]);
+        }
+        ph[nt] = __builtin_bit_cast(u32x4, h);
+        pl[F16 ? nt : 0] = __builtin_bit_cast(u32x4, l);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const float v = __builtin_amdgcn_exp2f(sv[i] - mn);
+          ps += v;
+          ph[nt][i] = __float_as_uint(v);
+        }
+      }
+      lrun[nt] = fmaf(lrun[nt], corr, ps);
+      mrun[nt] = mn;
+      if (__ballot(corr != 1.f)) {
+#pragma unroll
+        for (int f = 0; f < NF; f++) o[nt][f] *= corr;
+      }
+    }
+    k_read();
+    auto weigh = [&](const u32x4& v, int nt, f32x4 y) -> f32x4 {
+      if (F16) {
+        const ph8_t vh = __builtin_bit_cast(ph8_t, v);
+        y = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, __builtin_bit_cast(ph8_t, ph[nt]), y, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, __builtin_bit_cast(ph8_t, pl[F16 ? nt : 0]), y, 0, 0, 0);
+      }
+      const f32x4 vf = __builtin_bit_cast(f32x4, v), pf = __builtin_bit_cast(f32x4, ph[nt]);
+#pragma unroll
+      for (int e = 0; e < 4; e++) y = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[e], pf[e], y, 0, 0, 0);
+      return y;
+    };
+    if (!apart) {
+#pragma unroll
+      for (int f = 0; f < NF; f++)
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) o[nt][f] = weigh(x.v[f], nt, o[nt][f]);
+      v_read();
+      return;
+    }
+    // token by token, each over the positions that it sees, kept in its rows' columns
+    for (int j = ja; j <= jb; j++) {
+      const int first = a.window > 0 ? start + j - a.window + 1 : 0, last = start + j;
+#pragma unroll
+      for (int f = 0; f < NF; f++) {
+        const u32x4 v = keep(x.v[f], p, first, last);
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+          const f32x4 y = weigh(v, nt, o[nt][f]);
+          if (hi[nt] == last) o[nt][f] = y;
+        }
+      }
+    }
+    v_read();
+  };
+
+  // The wave's tiles t0 + w, t0 + w + W, ...  Their pages, 64 at a time, a lane each.
+  // One row tile: a position tile in work, the next in flight.  More: their outputs
+  // take the registers of a second one, and the next tile's K goes out when this
+  // one's has been read, its V likewise.
+  const auto none = [] {};
+  for (int tb = t0 + w; tb < t1; tb += 64 * W) {
+    const int tl = tb + lane * W, n = min(64, (t1 - tb + W - 1) / W);
+    const int page = paged_page(table, min(tl, t1 - 1) << T::SHIFT, a.page_shift, a.num_pages);
+    if (page < 0 && tl < t1) paged_flag(a.status, kPagedStatusPage);
+    auto page_of = [&](int i) { return __builtin_amdgcn_readlane(page, min(i, n - 1)); };
+    auto load_k = [&](Tile& x, int i) { load(x.k, a.kc, tb + min(i, n - 1) * W, page_of(i)); };
+    auto load_v = [&](Tile& x, int i) { load(x.v, a.vc, tb + min(i, n - 1) * W, page_of(i)); };
+    Tile x;
+    load_k(x, 0);
+    load_v(x, 0);
+    if constexpr (NT == 1) {
+      Tile y;
+      for (int i = 0; i < n; i += 2) {
+        load_k(y, i + 1);
+        load_v(y, i + 1);
+        if (page_of(i) >= 0) process(x, tb + i * W, none, none);
+        if (i + 1 >= n) break;
+        load_k(x, i + 2);
+        load_v(x, i + 2);
+        if (page_of(i + 1) >= 0) process(y, tb + (i + 1) * W, none, none);
+      }
+    } else {
+      for (int i = 0; i < n; i++) {
+        if (page_of(i) >= 0) {
+          process(x, tb + i * W, [&] { load_k(x, i + 1); }, [&] { load_v(x, i + 1); });
+        } else {
+          load_k(x, i + 1);
+          load_v(x, i + 1);
+        }
+      }
+    }
+  }
+
+  // the waves' results, 16 rows at a time, through LDS
+  const bool whole = sc.n == 1;
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++) {
+    float l = lrun[nt];
+    l += lane_swap16(l);
+    l += lane_swap32(l);
+    if (r0 + 16 * nt >= R) break;  // block-uniform
+    __syncthreads();
+    float* rec = lds + (w * 16 + i16) * RS;
+#pragma unroll
+    for (int f = 0; f < NF; f++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) rec[2 + 16 * f + 4 * qd + e] = o[nt][f][e];
+    if (qd == 0) rec[0] = mrun[nt], rec[1] = l;
+    __syncthreads();
+    for (int e = tid; e < 16 * DT; e += 64 * W) {
+      const int row = e / DT, d = e % DT, r = r0 + 16 * nt + row;
+      if (r >= R) break;
+      float M = -FLT_MAX, L = 0.f, O = 0.f;
+#pragma unroll
+      for (int x = 0; x < W; x++) M = fmaxf(M, lds[(x * 16 + row) * RS]);
+#pragma unroll
+      for (int x = 0; x < W; x++) {
+        const float* y = lds + (x * 16 + row) * RS;
+        const float f = __builtin_amdgcn_exp2f(y[0] - M);
+        L = fmaf(y[1], f, L);
+        O = fmaf(y[2 + d], f, O);
+      }
+      if (whole) {
+        const float y = L == 0.f ? 0.f : O / L;  // 0: no position has a page
+        const size_t at = (((size_t)sc.s * a.tokens + r / a.G) * a.Hq + hk * a.G + r % a.G) * DT + d;
+        if (a.out_f32) static_cast<float*>(a.out)[at] = y;
+        else static_cast<uint16_t*>(a.out)[at] = kv_store<uint16_t>(y);
+      } else {
+        float* p = part_row(a, sc.slot + ci, unit, 16 * nt + row, 16 * NT, DT);
+        p[d] = O;
+        if (d == 0) p[DT] = M, p[DT + 1] = L;
+      }
+    }
+  }
+}
+
+// The chunks of a row joined: a block per sequence, unit and row (`used` of the
+// `rows` that a unit's record holds).
+template <int SHIFT, int DT>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int rows, int used) {
+  constexpr int P = DT / 2, NG = 256 / P;  // threads of a record, two dims each; records at a time
+  __shared__ float red[NG][DT + 2];
+  const int row = blockIdx.x % used, unit = blockIdx.x / used % a.units, s = blockIdx.x / used / a.units;
+  SeqChunks sc;
+  plan<SHIFT>(a, sc, [&](int i, int, int) { return i == s; });
+  const int r = unit / a.Hkv * rows + row, hk = unit % a.Hkv;
+  if (sc.n < 2 || r >= sc.w.rows * a.G) return;
+  const int d2 = threadIdx.x % P, grp = threadIdx.x / P;
+  if (grp < NG) {
+    float M = -FLT_MAX, L = 0.f, O0 = 0.f, O1 = 0.f;
+    for (int c = grp; c < sc.n; c += NG) {
+      const float* p = part_row(a, sc.slot + c, unit, row, rows, DT);
+      const float2 v = *reinterpret_cast<const float2*>(p + 2 * d2), ml = *reinterpret_cast<const float2*>(p + DT);
+      const float mn = fmaxf(M, ml.x), f = __builtin_amdgcn_exp2f(M - mn), h = __builtin_amdgcn_exp2f(ml.x - mn);
+      L = L * f + ml.y * h;
+      O0 = O0 * f + v.x * h;
+      O1 = O1 * f + v.y * h;
+      M = mn;
+    }
+    red[grp][2 * d2] = O0;
+    red[grp][2 * d2 + 1] = O1;
+    if (d2 == 0) red[grp][DT] = M, red[grp][DT + 1] = L;
+  }
+  __syncthreads();
+  const int d = threadIdx.x;
+  if (d >= DT) return;
+  float M = -FLT_MAX, L = 0.f, O = 0.f;
+#pragma unroll
+  for (int x = 0; x < NG; x++) M = fmaxf(M, red[x][DT]);
+#pragma unroll
+  for (int x = 0; x < NG; x++) {
+    const float f = __builtin_amdgcn_exp2f(red[x][DT] - M);
+    L = fmaf(red[x][DT + 1], f, L);
+    O = fmaf(red[x][d], f, O);
+  }
+  const float y = L == 0.f ? 0.f : O / L;
+  const size_t at = (((size_t)s * a.tokens + r / a.G) * a.Hq + hk * a.G + r % a.G) * DT + d;
   if (a.out_f32) static_cast<float*>(a.out)[at] = y;
   else static_cast<uint16_t*>(a.out)[at] = kv_store<uint16_t>(y);
+}
+
+template <typename KT, int DT, int NT, int W>
+void launch_attention_of(PagedArgs a, int cus, size_t part_floats, hipStream_t st) {
+  using T = PagedTile<KT>;
+  const int rows = 16 * NT, groups = (a.tokens * a.G + rows - 1) / rows;
+  a.units = a.Hkv * groups;
+  // tiles that a sequence may have, as far as the host knows
+  int64_t most = a.limit;
+  if (a.window > 0) most = std::min<int64_t>(most, (int64_t)a.window + a.tokens);
+  const int64_t tiles = most / T::TS + 2;
+  a.plan_shift = 0;
+  while (a.seqs * ((tiles >> a.plan_shift) + 1) >= ((int64_t)1 << 30)) a.plan_shift++;
+  // all blocks at once: `chunks` of them a unit
+  const int64_t record = (int64_t)rows * (DT + 2);
+  const int64_t fit = (int64_t)part_floats / (2 * a.units * record);  // sequences of two chunks or more: 2 * chunks at most
+  a.chunks = (int)std::max<int64_t>(1, std::min<int64_t>(fit, 2 * cus / a.units));
+  a.chunk_min = fit < 1 ? INT_MAX / 2 : W;
+  const int64_t per_seq = fit < 1 ? 1 : (tiles + a.chunk_min - 1) / a.chunk_min;
+  const int64_t blocks = std::min<int64_t>(a.chunks + a.seqs, a.seqs * per_seq) * a.units;
+  hipLaunchKernelGGL((paged_attention_kernel<KT, DT, NT, W>), dim3((unsigned)blocks), dim3(64 * W), 0, st, a);
+  if (per_seq < 2) return;
+  const int used = std::min(rows, a.tokens * a.G);
+  hipLaunchKernelGGL((paged_join_kernel<T::SHIFT, DT>), dim3((unsigned)(a.seqs * a.units * used)), dim3(256), 0, st, a,
+                     rows, used);
+}
+
+template <typename KT, int DT>
+void launch_attention_rows(const PagedArgs& a, int cus, size_t part_floats, hipStream_t st) {
+  const int rows = a.tokens * a.G;
+  if (rows <= 16) launch_attention_of<KT, DT, 1, 8>(a, cus, part_floats, st);
+  else if (rows <= 32) launch_attention_of<KT, DT, 2, 4>(a, cus, part_floats, st);
+  else launch_attention_of<KT, DT, 4, 4>(a, cus, part_floats, st);
 }
 
 }  // namespace
@@ -118,11 +565,15 @@ bool launch_paged_append(bool kv_f32, const PagedArgs& a, hipStream_t st) {
   return true;
 }
 
-bool launch_paged_attention(bool kv_f32, const PagedArgs& a, hipStream_t st) {
-  const dim3 grid((unsigned)(a.seqs * a.tokens * a.Hq));
-  if (kv_f32) hipLaunchKernelGGL(paged_attention_kernel<float>, grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL(paged_attention_kernel<uint16_t>, grid, dim3(256), 0, st, a);
-  return true;
+bool launch_paged_attention(bool kv_f32, const PagedArgs& a, int cus, size_t part_floats, hipStream_t st) {
+#define PAGED_D(DT)                                                                \
+  case DT:                                                                         \
+    if (kv_f32) launch_attention_rows<float, DT>(a, cus, part_floats, st);         \
+    else launch_attention_rows<uint16_t, DT>(a, cus, part_floats, st);             \
+    return true;
+  switch (a.D) { PAGED_D(32) PAGED_D(64) PAGED_D(96) PAGED_D(128) }
+#undef PAGED_D
+  return false;
 }
 
 }  // namespace tlm
