@@ -90,6 +90,7 @@ struct tlm_ctx {
   // tlm_op_logits: the blocks' folded best and their count (zero between launches)
   unsigned long long* arg_key = nullptr;
   unsigned* arg_arrived = nullptr;
+  unsigned* verify_arrived = nullptr;  // tlm_op_verify_drafts' blocks done, per sequence (zero between launches)
   unsigned* topk_arrived = nullptr;  // tlm_op_topk's blocks done (zero between launches)
   // top-k levels: two levels of kTopkWork (score, id) pairs
   float* topk_v = nullptr;
@@ -536,6 +537,8 @@ int tlm_open(int device, tlm_ctx** out) {
   if (e == hipSuccess) e = hipMalloc(&c->arg_key, sizeof(unsigned long long));
   if (e == hipSuccess) e = hipMalloc(&c->arg_arrived, sizeof(unsigned));
   if (e == hipSuccess) e = hipMalloc(&c->topk_arrived, sizeof(unsigned));
+  if (e == hipSuccess) e = hipMalloc(&c->verify_arrived, kVerifyCounters * sizeof(unsigned));
+  if (e == hipSuccess) e = hipMemset(c->verify_arrived, 0, kVerifyCounters * sizeof(unsigned));
   if (e == hipSuccess) e = hipMemset(c->topk_arrived, 0, sizeof(unsigned));
   if (e == hipSuccess) e = hipMemset(c->arg_key, 0, sizeof(unsigned long long));
   if (e == hipSuccess) e = hipMemset(c->arg_arrived, 0, sizeof(unsigned));
@@ -564,6 +567,7 @@ void tlm_close(tlm_ctx* ctx) {
   hipFree(ctx->arg_key);
   hipFree(ctx->arg_arrived);
   hipFree(ctx->topk_arrived);
+  hipFree(ctx->verify_arrived);
   if (ctx->stream) hipStreamDestroy(ctx->stream);
   delete ctx;
 }
@@ -1386,6 +1390,8 @@ int tlm_op_verify_drafts(tlm_ctx* ctx, const float* logits, const float* draft_l
     return fail(TLM_ERR_INVALID, "TLMVerify: invalid argument");
   if (tokens > kVerifyMaxTokens)
     return fail(TLM_ERR_INVALID, "TLMVerify: %d rows per sequence, at most %d", tokens, kVerifyMaxTokens);
+  if (vocab > kVerifyMaxVocab)
+    return fail(TLM_ERR_INVALID, "TLMVerify: a vocabulary of %d, at most %d", vocab, kVerifyMaxVocab);
   if (tokens > 1 && !drafts) return fail(TLM_ERR_INVALID, "TLMVerify: %d rows without drafts", tokens);
   if (!(temperature >= 0) || temperature > DBL_MAX)
     return fail(TLM_ERR_INVALID, "TLMVerify: temperature %g", temperature);
@@ -1404,12 +1410,16 @@ int tlm_op_verify_drafts(tlm_ctx* ctx, const float* logits, const float* draft_l
   a.seqs = seqs;
   a.tokens = tokens;
   a.vocab = vocab;
-  a.inv_temp = temperature > 0 ? 1.0 / std::max(temperature, 1e-6) : 0.0;
-  verify_plan(a, ctx->cus, kPartFloats * sizeof(float));
+  a.scale = temperature > 0 ? 1.4426950408889634 / std::max(temperature, 1e-6) : 0.0;
+  a.arrived = ctx->verify_arrived;
+  const size_t need = verify_plan(a);
+  if (need > kPartFloats * sizeof(float))
+    return fail(TLM_ERR_RANGE, "TLMVerify: %d sequences of %d rows over %d tokens need %zu bytes of workspace, of %zu",
+                seqs, tokens, vocab, need, kPartFloats * sizeof(float));
   const DeviceScope on(ctx->device);
   std::lock_guard<std::mutex> lock(ctx->part_mu);
   a.work = ctx->part;
-  launch_verify(a, ctx->stream);
+  launch_verify(a, ctx->cus, ctx->stream);
   CHECK_LAUNCH("TLMVerify");
   return TLM_OK;
 }

@@ -504,13 +504,16 @@ struct VerifyArgs {
   int32_t* accepted;          // [seqs]
   int32_t* ids;               // [seqs][tokens]
   int seqs, tokens, vocab;
-  double inv_temp;            // 0: greedy
-  int chunks, chunk;          // of the vocabulary
-  void* work;
+  double scale;               // log2(e) / temperature; 0: greedy
+  int rows, chunks;           // verify_plan: rows of a sequence that are read, chunks of a row
+  void* work;                 // verify_plan's bytes
+  unsigned* arrived;          // [kVerifyCounters], zero between launches
 };
 constexpr int kVerifyMaxTokens = 64;
-// chunk and chunks, for at most `most` bytes of work
-void verify_plan(VerifyArgs& a, int cus, size_t most);
-void launch_verify(const VerifyArgs& a, hipStream_t st);
+constexpr int kVerifyMaxVocab = 524288;
+constexpr int kVerifyCounters = 4096;
+// Fills in rows and chunks; the bytes that a.work has to hold.
+size_t verify_plan(VerifyArgs& a);
+void launch_verify(const VerifyArgs& a, int cus, hipStream_t st);
 
 }  // namespace tlm

@@ -9,6 +9,12 @@
 // Everything is in 64 bits: which token is drawn hangs on sums over the
 // vocabulary, and 32-bit ones (2^-24 a term) would move a border past u once in
 // some hundred draws from a flat distribution over 10^5 tokens.
+//
+// One pass over the logits: a wave takes kVChunk entries of a row into registers
+// and leaves their maximum and sum of exponentials (greedy: the best entry).  The
+// block that finishes a sequence's last chunk decides from these few numbers and
+// reads one more chunk for the token, in the same launch.  With draft logits the
+// refused row's max(p - q, 0) takes a second launch.
 #include <float.h>
 #include <limits.h>
 #include <math.h>
@@ -20,45 +26,111 @@
 namespace tlm {
 namespace {
 
-constexpr int kVT = 256;  // threads per block
-constexpr int kVE = 8;    // elements of a row a thread takes at a time
-constexpr int kVTile = kVT * kVE;
+constexpr int kVW = 8;                    // waves per block, a chunk each
+constexpr int kVT = 64 * kVW;             // threads
+constexpr int kVChunk = 2048;             // entries: 32 a lane of a wave, 4 a thread of a block
+constexpr int kVQuads = kVChunk / 4 / 64;
+constexpr int kVRow = kVerifyMaxVocab / kVChunk / 64;  // chunks of a row that a lane holds
+static_assert(kVChunk == 4 * kVT, "a block takes a chunk in one step");
 
-// What the steps pass on: per row of target logits, then of draft logits, and
-// chunk of the vocabulary the maximum and the sum of exp((l - max) / T), or the
-// greedy key; per sequence the decision and the chunks' sums of max(p - q, 0).
+typedef float vf4 __attribute__((ext_vector_type(4), aligned(4)));  // rows start at any 4-byte address
+
+// What the steps pass on.  Cells: per sequence and row (its target rows, then
+// its draft rows) and chunk.
 struct Decision {
-  double m, s, mq, sq;  // of the row the token is drawn from: maximum and sum, the draft's
-  int row;              // target row (of all), or -1: nothing is left to draw
-  int draft;            // draft row, or -1
+  double s, sq;  // 1 / sum of the row the token is drawn from, of the draft's (0: it has no entry)
+  float m, mq;   // their maxima
+  int row;       // target row (of all)
+  int draft;     // draft row, or -1: the token is known already
 };
 struct VerifyWork {
-  double* sum;
+  unsigned long long* cell;  // sum of exp((l - max) / T), greedy: the best entry's key
   float* max;
-  unsigned long long* key;
-  double* rest;
+  double* rest;  // per sequence and chunk: the sum of max(p - q, 0)
   Decision* dec;
 };
 __host__ __device__ inline VerifyWork verify_work(const VerifyArgs& a) {
-  const size_t rows = (size_t)a.seqs * (2 * a.tokens - 1), cells = rows * a.chunks;
+  const size_t cells = (size_t)a.seqs * a.rows * a.chunks;
   VerifyWork w;
-  w.sum = static_cast<double*>(a.work);
-  w.key = reinterpret_cast<unsigned long long*>(w.sum);  // greedy has no sums
-  w.rest = w.sum + cells;
+  w.cell = static_cast<unsigned long long*>(a.work);
+  w.rest = reinterpret_cast<double*>(w.cell + cells);
   w.dec = reinterpret_cast<Decision*>(w.rest + (size_t)a.seqs * a.chunks);
   w.max = reinterpret_cast<float*>(w.dec + a.seqs);
   return w;
 }
 
-// Entries at or below LOWEST_FLOAT (-inf and NaN included) never take part.
-__device__ __forceinline__ double weight(float l, double m, double inv_temp) {
-  if (!(l > kLowest)) return 0.0;
-  return l == m ? 1.0 : exp(((double)l - m) * inv_temp);
+// Values that another block of the same launch reads: past the XCD's L2.
+template <typename T>
+__device__ __forceinline__ void publish(T* p, T v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <typename T>
+__device__ __forceinline__ T published(const T* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-__device__ __forceinline__ double wave_sum_f64(double v) {
+// exp((l - m) / T) = 2^((l - m) c), c = log2(e) / T, for a row's maximum m.
+// Entries at or below LOWEST_FLOAT (-inf and NaN included) never take part.
+// 2^t, t <= 0: t's nearest whole number through the sum with 1.5 * 2^52, and the
+// series of 2^f, |f| <= 1/2, up to f^9: short of it by (ln 2 / 2)^10 / 10! = 7e-12
+// (a border between tokens moves by 7e-12 of what lies below it).  The series'
+// coefficients stay in scalar registers (as literals each took two moves a term).
+// No entry is below `floor`, 2^-1100 of the maximum, which is 0: one 32-bit maximum
+// for masked entries, NaN and the exponent's range.
+constexpr double kLn2 = 0.693147180559945309417232121458;
+constexpr double coef(int n) { return n == 0 ? 1.0 : coef(n - 1) * kLn2 / n; }
+struct Weights {
+  double c, m, co[10];
+  float mf, floor;
+  bool plain;  // else the floor is none: m is infinite, the temperature past 1e35 or so low that m - floor is lost
+  __device__ __forceinline__ Weights(float max, double scale) : c(scale), m(max), mf(max) {
+    constexpr double k[10] = {coef(0), coef(1), coef(2), coef(3), coef(4), coef(5), coef(6), coef(7), coef(8), coef(9)};
 #pragma unroll
-  for (int o = 1; o < 64; o *= 2) v += __shfl_xor(v, o);
+    for (int i = 0; i < 10; i++) {
+      co[i] = k[i];
+      asm("" : "+s"(co[i]));
+    }
+    const double deep = 1100.0 / scale;
+    floor = (float)(m - deep);
+    plain = floor > kLowest && 1024.0 * deep >= fabs(m);
+  }
+  __device__ __forceinline__ double power(double t) const {
+    const double big = 6755399441055744.0;
+    const double k = t + big, f = t - (k - big);
+    double p = co[9];
+#pragma unroll
+    for (int n = 8; n >= 0; n--) p = fma(p, f, co[n]);
+    return ldexp(p, __double2loint(k));
+  }
+  __device__ __forceinline__ double series(float l) const { return power(((double)fmaxf(l, floor) - m) * c); }
+  __device__ __forceinline__ double of(float l) const {  // any entry and maximum
+    const double p = power(fmax(((double)l - m) * c, -1100.0));
+    return !(l > kLowest) ? 0.0 : l == mf ? 1.0 : p;
+  }
+};
+
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ double dpp_f64(double v) {  // lanes without a source: 0
+  return __hiloint2double(__builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, ROWS, 0xF, false),
+                          __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, ROWS, 0xF, false));
+}
+__device__ __forceinline__ double readlane_f64(double v, int l) {
+  return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), l), __builtin_amdgcn_readlane(__double2loint(v), l));
+}
+__device__ __forceinline__ double wave_sum_f64(double v) {
+  v += dpp_f64<kDppXor1>(v);
+  v += dpp_f64<kDppXor2>(v);
+  v += dpp_f64<kDppHalfMirror>(v);
+  v += dpp_f64<kDppMirror>(v);
+  return (readlane_f64(v, 0) + readlane_f64(v, 16)) + (readlane_f64(v, 32) + readlane_f64(v, 48));
+}
+__device__ __forceinline__ double wave_scan_f64(double v) {  // inclusive
+  v += dpp_f64<0x111>(v);       // row_shr:1, within 16 lanes
+  v += dpp_f64<0x112>(v);
+  v += dpp_f64<0x114>(v);
+  v += dpp_f64<0x118>(v);
+  v += dpp_f64<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
+  v += dpp_f64<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
   return v;
 }
 __device__ __forceinline__ unsigned long long wave_max_key(unsigned long long k) {
@@ -69,324 +141,543 @@ __device__ __forceinline__ unsigned long long wave_max_key(unsigned long long k)
   }
   return k;
 }
-__device__ double block_sum_f64(double v, double* scratch) {  // scratch: a double per wave
-  v = wave_sum_f64(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
-  __syncthreads();
-  double r = 0.0;
-  for (int i = 0; i < kVT / 64; i++) r += scratch[i];
-  return r;
-}
 
 __device__ __forceinline__ int row_count(const VerifyArgs& a, int s) {
   return a.counts ? min(a.counts[s], a.tokens) : a.tokens;
 }
 
-// A block per chunk of a row.
-template <bool GREEDY>
-__global__ __launch_bounds__(kVT) void verify_stats_kernel(VerifyArgs a) {
-  __shared__ double red[kVT / 64];
-  __shared__ float redm[kVT / 64];
-  __shared__ unsigned long long redk[kVT / 64];
-  const int row = blockIdx.x / a.chunks, c = blockIdx.x % a.chunks, targets = a.seqs * a.tokens;
-  const bool target = row < targets;
-  const int s = target ? row / a.tokens : (row - targets) / (a.tokens - 1);
-  const int j = target ? row % a.tokens : (row - targets) % (a.tokens - 1);
-  if (j >= row_count(a, s) - (target ? 0 : 1)) return;
-  const float* x = target ? a.logits + (size_t)row * a.vocab : a.draft_logits + (size_t)(row - targets) * a.vocab;
-  const int i0 = c * a.chunk, i1 = min(i0 + a.chunk, a.vocab), tid = threadIdx.x;
-  const VerifyWork w = verify_work(a);
-  const size_t cell = (size_t)row * a.chunks + c;
-  if (GREEDY) {
-    unsigned long long best = 0;
-    for (int i = i0 + tid; i < i1; i += kVT)
-      if (x[i] > kLowest) {
-        const unsigned long long k = greedy_key(x[i], i);
-        best = k > best ? k : best;
-      }
-    best = wave_max_key(best);
-    if ((tid & 63) == 0) redk[tid >> 6] = best;
-    __syncthreads();
-    if (tid == 0) {
-      for (int i = 1; i < kVT / 64; i++) best = redk[i] > best ? redk[i] : best;
-      w.key[cell] = best;
-    }
-    return;
-  }
-  float m = -INFINITY;
-  for (int i = i0 + tid; i < i1; i += kVT)
-    if (x[i] > kLowest) m = fmaxf(m, x[i]);
-  m = wave_max(m);
-  if ((tid & 63) == 0) redm[tid >> 6] = m;
-  __syncthreads();
-  for (int i = 0; i < kVT / 64; i++) m = fmaxf(m, redm[i]);
-  double sum = 0.0;
-  for (int i = i0 + tid; i < i1; i += kVT) sum += weight(x[i], (double)m, a.inv_temp);
-  sum = block_sum_f64(sum, red);
-  if (tid == 0) {
-    w.max[cell] = m;
-    w.sum[cell] = sum;
-  }
-}
-
-// A chunk's sum relative to the row's maximum m (a chunk without entries: 0).
-__device__ __forceinline__ double chunk_sum(const VerifyArgs& a, const VerifyWork& w, size_t cell, double m) {
-  const double s = w.sum[cell];
-  const float cm = w.max[cell];
-  return s > 0.0 ? s * (cm == m ? 1.0 : exp(((double)cm - m) * a.inv_temp)) : 0.0;
-}
-
-// Maximum and sum of a row, in every lane of the wave.
-__device__ void row_stats(const VerifyArgs& a, const VerifyWork& w, size_t row, double* m, double* s) {
+// Entries 4 lane + 256 k + e of a wave's chunk at i0; past the end -inf.
+__device__ __forceinline__ void load_chunk(const float* x, int i0, int n, vf4* v) {
   const int lane = threadIdx.x & 63;
-  float mx = -INFINITY;
-  for (int c = lane; c < a.chunks; c += 64) mx = fmaxf(mx, w.max[row * a.chunks + c]);
+  if (i0 + kVChunk <= n) {
+#pragma unroll
+    for (int k = 0; k < kVQuads; k++) v[k] = *(const TLM_GLOBAL vf4*)(x + i0 + 256 * k + 4 * lane);
+  } else {
+#pragma unroll
+    for (int k = 0; k < kVQuads; k++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const int i = i0 + 256 * k + 4 * lane + e;
+        v[k][e] = i < n ? x[i] : -INFINITY;
+      }
+  }
+}
+
+struct VerifyShared {
+  double red[kVW], s[kVerifyMaxTokens], sq[kVerifyMaxTokens], wx[kVerifyMaxTokens];
+  float m[kVerifyMaxTokens], mq[kVerifyMaxTokens];
+  int ok[kVerifyMaxTokens], top[kVerifyMaxTokens], x[kVerifyMaxTokens], hit[kVW], last[kVW];
+  unsigned long long done;
+  unsigned before;
+  int chunk, again;  // find_chunk's
+  double base, border;
+};
+
+// A row's chunks in a wave's registers: chunk lane + 64 k.
+struct RowSums {
+  float max[kVRow];
+  double sum[kVRow];  // row_load: relative to max; row_scale: to the row's maximum
+};
+__device__ __forceinline__ void row_load(const VerifyArgs& a, const VerifyWork& w, size_t row, RowSums& r) {
+#pragma unroll
+  for (int k = 0; k < kVRow; k++) {
+    const int c = (threadIdx.x & 63) + 64 * k;
+    r.sum[k] = c < a.chunks ? __longlong_as_double((long long)published(w.cell + row * a.chunks + c)) : 0.0;
+    r.max[k] = c < a.chunks ? published(w.max + row * a.chunks + c) : -INFINITY;
+  }
+}
+// The row's maximum and sum, in every lane (a chunk or a row without entries: 0).
+__device__ __forceinline__ void row_scale(const VerifyArgs& a, RowSums& r, float* m, double* s) {
+  float mx = r.max[0];
+#pragma unroll
+  for (int k = 1; k < kVRow; k++) mx = fmaxf(mx, r.max[k]);
   mx = wave_max(mx);
+  const Weights w(mx, a.scale);
   double sum = 0.0;
-  for (int c = lane; c < a.chunks; c += 64) sum += chunk_sum(a, w, row * a.chunks + c, (double)mx);
-  *m = (double)mx;
+#pragma unroll
+  for (int k = 0; k < kVRow; k++) {
+    if (64 * k < a.chunks) r.sum[k] = r.sum[k] > 0.0 ? r.sum[k] * w.of(r.max[k]) : 0.0;
+    sum += r.sum[k];
+  }
+  *m = mx;
   *s = wave_sum_f64(sum);
 }
 
-// The block finds the lowest index whose running sum passes u times the whole:
-// `sums(c)` the chunks' sums, `at(i)` an entry's weight.  Rounding may leave the
-// last border at u: then it is the last index with a weight.  -1: all are zero.
-template <typename Sums, typename At>
-__device__ int draw(const VerifyArgs& a, float u, Sums sums, At at, double* red, int* pick) {
-  const int tid = threadIdx.x, lane = tid & 63;
-  // every wave: the whole, then the chunk
-  double total = 0.0;
-  for (int c = lane; c < a.chunks; c += 64) total += sums(c);
-  total = wave_sum_f64(total);
-  if (!(total > 0.0)) return -1;
+// One wave: the chunk in which the running sum of the chunks passes u times the
+// whole, the sum before it and that border, into sh.  Rounding may leave the last
+// border at u: then the last chunk with a weight.  -1: all are zero.
+__device__ void find_chunk(const double* v, float u, VerifyShared& sh) {
+  const int lane = threadIdx.x & 63;
+  double incl[kVRow], total = 0.0;
+#pragma unroll
+  for (int k = 0; k < kVRow; k++) {
+    incl[k] = total + wave_scan_f64(v[k]);
+    total = readlane_f64(incl[k], 63);
+  }
   const double border = (double)u * total;
-  double before = 0.0, found_before = 0.0;
   int chunk = -1, last = -1;
-  double last_before = 0.0;
-  for (int c0 = 0; c0 < a.chunks && chunk < 0; c0 += 64) {
-    const double v = c0 + lane < a.chunks ? sums(c0 + lane) : 0.0;
-    double run = v;
+  double base = 0.0, last_base = 0.0;
 #pragma unroll
-    for (int o = 1; o < 64; o *= 2) {
-      const double y = __shfl_up(run, o);
-      if (lane >= o) run += y;
+  for (int k = 0; k < kVRow; k++) {
+    const unsigned long long some = __ballot(v[k] > 0.0), over = __ballot(v[k] > 0.0 && incl[k] > border);
+    const double before = incl[k] - v[k];
+    if (chunk < 0 && over) {
+      const int l = __builtin_ctzll(over);
+      chunk = 64 * k + l;
+      base = readlane_f64(before, l);
     }
-    const unsigned long long over = __ballot(v > 0.0 && before + run > border), some = __ballot(v > 0.0);
-    const double excl = before + (run - v);
-    if (over) {
-      const int l = __ffsll(over) - 1;
-      chunk = c0 + l;
-      found_before = __shfl(excl, l);
-    } else if (some) {
-      const int l = 63 - __clzll(some);
-      last = c0 + l;
-      last_before = __shfl(excl, l);
+    if (some) {
+      const int l = 63 - __builtin_clzll(some);
+      last = 64 * k + l;
+      last_base = readlane_f64(before, l);
     }
-    before += __shfl(run, 63);
   }
-  if (chunk < 0) {
-    chunk = last;
-    found_before = last_before;
+  if (lane == 0) {
+    sh.chunk = chunk < 0 ? last : chunk;
+    sh.base = chunk < 0 ? last_base : base;
+    sh.border = border;
   }
-  // the block: kVE entries a thread, in order
-  const int i1 = min((chunk + 1) * a.chunk, a.vocab);
-  double run = found_before;
-  int best = -1;
-  for (int i0 = chunk * a.chunk; i0 < i1; i0 += kVTile) {
-    double v[kVE], mine = 0.0;
-    int mlast = -1;
-#pragma unroll
-    for (int e = 0; e < kVE; e++) {
-      const int i = i0 + tid * kVE + e;
-      v[e] = i < i1 ? at(i) : 0.0;
-      mine += v[e];
-      if (v[e] > 0.0) mlast = i;
-    }
-    double incl = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) {
-      const double y = __shfl_up(incl, o);
-      if (lane >= o) incl += y;
-    }
-    __syncthreads();
-    if (lane == 63) red[tid >> 6] = incl;
-    if (tid == 0) pick[0] = 0x7fffffff, pick[1] = -1;
-    __syncthreads();
-    double c = run + (incl - mine);
-    for (int k = 0; k < tid >> 6; k++) c += red[k];
-    int hit = 0x7fffffff;
-#pragma unroll
-    for (int e = kVE - 1; e >= 0; e--) {
-      double upto = c;
-      for (int f = 0; f <= e; f++) upto += v[f];
-      if (v[e] > 0.0 && upto > border) hit = i0 + tid * kVE + e;
-    }
-    if (hit != 0x7fffffff) atomicMin(&pick[0], hit);
-    if (mlast >= 0) atomicMax(&pick[1], mlast);
-    __syncthreads();
-    if (pick[0] != 0x7fffffff) return pick[0];
-    if (pick[1] >= 0) best = pick[1];
-    for (int k = 0; k < kVT / 64; k++) run += red[k];
-  }
-  return best;
 }
 
-// A block per sequence: which drafts stand, and the token after them where no
-// draft logits are to be subtracted.
+// The block: the entry of sh.chunk, at(i, v) an entry's four weights from i on.
+template <typename At>
+__device__ int find_entry(const VerifyArgs& a, At at, VerifyShared& sh) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int i0 = sh.chunk * kVChunk + 4 * tid;
+  double v[4], mine = 0.0;
+  at(i0, v);
+  int mlast = -1;
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    mine += v[e];
+    if (v[e] > 0.0) mlast = i0 + e;
+  }
+  const double incl = wave_scan_f64(mine), border = sh.border;
+  double run = sh.base;
+  const unsigned long long some = __ballot(mlast >= 0);
+  const int wlast = some ? __builtin_amdgcn_readlane(mlast, 63 - __builtin_clzll(some)) : -1;
+  if (lane == 63) sh.red[tid >> 6] = incl;
+  __syncthreads();
+  for (int k = 0; k < tid >> 6; k++) run += sh.red[k];
+  run += incl - mine;
+  int hit = -1;
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    run += v[e];
+    if (hit < 0 && v[e] > 0.0 && run > border) hit = i0 + e;
+  }
+  const unsigned long long over = __ballot(hit >= 0);
+  const int whit = over ? __builtin_amdgcn_readlane(hit, __builtin_ctzll(over)) : -1;
+  if (lane == 0) sh.hit[tid >> 6] = whit, sh.last[tid >> 6] = wlast;
+  __syncthreads();
+  int last = -1;
+  for (int k = 0; k < kVW; k++) {
+    if (sh.hit[k] >= 0) return sh.hit[k];
+    if (sh.last[k] >= 0) last = sh.last[k];
+  }
+  return last;
+}
+
+// Four entries of a row from i on; past the end -inf (of no weight).
+__device__ __forceinline__ vf4 row_quad(const float* x, int i, int n) {
+  if (i + 4 <= n) return *(const TLM_GLOBAL vf4*)(x + i);
+  vf4 v;
+#pragma unroll
+  for (int e = 0; e < 4; e++) v[e] = i + e < n ? x[i + e] : -INFINITY;
+  return v;
+}
+
+__device__ double block_sum_f64(double v, VerifyShared& sh) {
+  v = wave_sum_f64(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) sh.red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  double r = 0.0;
+#pragma unroll
+  for (int i = 0; i < kVW; i++) r += sh.red[i];
+  __syncthreads();
+  return r;
+}
+
+// Which drafts of a sequence stand, and the token after them where no draft
+// logits are to be subtracted.  The whole block.
 template <bool GREEDY>
-__global__ __launch_bounds__(kVT) void verify_decide_kernel(VerifyArgs a) {
-  __shared__ double red[kVT / 64], rm[kVerifyMaxTokens], rs[kVerifyMaxTokens], qm[kVerifyMaxTokens],
-      qs[kVerifyMaxTokens];
-  __shared__ int ok[kVerifyMaxTokens], top[kVerifyMaxTokens], pick[2];
-  const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63, T = a.tokens, targets = a.seqs * T;
+__device__ void decide(const VerifyArgs& a, int s, VerifyShared& sh) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, T = a.tokens;
   const VerifyWork w = verify_work(a);
   const int n = row_count(a, s);
-  if (n < 1) {  // idle: its results stay as they are
-    if (!GREEDY && tid == 0) w.dec[s].row = -1, w.dec[s].draft = -1;
-    return;
-  }
-  for (int j = tid >> 6; j < n; j += kVT / 64) {
-    const int row = s * T + j, x = j < n - 1 ? a.drafts[s * (T - 1) + j] : -1;
-    const bool in = x >= 0 && x < a.vocab;
+  __syncthreads();  // sh of the sequence before has been read
+  RowSums rp;
+  for (int j = wave; j < n; j += kVW) {
+    const size_t row = (size_t)s * a.rows + j;
+    const bool model = !GREEDY && a.draft_logits && j < n - 1;
+    RowSums rq;
+    unsigned long long best = 0;
     if (GREEDY) {
-      unsigned long long k = 0;
-      for (int c = lane; c < a.chunks; c += 64) {
-        const unsigned long long y = w.key[(size_t)row * a.chunks + c];
-        k = y > k ? y : k;
+#pragma unroll
+      for (int i = 0; i < kVRow; i++) {
+        const int c = lane + 64 * i;
+        const unsigned long long y = c < a.chunks ? published(w.cell + row * a.chunks + c) : 0;
+        best = y > best ? y : best;
       }
-      k = wave_max_key(k);
+    } else {
+      row_load(a, w, row, rp);
+      if (model) row_load(a, w, (size_t)s * a.rows + T + j, rq);
+    }
+    const int id = j < n - 1 ? a.drafts[s * (T - 1) + j] : -1, x = id < a.vocab ? id : -1;
+    if (lane == 0) sh.x[j] = x;
+    if (GREEDY) {
+      best = wave_max_key(best);
       if (lane == 0) {
-        top[j] = k ? greedy_key_id(k) : -1;
-        ok[j] = in && x == top[j];
+        sh.top[j] = best ? greedy_key_id(best) : -1;
+        sh.ok[j] = x >= 0 && x == sh.top[j];
       }
       continue;
     }
-    double m, sum, dm = 0.0, ds = 0.0;
-    row_stats(a, w, row, &m, &sum);
-    if (a.draft_logits && j < n - 1) row_stats(a, w, targets + s * (T - 1) + j, &dm, &ds);
+    const float lx = x >= 0 ? a.logits[((size_t)s * T + j) * a.vocab + x] : -INFINITY;
+    const float qx = x >= 0 && model ? a.draft_logits[((size_t)s * (T - 1) + j) * a.vocab + x] : -INFINITY;
+    const float u = a.uniforms[s * T + j];
+    float m, mq = 0.f;
+    double sum, sq = 0.0;
+    row_scale(a, rp, &m, &sum);
+    if (model) row_scale(a, rq, &mq, &sq);
+    const double wx = Weights(m, a.scale).of(lx), p = sum > 0.0 ? wx / sum : 0.0;
+    const double q = !model ? 1.0 : sq > 0.0 ? Weights(mq, a.scale).of(qx) / sq : 0.0;
     if (lane == 0) {
-      rm[j] = m, rs[j] = sum, qm[j] = dm, qs[j] = ds;
-      double p = 0.0, q = 1.0;
-      if (in && sum > 0.0) p = weight(a.logits[(size_t)row * a.vocab + x], m, a.inv_temp) / sum;
-      if (in && a.draft_logits)
-        q = ds > 0.0 ? weight(a.draft_logits[((size_t)s * (T - 1) + j) * a.vocab + x], dm, a.inv_temp) / ds : 0.0;
-      ok[j] = in && (double)a.uniforms[s * T + j] * q < p;
+      sh.m[j] = m, sh.s[j] = sum, sh.mq[j] = mq, sh.sq[j] = sq, sh.wx[j] = wx;
+      sh.ok[j] = x >= 0 && (double)u * q < p;
     }
   }
   __syncthreads();
-  int taken = 0;
-  while (taken < n - 1 && ok[taken]) taken++;
+  const unsigned long long no = __ballot(lane >= n - 1 || !sh.ok[min(lane, n - 1)]);
+  const int taken = __builtin_ctzll(no);  // n - 1 <= 63
   const bool refused = taken < n - 1;
-  for (int j = tid; j < T; j += kVT)
-    if (j != taken) a.ids[(size_t)s * T + j] = j < taken ? a.drafts[s * (T - 1) + j] : -1;
+  if (tid < T && tid != taken) a.ids[(size_t)s * T + tid] = tid < taken ? sh.x[tid] : -1;
   if (tid == 0) a.accepted[s] = taken;
   int token;
   if (GREEDY) {
-    token = top[taken];
+    token = sh.top[taken];
   } else {
-    const int row = s * T + taken;
-    const double m = rm[taken];
-    const bool split = refused && a.draft_logits && rs[taken] > 0.0;
-    if (tid == 0) w.dec[s] = Decision{m, rs[taken], qm[taken], qs[taken], row, split ? s * (T - 1) + taken : -1};
-    if (split) return;
-    const float* l = a.logits + (size_t)row * a.vocab;
+    const bool rest = refused && a.draft_logits && sh.s[taken] > 0.0;
+    if (a.draft_logits && tid == 0)
+      w.dec[s] = Decision{1.0 / sh.s[taken], sh.sq[taken] > 0.0 ? 1.0 / sh.sq[taken] : 0.0, sh.m[taken], sh.mq[taken],
+                          s * T + taken, rest ? s * (T - 1) + taken : -1};
+    if (rest) return;
+    const float* l = a.logits + ((size_t)s * T + taken) * a.vocab;
+    const Weights of(sh.m[taken], a.scale);
     const float u = a.uniforms[s * T + T - 1];
-    // a certain draft's residual is p without it
-    const int x = refused && !a.draft_logits ? a.drafts[s * (T - 1) + taken] : -1;
-    const int cx = x >= 0 && x < a.vocab ? x / a.chunk : -1;
-    double without = 0.0;
-    if (cx >= 0) {  // its chunk again, as a difference would lose what is left beside a likely draft
-      for (int i = cx * a.chunk + tid; i < min((cx + 1) * a.chunk, a.vocab); i += kVT)
-        without += i == x ? 0.0 : weight(l[i], m, a.inv_temp);
-      without = block_sum_f64(without, red);
+    int x = refused && !a.draft_logits ? sh.x[taken] : -1;  // a certain draft's residual is p without it
+    auto at = [&](int i, double* v) {
+      const vf4 y = row_quad(l, i, a.vocab);
+#pragma unroll
+      for (int e = 0; e < 4; e++) v[e] = i + e == x ? 0.0 : of.of(y[e]);
+    };
+    const bool mine = wave == taken % kVW;  // this wave has the row's sums, if no row came after it
+    double v[kVRow];
+    if (mine) {
+      if (n > kVW) {
+        float dm;
+        double ds;
+        row_load(a, w, (size_t)s * a.rows + taken, rp);
+        row_scale(a, rp, &dm, &ds);
+      }
+      bool much = false;
+#pragma unroll
+      for (int k = 0; k < kVRow; k++) {
+        const bool here = x >= 0 && lane + 64 * k == x / kVChunk;
+        v[k] = here ? rp.sum[k] - sh.wx[taken] : rp.sum[k];
+        much |= here && !(sh.wx[taken] <= 0.5 * rp.sum[k]);
+      }
+      const bool again = __ballot(much) != 0;
+      if (!again) find_chunk(v, u, sh);
+      if (lane == 0) sh.again = again;
     }
-    token = draw(a, u, [&](int c) { return c == cx ? without : chunk_sum(a, w, (size_t)row * a.chunks + c, m); },
-                 [&](int i) { return i == x ? 0.0 : weight(l[i], m, a.inv_temp); }, red, pick);
-    if (token < 0 && x >= 0) {  // nothing beside the draft: p itself
+    __syncthreads();
+    if (sh.again) {  // a difference would lose what is left beside a likely draft: its chunk's sum without it
+      double y[4];
+      at(x / kVChunk * kVChunk + 4 * tid, y);
+      const double without = block_sum_f64((y[0] + y[1]) + (y[2] + y[3]), sh);
+      if (mine) {
+#pragma unroll
+        for (int k = 0; k < kVRow; k++)
+          if (lane + 64 * k == x / kVChunk) v[k] = without;
+        find_chunk(v, u, sh);
+      }
       __syncthreads();
-      token = draw(a, u, [&](int c) { return chunk_sum(a, w, (size_t)row * a.chunks + c, m); },
-                   [&](int i) { return weight(l[i], m, a.inv_temp); }, red, pick);
     }
+    if (sh.chunk < 0 && x >= 0) {  // nothing beside the draft: p itself
+      x = -1;
+      __syncthreads();
+      if (mine) find_chunk(rp.sum, u, sh);
+      __syncthreads();
+    }
+    token = sh.chunk < 0 ? -1 : find_entry(a, at, sh);
   }
   if (tid == 0) a.ids[(size_t)s * T + taken] = token;
 }
 
-__device__ __forceinline__ double residual(const VerifyArgs& a, const Decision& d, const float* l, const float* q, int i) {
-  const double p = weight(l[i], d.m, a.inv_temp) / d.s;
-  const double y = d.sq > 0.0 ? weight(q[i], d.mq, a.inv_temp) / d.sq : 0.0;
-  return p > y ? p - y : 0.0;
+// Where the rows that are there lie, a wave's own view: 64 sequences at a time, a
+// lane each, their rows (targets, then drafts) numbered through.
+struct RowWalk {
+  int s0, before, rows, incl, total;  // rows before the 64, this lane's, theirs up to this lane's, all theirs
+  __device__ __forceinline__ void group(const VerifyArgs& a, int s) {
+    const int l = s + (threadIdx.x & 63), n = l < a.seqs ? row_count(a, l) : 0;
+    s0 = s;
+    rows = n < 1 ? 0 : a.rows > a.tokens ? 2 * n - 1 : n;
+    incl = rows;
+    incl += __builtin_amdgcn_update_dpp(0, incl, 0x111, 0xF, 0xF, false);  // as wave_scan_f64
+    incl += __builtin_amdgcn_update_dpp(0, incl, 0x112, 0xF, 0xF, false);
+    incl += __builtin_amdgcn_update_dpp(0, incl, 0x114, 0xF, 0xF, false);
+    incl += __builtin_amdgcn_update_dpp(0, incl, 0x118, 0xF, 0xF, false);
+    incl += __builtin_amdgcn_update_dpp(0, incl, 0x142, 0xA, 0xF, false);
+    incl += __builtin_amdgcn_update_dpp(0, incl, 0x143, 0xC, 0xF, false);
+    total = __builtin_amdgcn_readlane(incl, 63);
+  }
+  // All rows; the walk then stands at the first 64 sequences.
+  __device__ __forceinline__ int start(const VerifyArgs& a) {
+    int all = 0;
+    for (int s = 0; s < a.seqs; s += 64) {
+      group(a, s);
+      all += total;
+    }
+    if (a.seqs > 64) group(a, 0);
+    before = 0;
+    return all;
+  }
+  // The lane of the sequence that holds a row, no earlier than the last one asked for.
+  __device__ __forceinline__ int seek(const VerifyArgs& a, int row) {
+    while (row >= before + total) {
+      const int t = total;
+      group(a, s0 + 64);
+      before += t;
+    }
+    return __builtin_popcountll(__ballot(before + incl <= row));
+  }
+};
+
+// All chunks of all rows that are there, shared out evenly: a block takes a run of
+// them, its waves in turn.  Having published its results it counts them for their
+// sequences; the block that completes a sequence decides it (every value of the
+// sequence has then been performed) and clears the count.
+template <bool GREEDY>
+__global__ __launch_bounds__(kVT, 4) void verify_kernel(VerifyArgs a) {
+  __shared__ VerifyShared sh;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), T = a.tokens;
+  const VerifyWork w = verify_work(a);
+  RowWalk walk;
+  const int cells = walk.start(a) * a.chunks, run = (cells + gridDim.x - 1) / gridDim.x;
+  const int c0 = min((int)blockIdx.x * run, cells), c1 = min(c0 + run, cells);
+  if (c0 >= c1) return;
+  struct Place {
+    int s, r, c;  // sequence, row (drafts after the targets), chunk
+  };
+  auto place = [&](int cell) {
+    const int row = cell / a.chunks, l = walk.seek(a, row), rows = __builtin_amdgcn_readlane(walk.rows, l);
+    const int k = row - walk.before - (__builtin_amdgcn_readlane(walk.incl, l) - rows);
+    const int n = a.rows > T ? (rows + 1) / 2 : rows;
+    return Place{walk.s0 + l, k < n ? k : T + k - n, cell - row * a.chunks};
+  };
+  auto fetch = [&](int cell, vf4* v) {  // past the run's end: its last chunk
+    const Place p = place(min(cell, c1 - 1));
+    load_chunk(p.r < T ? a.logits + ((size_t)p.s * T + p.r) * a.vocab
+                       : a.draft_logits + ((size_t)p.s * (T - 1) + p.r - T) * a.vocab,
+               p.c * kVChunk, a.vocab, v);
+    return p;
+  };
+  auto reduce = [&](const Place& p, vf4* v) {
+    const size_t at = ((size_t)p.s * a.rows + p.r) * a.chunks + p.c;
+    if (GREEDY) {
+      const int i0 = p.c * kVChunk + 4 * lane;
+      float best = kLowest;
+      int id = 0;
+#pragma unroll
+      for (int k = 0; k < kVQuads; k++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          if (v[k][e] > best) best = v[k][e], id = i0 + 256 * k + e;  // ids ascend: the lower one stays
+      const unsigned long long key = wave_max_key(best > kLowest ? greedy_key(best, id) : 0ull);
+      if (lane == 0) publish(w.cell + at, key);
+      return;
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kVQuads; k++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) mx = fmaxf(mx, v[k][e]);
+    mx = wave_max(mx);
+    if (!(mx > kLowest)) mx = -INFINITY;  // no entry
+    const Weights of(mx, a.scale);
+    double sum = 0.0;
+    if (of.plain) {
+#pragma unroll
+      for (int k = 0; k < kVQuads; k++) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) sum += of.series(v[k][e]);
+        __builtin_amdgcn_sched_barrier(0);  // four series at once: 32 would take twice the registers
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < kVQuads; k++) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) sum += of.of(v[k][e]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    sum = wave_sum_f64(sum);
+    if (lane == 0) {
+      publish(w.cell + at, (unsigned long long)__double_as_longlong(sum));
+      publish(w.max + at, mx);
+    }
+  };
+  // one chunk in work, the next in flight
+  if (c0 + wave < c1) {
+    vf4 x[kVQuads], y[kVQuads];
+    Place px = fetch(c0 + wave, x), py;
+    for (int c = c0 + wave;; c += 2 * kVW) {
+      py = fetch(c + kVW, y);
+      reduce(px, x);
+      if (c + kVW >= c1) break;
+      px = fetch(c + 2 * kVW, x);
+      reduce(py, y);
+      if (c + 2 * kVW >= c1) break;
+    }
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's results are performed
+  __syncthreads();                                  // and every wave's
+  walk.group(a, 0);
+  walk.before = 0;
+  walk.seek(a, c0 / a.chunks);
+  while (true) {  // 64 sequences at a time
+    if (wave == 0) {
+      const int s = walk.s0 + lane, end = (walk.before + walk.incl) * a.chunks, all = walk.rows * a.chunks;
+      const int mine = min(c1, end) - max(c0, end - all);
+      bool done = false;
+      if (mine > 0) {
+        const unsigned count =
+            __hip_atomic_fetch_add(a.arrived + s, (unsigned)mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        done = (int)count + mine == all;
+        if (done) __hip_atomic_store(a.arrived + s, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+      const unsigned long long which = __ballot(done);
+      if (lane == 0) sh.done = which;
+    }
+    __syncthreads();
+    for (unsigned long long left = sh.done; left; left &= left - 1)
+      decide<GREEDY>(a, walk.s0 + __builtin_ctzll(left), sh);
+    const int rows = walk.before + walk.total;
+    if (rows * a.chunks >= c1) break;
+    walk.seek(a, rows);
+    __syncthreads();  // sh.done has been read
+  }
 }
 
-// A block per chunk and sequence: the chunk's sum of max(p - q, 0).
-__global__ __launch_bounds__(kVT) void verify_rest_kernel(VerifyArgs a) {
-  __shared__ double red[kVT / 64];
-  const int s = blockIdx.x / a.chunks, c = blockIdx.x % a.chunks;
+// A wave per chunk of every sequence whose token is still to be drawn: the
+// chunk's sum of max(p - q, 0); the last of a sequence's `per` blocks draws.
+__global__ __launch_bounds__(kVT) void verify_rest_kernel(VerifyArgs a, int per) {
+  __shared__ VerifyShared sh;
   const VerifyWork w = verify_work(a);
-  const Decision d = w.dec[s];
-  if (d.draft < 0) return;
-  const float* l = a.logits + (size_t)d.row * a.vocab;
-  const float* q = a.draft_logits + (size_t)d.draft * a.vocab;
-  double sum = 0.0;
-  for (int i = c * a.chunk + threadIdx.x; i < min((c + 1) * a.chunk, a.vocab); i += kVT) sum += residual(a, d, l, q, i);
-  sum = block_sum_f64(sum, red);
-  if (threadIdx.x == 0) w.rest[(size_t)s * a.chunks + c] = sum;
-}
-
-// A block per sequence: the token from those sums.
-__global__ __launch_bounds__(kVT) void verify_draw_kernel(VerifyArgs a) {
-  __shared__ double red[kVT / 64];
-  __shared__ int pick[2];
-  const int s = blockIdx.x;
-  const VerifyWork w = verify_work(a);
+  const int s = blockIdx.x / per, c = blockIdx.x % per * kVW + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (row_count(a, s) < 1) return;
   const Decision d = w.dec[s];
   if (d.draft < 0) return;
   const float* l = a.logits + (size_t)d.row * a.vocab;
   const float* q = a.draft_logits + (size_t)d.draft * a.vocab;
   const float u = a.uniforms[s * a.tokens + a.tokens - 1];
-  int token = draw(a, u, [&](int c) { return w.rest[(size_t)s * a.chunks + c]; },
-                   [&](int i) { return residual(a, d, l, q, i); }, red, pick);
-  if (token < 0) {  // p and q are the same: p itself
-    __syncthreads();
-    token = draw(a, u, [&](int c) { return chunk_sum(a, w, (size_t)d.row * a.chunks + c, d.m); },
-                 [&](int i) { return weight(l[i], d.m, a.inv_temp); }, red, pick);
+  const Weights lw(d.m, a.scale), qw(d.mq, a.scale);
+  auto residual = [&](float x, float y) { return fmax(lw.of(x) * d.s - (d.sq > 0.0 ? qw.of(y) * d.sq : 0.0), 0.0); };
+  if (c < a.chunks) {
+    vf4 x[kVQuads], y[kVQuads];
+    load_chunk(l, c * kVChunk, a.vocab, x);
+    load_chunk(q, c * kVChunk, a.vocab, y);
+    double sum = 0.0;
+    if (lw.plain && qw.plain && d.sq > 0.0) {
+#pragma unroll
+      for (int k = 0; k < kVQuads; k++) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) sum += fmax(lw.series(x[k][e]) * d.s - qw.series(y[k][e]) * d.sq, 0.0);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < kVQuads; k++) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) sum += residual(x[k][e], y[k][e]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    sum = wave_sum_f64(sum);
+    if (lane == 0) publish(w.rest + (size_t)s * a.chunks + c, sum);
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0)
+    sh.before = __hip_atomic_fetch_add(a.arrived + s, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  if (sh.before != (unsigned)per - 1) return;
+  if (threadIdx.x == 0) __hip_atomic_store(a.arrived + s, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (threadIdx.x < 64) {
+    double v[kVRow];
+#pragma unroll
+    for (int i = 0; i < kVRow; i++)
+      v[i] = lane + 64 * i < a.chunks ? published(w.rest + (size_t)s * a.chunks + lane + 64 * i) : 0.0;
+    find_chunk(v, u, sh);
+  }
+  __syncthreads();
+  const bool same = sh.chunk < 0;  // p and q are: p itself
+  if (same) {
+    __syncthreads();
+    if (threadIdx.x < 64) {
+      RowSums r;
+      float dm;
+      double ds;
+      row_load(a, w, (size_t)s * a.rows + d.row % a.tokens, r);
+      row_scale(a, r, &dm, &ds);
+      find_chunk(r.sum, u, sh);
+    }
+    __syncthreads();
+  }
+  const int token = find_entry(a, [&](int i, double* v) {
+    const vf4 y = row_quad(l, i, a.vocab), z = row_quad(q, i, a.vocab);
+#pragma unroll
+    for (int f = 0; f < 4; f++) v[f] = same ? lw.of(y[f]) : residual(y[f], z[f]);
+  }, sh);
   if (threadIdx.x == 0) a.ids[d.row] = token;
 }
 
 }  // namespace
 
-static size_t work_bytes(const VerifyArgs& a) {
-  const size_t cells = (size_t)a.seqs * (2 * a.tokens - 1) * a.chunks;
-  return cells * (sizeof(double) + sizeof(float)) + (size_t)a.seqs * (a.chunks * sizeof(double) + sizeof(Decision));
+size_t verify_plan(VerifyArgs& a) {
+  a.rows = a.draft_logits && a.scale > 0.0 ? 2 * a.tokens - 1 : a.tokens;
+  a.chunks = (a.vocab + kVChunk - 1) / kVChunk;
+  const size_t seqs = std::min(a.seqs, kVerifyCounters), cells = seqs * a.rows * a.chunks;
+  return cells * (sizeof(unsigned long long) + sizeof(float)) + seqs * (a.chunks * sizeof(double) + sizeof(Decision));
 }
 
-void verify_plan(VerifyArgs& a, int cus, size_t most) {
-  const int64_t rows = (int64_t)a.seqs * a.tokens;
-  int64_t chunk = kVTile;
-  while (chunk < 4 * kVTile && rows * (a.vocab / chunk) > 8 * cus) chunk *= 2;
-  for (;; chunk *= 2) {
-    a.chunk = (int)std::min<int64_t>(chunk, INT_MAX);
-    a.chunks = (int)((a.vocab + (int64_t)a.chunk - 1) / a.chunk);
-    if (work_bytes(a) <= most || a.chunks == 1) return;
+// kVerifyCounters sequences at a time.  Two blocks a CU are resident: several
+// chunks a wave from there on, so that the next one is in flight during a chunk's
+// sum and a block waits for its counts only once.
+void launch_verify(const VerifyArgs& all, int cus, hipStream_t st) {
+  for (int s0 = 0; s0 < all.seqs; s0 += kVerifyCounters) {
+    VerifyArgs a = all;
+    const size_t row = (size_t)s0 * a.tokens, draft = (size_t)s0 * (a.tokens - 1);
+    a.seqs = std::min(all.seqs - s0, kVerifyCounters);
+    a.logits += row * a.vocab;
+    if (a.draft_logits) a.draft_logits += draft * a.vocab;
+    if (a.drafts) a.drafts += draft;
+    if (a.counts) a.counts += s0;
+    if (a.uniforms) a.uniforms += row;
+    a.accepted += s0;
+    a.ids += row;
+    const int64_t cells = (int64_t)a.seqs * a.rows * a.chunks;
+    const dim3 grid((unsigned)std::min<int64_t>(2 * cus, (cells + kVW - 1) / kVW)), block(kVT);
+    if (a.scale == 0.0) {
+      hipLaunchKernelGGL(verify_kernel<true>, grid, block, 0, st, a);
+      continue;
+    }
+    hipLaunchKernelGGL(verify_kernel<false>, grid, block, 0, st, a);
+    const int per = (a.chunks + kVW - 1) / kVW;
+    if (a.rows > a.tokens) hipLaunchKernelGGL(verify_rest_kernel, dim3((unsigned)(a.seqs * per)), block, 0, st, a, per);
   }
-}
-
-void launch_verify(const VerifyArgs& a, hipStream_t st) {
-  const bool greedy = a.inv_temp == 0.0;
-  const bool model = !greedy && a.draft_logits && a.tokens > 1;
-  const int rows = a.seqs * (model ? 2 * a.tokens - 1 : a.tokens);
-  const dim3 grid((unsigned)(rows * a.chunks)), seqs((unsigned)a.seqs), block(kVT);
-  if (greedy) {
-    hipLaunchKernelGGL(verify_stats_kernel<true>, grid, block, 0, st, a);
-    hipLaunchKernelGGL(verify_decide_kernel<true>, seqs, block, 0, st, a);
-    return;
-  }
-  hipLaunchKernelGGL(verify_stats_kernel<false>, grid, block, 0, st, a);
-  hipLaunchKernelGGL(verify_decide_kernel<false>, seqs, block, 0, st, a);
-  if (!model) return;
-  hipLaunchKernelGGL(verify_rest_kernel, dim3((unsigned)(a.seqs * a.chunks)), block, 0, st, a);
-  hipLaunchKernelGGL(verify_draw_kernel, seqs, block, 0, st, a);
 }
 
 }  // namespace tlm
