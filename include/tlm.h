@@ -189,7 +189,7 @@ typedef struct tlm_paged_desc {
  * given back, their entries anything).  Sequences may share pages that they
  * read; a position that two of them append to gets either's row.
  * All pointers are device memory; the struct itself is the host's and is read
- * during the call. */
+ * during the call.  seqs * tokens * heads is at most 2^22. */
 typedef struct tlm_paged_batch {
   void* k_pages;            /* pools of num_pages * kv_heads * page_tokens * head_dim kv_fmt elements, 16-byte */
   void* v_pages;            /* aligned, in the order that tlm_paged_locate tells */

@@ -1217,8 +1217,9 @@ static int paged_args(const tlm_paged* P, const tlm_paged_batch* b, PagedArgs& a
   if (b->num_pages < 1 || b->table_width < 1 || b->seqs < 1 || b->tokens < 1)
     return fail(TLM_ERR_INVALID, "TLMPaged: %d pages, tables of %d, %d sequences of %d rows", b->num_pages,
                 b->table_width, b->seqs, b->tokens);
-  if ((int64_t)b->seqs * b->tokens > (1 << 20))
-    return fail(TLM_ERR_RANGE, "TLMPaged: %d sequences of %d rows are more than 2^20 rows", b->seqs, b->tokens);
+  if ((int64_t)b->seqs * b->tokens > (1 << 22) / P->d.heads)
+    return fail(TLM_ERR_RANGE, "TLMPaged: %d sequences of %d rows of %d heads are more than 2^22", b->seqs, b->tokens,
+                P->d.heads);
   if ((reinterpret_cast<uintptr_t>(b->k_pages) | reinterpret_cast<uintptr_t>(b->v_pages)) % 16)
     return fail(TLM_ERR_INVALID, "TLMPaged: a pool is not 16-byte aligned");
   memset(&a, 0, sizeof a);
