@@ -90,6 +90,7 @@ struct tlm_ctx {
   // tlm_op_logits: the blocks' folded best and their count (zero between launches)
   unsigned long long* arg_key = nullptr;
   unsigned* arg_arrived = nullptr;
+  unsigned* paged_arrived = nullptr;  // tlm_op_paged_attention's chunks done (zero between launches)
   unsigned* verify_arrived = nullptr;  // tlm_op_verify_drafts' blocks done, per sequence (zero between launches)
   unsigned* topk_arrived = nullptr;  // tlm_op_topk's blocks done (zero between launches)
   // top-k levels: two levels of kTopkWork (score, id) pairs
@@ -537,6 +538,8 @@ int tlm_open(int device, tlm_ctx** out) {
   if (e == hipSuccess) e = hipMalloc(&c->arg_key, sizeof(unsigned long long));
   if (e == hipSuccess) e = hipMalloc(&c->arg_arrived, sizeof(unsigned));
   if (e == hipSuccess) e = hipMalloc(&c->topk_arrived, sizeof(unsigned));
+  if (e == hipSuccess) e = hipMalloc(&c->paged_arrived, kPagedCounters * sizeof(unsigned));
+  if (e == hipSuccess) e = hipMemset(c->paged_arrived, 0, kPagedCounters * sizeof(unsigned));
   if (e == hipSuccess) e = hipMalloc(&c->verify_arrived, kVerifyCounters * sizeof(unsigned));
   if (e == hipSuccess) e = hipMemset(c->verify_arrived, 0, kVerifyCounters * sizeof(unsigned));
   if (e == hipSuccess) e = hipMemset(c->topk_arrived, 0, sizeof(unsigned));
@@ -567,6 +570,7 @@ void tlm_close(tlm_ctx* ctx) {
   hipFree(ctx->arg_key);
   hipFree(ctx->arg_arrived);
   hipFree(ctx->topk_arrived);
+  hipFree(ctx->paged_arrived);
   hipFree(ctx->verify_arrived);
   if (ctx->stream) hipStreamDestroy(ctx->stream);
   delete ctx;
@@ -1279,6 +1283,7 @@ int tlm_op_paged_attention(tlm_paged* P, const tlm_paged_batch* b, const float* 
   // the chunks' results live in the context's buffer from one launch to the next
   std::lock_guard<std::mutex> lock(P->ctx->part_mu);
   a.part = P->ctx->part;
+  a.arrived = P->ctx->paged_arrived;
   if (!launch_paged_attention(P->d.kv_fmt == TLM_FMT_F32, a, P->ctx->cus, kPartFloats, P->ctx->stream))
     return fail(TLM_ERR_STATE, "TLMPaged: no attention kernel for this shape");
   CHECK_LAUNCH("TLMPaged");

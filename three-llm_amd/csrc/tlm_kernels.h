@@ -489,8 +489,10 @@ struct PagedArgs {
   float scale;
   // attention: how the sequences' position tiles are shared out (launch_paged_attention)
   float* part;
-  int units, chunks, chunk_min, plan_shift;
+  unsigned* arrived;  // [kPagedCounters], zero between launches
+  int units, chunks, round, chunk_min, plan_shift;
 };
+constexpr int kPagedCounters = 16384;
 bool launch_paged_append(bool kv_f32, const PagedArgs& a, hipStream_t st);
 // part_floats: what a.part holds
 bool launch_paged_attention(bool kv_f32, const PagedArgs& a, int cus, size_t part_floats, hipStream_t st);

@@ -309,57 +309,77 @@ __device__ __forceinline__ SeqWork seq_work(const PagedArgs& a, int s, bool* bad
   return w;
 }
 
-// Chunks of equal size over sequences of unequal length: c tiles a chunk, such
-// that all sequences together have at most a.chunks more chunks than sequences.
-// Every wave works it out for itself from the starts (which only the device
-// knows): the sum of the tiles, then a running sum of the sequences' chunks up to
-// the one that `found` accepts (excl: chunks of the sequences before, n: its own).
-// slot: records of partial results before it (sequences of one chunk have none).
-struct SeqChunks {
+// Values that another block of the same launch reads: past the XCD's L2.
+__device__ __forceinline__ void publish2(float* p, float x, float y) {
+  const unsigned long long v = (unsigned long long)__float_as_uint(y) << 32 | __float_as_uint(x);
+  __hip_atomic_store(reinterpret_cast<unsigned long long*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 published2(const float* p) {
+  const unsigned long long v = __hip_atomic_load(reinterpret_cast<const unsigned long long*>(p), __ATOMIC_RELAXED,
+                                                 __HIP_MEMORY_SCOPE_AGENT);
+  return make_float2(__uint_as_float((unsigned)v), __uint_as_float((unsigned)(v >> 32)));
+}
+
+// Sum over the wave's lanes up to each, over integers.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr:1, within 16 lanes
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
+  return v;
+}
+
+// Chunks of equal size over sequences of unequal length, c tiles each: all
+// sequences together have at most a.chunks more of them than sequences.  Every
+// wave works it out for itself from the starts (which only the device knows): the
+// sum of the tiles, then a running sum of the sequences' chunks up to chunk g.
+// slot: records of partial results before the sequence's (one of a single chunk has
+// none).  False: there is no chunk g.
+struct SeqChunk {
   SeqWork w;
-  int s, n, chunk, slot;  // chunk: which of the sequence's (plan_chunk)
+  int s, n, chunk, slot;  // sequence, its chunks, which of them
   bool bad;
 };
-template <int SHIFT, typename Found>
-__device__ __forceinline__ bool plan(const PagedArgs& a, SeqChunks& r, Found found) {
+template <int SHIFT>
+__device__ __forceinline__ bool plan(const PagedArgs& a, int g, SeqChunk& r) {
   const int lane = threadIdx.x & 63;
   bool bad = false;
   SeqWork w = lane < a.seqs ? seq_work<SHIFT>(a, lane, &bad) : SeqWork{0, 0, 0, 0};
-  int total = (w.tiles + (1 << a.plan_shift) - 1) >> a.plan_shift;
+  int part = (w.tiles + (1 << a.plan_shift) - 1) >> a.plan_shift;
   for (int s = lane + 64; s < a.seqs; s += 64) {
     bool b;
-    total += (seq_work<SHIFT>(a, s, &b).tiles + (1 << a.plan_shift) - 1) >> a.plan_shift;
+    part += (seq_work<SHIFT>(a, s, &b).tiles + (1 << a.plan_shift) - 1) >> a.plan_shift;
   }
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) total += __shfl_xor(total, o);
-  const int c = max(a.chunk_min, ((total + a.chunks - 1) / a.chunks) << a.plan_shift);
+  const int total = __builtin_amdgcn_readlane(wave_scan(part), 63);
+  int c = max(a.chunk_min, ((total + a.chunks - 1) / a.chunks) << a.plan_shift);
+  if (a.seqs <= 64) {
+    // few sequences: all their chunks in one round of blocks
+    const int live = __builtin_popcountll(__ballot(w.tiles > 0));
+    if (2 * live <= a.round)
+      while (__builtin_amdgcn_readlane(wave_scan((w.tiles + c - 1) / c), 63) > a.round) c += (c + 7) / 8;
+  }
   int before = 0, slots = 0;
   for (int s0 = 0; s0 < a.seqs; s0 += 64) {
     if (s0) w = s0 + lane < a.seqs ? seq_work<SHIFT>(a, s0 + lane, &bad) : SeqWork{0, 0, 0, 0};
-    const int n = (w.tiles + c - 1) / c, m = n > 1 ? n : 0;
-    int incl = n, sincl = m;
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) {
-      const int x = __shfl_up(incl, o), y = __shfl_up(sincl, o);
-      if (lane >= o) incl += x, sincl += y;
-    }
-    const int excl = before + incl - n;
-    const unsigned long long hit = __ballot(found(s0 + lane, excl, n));
+    const int n = (w.tiles + c - 1) / c, incl = wave_scan(n);
+    const unsigned long long hit = __ballot(before + incl > g);
     if (hit) {
-      const int l = __builtin_ctzll(hit);
+      const int l = __builtin_ctzll(hit), m = n > 1 ? n : 0, sincl = wave_scan(m);
       r.s = s0 + l;
       r.w.start = __builtin_amdgcn_readlane(w.start, l);
       r.w.rows = __builtin_amdgcn_readlane(w.rows, l);
       r.w.first = __builtin_amdgcn_readlane(w.first, l);
       r.w.tiles = __builtin_amdgcn_readlane(w.tiles, l);
       r.n = __builtin_amdgcn_readlane(n, l);
-      r.chunk = __builtin_amdgcn_readlane(excl, l);  // chunks before the sequence
+      r.chunk = g - before - __builtin_amdgcn_readlane(incl - n, l);
       r.slot = slots + __builtin_amdgcn_readlane(sincl - m, l);
       r.bad = __builtin_amdgcn_readlane((int)bad, l);
       return true;
     }
     before += __builtin_amdgcn_readlane(incl, 63);
-    slots += __builtin_amdgcn_readlane(sincl, 63);
+    if (a.seqs > 64) slots += __builtin_amdgcn_readlane(wave_scan(n > 1 ? n : 0), 63);
   }
   return false;
 }
@@ -376,13 +396,14 @@ __global__ __launch_bounds__(64 * W) void paged_attention_kernel(PagedArgs a) {
   constexpr int SUB = T::SUB, TS = T::TS, NF = DT / 16;  // 1 KB operand pieces of a tile's K, of its V
   constexpr bool F16 = sizeof(KT) == 2, QREG = NT == 1;
   constexpr int RS = DT + 2;  // floats of a row's record: maximum, sum, output
-  constexpr int QB = QREG ? 0 : NT * NF * 64 * 4, MB = W * 16 * RS;  // floats
-  __shared__ __align__(16) float lds[QB > MB ? QB : MB];
+  constexpr int QB = QREG ? 0 : NT * (NF * 256 + 16), MB = W * 16 * RS;  // floats
+  constexpr int LDSF = QB > MB ? QB : MB;
+  __shared__ __align__(16) float lds[LDSF];
   const int unit = blockIdx.x % a.units, hk = unit % a.Hkv, r0 = unit / a.Hkv * 16 * NT;
   const int g = blockIdx.x / a.units;
-  SeqChunks sc;
-  if (!plan<T::SHIFT>(a, sc, [&](int, int excl, int n) { return excl <= g && g < excl + n; })) return;
-  const int ci = g - sc.chunk, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  SeqChunk sc;
+  if (!plan<T::SHIFT>(a, g, sc)) return;
+  const int ci = sc.chunk, tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   if (sc.bad && ci == 0 && unit == 0 && tid == 0) paged_flag(a.status, kPagedStatusRows);
   const int R = sc.w.rows * a.G;  // rows of the kv head
   if (r0 >= R) return;
@@ -397,59 +418,106 @@ __global__ __launch_bounds__(64 * W) void paged_attention_kernel(PagedArgs a) {
   const int32_t* const table = a.tables + (size_t)sc.s * a.width;
   const int tpp = a.page_shift - T::SHIFT;  // log2 of the tiles of a page
 
-  // this lane's rows (a column of each tile): their positions' bounds, q scaled by
-  // a power of two per row to at most 1
+  struct Tile {
+    u32x4 k[NF], v[NF];
+  };
+  auto load = [&](u32x4* x, const void* pool, int t, int page) {
+    const size_t at = paged_head_at(max(page, 0), hk, a.Hkv, a.page_shift, DT) +
+                      (size_t)(t & ((1 << tpp) - 1)) * (TS * DT) + lane * (16 / sizeof(KT));
+    const TLM_GLOBAL u32x4* p = gl(reinterpret_cast<const u32x4*>(static_cast<const KT*>(pool) + at));
+#pragma unroll
+    for (int f = 0; f < NF; f++) x[f] = p[64 * f];
+  };
+  // The wave's tiles t0 + w, t0 + w + W, ...  Their pages, 64 at a time, a lane each;
+  // the first tile is on its way while q is prepared.
+  int tb = t0 + w, n = 0, page = -1;
+  auto pages = [&] {
+    const int tl = tb + lane * W;
+    n = min(64, (t1 - tb + W - 1) / W);
+    page = paged_page(table, min(tl, t1 - 1) << T::SHIFT, a.page_shift, a.num_pages);
+    if (page < 0 && tl < t1) paged_flag(a.status, kPagedStatusPage);
+  };
+  auto page_of = [&](int i) { return __builtin_amdgcn_readlane(page, min(i, n - 1)); };
+  auto load_k = [&](Tile& x, int i) { load(x.k, a.kc, tb + min(i, n - 1) * W, page_of(i)); };
+  auto load_v = [&](Tile& x, int i) { load(x.v, a.vc, tb + min(i, n - 1) * W, page_of(i)); };
+  // this lane's rows (a column of each row tile): their positions' bounds, and q scaled
+  // by a power of two per row to at most 1.  q is requested before the first tile:
+  // loads return in order.  With more row tiles than one a wave prepares some of
+  // them, and all take them from LDS.
   int lo[NT], hi[NT];
   float mult[NT];
   u32x4 qreg[QREG ? NF : 1];
   u32x4* const qlds = reinterpret_cast<u32x4*>(lds);  // [NT][NF][64]
+  float* const mlds = lds + NT * NF * 256;            // [NT][16]
   const float qscale = a.scale * 1.4426950408889634f;  // log2 e: the softmax runs in base 2
-#pragma unroll
-  for (int nt = 0; nt < NT; nt++) {
-    const int r = r0 + 16 * nt + i16, rc = min(r, R - 1), j = rc / a.G, pos = start + j;
-    lo[nt] = a.window > 0 ? pos - a.window + 1 : 0;
-    hi[nt] = pos;
-    const float* q = a.x + (((size_t)sc.s * a.tokens + j) * a.Hq + hk * a.G + rc % a.G) * DT;
-    f32x4 x[NF];
+  f32x4 qx[NF];
+  auto load_q = [&](int nt) {
+    const int r = min(r0 + 16 * nt + i16, R - 1);
+    const float* q = a.x + (((size_t)sc.s * a.tokens + r / a.G) * a.Hq + hk * a.G + r % a.G) * DT;
 #pragma unroll
     for (int f = 0; f < NF; f++)  // fp16: dims 32 (f / 2) + 8 qd + 4 (f % 2) ..; fp32: 16 f + 4 qd ..
-      x[f] = *(const TLM_GLOBAL f32x4u*)(q + (F16 ? 32 * (f / 2) + 8 * qd + 4 * (f & 1) : 16 * f + 4 * qd));
+      qx[f] = *(const TLM_GLOBAL f32x4u*)(q + (F16 ? 32 * (f / 2) + 8 * qd + 4 * (f & 1) : 16 * f + 4 * qd));
+  };
+  auto prepare_q = [&](int nt, u32x4* to, int stride) {  // the row's multiplier
     float m = 0.f;
 #pragma unroll
     for (int f = 0; f < NF; f++)
 #pragma unroll
-      for (int e = 0; e < 4; e++) m = fmaxf(m, fabsf(x[f][e]));
+      for (int e = 0; e < 4; e++) m = fmaxf(m, fabsf(qx[f][e]));
     m = fmaxf(m, lane_swap16(m));
     m = fmaxf(m, lane_swap32(m));
     const int ex = max(-120, min(120, __builtin_amdgcn_frexp_expf(m)));
-    mult[nt] = ldexpf(qscale, ex);
+    const bool row = r0 + 16 * nt + i16 < R;
 #pragma unroll
     for (int f = 0; f < NF; f++)
 #pragma unroll
-      for (int e = 0; e < 4; e++) x[f][e] = r < R ? ldexpf(x[f][e], -ex) : 0.f;
+      for (int e = 0; e < 4; e++) qx[f][e] = row ? ldexpf(qx[f][e], -ex) : 0.f;
     if (F16) {
 #pragma unroll
       for (int jj = 0; jj < NF / 2; jj++) {
         ph8_t h, l;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-          const float v = x[2 * jj + e / 4][e & 3];
+          const float v = qx[2 * jj + e / 4][e & 3];
           h[e] = (_Float16)v;
           l[e] = (_Float16)(v - (float)h[e]);
         }
-        const u32x4 hb = __builtin_bit_cast(u32x4, h), lb = __builtin_bit_cast(u32x4, l);
-        if (QREG) qreg[QREG ? 2 * jj : 0] = hb, qreg[QREG ? 2 * jj + 1 : 0] = lb;
-        else if (w == nt % W) qlds[(nt * NF + 2 * jj) * 64 + lane] = hb, qlds[(nt * NF + 2 * jj + 1) * 64 + lane] = lb;
+        to[2 * jj * stride] = __builtin_bit_cast(u32x4, h);
+        to[(2 * jj + 1) * stride] = __builtin_bit_cast(u32x4, l);
       }
     } else {
 #pragma unroll
-      for (int f = 0; f < NF; f++) {
-        if (QREG) qreg[QREG ? f : 0] = __builtin_bit_cast(u32x4, x[f]);
-        else if (w == nt % W) qlds[(nt * NF + f) * 64 + lane] = __builtin_bit_cast(u32x4, x[f]);
-      }
+      for (int f = 0; f < NF; f++) to[f * stride] = __builtin_bit_cast(u32x4, qx[f]);
     }
+    return ldexpf(qscale, ex);
+  };
+  if (QREG || w < NT) load_q(QREG ? 0 : w);
+  __builtin_amdgcn_sched_barrier(0);
+  Tile x;
+  if (tb < t1) {
+    pages();
+    load_k(x, 0);
+    load_v(x, 0);
   }
-  if (!QREG) lds_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++) {
+    const int pos = start + min(r0 + 16 * nt + i16, R - 1) / a.G;
+    lo[nt] = a.window > 0 ? pos - a.window + 1 : 0;
+    hi[nt] = pos;
+  }
+  if constexpr (QREG) {
+    mult[0] = prepare_q(0, qreg, 1);
+  } else {
+    static_assert(NT <= W, "a wave per row tile");
+    if (w < NT) {
+      const float m = prepare_q(w, qlds + w * NF * 64 + lane, 64);
+      if (qd == 0) mlds[w * 16 + i16] = m;
+    }
+    lds_barrier();
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) mult[nt] = mlds[nt * 16 + i16];
+  }
 
   f32x4 o[NT][NF];
   float mrun[NT], lrun[NT];  // running maximum, this lane's share of the sum
@@ -461,16 +529,6 @@ __global__ __launch_bounds__(64 * W) void paged_attention_kernel(PagedArgs a) {
     for (int f = 0; f < NF; f++) o[nt][f] = (f32x4){0.f, 0.f, 0.f, 0.f};
   }
 
-  struct Tile {
-    u32x4 k[NF], v[NF];
-  };
-  auto load = [&](u32x4* x, const void* pool, int t, int page) {
-    const size_t at = paged_head_at(max(page, 0), hk, a.Hkv, a.page_shift, DT) +
-                      (size_t)(t & ((1 << tpp) - 1)) * (TS * DT) + lane * (16 / sizeof(KT));
-    const TLM_GLOBAL u32x4* p = gl(reinterpret_cast<const u32x4*>(static_cast<const KT*>(pool) + at));
-#pragma unroll
-    for (int f = 0; f < NF; f++) x[f] = p[64 * f];
-  };
   // V with positions outside [first, last] taken out (0 times what they hold may be NaN)
   auto keep = [&](const u32x4& v, int p, int first, int last) {
     u32x4 y;
@@ -486,6 +544,9 @@ __global__ __launch_bounds__(64 * W) void paged_attention_kernel(PagedArgs a) {
     }
     return y;
   };
+  auto not_finite = [](unsigned v) -> unsigned {  // the sign bits' places of values that are not finite
+    return F16 ? ((v & 0x7C007C00u) + 0x04000400u) & 0x80008000u : ((v & 0x7F800000u) + 0x00800000u) & 0x80000000u;
+  };
   // tile t; k_read() and v_read() run once x.k and x.v have been read
   auto process = [&](Tile& x, int t, auto k_read, auto v_read) {
     if (!QREG) asm volatile("" ::: "memory");  // q is read again, not kept in registers that o needs
@@ -499,9 +560,7 @@ __global__ __launch_bounds__(64 * W) void paged_attention_kernel(PagedArgs a) {
       for (int f = 0; f < NF; f++) {
         x.v[f] = keep(x.v[f], p, lo_any, hi_any);
 #pragma unroll
-        for (int d = 0; d < 4; d++)
-          nf |= F16 ? ((x.v[f][d] & 0x7C007C00u) + 0x04000400u) & 0x80008000u
-                    : ((x.v[f][d] & 0x7F800000u) + 0x00800000u) & 0x80000000u;
+        for (int d = 0; d < 4; d++) nf |= not_finite(x.v[f][d]);
       }
       apart = ja != jb && __ballot(nf != 0) != 0;
     }
@@ -590,46 +649,40 @@ __global__ __launch_bounds__(64 * W) void paged_attention_kernel(PagedArgs a) {
       for (int e = 0; e < 4; e++) y = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[e], pf[e], y, 0, 0, 0);
       return y;
     };
-    if (!apart) {
-#pragma unroll
-      for (int f = 0; f < NF; f++)
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) o[nt][f] = weigh(x.v[f], nt, o[nt][f]);
-      v_read();
-      return;
-    }
-    // token by token, each over the positions that it sees, kept in its rows' columns
-    for (int j = ja; j <= jb; j++) {
-      const int first = a.window > 0 ? start + j - a.window + 1 : 0, last = start + j;
+    if (apart) {
+      // a row that does give such a value a weight becomes NaN there; the others get 0
+      // times 0
 #pragma unroll
       for (int f = 0; f < NF; f++) {
-        const u32x4 v = keep(x.v[f], p, first, last);
+        u32x4 one;
+#pragma unroll
+        for (int d = 0; d < 4; d++) {
+          const unsigned t = not_finite(x.v[f][d]);  // a bit per value, its highest
+          one[d] = F16 ? (t >> 15) * 0x3C00u : (t >> 31) * 0x3F800000u;
+          x.v[f][d] &= ~(F16 ? (t >> 15) * 0xFFFFu : (t >> 31) * 0xFFFFFFFFu);
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-          const f32x4 y = weigh(v, nt, o[nt][f]);
-          if (hi[nt] == last) o[nt][f] = y;
+          const f32x4 y = weigh(one, nt, (f32x4){0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            if (y[e] > 0.f) o[nt][f][e] = __uint_as_float(0x7FC00000u);
         }
       }
     }
+#pragma unroll
+    for (int f = 0; f < NF; f++)
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++) o[nt][f] = weigh(x.v[f], nt, o[nt][f]);
     v_read();
   };
 
-  // The wave's tiles t0 + w, t0 + w + W, ...  Their pages, 64 at a time, a lane each.
   // One row tile: a position tile in work, the next in flight.  More: their outputs
   // take the registers of a second one, and the next tile's K goes out when this
   // one's has been read, its V likewise.
   const auto none = [] {};
-  for (int tb = t0 + w; tb < t1; tb += 64 * W) {
-    const int tl = tb + lane * W, n = min(64, (t1 - tb + W - 1) / W);
-    const int page = paged_page(table, min(tl, t1 - 1) << T::SHIFT, a.page_shift, a.num_pages);
-    if (page < 0 && tl < t1) paged_flag(a.status, kPagedStatusPage);
-    auto page_of = [&](int i) { return __builtin_amdgcn_readlane(page, min(i, n - 1)); };
-    auto load_k = [&](Tile& x, int i) { load(x.k, a.kc, tb + min(i, n - 1) * W, page_of(i)); };
-    auto load_v = [&](Tile& x, int i) { load(x.v, a.vc, tb + min(i, n - 1) * W, page_of(i)); };
-    Tile x;
-    load_k(x, 0);
-    load_v(x, 0);
-    if constexpr (NT == 1) {
+  while (tb < t1) {
+    if constexpr (NT == 1 && DT <= 64) {
       Tile y;
       for (int i = 0; i < n; i += 2) {
         load_k(y, i + 1);
@@ -650,10 +703,26 @@ __global__ __launch_bounds__(64 * W) void paged_attention_kernel(PagedArgs a) {
         }
       }
     }
+    tb += 64 * W;
+    if (tb < t1) {
+      pages();
+      load_k(x, 0);
+      load_v(x, 0);
+    }
   }
 
   // the waves' results, 16 rows at a time, through LDS
   const bool whole = sc.n == 1;
+  auto put = [&](int r, int d, float y0, float y1) {  // dims d and d + 1 of row r
+    const size_t at = (((size_t)sc.s * a.tokens + r / a.G) * a.Hq + hk * a.G + r % a.G) * DT + d;
+    if (a.out_f32) {
+      static_cast<float*>(a.out)[at] = y0;
+      static_cast<float*>(a.out)[at + 1] = y1;
+    } else {
+      static_cast<uint16_t*>(a.out)[at] = kv_store<uint16_t>(y0);
+      static_cast<uint16_t*>(a.out)[at + 1] = kv_store<uint16_t>(y1);
+    }
+  };
 #pragma unroll
   for (int nt = 0; nt < NT; nt++) {
     float l = lrun[nt];
@@ -668,10 +737,10 @@ __global__ __launch_bounds__(64 * W) void paged_attention_kernel(PagedArgs a) {
       for (int e = 0; e < 4; e++) rec[2 + 16 * f + 4 * qd + e] = o[nt][f][e];
     if (qd == 0) rec[0] = mrun[nt], rec[1] = l;
     __syncthreads();
-    for (int e = tid; e < 16 * DT; e += 64 * W) {
-      const int row = e / DT, d = e % DT, r = r0 + 16 * nt + row;
+    for (int e = tid; e < 8 * DT; e += 64 * W) {
+      const int row = e / (DT / 2), d = 2 * (e % (DT / 2)), r = r0 + 16 * nt + row;
       if (r >= R) break;
-      float M = -FLT_MAX, L = 0.f, O = 0.f;
+      float M = -FLT_MAX, L = 0.f, O0 = 0.f, O1 = 0.f;
 #pragma unroll
       for (int x = 0; x < W; x++) M = fmaxf(M, lds[(x * 16 + row) * RS]);
 #pragma unroll
@@ -679,65 +748,77 @@ __global__ __launch_bounds__(64 * W) void paged_attention_kernel(PagedArgs a) {
         const float* y = lds + (x * 16 + row) * RS;
         const float f = __builtin_amdgcn_exp2f(y[0] - M);
         L = fmaf(y[1], f, L);
-        O = fmaf(y[2 + d], f, O);
+        O0 = fmaf(y[2 + d], f, O0);
+        O1 = fmaf(y[3 + d], f, O1);
       }
       if (whole) {
-        const float y = L == 0.f ? 0.f : O / L;  // 0: no position has a page
-        const size_t at = (((size_t)sc.s * a.tokens + r / a.G) * a.Hq + hk * a.G + r % a.G) * DT + d;
-        if (a.out_f32) static_cast<float*>(a.out)[at] = y;
-        else static_cast<uint16_t*>(a.out)[at] = kv_store<uint16_t>(y);
+        put(r, d, L == 0.f ? 0.f : O0 / L, L == 0.f ? 0.f : O1 / L);  // 0: no position has a page
       } else {
         float* p = part_row(a, sc.slot + ci, unit, 16 * nt + row, 16 * NT, DT);
-        p[d] = O;
-        if (d == 0) p[DT] = M, p[DT + 1] = L;
+        publish2(p + d, O0, O1);
+        if (d == 0) publish2(p + DT, M, L);
       }
     }
   }
-}
+  if (whole) return;
 
-// The chunks of a row joined: a block per sequence, unit and row (`used` of the
-// `rows` that a unit's record holds).
-template <int SHIFT, int DT>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int rows, int used) {
-  constexpr int P = DT / 2, NG = 256 / P;  // threads of a record, two dims each; records at a time
-  __shared__ float red[NG][DT + 2];
-  const int row = blockIdx.x % used, unit = blockIdx.x / used % a.units, s = blockIdx.x / used / a.units;
-  SeqChunks sc;
-  plan<SHIFT>(a, sc, [&](int i, int, int) { return i == s; });
-  const int r = unit / a.Hkv * rows + row, hk = unit % a.Hkv;
-  if (sc.n < 2 || r >= sc.w.rows * a.G) return;
-  const int d2 = threadIdx.x % P, grp = threadIdx.x / P;
-  if (grp < NG) {
-    float M = -FLT_MAX, L = 0.f, O0 = 0.f, O1 = 0.f;
-    for (int c = grp; c < sc.n; c += NG) {
-      const float* p = part_row(a, sc.slot + c, unit, row, rows, DT);
-      const float2 v = *reinterpret_cast<const float2*>(p + 2 * d2), ml = *reinterpret_cast<const float2*>(p + DT);
-      const float mn = fmaxf(M, ml.x), f = __builtin_amdgcn_exp2f(M - mn), h = __builtin_amdgcn_exp2f(ml.x - mn);
-      L = L * f + ml.y * h;
-      O0 = O0 * f + v.x * h;
-      O1 = O1 * f + v.y * h;
-      M = mn;
-    }
-    red[grp][2 * d2] = O0;
-    red[grp][2 * d2 + 1] = O1;
-    if (d2 == 0) red[grp][DT] = M, red[grp][DT + 1] = L;
-  }
+  // The last of the sequence's blocks joins the chunks: it counts last, when every
+  // block's results have been performed, and clears the count.
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's results are performed
+  __syncthreads();                                  // and every wave's
+  unsigned* const count = a.arrived + (size_t)sc.slot * a.units + unit;
+  if (tid == 0) lds[0] = __uint_as_float(__hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
   __syncthreads();
-  const int d = threadIdx.x;
-  if (d >= DT) return;
-  float M = -FLT_MAX, L = 0.f, O = 0.f;
+  if (__float_as_uint(lds[0]) != (unsigned)sc.n - 1) return;
+  __syncthreads();  // lds[0] has been read
+  if (tid == 0) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  // A thread per row and pair of dims, the chunks in `groups` where there are threads
+  // for it; eight chunks' values in flight at a time.
+  constexpr int TH = 64 * W, P = DT / 2;
+  static_assert(4 * TH <= LDSF, "a record per thread");
+  const int rows = min(16 * NT, R - r0), items = rows * P, groups = max(1, TH / items);
+  const size_t step = (size_t)a.units * 16 * NT * RS;
+  for (int i0 = 0; i0 < items; i0 += TH) {
+    const int i = groups > 1 ? tid % items : i0 + tid, grp = groups > 1 ? tid / items : 0;
+    const bool here = i < items && grp < groups;
+    float M = -FLT_MAX, L = 0.f, O0 = 0.f, O1 = 0.f;
+    const float* rec = part_row(a, sc.slot, unit, min(i, items - 1) / P, 16 * NT, DT);
+    for (int c0 = grp; here && c0 < sc.n; c0 += 8 * groups) {
+      float2 v[8], ml[8];
 #pragma unroll
-  for (int x = 0; x < NG; x++) M = fmaxf(M, red[x][DT]);
+      for (int k = 0; k < 8; k++) {
+        const float* p = rec + min(c0 + k * groups, sc.n - 1) * step;
+        v[k] = published2(p + 2 * (i % P));
+        ml[k] = published2(p + DT);
+      }
+      float m = M;
 #pragma unroll
-  for (int x = 0; x < NG; x++) {
-    const float f = __builtin_amdgcn_exp2f(red[x][DT] - M);
-    L = fmaf(red[x][DT + 1], f, L);
-    O = fmaf(red[x][d], f, O);
+      for (int k = 0; k < 8; k++) m = fmaxf(m, ml[k].x);
+      const float f = __builtin_amdgcn_exp2f(M - m);
+      L *= f, O0 *= f, O1 *= f;
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        const float h = c0 + k * groups < sc.n ? __builtin_amdgcn_exp2f(ml[k].x - m) : 0.f;
+        L = fmaf(ml[k].y, h, L);
+        O0 = fmaf(v[k].x, h, O0);
+        O1 = fmaf(v[k].y, h, O1);
+      }
+      M = m;
+    }
+    if (groups > 1) {
+      float* const mine = lds + 4 * tid;
+      mine[0] = M, mine[1] = L, mine[2] = O0, mine[3] = O1;
+      __syncthreads();
+      for (int x = 1; x < groups && tid < items; x++) {
+        const float* y = lds + 4 * (tid + x * items);
+        const float m = fmaxf(M, y[0]), f = __builtin_amdgcn_exp2f(M - m), h = __builtin_amdgcn_exp2f(y[0] - m);
+        L = L * f + y[1] * h, O0 = O0 * f + y[2] * h, O1 = O1 * f + y[3] * h;
+        M = m;
+      }
+    }
+    if (here && grp == 0)
+      put(r0 + i / P, 2 * (i % P), L == 0.f ? 0.f : O0 / L, L == 0.f ? 0.f : O1 / L);
   }
-  const float y = L == 0.f ? 0.f : O / L;
-  const size_t at = (((size_t)s * a.tokens + r / a.G) * a.Hq + hk * a.G + r % a.G) * DT + d;
-  if (a.out_f32) static_cast<float*>(a.out)[at] = y;
-  else static_cast<uint16_t*>(a.out)[at] = kv_store<uint16_t>(y);
 }
 
 template <typename KT, int DT, int NT, int W>
@@ -751,18 +832,15 @@ void launch_attention_of(PagedArgs a, int cus, size_t part_floats, hipStream_t s
   const int64_t tiles = most / T::TS + 2;
   a.plan_shift = 0;
   while (a.seqs * ((tiles >> a.plan_shift) + 1) >= ((int64_t)1 << 30)) a.plan_shift++;
-  // all blocks at once: `chunks` of them a unit
   const int64_t record = (int64_t)rows * (DT + 2);
-  const int64_t fit = (int64_t)part_floats / (2 * a.units * record);  // sequences of two chunks or more: 2 * chunks at most
-  a.chunks = (int)std::max<int64_t>(1, std::min<int64_t>(fit, 2 * cus / a.units));
-  a.chunk_min = fit < 1 ? INT_MAX / 2 : W;
+  // sequences of two chunks or more have 2 * chunks at most, each a record and a count
+  const int64_t fit = std::min<int64_t>((int64_t)part_floats / (2 * a.units * record), kPagedCounters / (2 * a.units));
+  a.round = std::max(1, cus / a.units);
+  a.chunks = (int)std::max<int64_t>(1, std::min<int64_t>(fit, a.round));
+  a.chunk_min = fit < 1 ? INT_MAX / 2 : 2 * W;
   const int64_t per_seq = fit < 1 ? 1 : (tiles + a.chunk_min - 1) / a.chunk_min;
   const int64_t blocks = std::min<int64_t>(a.chunks + a.seqs, a.seqs * per_seq) * a.units;
   hipLaunchKernelGGL((paged_attention_kernel<KT, DT, NT, W>), dim3((unsigned)blocks), dim3(64 * W), 0, st, a);
-  if (per_seq < 2) return;
-  const int used = std::min(rows, a.tokens * a.G);
-  hipLaunchKernelGGL((paged_join_kernel<T::SHIFT, DT>), dim3((unsigned)(a.seqs * a.units * used)), dim3(256), 0, st, a,
-                     rows, used);
 }
 
 template <typename KT, int DT>
