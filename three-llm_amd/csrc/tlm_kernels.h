@@ -490,7 +490,7 @@ struct PagedArgs {
   // attention: how the sequences' position tiles are shared out (launch_paged_attention)
   float* part;
   unsigned* arrived;  // [kPagedCounters], zero between launches
-  int units, chunks, round, chunk_min, plan_shift;
+  int units, chunks, round, chunk_min, whole, plan_shift;
 };
 constexpr int kPagedCounters = 16384;
 bool launch_paged_append(bool kv_f32, const PagedArgs& a, hipStream_t st);

@@ -345,41 +345,58 @@ struct SeqChunk {
 template <int SHIFT>
 __device__ __forceinline__ bool plan(const PagedArgs& a, int g, SeqChunk& r) {
   const int lane = threadIdx.x & 63;
-  bool bad = false;
-  SeqWork w = lane < a.seqs ? seq_work<SHIFT>(a, lane, &bad) : SeqWork{0, 0, 0, 0};
-  int part = (w.tiles + (1 << a.plan_shift) - 1) >> a.plan_shift;
-  for (int s = lane + 64; s < a.seqs; s += 64) {
-    bool b;
-    part += (seq_work<SHIFT>(a, s, &b).tiles + (1 << a.plan_shift) - 1) >> a.plan_shift;
+  // the first kSeqs times 64 sequences stay in registers, a lane each
+  constexpr int kSeqs = 4;
+  const SeqWork none{0, 0, 0, 0};
+  SeqWork w[kSeqs];
+  bool bad[kSeqs], b;
+  auto part = [&](int tiles) { return (tiles + (1 << a.plan_shift) - 1) >> a.plan_shift; };
+  int sum = 0;
+#pragma unroll
+  for (int k = 0; k < kSeqs; k++) {
+    w[k] = none, bad[k] = false;
+    if (64 * k < a.seqs && 64 * k + lane < a.seqs) w[k] = seq_work<SHIFT>(a, 64 * k + lane, &bad[k]);
   }
-  const int total = __builtin_amdgcn_readlane(wave_scan(part), 63);
+#pragma unroll
+  for (int k = 0; k < kSeqs; k++) sum += part(w[k].tiles);
+  for (int s = 64 * kSeqs + lane; s < a.seqs; s += 64) sum += part(seq_work<SHIFT>(a, s, &b).tiles);
+  const int total = __builtin_amdgcn_readlane(wave_scan(sum), 63);
   int c = max(a.chunk_min, ((total + a.chunks - 1) / a.chunks) << a.plan_shift);
+  auto chunks_of = [&](int tiles) { return tiles <= a.whole ? min(tiles, 1) : (tiles + c - 1) / c; };
   if (a.seqs <= 64) {
     // few sequences: all their chunks in one round of blocks
-    const int live = __builtin_popcountll(__ballot(w.tiles > 0));
+    const int live = __builtin_popcountll(__ballot(w[0].tiles > 0));
     if (2 * live <= a.round)
-      while (__builtin_amdgcn_readlane(wave_scan((w.tiles + c - 1) / c), 63) > a.round) c += (c + 7) / 8;
+      while (__builtin_amdgcn_readlane(wave_scan(chunks_of(w[0].tiles)), 63) > a.round) c += (c + 7) / 8;
   }
   int before = 0, slots = 0;
-  for (int s0 = 0; s0 < a.seqs; s0 += 64) {
-    if (s0) w = s0 + lane < a.seqs ? seq_work<SHIFT>(a, s0 + lane, &bad) : SeqWork{0, 0, 0, 0};
-    const int n = (w.tiles + c - 1) / c, incl = wave_scan(n);
+  auto find = [&](const SeqWork& w, bool bad, int s0) {
+    const int n = chunks_of(w.tiles), incl = wave_scan(n), m = n > 1 ? n : 0, sincl = wave_scan(m);
     const unsigned long long hit = __ballot(before + incl > g);
-    if (hit) {
-      const int l = __builtin_ctzll(hit), m = n > 1 ? n : 0, sincl = wave_scan(m);
-      r.s = s0 + l;
-      r.w.start = __builtin_amdgcn_readlane(w.start, l);
-      r.w.rows = __builtin_amdgcn_readlane(w.rows, l);
-      r.w.first = __builtin_amdgcn_readlane(w.first, l);
-      r.w.tiles = __builtin_amdgcn_readlane(w.tiles, l);
-      r.n = __builtin_amdgcn_readlane(n, l);
-      r.chunk = g - before - __builtin_amdgcn_readlane(incl - n, l);
-      r.slot = slots + __builtin_amdgcn_readlane(sincl - m, l);
-      r.bad = __builtin_amdgcn_readlane((int)bad, l);
-      return true;
+    if (!hit) {
+      before += __builtin_amdgcn_readlane(incl, 63);
+      slots += __builtin_amdgcn_readlane(sincl, 63);
+      return false;
     }
-    before += __builtin_amdgcn_readlane(incl, 63);
-    if (a.seqs > 64) slots += __builtin_amdgcn_readlane(wave_scan(n > 1 ? n : 0), 63);
+    const int l = __builtin_ctzll(hit);
+    r.s = s0 + l;
+    r.w.start = __builtin_amdgcn_readlane(w.start, l);
+    r.w.rows = __builtin_amdgcn_readlane(w.rows, l);
+    r.w.first = __builtin_amdgcn_readlane(w.first, l);
+    r.w.tiles = __builtin_amdgcn_readlane(w.tiles, l);
+    r.n = __builtin_amdgcn_readlane(n, l);
+    r.chunk = g - before - __builtin_amdgcn_readlane(incl - n, l);
+    r.slot = slots + __builtin_amdgcn_readlane(sincl - m, l);
+    r.bad = __builtin_amdgcn_readlane((int)bad, l);
+    return true;
+  };
+#pragma unroll
+  for (int k = 0; k < kSeqs; k++)
+    if (64 * k < a.seqs && find(w[k], bad[k], 64 * k)) return true;
+  for (int s0 = 64 * kSeqs; s0 < a.seqs; s0 += 64) {
+    b = false;
+    const SeqWork v = s0 + lane < a.seqs ? seq_work<SHIFT>(a, s0 + lane, &b) : none;
+    if (find(v, b, s0)) return true;
   }
   return false;
 }
@@ -390,8 +407,8 @@ __device__ __forceinline__ float* part_row(const PagedArgs& a, int slot, int uni
   return a.part + (((size_t)slot * a.units + unit) * rows + row) * (DT + 2);
 }
 
-template <typename KT, int DT, int NT, int W>
-__global__ __launch_bounds__(64 * W) void paged_attention_kernel(PagedArgs a) {
+template <typename KT, int DT, int NT, int W, bool STREAM>
+__global__ __launch_bounds__(64 * W, NT == 1 ? (DT <= 64 ? 4 : 2) : 1) void paged_attention_kernel(PagedArgs a) {
   using T = PagedTile<KT>;
   constexpr int SUB = T::SUB, TS = T::TS, NF = DT / 16;  // 1 KB operand pieces of a tile's K, of its V
   constexpr bool F16 = sizeof(KT) == 2, QREG = NT == 1;
@@ -399,7 +416,8 @@ __global__ __launch_bounds__(64 * W) void paged_attention_kernel(PagedArgs a) {
   constexpr int QB = QREG ? 0 : NT * (NF * 256 + 16), MB = W * 16 * RS;  // floats
   constexpr int LDSF = QB > MB ? QB : MB;
   __shared__ __align__(16) float lds[LDSF];
-  const int unit = blockIdx.x % a.units, hk = unit % a.Hkv, r0 = unit / a.Hkv * 16 * NT;
+  // the row groups from the last one on: a prompt's last rows attend to the most
+  const int unit = blockIdx.x % a.units, hk = unit % a.Hkv, r0 = (a.units - 1 - unit) / a.Hkv * 16 * NT;
   const int g = blockIdx.x / a.units;
   SeqChunk sc;
   if (!plan<T::SHIFT>(a, g, sc)) return;
@@ -426,7 +444,7 @@ __global__ __launch_bounds__(64 * W) void paged_attention_kernel(PagedArgs a) {
                       (size_t)(t & ((1 << tpp) - 1)) * (TS * DT) + lane * (16 / sizeof(KT));
     const TLM_GLOBAL u32x4* p = gl(reinterpret_cast<const u32x4*>(static_cast<const KT*>(pool) + at));
 #pragma unroll
-    for (int f = 0; f < NF; f++) x[f] = p[64 * f];
+    for (int f = 0; f < NF; f++) x[f] = STREAM ? __builtin_nontemporal_load(p + 64 * f) : p[64 * f];
   };
   // The wave's tiles t0 + w, t0 + w + W, ...  Their pages, 64 at a time, a lane each;
   // the first tile is on its way while q is prepared.
@@ -677,30 +695,17 @@ __global__ __launch_bounds__(64 * W) void paged_attention_kernel(PagedArgs a) {
     v_read();
   };
 
-  // One row tile: a position tile in work, the next in flight.  More: their outputs
-  // take the registers of a second one, and the next tile's K goes out when this
-  // one's has been read, its V likewise.
-  const auto none = [] {};
+  // The next tile's K goes out when this one's has been read, its V likewise: half a
+  // tile or more in flight a wave, and the registers of one (with two, 8 waves a CU
+  // instead of 16 at head_dim 64 and less in flight: 64 x 1 Llama-3.2-1B at 1000
+  // positions 31.8 instead of 28.1 us).
   while (tb < t1) {
-    if constexpr (NT == 1 && DT <= 64) {
-      Tile y;
-      for (int i = 0; i < n; i += 2) {
-        load_k(y, i + 1);
-        load_v(y, i + 1);
-        if (page_of(i) >= 0) process(x, tb + i * W, none, none);
-        if (i + 1 >= n) break;
-        load_k(x, i + 2);
-        load_v(x, i + 2);
-        if (page_of(i + 1) >= 0) process(y, tb + (i + 1) * W, none, none);
-      }
-    } else {
-      for (int i = 0; i < n; i++) {
-        if (page_of(i) >= 0) {
-          process(x, tb + i * W, [&] { load_k(x, i + 1); }, [&] { load_v(x, i + 1); });
-        } else {
-          load_k(x, i + 1);
-          load_v(x, i + 1);
-        }
+    for (int i = 0; i < n; i++) {
+      if (page_of(i) >= 0) {
+        process(x, tb + i * W, [&] { load_k(x, i + 1); }, [&] { load_v(x, i + 1); });
+      } else {
+        load_k(x, i + 1);
+        load_v(x, i + 1);
       }
     }
     tb += 64 * W;
@@ -772,56 +777,67 @@ __global__ __launch_bounds__(64 * W) void paged_attention_kernel(PagedArgs a) {
   if (__float_as_uint(lds[0]) != (unsigned)sc.n - 1) return;
   __syncthreads();  // lds[0] has been read
   if (tid == 0) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  // A thread per row and pair of dims, the chunks in `groups` where there are threads
-  // for it; eight chunks' values in flight at a time.
-  constexpr int TH = 64 * W, P = DT / 2;
-  static_assert(4 * TH <= LDSF, "a record per thread");
-  const int rows = min(16 * NT, R - r0), items = rows * P, groups = max(1, TH / items);
+  // A thread per row and four dims, the chunks in `groups` where there are threads for
+  // it; four chunks' values in flight at a time.
+  constexpr int TH = 64 * W, P = DT / 4;
+  const int rows = min(16 * NT, R - r0), items = rows * P, groups = max(1, min(TH, LDSF / 6) / items);
   const size_t step = (size_t)a.units * 16 * NT * RS;
   for (int i0 = 0; i0 < items; i0 += TH) {
     const int i = groups > 1 ? tid % items : i0 + tid, grp = groups > 1 ? tid / items : 0;
     const bool here = i < items && grp < groups;
-    float M = -FLT_MAX, L = 0.f, O0 = 0.f, O1 = 0.f;
+    float M = -FLT_MAX, L = 0.f;
+    f32x4 O = {0.f, 0.f, 0.f, 0.f};
     const float* rec = part_row(a, sc.slot, unit, min(i, items - 1) / P, 16 * NT, DT);
-    for (int c0 = grp; here && c0 < sc.n; c0 += 8 * groups) {
-      float2 v[8], ml[8];
+    for (int c0 = grp; here && c0 < sc.n; c0 += 4 * groups) {
+      float2 v[4], u[4], ml[4];
 #pragma unroll
-      for (int k = 0; k < 8; k++) {
+      for (int k = 0; k < 4; k++) {
         const float* p = rec + min(c0 + k * groups, sc.n - 1) * step;
-        v[k] = published2(p + 2 * (i % P));
+        v[k] = published2(p + 4 * (i % P));
+        u[k] = published2(p + 4 * (i % P) + 2);
         ml[k] = published2(p + DT);
       }
-      float m = M;
-#pragma unroll
-      for (int k = 0; k < 8; k++) m = fmaxf(m, ml[k].x);
+      const float m = fmaxf(fmaxf(fmaxf(M, ml[0].x), fmaxf(ml[1].x, ml[2].x)), ml[3].x);
       const float f = __builtin_amdgcn_exp2f(M - m);
-      L *= f, O0 *= f, O1 *= f;
+      L *= f;
+      O *= f;
 #pragma unroll
-      for (int k = 0; k < 8; k++) {
+      for (int k = 0; k < 4; k++) {
         const float h = c0 + k * groups < sc.n ? __builtin_amdgcn_exp2f(ml[k].x - m) : 0.f;
         L = fmaf(ml[k].y, h, L);
-        O0 = fmaf(v[k].x, h, O0);
-        O1 = fmaf(v[k].y, h, O1);
+        O[0] = fmaf(v[k].x, h, O[0]);
+        O[1] = fmaf(v[k].y, h, O[1]);
+        O[2] = fmaf(u[k].x, h, O[2]);
+        O[3] = fmaf(u[k].y, h, O[3]);
       }
       M = m;
     }
     if (groups > 1) {
-      float* const mine = lds + 4 * tid;
-      mine[0] = M, mine[1] = L, mine[2] = O0, mine[3] = O1;
+      if (here) {
+        float* const mine = lds + 6 * tid;
+        mine[0] = M, mine[1] = L;
+#pragma unroll
+        for (int e = 0; e < 4; e++) mine[2 + e] = O[e];
+      }
       __syncthreads();
       for (int x = 1; x < groups && tid < items; x++) {
-        const float* y = lds + 4 * (tid + x * items);
+        const float* y = lds + 6 * (tid + x * items);
         const float m = fmaxf(M, y[0]), f = __builtin_amdgcn_exp2f(M - m), h = __builtin_amdgcn_exp2f(y[0] - m);
-        L = L * f + y[1] * h, O0 = O0 * f + y[2] * h, O1 = O1 * f + y[3] * h;
+        L = L * f + y[1] * h;
+#pragma unroll
+        for (int e = 0; e < 4; e++) O[e] = O[e] * f + y[2 + e] * h;
         M = m;
       }
     }
-    if (here && grp == 0)
-      put(r0 + i / P, 2 * (i % P), L == 0.f ? 0.f : O0 / L, L == 0.f ? 0.f : O1 / L);
+    if (here && grp == 0) {
+      const float d = L == 0.f ? 0.f : 1.f / L;
+      put(r0 + i / P, 4 * (i % P), O[0] * d, O[1] * d);
+      put(r0 + i / P, 4 * (i % P) + 2, O[2] * d, O[3] * d);
+    }
   }
 }
 
-template <typename KT, int DT, int NT, int W>
+template <typename KT, int DT, int NT, int W, bool STREAM = false>
 void launch_attention_of(PagedArgs a, int cus, size_t part_floats, hipStream_t st) {
   using T = PagedTile<KT>;
   const int rows = 16 * NT, groups = (a.tokens * a.G + rows - 1) / rows;
@@ -833,20 +849,40 @@ void launch_attention_of(PagedArgs a, int cus, size_t part_floats, hipStream_t s
   a.plan_shift = 0;
   while (a.seqs * ((tiles >> a.plan_shift) + 1) >= ((int64_t)1 << 30)) a.plan_shift++;
   const int64_t record = (int64_t)rows * (DT + 2);
-  // sequences of two chunks or more have 2 * chunks at most, each a record and a count
+  // Sequences of two chunks or more have 2 * chunks at most, each a record and a count.
+  // A split costs about 3.5 us (counting, joining), a round of the waves' tiles 0.8: up to
+  // 32 tiles a sequence stays whole, and chunks have 16 at least (16 x 8 Llama-3.2-1B at 2000
+  // 18.3 us with 16 tiles whole, 17.0 with 24, 16.6 with 32; four column tiles, whose rounds
+  // are longer: 16 x 5 Qwen2.5-0.5B 18.8 with 16, 25.3 with 32).
   const int64_t fit = std::min<int64_t>((int64_t)part_floats / (2 * a.units * record), kPagedCounters / (2 * a.units));
-  a.round = std::max(1, cus / a.units);
+  a.round = std::max(1, (NT == 1 ? 8 / W : 1) * cus / a.units);
   a.chunks = (int)std::max<int64_t>(1, std::min<int64_t>(fit, a.round));
-  a.chunk_min = fit < 1 ? INT_MAX / 2 : 2 * W;
-  const int64_t per_seq = fit < 1 ? 1 : (tiles + a.chunk_min - 1) / a.chunk_min;
+  a.chunk_min = fit < 1 ? INT_MAX / 2 : 16;
+  a.whole = NT == 4 ? 16 : 32;
+  const int64_t per_seq = fit < 1 || tiles <= a.whole ? 1 : (tiles + a.chunk_min - 1) / a.chunk_min;
   const int64_t blocks = std::min<int64_t>(a.chunks + a.seqs, a.seqs * per_seq) * a.units;
-  hipLaunchKernelGGL((paged_attention_kernel<KT, DT, NT, W>), dim3((unsigned)blocks), dim3(64 * W), 0, st, a);
+  hipLaunchKernelGGL((paged_attention_kernel<KT, DT, NT, W, STREAM>), dim3((unsigned)blocks), dim3(64 * W), 0, st, a);
 }
 
+// Waves a block: four where the sequences' kv heads alone give two blocks a CU (a
+// short sequence then leaves no waves idle), else eight.  us a call, 8 / 4 waves:
+// 128 x 1 Llama-3.2-1B at 1000 positions 28.1 / 24.2, 256 x 1 51.1 / 42.7, 64 x 1 Llama-3.2-3B 30.6 /
+// 28.4; 16 x 5 at 2500 17.6 / 19.3, Qwen2.5-0.5B 1 x 1 at 300 5.7 / 6.2.
+// There, loads past the last-level cache (256 MB) where K and V may exceed it, as
+// nothing of them is still there for the next call: 64 x 1 Llama-3.2-1B at 8192 (297 MB)
+// 60.7 -> 56.4; what fits it is faster kept (64 x 1 Llama-3.2-3B at 1000 28.3 -> 29.6).
+// More rows than 16: two or four column tiles, whose outputs leave room for four waves.
 template <typename KT, int DT>
 void launch_attention_rows(const PagedArgs& a, int cus, size_t part_floats, hipStream_t st) {
   const int rows = a.tokens * a.G;
-  if (rows <= 16) launch_attention_of<KT, DT, 1, 8>(a, cus, part_floats, st);
+  if (rows <= 16 && (int64_t)a.seqs * a.Hkv >= 2 * cus) {
+    const int64_t held = std::min<int64_t>(a.limit, a.window > 0 ? (int64_t)a.window + a.tokens : INT_MAX);
+    if (a.seqs * held * 2 * a.Hkv * DT * (int64_t)sizeof(KT) > (int64_t)256 << 20)
+      launch_attention_of<KT, DT, 1, 4, true>(a, cus, part_floats, st);
+    else
+      launch_attention_of<KT, DT, 1, 4>(a, cus, part_floats, st);
+  }
+  else if (rows <= 16) launch_attention_of<KT, DT, 1, 8>(a, cus, part_floats, st);
   else if (rows <= 32) launch_attention_of<KT, DT, 2, 4>(a, cus, part_floats, st);
   else launch_attention_of<KT, DT, 4, 4>(a, cus, part_floats, st);
 }
