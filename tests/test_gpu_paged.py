@@ -229,6 +229,18 @@ def test_attention_windows(ctx, window, tokens, kv):
     attend(Serving(ctx, 8, 2, 64, [0, window - 1, window, window + 45, 1500], tokens, 32, kv, window=window))
 
 
+@pytest.mark.parametrize("n", [65, 130, 300])
+@pytest.mark.parametrize("hq,hkv", [(4, 2), (8, 8)])
+def test_attention_long_caches_among_many(ctx, n, hq, hkv):
+    """Some sequences in several chunks, in every group of 64 that a block looks through."""
+    rng = np.random.default_rng(n + hq)
+    lengths = [int(x) for x in rng.integers(0, 60, n)]
+    for s in (1, 63, 64, n - 2, n - 1):
+        lengths[s] = 3000 + 7 * s
+    lengths[5] = -1
+    attend(Serving(ctx, hq, hkv, 64, lengths, 1, 64))
+
+
 @pytest.mark.parametrize("n", [1, 63, 64, 65, 200])
 def test_attention_many_sequences_of_all_lengths(ctx, n):
     rng = np.random.default_rng(n)
@@ -369,6 +381,25 @@ def test_rows_past_the_table_and_the_model_are_left_out(ctx):
     assert np.array_equal(after, before, equal_nan=True)
     with pytest.raises(tlm.TlmError):
         sv.paged.status()
+    sv.close()
+
+
+def test_starts_past_everything_are_reported_by_either_call(ctx):
+    sv = Serving(ctx, 4, 2, 64, [40, 3], 1, 32, counts=[1, 1], max_tokens=50)
+    sv.upload(*sv.pools([41, 4]))
+    q, x = normal(sv), np.zeros((2, 1, 8, 64), np.float32)
+    for start in (50, 64, 2 ** 31 - 1):
+        sv.batch.starts = ctx.array(np.array([start, 3], np.int32)).ptr
+        sv.rows, sv.starts = [0, 1], np.array([start, 3], np.int32)
+        sv.check(q, sv.attention(q, tlm.FMT_F32), tlm.FMT_F32, reported=True)
+        with pytest.raises(tlm.TlmError) as e:
+            sv.paged.status()
+        assert e.value.code == tlm.TLM_ERR_RANGE
+        sv.paged.append(sv.batch, ctx.array(x))
+        with pytest.raises(tlm.TlmError):
+            sv.paged.status()
+        sv.paged.status()
+        sv.upload(*sv.pools([0, 4]))
     sv.close()
 
 

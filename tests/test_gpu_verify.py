@@ -57,6 +57,16 @@ def test_large_vocabulary_many_sequences(ctx, by):
     check(ctx, logits, drafts, u, 0.8, counts=[4, 1, 0, 3, 2, 4, 4, -3, 4, 1, 2, 4], draft_logits=q)
 
 
+@pytest.mark.parametrize("n,v", [(64, 3000), (65, 4097), (200, 2049), (4097, 40), (9000, 7)])
+@pytest.mark.parametrize("by", ["lookup", "model"])
+@pytest.mark.parametrize("temp", [0.0, 0.9])
+def test_many_sequences_of_all_counts(ctx, n, v, by, temp):
+    """More sequences than a wave's lanes, than a launch's counters; idle ones in between."""
+    logits, drafts, u, q = inputs(n, 3, v, by=by)
+    counts = np.random.default_rng(n).integers(-1, 4, n)
+    check(ctx, logits, drafts, u, temp, counts=counts, draft_logits=q)
+
+
 def test_flat_distribution_draws_the_definition_s_token(ctx):
     """Every token equally likely but for noise: the sums decide."""
     logits, _, u, _ = inputs(48, 1, 128256, spread=0.05)

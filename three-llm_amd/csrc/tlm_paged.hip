@@ -340,7 +340,6 @@ __device__ __forceinline__ int wave_scan(int v) {
 struct SeqChunk {
   SeqWork w;
   int s, n, chunk, slot;  // sequence, its chunks, which of them
-  bool bad;
 };
 template <int SHIFT>
 __device__ __forceinline__ bool plan(const PagedArgs& a, int g, SeqChunk& r) {
@@ -359,7 +358,12 @@ __device__ __forceinline__ bool plan(const PagedArgs& a, int g, SeqChunk& r) {
   }
 #pragma unroll
   for (int k = 0; k < kSeqs; k++) sum += part(w[k].tiles);
-  for (int s = 64 * kSeqs + lane; s < a.seqs; s += 64) sum += part(seq_work<SHIFT>(a, s, &b).tiles);
+  bool any = bad[0] || bad[1] || bad[2] || bad[3];
+  for (int s = 64 * kSeqs + lane; s < a.seqs; s += 64) {
+    sum += part(seq_work<SHIFT>(a, s, &b).tiles);
+    any |= b;
+  }
+  if (any && blockIdx.x == 0 && threadIdx.x < 64) paged_flag(a.status, kPagedStatusRows);
   const int total = __builtin_amdgcn_readlane(wave_scan(sum), 63);
   int c = max(a.chunk_min, ((total + a.chunks - 1) / a.chunks) << a.plan_shift);
   auto chunks_of = [&](int tiles) { return tiles <= a.whole ? min(tiles, 1) : (tiles + c - 1) / c; };
@@ -370,7 +374,7 @@ __device__ __forceinline__ bool plan(const PagedArgs& a, int g, SeqChunk& r) {
       while (__builtin_amdgcn_readlane(wave_scan(chunks_of(w[0].tiles)), 63) > a.round) c += (c + 7) / 8;
   }
   int before = 0, slots = 0;
-  auto find = [&](const SeqWork& w, bool bad, int s0) {
+  auto find = [&](const SeqWork& w, int s0) {
     const int n = chunks_of(w.tiles), incl = wave_scan(n), m = n > 1 ? n : 0, sincl = wave_scan(m);
     const unsigned long long hit = __ballot(before + incl > g);
     if (!hit) {
@@ -387,16 +391,14 @@ __device__ __forceinline__ bool plan(const PagedArgs& a, int g, SeqChunk& r) {
     r.n = __builtin_amdgcn_readlane(n, l);
     r.chunk = g - before - __builtin_amdgcn_readlane(incl - n, l);
     r.slot = slots + __builtin_amdgcn_readlane(sincl - m, l);
-    r.bad = __builtin_amdgcn_readlane((int)bad, l);
     return true;
   };
 #pragma unroll
   for (int k = 0; k < kSeqs; k++)
-    if (64 * k < a.seqs && find(w[k], bad[k], 64 * k)) return true;
+    if (64 * k < a.seqs && find(w[k], 64 * k)) return true;
   for (int s0 = 64 * kSeqs; s0 < a.seqs; s0 += 64) {
-    b = false;
     const SeqWork v = s0 + lane < a.seqs ? seq_work<SHIFT>(a, s0 + lane, &b) : none;
-    if (find(v, b, s0)) return true;
+    if (find(v, s0)) return true;
   }
   return false;
 }
@@ -422,7 +424,6 @@ __global__ __launch_bounds__(64 * W, NT == 1 ? (DT <= 64 ? 4 : 2) : 1) void page
   SeqChunk sc;
   if (!plan<T::SHIFT>(a, g, sc)) return;
   const int ci = sc.chunk, tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  if (sc.bad && ci == 0 && unit == 0 && tid == 0) paged_flag(a.status, kPagedStatusRows);
   const int R = sc.w.rows * a.G;  // rows of the kv head
   if (r0 >= R) return;
   const int i16 = lane & 15, qd = lane >> 4;
