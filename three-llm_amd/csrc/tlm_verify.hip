@@ -164,8 +164,8 @@ __device__ __forceinline__ void load_chunk(const float* x, int i0, int n, vf4* v
 }
 
 struct VerifyShared {
-  double red[kVW], s[kVerifyMaxTokens], sq[kVerifyMaxTokens], wx[kVerifyMaxTokens];
-  float m[kVerifyMaxTokens], mq[kVerifyMaxTokens];
+  double red[kVW], s[kVerifyMaxTokens], sq[kVerifyMaxTokens];
+  float m[kVerifyMaxTokens], mq[kVerifyMaxTokens], lx[kVerifyMaxTokens];
   int ok[kVerifyMaxTokens], top[kVerifyMaxTokens], x[kVerifyMaxTokens], hit[kVW], last[kVW];
   unsigned long long done;
   unsigned before;
@@ -176,13 +176,13 @@ struct VerifyShared {
 // A row's chunks in a wave's registers: chunk lane + 64 k.
 struct RowSums {
   float max[kVRow];
-  double sum[kVRow];  // row_load: relative to max; row_scale: to the row's maximum
+  double raw[kVRow], sum[kVRow];  // relative to max; to the row's maximum
 };
 __device__ __forceinline__ void row_load(const VerifyArgs& a, const VerifyWork& w, size_t row, RowSums& r) {
 #pragma unroll
   for (int k = 0; k < kVRow; k++) {
     const int c = (threadIdx.x & 63) + 64 * k;
-    r.sum[k] = c < a.chunks ? __longlong_as_double((long long)published(w.cell + row * a.chunks + c)) : 0.0;
+    r.raw[k] = c < a.chunks ? __longlong_as_double((long long)published(w.cell + row * a.chunks + c)) : 0.0;
     r.max[k] = c < a.chunks ? published(w.max + row * a.chunks + c) : -INFINITY;
   }
 }
@@ -196,7 +196,7 @@ __device__ __forceinline__ void row_scale(const VerifyArgs& a, RowSums& r, float
   double sum = 0.0;
 #pragma unroll
   for (int k = 0; k < kVRow; k++) {
-    if (64 * k < a.chunks) r.sum[k] = r.sum[k] > 0.0 ? r.sum[k] * w.of(r.max[k]) : 0.0;
+    r.sum[k] = 64 * k < a.chunks && r.raw[k] > 0.0 ? r.raw[k] * w.of(r.max[k]) : 0.0;
     sum += r.sum[k];
   }
   *m = mx;
@@ -341,10 +341,10 @@ __device__ void decide(const VerifyArgs& a, int s, VerifyShared& sh) {
     double sum, sq = 0.0;
     row_scale(a, rp, &m, &sum);
     if (model) row_scale(a, rq, &mq, &sq);
-    const double wx = Weights(m, a.scale).of(lx), p = sum > 0.0 ? wx / sum : 0.0;
+    const double p = sum > 0.0 ? Weights(m, a.scale).of(lx) / sum : 0.0;
     const double q = !model ? 1.0 : sq > 0.0 ? Weights(mq, a.scale).of(qx) / sq : 0.0;
     if (lane == 0) {
-      sh.m[j] = m, sh.s[j] = sum, sh.mq[j] = mq, sh.sq[j] = sq, sh.wx[j] = wx;
+      sh.m[j] = m, sh.s[j] = sum, sh.mq[j] = mq, sh.sq[j] = sq, sh.lx[j] = lx;
       sh.ok[j] = x >= 0 && (double)u * q < p;
     }
   }
@@ -384,16 +384,20 @@ __device__ void decide(const VerifyArgs& a, int s, VerifyShared& sh) {
       bool much = false;
 #pragma unroll
       for (int k = 0; k < kVRow; k++) {
-        const bool here = x >= 0 && lane + 64 * k == x / kVChunk;
-        v[k] = here ? rp.sum[k] - sh.wx[taken] : rp.sum[k];
-        much |= here && !(sh.wx[taken] <= 0.5 * rp.sum[k]);
+        v[k] = rp.sum[k];
+        if (x >= 0 && lane + 64 * k == x / kVChunk) {  // less the draft's term, as it was added
+          const Weights c(rp.max[k], a.scale);
+          const double left = rp.raw[k] - (c.plain ? c.series(sh.lx[taken]) : c.of(sh.lx[taken]));
+          much = !(left >= rp.raw[k] * 0x1p-16);
+          v[k] = left * of.of(rp.max[k]);
+        }
       }
       const bool again = __ballot(much) != 0;
       if (!again) find_chunk(v, u, sh);
       if (lane == 0) sh.again = again;
     }
     __syncthreads();
-    if (sh.again) {  // a difference would lose what is left beside a likely draft: its chunk's sum without it
+    if (sh.again) {  // the difference has lost what is left beside a likely draft: its chunk's sum without it
       double y[4];
       at(x / kVChunk * kVChunk + 4 * tid, y);
       const double without = block_sum_f64((y[0] + y[1]) + (y[2] + y[3]), sh);
@@ -544,9 +548,11 @@ __global__ __launch_bounds__(kVT, 4) void verify_kernel(VerifyArgs a) {
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's results are performed
   __syncthreads();                                  // and every wave's
-  walk.group(a, 0);
-  walk.before = 0;
-  walk.seek(a, c0 / a.chunks);
+  if (a.seqs > 64) {
+    walk.group(a, 0);
+    walk.before = 0;
+    walk.seek(a, c0 / a.chunks);
+  }
   while (true) {  // 64 sequences at a time
     if (wave == 0) {
       const int s = walk.s0 + lane, end = (walk.before + walk.incl) * a.chunks, all = walk.rows * a.chunks;
