@@ -182,8 +182,8 @@ typedef struct tlm_paged_desc {
 
 /* One step's rows.  Sequence s has `tokens` rows, of which the first counts[s]
  * are there (counts NULL: all), at the positions starts[s], starts[s] + 1, ...
- * A sequence with starts[s] < 0 or counts[s] < 1 is idle.  Rows that are not
- * there are neither read nor written: what the outputs hold for them stays.
+ * A sequence with starts[s] < 0 or counts[s] < 1 is idle.  What rows
+ * that are not there hold does not matter, and what the outputs hold for them stays.
  * Position p lies in page tables[s][p / page_tokens]; only the entries of
  * pages that hold a position in use are read (a window's earlier pages may be
  * given back, their entries anything).  Sequences may share pages that they
@@ -258,8 +258,9 @@ int tlm_op_topk(tlm_ctx* ctx, const float* logits, int n, int k, double softcap,
  * Entries at or below LOWEST_FLOAT (-inf, NaN included) never take part; a draft
  * outside the vocabulary never stands; a row without entries gives -1.
  * accepted: [seqs] drafts that stand; out_tokens: [seqs][tokens] those, the token
- * after them, then -1.  tokens <= 64, vocab <= 524288; 12 bytes for every 2048 entries of a row fit the
- * context's 32 MiB (TLM_ERR_RANGE otherwise).  Enqueue only. */
+ * after them, then -1; both apart from the inputs.  tokens <= 64, vocab <= 524288;
+ * 12 bytes for every 2048 entries of 4096 sequences' rows fit the context's 32 MiB
+ * (TLM_ERR_RANGE otherwise).  Enqueue only. */
 int tlm_op_verify_drafts(tlm_ctx* ctx, const float* logits, const float* draft_logits, const int32_t* drafts,
                          const int32_t* counts, const float* uniforms, int32_t seqs, int32_t tokens, int32_t vocab,
                          double temperature, int32_t* accepted, int32_t* out_tokens);

@@ -508,7 +508,28 @@ def test_refusals(ctx):
     refuse(tlm.TLM_ERR_INVALID, sv.paged.attention, b, q, out, tlm.FMT_Q4)
     with pytest.raises(tlm.TlmError):
         tlm.Paged(ctx, 4, 2, 48, 100)
+    for small in (dict(k_pages=sv.kb, num_pages=sv.pages + 1), dict(tables=ctx.buffer(4), table_width=2),
+                  dict(starts=ctx.buffer(4), seqs=2), dict(counts=ctx.buffer(4), seqs=2)):
+        whole = dict(k_pages=sv.kb, v_pages=sv.vb, num_pages=sv.pages, tables=ctx.buffer(64), table_width=1,
+                     starts=ctx.buffer(64), seqs=1)
+        refuse(tlm.TLM_ERR_INVALID, lambda: sv.paged.batch(**{**whole, **small}))
     sv.paged.append(b, x, q)
+    sv.paged.status()
+    sv.close()
+
+
+def test_calls_allocate_nothing(ctx):
+    sv = Serving(ctx, 8, 2, 64, [5000, 90, -1], 4, 32)
+    sv.upload(*sv.pools([5004, 94, 0]))
+    x, q = ctx.array(np.ones((3, 4, 12, 64), np.float32)), ctx.buffer(4 * 3 * 4 * 8 * 64)
+    out = ctx.buffer(2 * 3 * 4 * 8 * 64)
+    free = None
+    for i in range(30):
+        sv.paged.append(sv.batch, x, q)
+        sv.paged.attention(sv.batch, q, out)
+        ctx.sync()
+        free = ctx.memory()[0] if i == 9 else free
+    assert ctx.memory()[0] == free
     sv.paged.status()
     sv.close()
 

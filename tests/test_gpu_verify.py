@@ -181,6 +181,8 @@ def test_refusals(ctx):
     refuse(tlm.TLM_ERR_INVALID, b, 1, 0, 10, b, b, uniforms=b)
     refuse(tlm.TLM_ERR_INVALID, b, 1, 1, 0, b, b, uniforms=b)
     refuse(tlm.TLM_ERR_INVALID, b, 1, 65, 2, b, b, drafts=b, uniforms=b)
+    refuse(tlm.TLM_ERR_INVALID, b, 1, 1, 524289, b, b, uniforms=b)
+    refuse(tlm.TLM_ERR_RANGE, b, 4096, 64, 524288, b, b, drafts=b, uniforms=b)  # the workspace
     refuse(tlm.TLM_ERR_INVALID, b, 1, 2, 10, b, b, uniforms=b)
     refuse(tlm.TLM_ERR_INVALID, b, 1, 2, 10, b, b, drafts=b)
     for temp in (-0.5, float("nan"), float("inf")):

@@ -427,6 +427,12 @@ class Paged:
     def batch(self, k_pages: Buffer, v_pages: Buffer, num_pages: int, tables: Buffer, table_width: int, starts: Buffer,
               seqs: int, tokens: int = 1, counts: Optional[Buffer] = None) -> PagedBatch:
         """One step's rows: tables int32 [seqs][table_width], starts (and counts) int32 [seqs]."""
+        pool = num_pages * self.page_bytes()
+        for name, b, need in (("k_pages", k_pages, pool), ("v_pages", v_pages, pool),
+                              ("tables", tables, 4 * seqs * table_width), ("starts", starts, 4 * seqs),
+                              ("counts", counts, 4 * seqs)):
+            if getattr(b, "nbytes", need) < need:  # the kernels read that much
+                raise TlmError(TLM_ERR_INVALID, f"TLMPaged: {name} holds {b.nbytes} bytes of {need}")
         b = PagedBatch(k_pages.ptr, v_pages.ptr, tables.ptr, starts.ptr, _addr(counts), num_pages, table_width, seqs,
                        tokens)
         b.keep = (k_pages, v_pages, tables, starts, counts)
