@@ -275,10 +275,12 @@ __global__ __launch_bounds__(256) void paged_append_group_kernel(PagedArgs a, in
 
 typedef _Float16 ph8_t __attribute__((ext_vector_type(8)));
 // Attention of the rows of a step.  A kv head's rows r = j G + g (token j, head g
-// of its group) are the columns of 16-column matrix-core tiles, so that K and V
-// are read once for all of them; a block holds NT of those tiles (`a.groups` row
-// groups of 16 NT cover tokens x G).  Its W waves take the position tiles of one
-// chunk of the sequence in turn:
+// of its group) are the columns of 16-column matrix-core tiles, so that K and V are
+// read once for 16 of them; a block has one column tile (a unit is a kv head and a
+// row group).  Several tiles a block were slower everywhere, as their outputs leave
+// room for fewer waves (16 x 16 Llama-3.2-3B at 2000 positions 31.9 us with four, 22.9 so;
+// Qwen2.5-0.5B 16 x 5 20.5 and 10.3; a 2048-token prompt of Llama-3.2-1B 112 and 69).  The W
+// waves take the position tiles of one chunk of the sequence in turn:
 //   * scores S^T (positions x rows) = K Q^T, K the A operand, q the B operand;
 //   * softmax with a running maximum and sum per row, base 2;
 //   * O^T (dims x rows) += V^T P^T, V^T the A operand, P^T from the score registers.
@@ -403,23 +405,22 @@ __device__ __forceinline__ bool plan(const PagedArgs& a, int g, SeqChunk& r) {
   return false;
 }
 
-// Partial results: per slot, unit (kv head and row group) and row the unscaled
-// output, then per row (maximum in base 2, sum).
-__device__ __forceinline__ float* part_row(const PagedArgs& a, int slot, int unit, int row, int rows, int DT) {
-  return a.part + (((size_t)slot * a.units + unit) * rows + row) * (DT + 2);
+// Partial results: per slot, unit (kv head and row group) and row of its 16 the
+// unscaled output, then the maximum in base 2 and the sum.
+__device__ __forceinline__ float* part_row(const PagedArgs& a, int slot, int unit, int row, int DT) {
+  return a.part + (((size_t)slot * a.units + unit) * 16 + row) * (DT + 2);
 }
 
-template <typename KT, int DT, int NT, int W, bool STREAM>
-__global__ __launch_bounds__(64 * W, NT == 1 ? (DT <= 64 ? 4 : 2) : 1) void paged_attention_kernel(PagedArgs a) {
+template <typename KT, int DT, int W, bool STREAM>
+__global__ __launch_bounds__(64 * W, DT <= 64 ? 4 : 2) void paged_attention_kernel(PagedArgs a) {
   using T = PagedTile<KT>;
   constexpr int SUB = T::SUB, TS = T::TS, NF = DT / 16;  // 1 KB operand pieces of a tile's K, of its V
-  constexpr bool F16 = sizeof(KT) == 2, QREG = NT == 1;
+  constexpr bool F16 = sizeof(KT) == 2;
   constexpr int RS = DT + 2;  // floats of a row's record: maximum, sum, output
-  constexpr int QB = QREG ? 0 : NT * (NF * 256 + 16), MB = W * 16 * RS;  // floats
-  constexpr int LDSF = QB > MB ? QB : MB;
+  constexpr int LDSF = W * 16 * RS;
   __shared__ __align__(16) float lds[LDSF];
   // the row groups from the last one on: a prompt's last rows attend to the most
-  const int unit = blockIdx.x % a.units, hk = unit % a.Hkv, r0 = (a.units - 1 - unit) / a.Hkv * 16 * NT;
+  const int unit = blockIdx.x % a.units, hk = unit % a.Hkv, r0 = (a.units - 1 - unit) / a.Hkv * 16;
   const int g = blockIdx.x / a.units;
   SeqChunk sc;
   if (!plan<T::SHIFT>(a, g, sc)) return;
@@ -428,7 +429,7 @@ __global__ __launch_bounds__(64 * W, NT == 1 ? (DT <= 64 ? 4 : 2) : 1) void page
   if (r0 >= R) return;
   const int i16 = lane & 15, qd = lane >> 4;
   // positions that some row of the block attends to, and that all do
-  const int ja = r0 / a.G, jb = (min(r0 + 16 * NT, R) - 1) / a.G, start = sc.w.start;
+  const int ja = r0 / a.G, jb = (min(r0 + 16, R) - 1) / a.G, start = sc.w.start;
   const int lo_any = a.window > 0 ? max(0, start + ja - a.window + 1) : 0, hi_any = start + jb;
   const int lo_all = a.window > 0 ? max(0, start + jb - a.window + 1) : 0, hi_all = start + ja;
   const int per = (sc.w.tiles + sc.n - 1) / sc.n;
@@ -459,58 +460,17 @@ __global__ __launch_bounds__(64 * W, NT == 1 ? (DT <= 64 ? 4 : 2) : 1) void page
   auto page_of = [&](int i) { return __builtin_amdgcn_readlane(page, min(i, n - 1)); };
   auto load_k = [&](Tile& x, int i) { load(x.k, a.kc, tb + min(i, n - 1) * W, page_of(i)); };
   auto load_v = [&](Tile& x, int i) { load(x.v, a.vc, tb + min(i, n - 1) * W, page_of(i)); };
-  // this lane's rows (a column of each row tile): their positions' bounds, and q scaled
-  // by a power of two per row to at most 1.  q is requested before the first tile:
-  // loads return in order.  With more row tiles than one a wave prepares some of
-  // them, and all take them from LDS.
-  int lo[NT], hi[NT];
-  float mult[NT];
-  u32x4 qreg[QREG ? NF : 1];
-  u32x4* const qlds = reinterpret_cast<u32x4*>(lds);  // [NT][NF][64]
-  float* const mlds = lds + NT * NF * 256;            // [NT][16]
-  const float qscale = a.scale * 1.4426950408889634f;  // log2 e: the softmax runs in base 2
+  // This lane's row (its column of the tiles): its positions' bounds, and q scaled by
+  // a power of two to at most 1.  q is requested before the first tile: loads return
+  // in order.
+  const int row = r0 + i16, rc = min(row, R - 1), hi = start + rc / a.G;
+  const int lo = a.window > 0 ? hi - a.window + 1 : 0;
+  u32x4 qreg[NF];
   f32x4 qx[NF];
-  auto load_q = [&](int nt) {
-    const int r = min(r0 + 16 * nt + i16, R - 1);
-    const float* q = a.x + (((size_t)sc.s * a.tokens + r / a.G) * a.Hq + hk * a.G + r % a.G) * DT;
+  const float* const q = a.x + (((size_t)sc.s * a.tokens + rc / a.G) * a.Hq + hk * a.G + rc % a.G) * DT;
 #pragma unroll
-    for (int f = 0; f < NF; f++)  // fp16: dims 32 (f / 2) + 8 qd + 4 (f % 2) ..; fp32: 16 f + 4 qd ..
-      qx[f] = *(const TLM_GLOBAL f32x4u*)(q + (F16 ? 32 * (f / 2) + 8 * qd + 4 * (f & 1) : 16 * f + 4 * qd));
-  };
-  auto prepare_q = [&](int nt, u32x4* to, int stride) {  // the row's multiplier
-    float m = 0.f;
-#pragma unroll
-    for (int f = 0; f < NF; f++)
-#pragma unroll
-      for (int e = 0; e < 4; e++) m = fmaxf(m, fabsf(qx[f][e]));
-    m = fmaxf(m, lane_swap16(m));
-    m = fmaxf(m, lane_swap32(m));
-    const int ex = max(-120, min(120, __builtin_amdgcn_frexp_expf(m)));
-    const bool row = r0 + 16 * nt + i16 < R;
-#pragma unroll
-    for (int f = 0; f < NF; f++)
-#pragma unroll
-      for (int e = 0; e < 4; e++) qx[f][e] = row ? ldexpf(qx[f][e], -ex) : 0.f;
-    if (F16) {
-#pragma unroll
-      for (int jj = 0; jj < NF / 2; jj++) {
-        ph8_t h, l;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const float v = qx[2 * jj + e / 4][e & 3];
-          h[e] = (_Float16)v;
-          l[e] = (_Float16)(v - (float)h[e]);
-        }
-        to[2 * jj * stride] = __builtin_bit_cast(u32x4, h);
-        to[(2 * jj + 1) * stride] = __builtin_bit_cast(u32x4, l);
-      }
-    } else {
-#pragma unroll
-      for (int f = 0; f < NF; f++) to[f * stride] = __builtin_bit_cast(u32x4, qx[f]);
-    }
-    return ldexpf(qscale, ex);
-  };
-  if (QREG || w < NT) load_q(QREG ? 0 : w);
+  for (int f = 0; f < NF; f++)  // fp16: dims 32 (f / 2) + 8 qd + 4 (f % 2) ..; fp32: 16 f + 4 qd ..
+    qx[f] = *(const TLM_GLOBAL f32x4u*)(q + (F16 ? 32 * (f / 2) + 8 * qd + 4 * (f & 1) : 16 * f + 4 * qd));
   __builtin_amdgcn_sched_barrier(0);
   Tile x;
   if (tb < t1) {
@@ -519,34 +479,40 @@ __global__ __launch_bounds__(64 * W, NT == 1 ? (DT <= 64 ? 4 : 2) : 1) void page
     load_v(x, 0);
   }
   __builtin_amdgcn_sched_barrier(0);
+  float qmax = 0.f;
 #pragma unroll
-  for (int nt = 0; nt < NT; nt++) {
-    const int pos = start + min(r0 + 16 * nt + i16, R - 1) / a.G;
-    lo[nt] = a.window > 0 ? pos - a.window + 1 : 0;
-    hi[nt] = pos;
-  }
-  if constexpr (QREG) {
-    mult[0] = prepare_q(0, qreg, 1);
-  } else {
-    static_assert(NT <= W, "a wave per row tile");
-    if (w < NT) {
-      const float m = prepare_q(w, qlds + w * NF * 64 + lane, 64);
-      if (qd == 0) mlds[w * 16 + i16] = m;
+  for (int f = 0; f < NF; f++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) qmax = fmaxf(qmax, fabsf(qx[f][e]));
+  qmax = fmaxf(qmax, lane_swap16(qmax));
+  qmax = fmaxf(qmax, lane_swap32(qmax));
+  const int ex = max(-120, min(120, __builtin_amdgcn_frexp_expf(qmax)));
+#pragma unroll
+  for (int f = 0; f < NF; f++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) qx[f][e] = row < R ? ldexpf(qx[f][e], -ex) : 0.f;
+  const float mult = ldexpf(a.scale * 1.4426950408889634f, ex);  // log2 e: the softmax runs in base 2
+#pragma unroll
+  for (int f = 0; f < NF; f++) {
+    if (!F16) {
+      qreg[f] = __builtin_bit_cast(u32x4, qx[f]);
+    } else if (f % 2 == 0) {  // dims of one slab of 32: the high parts, then the low ones
+      ph8_t h, l;
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const float v = qx[f + e / 4][e & 3];
+        h[e] = (_Float16)v;
+        l[e] = (_Float16)(v - (float)h[e]);
+      }
+      qreg[f] = __builtin_bit_cast(u32x4, h);
+      qreg[f + 1] = __builtin_bit_cast(u32x4, l);
     }
-    lds_barrier();
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) mult[nt] = mlds[nt * 16 + i16];
   }
 
-  f32x4 o[NT][NF];
-  float mrun[NT], lrun[NT];  // running maximum, this lane's share of the sum
+  f32x4 o[NF];
+  float mrun = -FLT_MAX, lrun = 0.f;  // running maximum, this lane's share of the sum
 #pragma unroll
-  for (int nt = 0; nt < NT; nt++) {
-    mrun[nt] = -FLT_MAX;
-    lrun[nt] = 0.f;
-#pragma unroll
-    for (int f = 0; f < NF; f++) o[nt][f] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  }
+  for (int f = 0; f < NF; f++) o[f] = (f32x4){0.f, 0.f, 0.f, 0.f};
 
   // V with positions outside [first, last] taken out (0 times what they hold may be NaN)
   auto keep = [&](const u32x4& v, int p, int first, int last) {
@@ -568,7 +534,6 @@ __global__ __launch_bounds__(64 * W, NT == 1 ? (DT <= 64 ? 4 : 2) : 1) void page
   };
   // tile t; k_read() and v_read() run once x.k and x.v have been read
   auto process = [&](Tile& x, int t, auto k_read, auto v_read) {
-    if (!QREG) asm volatile("" ::: "memory");  // q is read again, not kept in registers that o needs
     const int p = t << T::SHIFT;
     const bool edge = p < lo_all || p + TS - 1 > hi_all;  // some row does not see all of it (wave-uniform)
     bool apart = false;
@@ -583,87 +548,82 @@ __global__ __launch_bounds__(64 * W, NT == 1 ? (DT <= 64 ? 4 : 2) : 1) void page
       }
       apart = ja != jb && __ballot(nf != 0) != 0;
     }
-    u32x4 ph[NT], pl[F16 ? NT : 1];
+    f32x4 acc[2] = {(f32x4){0.f, 0.f, 0.f, 0.f}, (f32x4){0.f, 0.f, 0.f, 0.f}};
+    if (F16) {
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-      f32x4 acc[2] = {(f32x4){0.f, 0.f, 0.f, 0.f}, (f32x4){0.f, 0.f, 0.f, 0.f}};
-      if (F16) {
+      for (int jj = 0; jj < NF / 2; jj++) {
+        const ph8_t qh = __builtin_bit_cast(ph8_t, qreg[2 * jj]), ql = __builtin_bit_cast(ph8_t, qreg[2 * jj + 1]);
 #pragma unroll
-        for (int jj = 0; jj < NF / 2; jj++) {
-          const ph8_t qh = __builtin_bit_cast(ph8_t, QREG ? qreg[QREG ? 2 * jj : 0] : qlds[(nt * NF + 2 * jj) * 64 + lane]);
-          const ph8_t ql = __builtin_bit_cast(ph8_t, QREG ? qreg[QREG ? 2 * jj + 1 : 0] : qlds[(nt * NF + 2 * jj + 1) * 64 + lane]);
-#pragma unroll
-          for (int st = 0; st < SUB; st++) {
-            const ph8_t k = __builtin_bit_cast(ph8_t, x.k[st * (NF / SUB) + jj]);
-            acc[st] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh, acc[st], 0, 0, 0);
-            acc[st] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql, acc[st], 0, 0, 0);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int f = 0; f < NF; f++) {
-          const f32x4 q = __builtin_bit_cast(f32x4, QREG ? qreg[QREG ? f : 0] : qlds[(nt * NF + f) * 64 + lane]);
-          const f32x4 k = __builtin_bit_cast(f32x4, x.k[f]);
-#pragma unroll
-          for (int e = 0; e < 4; e++) acc[e & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[e], q[e], acc[e & 1], 0, 0, 0);
-        }
-        acc[0] += acc[1];
-      }
-      // lane (row i16, qd): positions p + 16 st + 4 qd + e
-      float sv[4 * SUB];
-#pragma unroll
-      for (int st = 0; st < SUB; st++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) sv[4 * st + e] = acc[st][e] * mult[nt];
-      if (edge) {
-#pragma unroll
-        for (int i = 0; i < 4 * SUB; i++) {
-          const int y = p + 16 * (i / 4) + 4 * qd + (i & 3);
-          if (y < lo[nt] || y > hi[nt]) sv[i] = -INFINITY;
+        for (int st = 0; st < SUB; st++) {
+          const ph8_t k = __builtin_bit_cast(ph8_t, x.k[st * (NF / SUB) + jj]);
+          acc[st] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh, acc[st], 0, 0, 0);
+          acc[st] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql, acc[st], 0, 0, 0);
         }
       }
-      float mx = sv[0];
+    } else {
 #pragma unroll
-      for (int i = 1; i < 4 * SUB; i++) mx = fmaxf(mx, sv[i]);
-      mx = fmaxf(mx, lane_swap16(mx));
-      mx = fmaxf(mx, lane_swap32(mx));
-      const float mn = fmaxf(mrun[nt], mx);  // finite: it starts at -FLT_MAX
-      const float corr = __builtin_amdgcn_exp2f(mrun[nt] - mn);
-      float ps = 0.f;
-      if (F16) {
-        ph8_t h, l;
+      for (int f = 0; f < NF; f++) {
+        const f32x4 qf = __builtin_bit_cast(f32x4, qreg[f]), k = __builtin_bit_cast(f32x4, x.k[f]);
 #pragma unroll
-        for (int i = 0; i < 4 * SUB; i++) {
-          const float v = __builtin_amdgcn_exp2f(sv[i] - mn);
-          ps += v;
-          h[i % 8] = (_Float16)v;
-          l[i % 8] = (_Float16)(v - (float)h[i % 8]);
-        }
-        ph[nt] = __builtin_bit_cast(u32x4, h);
-        pl[F16 ? nt : 0] = __builtin_bit_cast(u32x4, l);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const float v = __builtin_amdgcn_exp2f(sv[i] - mn);
-          ps += v;
-          ph[nt][i] = __float_as_uint(v);
-        }
+        for (int e = 0; e < 4; e++) acc[e & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[e], qf[e], acc[e & 1], 0, 0, 0);
       }
-      lrun[nt] = fmaf(lrun[nt], corr, ps);
-      mrun[nt] = mn;
-      if (__ballot(corr != 1.f)) {
+      acc[0] += acc[1];
+    }
+    // lane (row i16, qd): positions p + 16 st + 4 qd + e
+    float sv[4 * SUB];
 #pragma unroll
-        for (int f = 0; f < NF; f++) o[nt][f] *= corr;
+    for (int st = 0; st < SUB; st++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) sv[4 * st + e] = acc[st][e] * mult;
+    if (edge) {
+#pragma unroll
+      for (int i = 0; i < 4 * SUB; i++) {
+        const int y = p + 16 * (i / 4) + 4 * qd + (i & 3);
+        if (y < lo || y > hi) sv[i] = -INFINITY;
       }
     }
+    float mx = sv[0];
+#pragma unroll
+    for (int i = 1; i < 4 * SUB; i++) mx = fmaxf(mx, sv[i]);
+    mx = fmaxf(mx, lane_swap16(mx));
+    mx = fmaxf(mx, lane_swap32(mx));
+    const float mn = fmaxf(mrun, mx);  // finite: it starts at -FLT_MAX
+    const float corr = __builtin_amdgcn_exp2f(mrun - mn);
+    float ps = 0.f;
+    u32x4 ph, pl;  // fp16: high and low parts
+    if (F16) {
+      ph8_t h, l;
+#pragma unroll
+      for (int i = 0; i < 4 * SUB; i++) {
+        const float v = __builtin_amdgcn_exp2f(sv[i] - mn);
+        ps += v;
+        h[i % 8] = (_Float16)v;
+        l[i % 8] = (_Float16)(v - (float)h[i % 8]);
+      }
+      ph = __builtin_bit_cast(u32x4, h);
+      pl = __builtin_bit_cast(u32x4, l);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float v = __builtin_amdgcn_exp2f(sv[i] - mn);
+        ps += v;
+        ph[i] = __float_as_uint(v);
+      }
+    }
+    lrun = fmaf(lrun, corr, ps);
+    mrun = mn;
+    if (__ballot(corr != 1.f)) {
+#pragma unroll
+      for (int f = 0; f < NF; f++) o[f] *= corr;
+    }
     k_read();
-    auto weigh = [&](const u32x4& v, int nt, f32x4 y) -> f32x4 {
+    auto weigh = [&](const u32x4& v, f32x4 y) -> f32x4 {
       if (F16) {
         const ph8_t vh = __builtin_bit_cast(ph8_t, v);
-        y = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, __builtin_bit_cast(ph8_t, ph[nt]), y, 0, 0, 0);
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, __builtin_bit_cast(ph8_t, pl[F16 ? nt : 0]), y, 0, 0, 0);
+        y = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, __builtin_bit_cast(ph8_t, ph), y, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, __builtin_bit_cast(ph8_t, pl), y, 0, 0, 0);
       }
-      const f32x4 vf = __builtin_bit_cast(f32x4, v), pf = __builtin_bit_cast(f32x4, ph[nt]);
+      const f32x4 vf = __builtin_bit_cast(f32x4, v), pf = __builtin_bit_cast(f32x4, ph);
 #pragma unroll
       for (int e = 0; e < 4; e++) y = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[e], pf[e], y, 0, 0, 0);
       return y;
@@ -680,19 +640,14 @@ __global__ __launch_bounds__(64 * W, NT == 1 ? (DT <= 64 ? 4 : 2) : 1) void page
           one[d] = F16 ? (t >> 15) * 0x3C00u : (t >> 31) * 0x3F800000u;
           x.v[f][d] &= ~(F16 ? (t >> 15) * 0xFFFFu : (t >> 31) * 0xFFFFFFFFu);
         }
+        const f32x4 y = weigh(one, (f32x4){0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-          const f32x4 y = weigh(one, nt, (f32x4){0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-          for (int e = 0; e < 4; e++)
-            if (y[e] > 0.f) o[nt][f][e] = __uint_as_float(0x7FC00000u);
-        }
+        for (int e = 0; e < 4; e++)
+          if (y[e] > 0.f) o[f][e] = __uint_as_float(0x7FC00000u);
       }
     }
 #pragma unroll
-    for (int f = 0; f < NF; f++)
-#pragma unroll
-      for (int nt = 0; nt < NT; nt++) o[nt][f] = weigh(x.v[f], nt, o[nt][f]);
+    for (int f = 0; f < NF; f++) o[f] = weigh(x.v[f], o[f]);
     v_read();
   };
 
@@ -717,7 +672,7 @@ __global__ __launch_bounds__(64 * W, NT == 1 ? (DT <= 64 ? 4 : 2) : 1) void page
     }
   }
 
-  // the waves' results, 16 rows at a time, through LDS
+  // the waves' results joined through LDS
   const bool whole = sc.n == 1;
   auto put = [&](int r, int d, float y0, float y1) {  // dims d and d + 1 of row r
     const size_t at = (((size_t)sc.s * a.tokens + r / a.G) * a.Hq + hk * a.G + r % a.G) * DT + d;
@@ -729,41 +684,35 @@ __global__ __launch_bounds__(64 * W, NT == 1 ? (DT <= 64 ? 4 : 2) : 1) void page
       static_cast<uint16_t*>(a.out)[at + 1] = kv_store<uint16_t>(y1);
     }
   };
+  lrun += lane_swap16(lrun);
+  lrun += lane_swap32(lrun);
+  float* const rec = lds + (w * 16 + i16) * RS;
 #pragma unroll
-  for (int nt = 0; nt < NT; nt++) {
-    float l = lrun[nt];
-    l += lane_swap16(l);
-    l += lane_swap32(l);
-    if (r0 + 16 * nt >= R) break;  // block-uniform
-    __syncthreads();
-    float* rec = lds + (w * 16 + i16) * RS;
+  for (int f = 0; f < NF; f++)
 #pragma unroll
-    for (int f = 0; f < NF; f++)
+    for (int e = 0; e < 4; e++) rec[2 + 16 * f + 4 * qd + e] = o[f][e];
+  if (qd == 0) rec[0] = mrun, rec[1] = lrun;
+  __syncthreads();
+  const int rows = min(16, R - r0);
+  for (int e = tid; e < rows * (DT / 2); e += 64 * W) {
+    const int i = e / (DT / 2), d = 2 * (e % (DT / 2));
+    float M = -FLT_MAX, L = 0.f, O0 = 0.f, O1 = 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; e++) rec[2 + 16 * f + 4 * qd + e] = o[nt][f][e];
-    if (qd == 0) rec[0] = mrun[nt], rec[1] = l;
-    __syncthreads();
-    for (int e = tid; e < 8 * DT; e += 64 * W) {
-      const int row = e / (DT / 2), d = 2 * (e % (DT / 2)), r = r0 + 16 * nt + row;
-      if (r >= R) break;
-      float M = -FLT_MAX, L = 0.f, O0 = 0.f, O1 = 0.f;
+    for (int x = 0; x < W; x++) M = fmaxf(M, lds[(x * 16 + i) * RS]);
 #pragma unroll
-      for (int x = 0; x < W; x++) M = fmaxf(M, lds[(x * 16 + row) * RS]);
-#pragma unroll
-      for (int x = 0; x < W; x++) {
-        const float* y = lds + (x * 16 + row) * RS;
-        const float f = __builtin_amdgcn_exp2f(y[0] - M);
-        L = fmaf(y[1], f, L);
-        O0 = fmaf(y[2 + d], f, O0);
-        O1 = fmaf(y[3 + d], f, O1);
-      }
-      if (whole) {
-        put(r, d, L == 0.f ? 0.f : O0 / L, L == 0.f ? 0.f : O1 / L);  // 0: no position has a page
-      } else {
-        float* p = part_row(a, sc.slot + ci, unit, 16 * nt + row, 16 * NT, DT);
-        publish2(p + d, O0, O1);
-        if (d == 0) publish2(p + DT, M, L);
-      }
+    for (int x = 0; x < W; x++) {
+      const float* y = lds + (x * 16 + i) * RS;
+      const float f = __builtin_amdgcn_exp2f(y[0] - M);
+      L = fmaf(y[1], f, L);
+      O0 = fmaf(y[2 + d], f, O0);
+      O1 = fmaf(y[3 + d], f, O1);
+    }
+    if (whole) {
+      put(r0 + i, d, L == 0.f ? 0.f : O0 / L, L == 0.f ? 0.f : O1 / L);  // 0: no position has a page
+    } else {
+      float* p = part_row(a, sc.slot + ci, unit, i, DT);
+      publish2(p + d, O0, O1);
+      if (d == 0) publish2(p + DT, M, L);
     }
   }
   if (whole) return;
@@ -781,19 +730,19 @@ __global__ __launch_bounds__(64 * W, NT == 1 ? (DT <= 64 ? 4 : 2) : 1) void page
   // A thread per row and four dims, the chunks in `groups` where there are threads for
   // it; four chunks' values in flight at a time.
   constexpr int TH = 64 * W, P = DT / 4;
-  const int rows = min(16 * NT, R - r0), items = rows * P, groups = max(1, min(TH, LDSF / 6) / items);
-  const size_t step = (size_t)a.units * 16 * NT * RS;
+  const int items = rows * P, groups = max(1, min(TH, LDSF / 6) / items);
+  const size_t step = (size_t)a.units * 16 * RS;
   for (int i0 = 0; i0 < items; i0 += TH) {
     const int i = groups > 1 ? tid % items : i0 + tid, grp = groups > 1 ? tid / items : 0;
     const bool here = i < items && grp < groups;
     float M = -FLT_MAX, L = 0.f;
     f32x4 O = {0.f, 0.f, 0.f, 0.f};
-    const float* rec = part_row(a, sc.slot, unit, min(i, items - 1) / P, 16 * NT, DT);
+    const float* from = part_row(a, sc.slot, unit, min(i, items - 1) / P, DT);
     for (int c0 = grp; here && c0 < sc.n; c0 += 4 * groups) {
       float2 v[4], u[4], ml[4];
 #pragma unroll
       for (int k = 0; k < 4; k++) {
-        const float* p = rec + min(c0 + k * groups, sc.n - 1) * step;
+        const float* p = from + min(c0 + k * groups, sc.n - 1) * step;
         v[k] = published2(p + 4 * (i % P));
         u[k] = published2(p + 4 * (i % P) + 2);
         ml[k] = published2(p + DT);
@@ -838,54 +787,49 @@ __global__ __launch_bounds__(64 * W, NT == 1 ? (DT <= 64 ? 4 : 2) : 1) void page
   }
 }
 
-template <typename KT, int DT, int NT, int W, bool STREAM = false>
+template <typename KT, int DT, int W, bool STREAM>
 void launch_attention_of(PagedArgs a, int cus, size_t part_floats, hipStream_t st) {
   using T = PagedTile<KT>;
-  const int rows = 16 * NT, groups = (a.tokens * a.G + rows - 1) / rows;
-  a.units = a.Hkv * groups;
   // tiles that a sequence may have, as far as the host knows
   int64_t most = a.limit;
   if (a.window > 0) most = std::min<int64_t>(most, (int64_t)a.window + a.tokens);
   const int64_t tiles = most / T::TS + 2;
   a.plan_shift = 0;
   while (a.seqs * ((tiles >> a.plan_shift) + 1) >= ((int64_t)1 << 30)) a.plan_shift++;
-  const int64_t record = (int64_t)rows * (DT + 2);
   // Sequences of two chunks or more have 2 * chunks at most, each a record and a count.
   // A split costs about 3.5 us (counting, joining), a round of the waves' tiles 0.8: up to
-  // 32 tiles a sequence stays whole, and chunks have 16 at least (16 x 8 Llama-3.2-1B at 2000
-  // 18.3 us with 16 tiles whole, 17.0 with 24, 16.6 with 32; four column tiles, whose rounds
-  // are longer: 16 x 5 Qwen2.5-0.5B 18.8 with 16, 25.3 with 32).
+  // 32 tiles a sequence stays whole, and chunks have 16 at least.
+  const int64_t record = 16 * (DT + 2);
   const int64_t fit = std::min<int64_t>((int64_t)part_floats / (2 * a.units * record), kPagedCounters / (2 * a.units));
-  a.round = std::max(1, (NT == 1 ? 8 / W : 1) * cus / a.units);
+  a.round = std::max(1, 8 / W * cus / a.units);
   a.chunks = (int)std::max<int64_t>(1, std::min<int64_t>(fit, a.round));
   a.chunk_min = fit < 1 ? INT_MAX / 2 : 16;
-  a.whole = NT == 4 ? 16 : 32;
+  a.whole = 32;
   const int64_t per_seq = fit < 1 || tiles <= a.whole ? 1 : (tiles + a.chunk_min - 1) / a.chunk_min;
   const int64_t blocks = std::min<int64_t>(a.chunks + a.seqs, a.seqs * per_seq) * a.units;
-  hipLaunchKernelGGL((paged_attention_kernel<KT, DT, NT, W, STREAM>), dim3((unsigned)blocks), dim3(64 * W), 0, st, a);
+  hipLaunchKernelGGL((paged_attention_kernel<KT, DT, W, STREAM>), dim3((unsigned)blocks), dim3(64 * W), 0, st, a);
 }
 
-// Waves a block: four where the sequences' kv heads alone give two blocks a CU (a
-// short sequence then leaves no waves idle), else eight.  us a call, 8 / 4 waves:
-// 128 x 1 Llama-3.2-1B at 1000 positions 28.1 / 24.2, 256 x 1 51.1 / 42.7, 64 x 1 Llama-3.2-3B 30.6 /
-// 28.4; 16 x 5 at 2500 17.6 / 19.3, Qwen2.5-0.5B 1 x 1 at 300 5.7 / 6.2.
-// There, loads past the last-level cache (256 MB) where K and V may exceed it, as
-// nothing of them is still there for the next call: 64 x 1 Llama-3.2-1B at 8192 (297 MB)
-// 60.7 -> 56.4; what fits it is faster kept (64 x 1 Llama-3.2-3B at 1000 28.3 -> 29.6).
-// More rows than 16: two or four column tiles, whose outputs leave room for four waves.
+// Waves a block: four where the sequences' kv heads and row groups alone give a
+// block a CU (a short sequence then leaves no waves idle), else eight.  us a call,
+// 8 / 4 waves: 128 x 1 Llama-3.2-1B at 1000 positions 28.1 / 24.2, 256 x 1 51.1 / 42.7, 64 x 1
+// Llama-3.2-3B 30.6 / 28.4, 16 x 8 at 2000 21.9 / 18.1; 16 x 5 at 2500 17.6 / 19.3, Qwen2.5-0.5B
+// 1 x 1 at 300 5.7 / 6.2, 16 x 5 at 2000 10.3 / 11.1.
+// Past the last-level cache (256 MB), streaming loads where K and V may exceed it and
+// are read once, as nothing of them is still there for the next call: 64 x 1
+// Llama-3.2-1B at 8192 (297 MB) 60.7 -> 56.4; what fits it is faster kept (64 x 1 Llama-3.2-3B
+// at 1000 28.3, streaming 29.6).
 template <typename KT, int DT>
-void launch_attention_rows(const PagedArgs& a, int cus, size_t part_floats, hipStream_t st) {
-  const int rows = a.tokens * a.G;
-  if (rows <= 16 && (int64_t)a.seqs * a.Hkv >= 2 * cus) {
-    const int64_t held = std::min<int64_t>(a.limit, a.window > 0 ? (int64_t)a.window + a.tokens : INT_MAX);
-    if (a.seqs * held * 2 * a.Hkv * DT * (int64_t)sizeof(KT) > (int64_t)256 << 20)
-      launch_attention_of<KT, DT, 1, 4, true>(a, cus, part_floats, st);
-    else
-      launch_attention_of<KT, DT, 1, 4>(a, cus, part_floats, st);
-  }
-  else if (rows <= 16) launch_attention_of<KT, DT, 1, 8>(a, cus, part_floats, st);
-  else if (rows <= 32) launch_attention_of<KT, DT, 2, 4>(a, cus, part_floats, st);
-  else launch_attention_of<KT, DT, 4, 4>(a, cus, part_floats, st);
+void launch_attention_rows(PagedArgs a, int cus, size_t part_floats, hipStream_t st) {
+  const int groups = (a.tokens * a.G + 15) / 16;
+  a.units = a.Hkv * groups;
+  const int64_t held = std::min<int64_t>(a.limit, a.window > 0 ? (int64_t)a.window + a.tokens : INT_MAX);
+  if ((int64_t)a.seqs * a.units < cus)
+    launch_attention_of<KT, DT, 8, false>(a, cus, part_floats, st);
+  else if (groups > 1 || a.seqs * held * 2 * a.Hkv * DT * (int64_t)sizeof(KT) <= (int64_t)256 << 20)
+    launch_attention_of<KT, DT, 4, false>(a, cus, part_floats, st);
+  else
+    launch_attention_of<KT, DT, 4, true>(a, cus, part_floats, st);
 }
 
 }  // namespace
