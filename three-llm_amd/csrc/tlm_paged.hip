@@ -457,9 +457,9 @@ __global__ __launch_bounds__(64 * W, DT <= 64 ? 4 : 2) void paged_attention_kern
     page = paged_page(table, min(tl, t1 - 1) << T::SHIFT, a.page_shift, a.num_pages);
     if (page < 0 && tl < t1) paged_flag(a.status, kPagedStatusPage);
   };
-  auto page_of = [&](int i) { return __builtin_amdgcn_readlane(page, min(i, n - 1)); };
-  auto load_k = [&](Tile& x, int i) { load(x.k, a.kc, tb + min(i, n - 1) * W, page_of(i)); };
-  auto load_v = [&](Tile& x, int i) { load(x.v, a.vc, tb + min(i, n - 1) * W, page_of(i)); };
+  auto page_of = [&](int i) { return __builtin_amdgcn_readlane(page, i); };
+  auto load_k = [&](Tile& x, int i) { load(x.k, a.kc, tb + i * W, page_of(i)); };
+  auto load_v = [&](Tile& x, int i) { load(x.v, a.vc, tb + i * W, page_of(i)); };
   // This lane's row (its column of the tiles): its positions' bounds, and q scaled by
   // a power of two to at most 1.  q is requested before the first tile: loads return
   // in order.
@@ -657,9 +657,10 @@ __global__ __launch_bounds__(64 * W, DT <= 64 ? 4 : 2) void paged_attention_kern
   // positions 31.8 instead of 28.1 us).
   while (tb < t1) {
     for (int i = 0; i < n; i++) {
+      const bool more = i + 1 < n;
       if (page_of(i) >= 0) {
-        process(x, tb + i * W, [&] { load_k(x, i + 1); }, [&] { load_v(x, i + 1); });
-      } else {
+        process(x, tb + i * W, [&] { if (more) load_k(x, i + 1); }, [&] { if (more) load_v(x, i + 1); });
+      } else if (more) {
         load_k(x, i + 1);
         load_v(x, i + 1);
       }
