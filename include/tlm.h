@@ -258,7 +258,7 @@ int tlm_op_topk(tlm_ctx* ctx, const float* logits, int n, int k, double softcap,
  * Entries at or below LOWEST_FLOAT (-inf, NaN included) never take part; a draft
  * outside the vocabulary never stands; a row without entries gives -1.
  * accepted: [seqs] drafts that stand; out_tokens: [seqs][tokens] those, the token
- * after them, then -1; both apart from the inputs.  tokens <= 64, vocab <= 524288;
+ * after them, then -1; both apart from the inputs and each other.  tokens <= 64, vocab <= 524288;
  * 12 bytes for every 2048 entries of 4096 sequences' rows fit the context's 32 MiB
  * (TLM_ERR_RANGE otherwise).  Enqueue only. */
 int tlm_op_verify_drafts(tlm_ctx* ctx, const float* logits, const float* draft_logits, const int32_t* drafts,

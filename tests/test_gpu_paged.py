@@ -499,6 +499,10 @@ def test_refusals(ctx):
         refuse(tlm.TLM_ERR_INVALID, sv.paged.append, b, x, q)
         refuse(tlm.TLM_ERR_INVALID, sv.paged.attention, b, q, out)
         setattr(b, field, keep)
+    keep, b.v_pages = b.v_pages, sv.kb.ptr.value + 16  # the pools overlap
+    refuse(tlm.TLM_ERR_INVALID, sv.paged.append, b, x, q)
+    refuse(tlm.TLM_ERR_INVALID, sv.paged.attention, b, q, out)
+    b.v_pages = keep
     b.seqs, b.tokens = 1 << 20, 1 << 20
     refuse(tlm.TLM_ERR_RANGE, sv.paged.append, b, x, q)
     refuse(tlm.TLM_ERR_RANGE, sv.paged.attention, b, q, out)

@@ -188,3 +188,24 @@ def test_refusals(ctx):
     for temp in (-0.5, float("nan"), float("inf")):
         refuse(tlm.TLM_ERR_INVALID, b, 1, 1, 10, b, b, uniforms=b, temperature=temp)
     refuse(tlm.TLM_ERR_RANGE, b, 1 << 20, 2, 10, b, b, drafts=b, uniforms=b)
+
+
+@pytest.mark.parametrize("name", ["logits", "draft_logits", "drafts", "counts", "uniforms", "accepted"])
+def test_results_over_an_input_are_refused(ctx, name):
+    # a sequence's results are written while others' inputs are still read
+    S, T, V = 3, 4, 10
+    held = {k: ctx.buffer(4 * S * T * V) for k in ("logits", "draft_logits", "drafts", "counts", "uniforms", "accepted",
+                                                   "out_tokens")}
+    held["out_tokens"] = held[name]
+
+    def call(temperature):
+        b = dict(held)
+        tlm.verify_drafts(ctx, b.pop("logits"), S, T, V, b.pop("accepted"), b.pop("out_tokens"), temperature=temperature,
+                          **b)
+
+    with pytest.raises(tlm.TlmError) as e:
+        call(1.0)
+    assert e.value.code == tlm.TLM_ERR_INVALID and "overlap" in str(e.value)
+    if name in ("draft_logits", "uniforms"):  # not read there
+        held["counts"].write(np.zeros(S, np.int32))
+        call(0.0)

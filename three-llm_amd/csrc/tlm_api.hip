@@ -689,8 +689,8 @@ static OpGemvArgs op_gemv_args(const tlm_linear* L, const float* x, const float*
   return a;
 }
 
-// Whether [p, p + n) and [q, q + m) share an address.
-static bool overlap(const float* p, size_t n, const float* q, size_t m) {
+// Whether [p, p + n) and [q, q + m), of 4-byte elements, share an address.
+static bool overlap(const void* p, size_t n, const void* q, size_t m) {
   const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
   return a < b + m * sizeof(float) && b < a + n * sizeof(float);
 }
@@ -1226,6 +1226,9 @@ static int paged_args(const tlm_paged* P, const tlm_paged_batch* b, PagedArgs& a
                 P->d.heads);
   if ((reinterpret_cast<uintptr_t>(b->k_pages) | reinterpret_cast<uintptr_t>(b->v_pages)) % 16)
     return fail(TLM_ERR_INVALID, "TLMPaged: a pool is not 16-byte aligned");
+  const size_t page = (size_t)P->d.kv_heads * P->d.page_tokens * P->d.head_dim;
+  const size_t pool = b->num_pages * (P->d.kv_fmt == TLM_FMT_F32 ? page : page / 2);
+  if (overlap(b->k_pages, pool, b->v_pages, pool)) return fail(TLM_ERR_INVALID, "TLMPaged: the pools overlap");
   memset(&a, 0, sizeof a);
   a.kc = b->k_pages;
   a.vc = b->v_pages;
@@ -1274,7 +1277,7 @@ int tlm_op_paged_attention(tlm_paged* P, const tlm_paged_batch* b, const float* 
   if (out_fmt != TLM_FMT_F16 && out_fmt != TLM_FMT_F32)
     return fail(TLM_ERR_INVALID, "TLMPaged: output format %d is not fp16 or fp32", out_fmt);
   const size_t n = (size_t)a.seqs * a.tokens * a.Hq * a.D;  // a multiple of 32
-  if (overlap(q, n, static_cast<const float*>(out), out_fmt == TLM_FMT_F32 ? n : n / 2))
+  if (overlap(q, n, out, out_fmt == TLM_FMT_F32 ? n : n / 2))
     return fail(TLM_ERR_INVALID, "TLMPaged: out overlaps q");
   a.x = q;
   a.out = out;
@@ -1422,6 +1425,20 @@ int tlm_op_verify_drafts(tlm_ctx* ctx, const float* logits, const float* draft_l
   if (need > kPartFloats * sizeof(float))
     return fail(TLM_ERR_RANGE, "TLMVerify: %d sequences of %d rows over %d tokens need %zu bytes of workspace, of %zu",
                 seqs, tokens, vocab, need, kPartFloats * sizeof(float));
+  // a sequence is decided while others' inputs are still read
+  const size_t rows = (size_t)seqs * tokens, drafted = rows - seqs, drawn = temperature > 0 ? 1 : 0;
+  const struct {
+    const void* p;
+    size_t n;
+  } in[] = {{logits, rows * vocab},
+            {draft_logits, drawn * drafted * vocab},
+            {drafts, drafted},
+            {counts, (size_t)seqs},
+            {uniforms, drawn * rows}};
+  bool apart = !overlap(accepted, seqs, out_tokens, rows);
+  for (const auto& x : in)
+    if (x.p && x.n && (overlap(x.p, x.n, accepted, seqs) || overlap(x.p, x.n, out_tokens, rows))) apart = false;
+  if (!apart) return fail(TLM_ERR_INVALID, "TLMVerify: the results overlap each other or an input");
   const DeviceScope on(ctx->device);
   std::lock_guard<std::mutex> lock(ctx->part_mu);
   a.work = ctx->part;
