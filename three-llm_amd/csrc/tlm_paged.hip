@@ -166,7 +166,7 @@ __global__ __launch_bounds__(256) void paged_append_row_kernel(PagedArgs a) {
 //     are read once for the G heads; a wave covers whole cache lines);
 //   K: eight dims with their partners;
 //   V: a dim of the E tokens of a piece, 4 q .. 4 q + 3 of each of SUB sixteens.
-// Latency and bandwidth: 3548 rows of Llama-3.2-3B (115 MB) 27.6 us, 4.2 TB/s; one
+// Latency and bandwidth: 3548 rows of Llama-3.2-3B (115 MB) 27.1 us, 4.2 TB/s; one
 // block for all of a group's items, one after the other, 36.1.
 struct AppendItems {
   int q, k, v, slices;
@@ -278,8 +278,8 @@ typedef _Float16 ph8_t __attribute__((ext_vector_type(8)));
 // of its group) are the columns of 16-column matrix-core tiles, so that K and V are
 // read once for 16 of them; a block has one column tile (a unit is a kv head and a
 // row group).  Several tiles a block were slower everywhere, as their outputs leave
-// room for fewer waves (16 x 16 Llama-3.2-3B at 2000 positions 31.9 us with four, 22.9 so;
-// Qwen2.5-0.5B 16 x 5 20.5 and 10.3; a 2048-token prompt of Llama-3.2-1B 112 and 69).  The W
+// room for fewer waves (16 x 16 Llama-3.2-3B at 2000 positions 31.9 us with four, 22.1 so;
+// Qwen2.5-0.5B 16 x 5 20.5 and 10.2; a 2048-token prompt of Llama-3.2-1B 112 and 65).  The W
 // waves take the position tiles of one chunk of the sequence in turn:
 //   * scores S^T (positions x rows) = K Q^T, K the A operand, q the B operand;
 //   * softmax with a running maximum and sum per row, base 2;
@@ -653,7 +653,7 @@ __global__ __launch_bounds__(64 * W, DT <= 64 ? 4 : 2) void paged_attention_kern
 
   // The next tile's K goes out when this one's has been read, its V likewise: half a
   // tile or more in flight a wave, and the registers of one (with two, 8 waves a CU
-  // instead of 16 at head_dim 64 and less in flight: 64 x 1 Llama-3.2-1B at 1000
+  // instead of 16 at head_dim 64 and less in flight: 128 x 1 Llama-3.2-1B at 1000
   // positions 31.8 instead of 28.1 us).
   while (tb < t1) {
     for (int i = 0; i < n; i++) {
@@ -813,13 +813,13 @@ void launch_attention_of(PagedArgs a, int cus, size_t part_floats, hipStream_t s
 
 // Waves a block: four where the sequences' kv heads and row groups alone give a
 // block a CU (a short sequence then leaves no waves idle), else eight.  us a call,
-// 8 / 4 waves: 128 x 1 Llama-3.2-1B at 1000 positions 28.1 / 24.2, 256 x 1 51.1 / 42.7, 64 x 1
-// Llama-3.2-3B 30.6 / 28.4, 16 x 8 at 2000 21.9 / 18.1; 16 x 5 at 2500 17.6 / 19.3, Qwen2.5-0.5B
-// 1 x 1 at 300 5.7 / 6.2, 16 x 5 at 2000 10.3 / 11.1.
+// 8 / 4 waves: 128 x 1 Llama-3.2-1B at 1000 positions 25.1 / 22.7, 256 x 1 44.6 / 36.3, 64 x 1
+// Llama-3.2-3B 28.9 / 26.7, 16 x 8 at 2000 20.3 / 18.4; 16 x 5 at 2500 17.0 / 19.7, Qwen2.5-0.5B
+// 1 x 1 at 300 5.6 / 6.2, 16 x 5 at 2000 10.2 / 11.5.
 // Past the last-level cache (256 MB), streaming loads where K and V may exceed it and
-// are read once, as nothing of them is still there for the next call: 64 x 1
-// Llama-3.2-1B at 8192 (297 MB) 60.7 -> 56.4; what fits it is faster kept (64 x 1 Llama-3.2-3B
-// at 1000 28.3, streaming 29.6).
+// are read once, as nothing of them is still there for the next call: 256 x 1
+// Llama-3.2-1B at 1000 40.3 -> 36.3, 64 x 1 at 8192 76.4 -> 70.9; what fits it is faster kept
+// (64 x 1 at 1000 13.5, streaming 15.4).
 template <typename KT, int DT>
 void launch_attention_rows(PagedArgs a, int cus, size_t part_floats, hipStream_t st) {
   const int groups = (a.tokens * a.G + 15) / 16;

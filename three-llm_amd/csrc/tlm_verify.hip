@@ -665,9 +665,9 @@ size_t verify_plan(VerifyArgs& a) {
 // block, a SIMD each (64 x 1 over 32000 tokens 14.6 -> 12.7 us).
 //
 // What bounds it: the logits' bytes for many rows (32 x 5 over 151936 tokens with draft
-// logits 42 us for 132 MB of live rows and 13 for the second launch; each chunk's
+// logits 43 us for 135 MB of live rows and 14 for the second launch; each chunk's
 // terms take 20 64-bit operations beside 4 bytes), for few a chain of a dozen
-// memory round trips and barriers in one block (1 x 5 over 128256: 11.4 us, of which
+// memory round trips and barriers in one block (1 x 5 over 128256: 11.6 us, of which
 // 3.7 until the sums are there, 3.5 to publish and count them, 5 to decide and draw).
 void launch_verify(const VerifyArgs& all, int cus, hipStream_t st) {
   for (int s0 = 0; s0 < all.seqs; s0 += kVerifyCounters) {
