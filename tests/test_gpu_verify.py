@@ -145,6 +145,21 @@ def test_target_and_draft_model_the_same(ctx):
     assert np.all(a == 3)
 
 
+@pytest.mark.parametrize("shift", [0.5, -3.0, 1e-3])
+@pytest.mark.parametrize("v", [700, 9000])
+def test_nothing_but_rounding_beside_a_draft_model(ctx, shift, v):
+    """q's logits are p's and a constant, and no draft can stand: what is left of p - q is rounding or nothing, and some
+    token of the vocabulary is drawn all the same."""
+    n = 40
+    logits, _, u, _ = inputs(n, 2, v)
+    acc, ids = ctx.buffer(4 * n), ctx.buffer(8 * n)
+    tlm.verify_drafts(ctx, ctx.array(logits), n, 2, v, acc, ids, drafts=ctx.array(np.full((n, 1), -1, np.int32)),
+                      draft_logits=ctx.array(logits[:, :1] + np.float32(shift)), uniforms=ctx.array(u), temperature=1.0)
+    assert np.all(acc.read(np.int32) == 0)
+    first = ids.read(np.int32).reshape(n, 2)[:, 0]
+    assert np.all((first >= 0) & (first < v))
+
+
 @pytest.mark.parametrize("temp", [1e-9, 1e-6, 0.01, 50.0, 1e30])
 def test_temperatures(ctx, temp):
     logits, drafts, u, q = inputs(5, 3, 4000, by="model")

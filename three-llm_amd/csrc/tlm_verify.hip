@@ -30,6 +30,7 @@ constexpr int kVW = 8;                    // waves per block, a chunk each
 constexpr int kVT = 64 * kVW;             // threads
 constexpr int kVChunk = 2048;             // entries: 32 a lane of a wave, 4 a thread of a block
 constexpr int kVQuads = kVChunk / 4 / 64;
+constexpr int kRestWaves = 2;             // waves that share a chunk of the second launch
 constexpr int kVRow = kVerifyMaxVocab / kVChunk / 64;  // chunks of a row that a lane holds
 static_assert(kVChunk == 4 * kVT, "a block takes a chunk in one step");
 
@@ -72,21 +73,26 @@ __device__ __forceinline__ T published(const T* p) {
 // exp((l - m) / T) = 2^((l - m) c), c = log2(e) / T, for a row's maximum m.
 // Entries at or below LOWEST_FLOAT (-inf and NaN included) never take part.
 // 2^t, t <= 0: t's nearest whole number through the sum with 1.5 * 2^52, and the
-// series of 2^f, |f| <= 1/2, up to f^9: short of it by (ln 2 / 2)^10 / 10! = 7e-12
-// (a border between tokens moves by 7e-12 of what lies below it).  The series'
+// series of 2^f, |f| <= 1/2, up to f^9, its last term spread over f .. f^7 by the
+// Chebyshev polynomial T9(2 f) = 0 (2^0 stays 1).  Off by (ln 2 / 2)^10 / 10! = 7e-12
+// for what the series leaves out and (ln 2 / 2)^9 / 9! / 256 = 8e-13 for T9, together
+// 8.4e-12 of 2^f (a border between tokens moves by so much of what lies below it).  The
 // coefficients stay in scalar registers (as literals each took two moves a term).
 // No entry is below `floor`, 2^-1100 of the maximum, which is 0: one 32-bit maximum
 // for masked entries, NaN and the exponent's range.
 constexpr double kLn2 = 0.693147180559945309417232121458;
 constexpr double coef(int n) { return n == 0 ? 1.0 : coef(n - 1) * kLn2 / n; }
+// f^9 = (576 y^7 - 432 y^5 + 120 y^3 - 9 y) / 256 / 2^9 where T9(y) = 0, y = 2 f
+constexpr double spread(int n, double of_y) { return coef(n) + coef(9) * of_y / 256 / (1 << (9 - n)); }
 struct Weights {
-  double c, m, co[10];
+  double c, m, co[9];
   float mf, floor;
   bool plain;  // else the floor is none: m is infinite, the temperature past 1e35 or so low that m - floor is lost
   __device__ __forceinline__ Weights(float max, double scale) : c(scale), m(max), mf(max) {
-    constexpr double k[10] = {coef(0), coef(1), coef(2), coef(3), coef(4), coef(5), coef(6), coef(7), coef(8), coef(9)};
+    constexpr double k[9] = {1.0,     spread(1, -9),   coef(2), spread(3, 120), coef(4),
+                             spread(5, -432), coef(6), spread(7, 576), coef(8)};
 #pragma unroll
-    for (int i = 0; i < 10; i++) {
+    for (int i = 0; i < 9; i++) {
       co[i] = k[i];
       asm("" : "+s"(co[i]));
     }
@@ -94,17 +100,21 @@ struct Weights {
     floor = (float)(m - deep);
     plain = floor > kLowest && 1024.0 * deep >= fabs(m);
   }
-  __device__ __forceinline__ double power(double t) const {
-    const double big = 6755399441055744.0;
-    const double k = t + big, f = t - (k - big);
-    double p = co[9];
+  static constexpr double kBig = 6755399441055744.0;
+  __device__ __forceinline__ double power(double k, double f) const {  // 2^(k - kBig + f)
+    double p = co[8];
 #pragma unroll
-    for (int n = 8; n >= 0; n--) p = fma(p, f, co[n]);
+    for (int n = 7; n >= 0; n--) p = fma(p, f, co[n]);
     return ldexp(p, __double2loint(k));
   }
-  __device__ __forceinline__ double series(float l) const { return power(((double)fmaxf(l, floor) - m) * c); }
+  __device__ __forceinline__ double series(float l) const {
+    const double d = (double)fmaxf(l, floor) - m, k = fma(d, c, kBig);
+    return power(k, fma(d, c, kBig - k));
+  }
   __device__ __forceinline__ double of(float l) const {  // any entry and maximum
-    const double p = power(fmax(((double)l - m) * c, -1100.0));
+    if (plain) return series(l);
+    const double t = fmax(((double)l - m) * c, -1100.0), k = t + kBig;
+    const double p = power(k, t - (k - kBig));
     return !(l > kLowest) ? 0.0 : l == mf ? 1.0 : p;
   }
 };
@@ -146,15 +156,16 @@ __device__ __forceinline__ int row_count(const VerifyArgs& a, int s) {
   return a.counts ? min(a.counts[s], a.tokens) : a.tokens;
 }
 
-// Entries 4 lane + 256 k + e of a wave's chunk at i0; past the end -inf.
-__device__ __forceinline__ void load_chunk(const float* x, int i0, int n, vf4* v) {
+// Entries 4 lane + 256 k + e from i0 on, k < N; past the end -inf.
+template <int N>
+__device__ __forceinline__ void load_quads(const float* x, int i0, int n, vf4* v) {
   const int lane = threadIdx.x & 63;
-  if (i0 + kVChunk <= n) {
+  if (i0 + 256 * N <= n) {
 #pragma unroll
-    for (int k = 0; k < kVQuads; k++) v[k] = *(const TLM_GLOBAL vf4*)(x + i0 + 256 * k + 4 * lane);
+    for (int k = 0; k < N; k++) v[k] = *(const TLM_GLOBAL vf4*)(x + i0 + 256 * k + 4 * lane);
   } else {
 #pragma unroll
-    for (int k = 0; k < kVQuads; k++)
+    for (int k = 0; k < N; k++)
 #pragma unroll
       for (int e = 0; e < 4; e++) {
         const int i = i0 + 256 * k + 4 * lane + e;
@@ -387,7 +398,7 @@ __device__ void decide(const VerifyArgs& a, int s, VerifyShared& sh) {
         v[k] = rp.sum[k];
         if (x >= 0 && lane + 64 * k == x / kVChunk) {  // less the draft's term, as it was added
           const Weights c(rp.max[k], a.scale);
-          const double left = rp.raw[k] - (c.plain ? c.series(sh.lx[taken]) : c.of(sh.lx[taken]));
+          const double left = rp.raw[k] - c.of(sh.lx[taken]);
           much = !(left >= rp.raw[k] * 0x1p-16);
           v[k] = left * of.of(rp.max[k]);
         }
@@ -483,7 +494,7 @@ __global__ __launch_bounds__(kVT, 4) void verify_kernel(VerifyArgs a) {
   };
   auto fetch = [&](int cell, vf4* v) {  // past the run's end: its last chunk
     const Place p = place(min(cell, c1 - 1));
-    load_chunk(p.r < T ? a.logits + ((size_t)p.s * T + p.r) * a.vocab
+    load_quads<kVQuads>(p.r < T ? a.logits + ((size_t)p.s * T + p.r) * a.vocab
                        : a.draft_logits + ((size_t)p.s * (T - 1) + p.r - T) * a.vocab,
                p.c * kVChunk, a.vocab, v);
     return p;
@@ -577,47 +588,58 @@ __global__ __launch_bounds__(kVT, 4) void verify_kernel(VerifyArgs a) {
   }
 }
 
-// A wave per chunk of every sequence whose token is still to be drawn: the
-// chunk's sum of max(p - q, 0); the last of a sequence's `per` blocks draws.
+// kRestWaves waves per chunk of every sequence whose token is still to be drawn: the
+// chunk's sum of max(p - q, 0); the last of a sequence's `per` blocks draws.  Two
+// share a chunk, as only the refused sequences' blocks have work (32 x 5 over 151936
+// tokens with one, two and four 55.6, 55.1 and 56.0 us a call).
 __global__ __launch_bounds__(kVT) void verify_rest_kernel(VerifyArgs a, int per) {
   __shared__ VerifyShared sh;
+  constexpr int Q = kVQuads / kRestWaves;
   const VerifyWork w = verify_work(a);
-  const int s = blockIdx.x / per, c = blockIdx.x % per * kVW + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (row_count(a, s) < 1) return;
+  const int s = blockIdx.x / per, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = row_count(a, s);
   const Decision d = w.dec[s];
-  if (d.draft < 0) return;
+  if (n < 1 || d.draft < 0) return;
   const float* l = a.logits + (size_t)d.row * a.vocab;
   const float* q = a.draft_logits + (size_t)d.draft * a.vocab;
   const float u = a.uniforms[s * a.tokens + a.tokens - 1];
   const Weights lw(d.m, a.scale), qw(d.mq, a.scale);
   auto residual = [&](float x, float y) { return fmax(lw.of(x) * d.s - (d.sq > 0.0 ? qw.of(y) * d.sq : 0.0), 0.0); };
-  if (c < a.chunks) {
-    vf4 x[kVQuads], y[kVQuads];
-    load_chunk(l, c * kVChunk, a.vocab, x);
-    load_chunk(q, c * kVChunk, a.vocab, y);
-    double sum = 0.0;
+  const int c0 = blockIdx.x % per * (kVW / kRestWaves), i0 = c0 * kVChunk + wave * (256 * Q);
+  double sum = 0.0;
+  if (i0 < a.vocab) {
+    vf4 x[Q], y[Q];
+    load_quads<Q>(l, i0, a.vocab, x);
+    load_quads<Q>(q, i0, a.vocab, y);
     if (lw.plain && qw.plain && d.sq > 0.0) {
 #pragma unroll
-      for (int k = 0; k < kVQuads; k++) {
+      for (int k = 0; k < Q; k++) {
 #pragma unroll
         for (int e = 0; e < 4; e++) sum += fmax(lw.series(x[k][e]) * d.s - qw.series(y[k][e]) * d.sq, 0.0);
         __builtin_amdgcn_sched_barrier(0);
       }
     } else {
 #pragma unroll
-      for (int k = 0; k < kVQuads; k++) {
+      for (int k = 0; k < Q; k++) {
 #pragma unroll
         for (int e = 0; e < 4; e++) sum += residual(x[k][e], y[k][e]);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
     sum = wave_sum_f64(sum);
-    if (lane == 0) publish(w.rest + (size_t)s * a.chunks + c, sum);
   }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  if (lane == 0) sh.red[wave] = sum;
   __syncthreads();
-  if (threadIdx.x == 0)
-    sh.before = __hip_atomic_fetch_add(a.arrived + s, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (wave == 0) {
+    if (lane < kVW / kRestWaves && c0 + lane < a.chunks) {
+      double v = 0.0;
+#pragma unroll
+      for (int k = 0; k < kRestWaves; k++) v += sh.red[lane * kRestWaves + k];
+      publish(w.rest + (size_t)s * a.chunks + c0 + lane, v);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the block's sums are performed
+    if (lane == 0) sh.before = __hip_atomic_fetch_add(a.arrived + s, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
   __syncthreads();
   if (sh.before != (unsigned)per - 1) return;
   if (threadIdx.x == 0) __hip_atomic_store(a.arrived + s, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -665,9 +687,9 @@ size_t verify_plan(VerifyArgs& a) {
 // block, a SIMD each (64 x 1 over 32000 tokens 14.6 -> 12.7 us).
 //
 // What bounds it: the logits' bytes for many rows (32 x 5 over 151936 tokens with draft
-// logits 43 us for 135 MB of live rows and 14 for the second launch; each chunk's
-// terms take 20 64-bit operations beside 4 bytes), for few a chain of a dozen
-// memory round trips and barriers in one block (1 x 5 over 128256: 11.6 us, of which
+// logits 43 us for 135 MB of live rows and 13 for the second launch; each entry's
+// term takes 17 64-bit operations beside 4 bytes), for few a chain of a dozen
+// memory round trips and barriers in one block (1 x 5 over 128256: 11.3 us, of which
 // 3.7 until the sums are there, 3.5 to publish and count them, 5 to decide and draw).
 void launch_verify(const VerifyArgs& all, int cus, hipStream_t st) {
   for (int s0 = 0; s0 < all.seqs; s0 += kVerifyCounters) {
@@ -689,7 +711,7 @@ void launch_verify(const VerifyArgs& all, int cus, hipStream_t st) {
       continue;
     }
     hipLaunchKernelGGL(verify_kernel<false>, grid, block, 0, st, a);
-    const int per = (a.chunks + kVW - 1) / kVW;
+    const int per = (a.chunks * kRestWaves + kVW - 1) / kVW;
     if (a.rows > a.tokens) hipLaunchKernelGGL(verify_rest_kernel, dim3((unsigned)(a.seqs * per)), block, 0, st, a, per);
   }
 }
