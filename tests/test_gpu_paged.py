@@ -256,6 +256,43 @@ def test_attention_one_long_cache_among_short_ones(ctx, kv, tokens):
     attend(Serving(ctx, 8, 2, 128, [20000, 3, 700], tokens, 256, kv))
 
 
+def test_attention_of_few_rows_in_a_batch_with_room_for_many(ctx):
+    """Room for 8192 rows and 40 of them there: so many row groups leave no room for partial results, and a sequence is
+    one block's however long it is."""
+    attend(Serving(ctx, 16, 16, 32, [1500, 2, -1], 8192, 64, counts=[40, 3, 5]))
+
+
+@pytest.mark.parametrize("kv", [tlm.FMT_F16, tlm.FMT_F32])
+def test_attention_over_2_30_positions(ctx, kv):
+    """40 sequences of up to 2^30 positions (their tiles together pass 32 bits), three of them as long as that over
+    tables that name the same pages again and again.  K is 0 and V 0 or 1, ones in a 256th of the table: every sum is a
+    count.  A sequence's 2^30 is joined from at most 256 chunks of 8 waves, a rounding each, and one division."""
+    n, page, d, width, part = 40, 1024, 32, 1 << 20, 1 << 12
+    paged = tlm.Paged(ctx, 1, 1, d, 1 << 30, page_tokens=page, kv_fmt=kv)
+    k, v = np.zeros(2 * page * d, NP[kv]), np.repeat([0, 1], page * d).astype(NP[kv])
+    tables = np.zeros((n, width), np.int32)
+    starts = np.array([37 * s if s % 5 else -1 for s in range(n)], np.int32)
+    tables[1::2] = 1
+    for s, at in ((3, 0), (8, width // 2 + 5 * part + 77), (39, width - part)):
+        starts[s] = (1 << 30) - 1 - s
+        tables[s] = 0
+        tables[s, at:at + part] = 1
+    out = ctx.array(np.full((n, d), 77, np.float32))
+    batch = paged.batch(ctx.array(k), ctx.array(v), 2, ctx.array(tables), width, ctx.array(starts), n)
+    paged.attention(batch, ctx.array(np.ones((n, d), np.float32)), out, tlm.FMT_F32)
+    paged.status()
+    got = out.read(np.float32).reshape(n, d).astype(np.float64)
+    for s in range(n):
+        if starts[s] < 0:
+            ref = 77.0
+        elif starts[s] < 1 << 20:
+            ref = float(tables[s, 0])
+        else:
+            ones = part * page - (s if s == 39 else 0)
+            ref = ones / (starts[s] + 1.0)
+        assert np.all(np.abs(got[s] - ref) <= 272 * EPS * ref), (s, got[s, 0], ref)
+
+
 @pytest.mark.parametrize("size", [2.0 ** -40, 2.0 ** 18, 2.0 ** 60])
 @pytest.mark.parametrize("kv", [tlm.FMT_F16, tlm.FMT_F32])
 def test_queries_of_any_size(ctx, size, kv):
