@@ -82,6 +82,23 @@ def test_most_rows(ctx):
     check(ctx, logits, drafts, u, 0.3, counts=[64, 63, 2])
 
 
+@pytest.mark.parametrize("v", [131073, 524287, 524288])
+@pytest.mark.parametrize("by", ["lookup", "model"])
+def test_largest_vocabularies(ctx, v, by):
+    """Rows of more than 64 chunks, so several to a lane; the last sequence's tokens lie at the end of its rows."""
+    logits, drafts, u, q = inputs(6, 2, v, by=by)
+    logits[5, :, :v - 40] -= np.float32(60)
+    drafts[4, 0] = v - 1
+    for temp in (0.0, 0.8):
+        check(ctx, logits, drafts, u, temp, draft_logits=q)
+
+
+def test_most_rows_of_a_draft_model(ctx):
+    logits, drafts, u, q = inputs(5, 64, 2500, by="model", close=0.05)
+    check(ctx, logits, drafts, u * np.float32(0.5), 0.8, counts=[64, 63, 9, 33, 8], draft_logits=q)
+    check(ctx, logits, drafts, u, 0.8, draft_logits=q)
+
+
 @pytest.mark.parametrize("u", [0.0, 1.0 - 2.0 ** -24, 0.5])
 @pytest.mark.parametrize("by", ["lookup", "model"])
 def test_ends_of_the_random_numbers(ctx, u, by):
