@@ -192,7 +192,7 @@ typedef struct tlm_paged_desc {
  * during the call.  seqs * tokens * heads is at most 2^22. */
 typedef struct tlm_paged_batch {
   void* k_pages;            /* pools of num_pages * kv_heads * page_tokens * head_dim kv_fmt elements, 16-byte */
-  void* v_pages;            /* aligned, in the order that tlm_paged_locate tells */
+  void* v_pages;            /* aligned and apart, in the order that tlm_paged_locate tells */
   const int32_t* tables;    /* [seqs][table_width] */
   const int32_t* starts;    /* [seqs] */
   const int32_t* counts;    /* [seqs] or NULL */
