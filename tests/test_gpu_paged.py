@@ -323,6 +323,59 @@ def test_no_spread_and_one_certain_key(ctx):
 
 
 @pytest.mark.parametrize("kv", [tlm.FMT_F16, tlm.FMT_F32])
+@pytest.mark.parametrize("size", [2.0 ** 18, 2.0 ** 23, 2.0 ** 26, 2.0 ** 30, 2.0 ** 60, 2.0 ** 100])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_of_any_size(ctx, size, sign, kv):
+    """Scores past what a 32-bit number holds in whole steps, above and below 0: the best key's V, and nothing else.
+    The best two keys' scores are at least a 64th of the largest apart, far more than they are off by."""
+    sv = Serving(ctx, 4, 2, 64, [300, 40], 3, 64, kv, scale=1.0)
+    for k in sv.k:
+        k[..., 1:] = 0
+        for h in range(2):  # 1 .. 2 in steps of a 512th, each once, and one 2 + a 32nd (or, below 0, 1 - a 64th)
+            k[:, h, 0] = 1 + sv.rng.permutation(512)[:k.shape[0]] / 512
+            k[sv.rng.integers(0, 38), h, 0] = 2 + 1 / 32 if sign > 0 else 1 - 1 / 64
+    sv.upload(*sv.pools(sv.starts + 3))
+    q = np.zeros((2, 3, 4, 64), np.float32)
+    q[..., 0] = sign * size * (1 + np.arange(4) / 7)
+    got = sv.attention(q, tlm.FMT_F32)
+    sv.paged.status()
+    for s in range(2):
+        for h in range(4):
+            best = np.argmax(sign * sv.k[s][:38, h // 2, 0])
+            want = sv.v[s][best, h // 2].astype(np.float64)
+            assert np.all(np.abs(got[s, :, h] - want) <= 2.0 ** -21 * np.abs(want)), (s, h)
+    sv.close()
+
+
+@pytest.mark.parametrize("kv", [tlm.FMT_F16, tlm.FMT_F32])
+@pytest.mark.parametrize("octaves", [18.4, 22.4, 25.6])
+@pytest.mark.parametrize("every", [0, 32])
+def test_small_weights_beside_dominant_keys(ctx, kv, octaves, every):
+    """One key, or one in 32, weighs 2^octaves times each of the others, and has V = 0: the output is what the small
+    weights w bring.  All terms are positive, so errors are relative.  A weight is off by g = octaves ln 2 times q's
+    2^-22 and the scale's and score's three roundings, and exp2's 2^-23: 8 g + 2 of 2^-24; as a pair by 2^-22 or
+    2^-39 of the largest; numerator and denominator each by n / 16 + 96 roundings."""
+    sv = Serving(ctx, 4, 2, 64, [700, 5000], 1, 64, kv, scale=1.0)
+    for k, v in zip(sv.k, sv.v):
+        k[:] = 0
+        v[:] = sv.rng.uniform(0.5, 1, v.shape)
+        at = slice(5, None, every) if every else [5]
+        k[at, :, 0], v[at] = 1, 0
+    sv.upload(*sv.pools(sv.starts + 1))
+    gap = octaves * np.log(2)
+    q = sv.rng.uniform(0, 1, (2, 1, 4, 64)).astype(np.float32)
+    q[..., 0] = gap
+    got = sv.attention(q, tlm.FMT_F32).astype(np.float64)
+    sv.paged.status()
+    for s in range(2):
+        n = int(sv.starts[s]) + 1
+        ref = po.attend(q[s, 0], sv.k[s], sv.v[s], n - 1, 0, 1.0)
+        tol = (8 * gap + 2 + 4 + 2 * (n / 16 + 96)) * EPS + 2.0 ** (octaves - 39)
+        assert np.all(np.abs(got[s, 0] - ref) <= tol * ref), (s, np.abs(got[s, 0] / ref - 1).max(), tol)
+    sv.close()
+
+
+@pytest.mark.parametrize("kv", [tlm.FMT_F16, tlm.FMT_F32])
 @pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
 @pytest.mark.parametrize("hq", [2, 16])
 def test_masked_rows_of_drafts_are_not_seen(ctx, kv, bad, hq):

@@ -282,18 +282,24 @@ typedef _Float16 ph8_t __attribute__((ext_vector_type(8)));
 // Qwen2.5-0.5B 16 x 5 20.5 and 10.2; a 2048-token prompt of Llama-3.2-1B 112 and 65).  The W
 // waves take the position tiles of one chunk of the sequence in turn:
 //   * scores S^T (positions x rows) = K Q^T, K the A operand, q the B operand;
-//   * softmax with a running maximum and sum per row, base 2;
+//   * softmax with a running maximum and sum per row, base 2.  The maximum is a whole
+//     number at or above the scores, so that rescaling is exact and a weight takes one
+//     fma before its exponential;
 //   * O^T (dims x rows) += V^T P^T, V^T the A operand, P^T from the score registers.
 // The pages hold K and V in operand order (tlm_paged.h), so a tile's operands are
 // loaded straight into registers, 1 KB in a row per wave and instruction.
 // fp16 caches: 32 positions a tile, v_mfma_f32_16x16x32_f16 with q and P as hi +
-// lo pairs (x = hi + lo to 2^-22 of the row's largest q, resp. of 1; K and V are
-// exact).  fp32 caches: 16 positions a tile, v_mfma_f32_16x16x4_f32.
+// lo pairs (K and V are exact): q to 2^-22 of the row's largest element, P to 2^-22 of
+// itself or 2^-39 of the largest.  The latter takes P times 2^15, the largest power of
+// two in fp16's range: as a number up to 1 it ends at 2^-25, and many small weights
+// beside one large are lost while the sum has them.  L and O both carry the factor.
+// fp32 caches: 16 positions a tile, v_mfma_f32_16x16x4_f32.
 template <typename KT>
 struct PagedTile {
   static constexpr int SUB = 4 / sizeof(KT);  // 16-position score tiles
   static constexpr int TS = 16 * SUB;         // positions
   static constexpr int SHIFT = SUB == 2 ? 5 : 4;
+  static constexpr float kLift = SUB == 2 ? 15.f : 0.f;  // log2 of P's factor
 };
 
 // A sequence's part in a call: its rows and the position tiles that they attend to.
@@ -491,7 +497,8 @@ __global__ __launch_bounds__(64 * W, DT <= 64 ? 4 : 2) void paged_attention_kern
   for (int f = 0; f < NF; f++)
 #pragma unroll
     for (int e = 0; e < 4; e++) qx[f][e] = row < R ? ldexpf(qx[f][e], -ex) : 0.f;
-  const float mult = ldexpf(a.scale * 1.4426950408889634f, ex);  // log2 e: the softmax runs in base 2
+  // log2 e: the softmax runs in base 2; above 0, as masked scores are -inf before it
+  const float mult = fmaxf(ldexpf(a.scale * 1.4426950408889634f, ex), FLT_TRUE_MIN);
 #pragma unroll
   for (int f = 0; f < NF; f++) {
     if (!F16) {
@@ -574,7 +581,7 @@ __global__ __launch_bounds__(64 * W, DT <= 64 ? 4 : 2) void paged_attention_kern
 #pragma unroll
     for (int st = 0; st < SUB; st++)
 #pragma unroll
-      for (int e = 0; e < 4; e++) sv[4 * st + e] = acc[st][e] * mult;
+      for (int e = 0; e < 4; e++) sv[4 * st + e] = acc[st][e];
     if (edge) {
 #pragma unroll
       for (int i = 0; i < 4 * SUB; i++) {
@@ -587,7 +594,17 @@ __global__ __launch_bounds__(64 * W, DT <= 64 ? 4 : 2) void paged_attention_kern
     for (int i = 1; i < 4 * SUB; i++) mx = fmaxf(mx, sv[i]);
     mx = fmaxf(mx, lane_swap16(mx));
     mx = fmaxf(mx, lane_swap32(mx));
-    const float mn = fmaxf(mrun, mx);  // finite: it starts at -FLT_MAX
+    const float mn = fmaxf(mrun, ceilf(mx * mult));  // finite: it starts at -FLT_MAX
+    if (__ballot(fabsf(mn) >= 0x1p22f)) {
+      // kLift - mn is rounded there, and an unrounded product passes the maximum by as much
+#pragma clang fp contract(off)
+#pragma unroll
+      for (int i = 0; i < 4 * SUB; i++) sv[i] = (sv[i] * mult - mn) + T::kLift;
+    } else {
+      const float lift = T::kLift - mn;
+#pragma unroll
+      for (int i = 0; i < 4 * SUB; i++) sv[i] = fmaf(sv[i], mult, lift);
+    }
     const float corr = __builtin_amdgcn_exp2f(mrun - mn);
     float ps = 0.f;
     u32x4 ph, pl;  // fp16: high and low parts
@@ -595,7 +612,7 @@ __global__ __launch_bounds__(64 * W, DT <= 64 ? 4 : 2) void paged_attention_kern
       ph8_t h, l;
 #pragma unroll
       for (int i = 0; i < 4 * SUB; i++) {
-        const float v = __builtin_amdgcn_exp2f(sv[i] - mn);
+        const float v = __builtin_amdgcn_exp2f(sv[i]);
         ps += v;
         h[i % 8] = (_Float16)v;
         l[i % 8] = (_Float16)(v - (float)h[i % 8]);
@@ -605,7 +622,7 @@ __global__ __launch_bounds__(64 * W, DT <= 64 ? 4 : 2) void paged_attention_kern
     } else {
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        const float v = __builtin_amdgcn_exp2f(sv[i] - mn);
+        const float v = __builtin_amdgcn_exp2f(sv[i]);
         ps += v;
         ph[i] = __float_as_uint(v);
       }
