@@ -210,9 +210,9 @@ int tlm_op_paged_append(tlm_paged* paged, const tlm_paged_batch* batch, const fl
  * sequence, which the pages hold (append first).  q: fp32 [seqs][tokens]
  * [heads * head_dim], rotated; out: the same shape in out_fmt, TLM_FMT_F16 or
  * TLM_FMT_F32, apart from q.  Scores and the weighted sum to 32 bits: an fp16
- * cache's products take q (relative to its row's largest element) and the
- * probabilities as pairs of fp16 values.  What masked positions hold does not
- * matter; attended K and V are finite.  Enqueue only. */
+ * cache's products take q and the probabilities as pairs of fp16 values, each to
+ * 2^-22 of itself or 2^-39 of its row's largest.  What masked positions hold does
+ * not matter; attended K and V are finite.  Enqueue only. */
 int tlm_op_paged_attention(tlm_paged* paged, const tlm_paged_batch* batch, const float* q, int out_fmt, void* out);
 /* Waits for the stream and tells of what the calls since the last status met on
  * the device: TLM_ERR_RANGE where counts[s] was above `tokens`, a row's position

@@ -348,6 +348,36 @@ def test_scores_of_any_size(ctx, size, sign, kv):
 
 
 @pytest.mark.parametrize("kv", [tlm.FMT_F16, tlm.FMT_F32])
+@pytest.mark.parametrize("tokens", [1, 3])
+def test_small_elements_of_q_beside_a_large_one(ctx, kv, tokens):
+    """Elements 2^-20 of the row's largest decide the scores: K is 0 where q is large and of 2^13 elsewhere.  An element
+    is off by 2^-22 of itself or 2^-39 of the largest (1), so a score by A 2^-22 + 2^-39 sum |k| scale and a 32-bit sum's
+    (d / 4 + 8) 2^-24 A; the output as elsewhere."""
+    scale = 64.0
+    sv = Serving(ctx, 4, 2, 64, [700, 90], tokens, 64, kv, scale=scale)
+    for k in sv.k:
+        k *= NP[kv](2.0 ** 13)
+        k[..., 0] = 0
+    sv.upload(*sv.pools(sv.starts + tokens))
+    q = normal(sv) * np.float32(2.0 ** -20)
+    q[..., 0] = 1
+    got = sv.attention(q, tlm.FMT_F32).astype(np.float64)
+    sv.paged.status()
+    for s in range(2):
+        for j in range(tokens):
+            n = int(sv.starts[s]) + j + 1
+            ref = po.attend(q[s, j], sv.k[s], sv.v[s], n - 1, 0, scale)
+            kk = np.abs(sv.k[s][:n].astype(np.float64)).repeat(2, 1)
+            a = float((kk * np.abs(q[s, j])).sum(-1).max()) * scale
+            off = (4 + 16 + 8) * EPS * a + 2.0 ** -39 * float(kk.sum(-1).max()) * scale
+            mv = float(np.abs(sv.v[s][:n].astype(np.float64)).max())
+            tol = (2 * off + (n / 16 + 96) * EPS) * mv
+            err = np.abs(got[s, j] - ref).max()
+            assert err <= tol, f"sequence {s} row {j}: {err} over {tol}"
+    sv.close()
+
+
+@pytest.mark.parametrize("kv", [tlm.FMT_F16, tlm.FMT_F32])
 @pytest.mark.parametrize("octaves", [18.4, 22.4, 25.6])
 @pytest.mark.parametrize("every", [0, 32])
 def test_small_weights_beside_dominant_keys(ctx, kv, octaves, every):

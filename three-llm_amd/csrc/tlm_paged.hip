@@ -289,17 +289,18 @@ typedef _Float16 ph8_t __attribute__((ext_vector_type(8)));
 // The pages hold K and V in operand order (tlm_paged.h), so a tile's operands are
 // loaded straight into registers, 1 KB in a row per wave and instruction.
 // fp16 caches: 32 positions a tile, v_mfma_f32_16x16x32_f16 with q and P as hi +
-// lo pairs (K and V are exact): q to 2^-22 of the row's largest element, P to 2^-22 of
-// itself or 2^-39 of the largest.  The latter takes P times 2^15, the largest power of
-// two in fp16's range: as a number up to 1 it ends at 2^-25, and many small weights
-// beside one large are lost while the sum has them.  L and O both carry the factor.
+// lo pairs (K and V are exact): an element of q to 2^-22 of itself or 2^-39 of the
+// row's largest, P to 2^-22 of itself or 2^-39 of the largest.  That takes both times
+// 2^15, the largest power of two in fp16's range: as numbers up to 1 they end at
+// 2^-25, and many small weights beside one large are lost while the sum has them.  q's
+// factor is taken out of the scores, P's is in L and O alike.
 // fp32 caches: 16 positions a tile, v_mfma_f32_16x16x4_f32.
 template <typename KT>
 struct PagedTile {
   static constexpr int SUB = 4 / sizeof(KT);  // 16-position score tiles
   static constexpr int TS = 16 * SUB;         // positions
   static constexpr int SHIFT = SUB == 2 ? 5 : 4;
-  static constexpr float kLift = SUB == 2 ? 15.f : 0.f;  // log2 of P's factor
+  static constexpr float kLift = SUB == 2 ? 15.f : 0.f;  // log2 of q's and P's factor
 };
 
 // A sequence's part in a call: its rows and the position tiles that they attend to.
@@ -467,8 +468,8 @@ __global__ __launch_bounds__(64 * W, DT <= 64 ? 4 : 2) void paged_attention_kern
   auto load_k = [&](Tile& x, int i) { load(x.k, a.kc, tb + i * W, page_of(i)); };
   auto load_v = [&](Tile& x, int i) { load(x.v, a.vc, tb + i * W, page_of(i)); };
   // This lane's row (its column of the tiles): its positions' bounds, and q scaled by
-  // a power of two to at most 1.  q is requested before the first tile: loads return
-  // in order.
+  // a power of two to at most 1, or 2^15 as fp16.  q is requested before the first
+  // tile: loads return in order.
   const int row = r0 + i16, rc = min(row, R - 1), hi = start + rc / a.G;
   const int lo = a.window > 0 ? hi - a.window + 1 : 0;
   u32x4 qreg[NF];
@@ -492,7 +493,8 @@ __global__ __launch_bounds__(64 * W, DT <= 64 ? 4 : 2) void paged_attention_kern
     for (int e = 0; e < 4; e++) qmax = fmaxf(qmax, fabsf(qx[f][e]));
   qmax = fmaxf(qmax, lane_swap16(qmax));
   qmax = fmaxf(qmax, lane_swap32(qmax));
-  const int ex = max(-120, min(120, __builtin_amdgcn_frexp_expf(qmax)));
+  const int qe = __builtin_amdgcn_frexp_expf(qmax);
+  const int ex = F16 ? max(-100, qe - (int)T::kLift) : max(-120, min(120, qe));
 #pragma unroll
   for (int f = 0; f < NF; f++)
 #pragma unroll
