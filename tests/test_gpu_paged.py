@@ -250,6 +250,61 @@ def test_attention_many_sequences_of_all_lengths(ctx, n):
     attend(Serving(ctx, 4, 2, 64, lengths, 1, 32))
 
 
+@pytest.mark.parametrize("n,hq,hkv,tokens", [(384, 8, 8, 1), (385, 4, 2, 1), (1024, 2, 1, 1), (1500, 4, 4, 2), (4500, 2, 1, 1)])
+@pytest.mark.parametrize("kv", [tlm.FMT_F16, tlm.FMT_F32])
+def test_attention_of_more_sequences_than_a_wave_plans(ctx, n, hq, hkv, tokens, kv):
+    """Long caches in several chunks among many short ones and idle slots, whole groups of 64 of them; a row past the
+    model's positions is reported."""
+    rng = np.random.default_rng(n)
+    lengths = [int(x) for x in rng.integers(0, 40, n)]
+    for s in (1, 63, 64, n // 2, n - 70, n - 1):
+        lengths[s] = 2500 + 5 * (s % 64)
+    for s in range(128, 256):
+        lengths[s] = -1
+    attend(Serving(ctx, hq, hkv, 32, lengths, tokens, 32, kv, counts=[int(x) for x in rng.integers(0, tokens + 1, n)]))
+    sv = Serving(ctx, hq, hkv, 32, [3] * n, 1, 32, kv, max_tokens=40)
+    sv.upload(*sv.pools(sv.starts + 1))
+    starts = sv.starts.copy()
+    starts[n - 3] = 40
+    sv.batch.starts = ctx.array(starts).ptr
+    sv.rows[n - 3] = 0
+    q = normal(sv)
+    sv.check(q, sv.attention(q, tlm.FMT_F32), tlm.FMT_F32, reported=True)
+    with pytest.raises(tlm.TlmError) as e:
+        sv.paged.status()
+    assert e.value.code == tlm.TLM_ERR_RANGE and "left out" in str(e.value)
+    sv.close()
+
+
+def test_attention_of_2_22_sequences(ctx):
+    """The most sequences that a call takes, over tables that name two pages: K is 0 and V 0 in one page and 1 in the
+    other, so an output is the share of a sequence's positions in the second.  32-bit sums of up to 1500 ones are exact,
+    one division is not."""
+    n, page, d, width = 1 << 22, 512, 32, 3
+    rng = np.random.default_rng(0)
+    paged = tlm.Paged(ctx, 1, 1, d, width * page, page_tokens=page)
+    k, v = np.zeros(2 * page * d, np.float16), np.repeat([0, 1], page * d).astype(np.float16)
+    tables = rng.integers(0, 2, (n, width)).astype(np.int32)
+    starts = rng.integers(-1, 20, n).astype(np.int32)
+    long = rng.integers(0, n, 300)
+    starts[long] = rng.integers(0, 1500, 300)
+    starts[n - 1] = 1400
+    q, out = ctx.buffer(4 * n * d), ctx.buffer(2 * n * d)
+    q.write(np.ones((n, d), np.float32))
+    out.write(np.full((n, d), 77, np.float16))
+    batch = paged.batch(ctx.array(k), ctx.array(v), 2, ctx.array(tables), width, ctx.array(starts), n)
+    paged.attention(batch, q, out)
+    paged.status()
+    got = out.read(np.float16).reshape(n, d)
+    seen = np.clip((starts + 1)[:, None] - page * np.arange(width), 0, page)
+    ref = (seen * tables).sum(1) / np.maximum(starts + 1, 1)
+    ref = np.where(starts < 0, 77, ref)
+    assert np.all(np.abs(got - ref[:, None]) <= ref[:, None] * (2.0 ** -11 + 2.0 ** -22))
+    q.free()
+    out.free()
+    paged.close()
+
+
 @pytest.mark.parametrize("kv", [tlm.FMT_F16, tlm.FMT_F32])
 @pytest.mark.parametrize("tokens", [1, 5])
 def test_attention_one_long_cache_among_short_ones(ctx, kv, tokens):

@@ -490,6 +490,7 @@ struct PagedArgs {
   // attention: how the sequences' position tiles are shared out (launch_paged_attention)
   float* part;
   unsigned* arrived;  // [kPagedCounters], zero between launches
+  int* plan;          // of many sequences (paged_plan_kernel), or null
   int units, chunks, round, chunk_min, whole, plan_shift;
 };
 constexpr int kPagedCounters = 16384;

@@ -341,50 +341,83 @@ __device__ __forceinline__ int wave_scan(int v) {
 }
 
 // Chunks of equal size over sequences of unequal length, c tiles each: all
-// sequences together have at most a.chunks more of them than sequences.  Every
-// wave works it out for itself from the starts (which only the device knows): the
-// sum of the tiles, then a running sum of the sequences' chunks up to chunk g.
+// sequences together have at most a.chunks more of them than sequences.  Up to
+// kPlanInPlace sequences every wave works it out for itself from the starts (which
+// only the device knows): the sum of the tiles, then a running sum of the sequences'
+// chunks up to chunk g.  Its time grows with the sequences in each of a number of
+// blocks that does, too; past that a launch of one block leaves c and the running
+// sums before each 64 sequences, which a wave searches.  us a call in place / so, one
+// token each at 300 positions of Llama-3.2-1B: 300 sequences 35.0 / 35.8, 512 64.8 / 59.2,
+// 1024 160 / 114, 2048 416 / 228.
 // slot: records of partial results before the sequence's (one of a single chunk has
 // none).  False: there is no chunk g.
+constexpr int kPlanInPlace = 384;
+constexpr int kPlanThreads = 1024;
 struct SeqChunk {
   SeqWork w;
   int s, n, chunk, slot;  // sequence, its chunks, which of them
 };
+// a.plan: c, then the chunks and the slots before each 64 sequences
+__host__ __device__ inline int plan_groups(int seqs) { return (seqs + 63) / 64; }
+__device__ __forceinline__ int plan_part(const PagedArgs& a, int tiles) {  // their sum stays in 31 bits
+  return (tiles + (1 << a.plan_shift) - 1) >> a.plan_shift;
+}
+__device__ __forceinline__ int plan_chunk(const PagedArgs& a, int total) {
+  return max(a.chunk_min, ((total + a.chunks - 1) / a.chunks) << a.plan_shift);
+}
+__device__ __forceinline__ int plan_chunks_of(const PagedArgs& a, int c, int tiles) {
+  return tiles <= a.whole ? min(tiles, 1) : (tiles + c - 1) / c;
+}
+
+template <int SHIFT>
+__global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedArgs a) {
+  constexpr int W = kPlanThreads / 64;
+  __shared__ int sh[2][W];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int groups = plan_groups(a.seqs);
+  bool any = false, bad;
+  int sum = 0;
+  for (int s = tid; s < a.seqs; s += kPlanThreads) {
+    sum += plan_part(a, seq_work<SHIFT>(a, s, &bad).tiles);
+    any |= bad;
+  }
+  if (any) paged_flag(a.status, kPagedStatusRows);
+  sum = __builtin_amdgcn_readlane(wave_scan(sum), 63);
+  if (lane == 0) sh[0][w] = sum;
+  __syncthreads();
+  int total = 0;
+  for (int i = 0; i < W; i++) total += sh[0][i];
+  const int c = plan_chunk(a, total);
+  if (tid == 0) a.plan[0] = c;
+  int before = 0, slots = 0;
+  for (int g0 = 0; g0 < groups; g0 += W) {  // a wave per 64 sequences
+    const int s = 64 * (g0 + w) + lane;
+    const int n = s < a.seqs ? plan_chunks_of(a, c, seq_work<SHIFT>(a, s, &bad).tiles) : 0;
+    const int chunks = __builtin_amdgcn_readlane(wave_scan(n), 63);
+    const int parts = __builtin_amdgcn_readlane(wave_scan(n > 1 ? n : 0), 63);
+    __syncthreads();  // sh of the round before has been read
+    if (lane == 0) sh[0][w] = chunks, sh[1][w] = parts;
+    __syncthreads();
+    for (int i = 0; i < W; i++) {
+      if (i == w && lane == 0 && g0 + w < groups) {
+        a.plan[1 + g0 + w] = before;
+        a.plan[1 + groups + g0 + w] = slots;
+      }
+      before += sh[0][i];
+      slots += sh[1][i];
+    }
+  }
+}
+
 template <int SHIFT>
 __device__ __forceinline__ bool plan(const PagedArgs& a, int g, SeqChunk& r) {
   const int lane = threadIdx.x & 63;
-  // the first kSeqs times 64 sequences stay in registers, a lane each
-  constexpr int kSeqs = 4;
   const SeqWork none{0, 0, 0, 0};
-  SeqWork w[kSeqs];
-  bool bad[kSeqs], b;
-  auto part = [&](int tiles) { return (tiles + (1 << a.plan_shift) - 1) >> a.plan_shift; };
-  int sum = 0;
-#pragma unroll
-  for (int k = 0; k < kSeqs; k++) {
-    w[k] = none, bad[k] = false;
-    if (64 * k < a.seqs && 64 * k + lane < a.seqs) w[k] = seq_work<SHIFT>(a, 64 * k + lane, &bad[k]);
-  }
-#pragma unroll
-  for (int k = 0; k < kSeqs; k++) sum += part(w[k].tiles);
-  bool any = bad[0] || bad[1] || bad[2] || bad[3];
-  for (int s = 64 * kSeqs + lane; s < a.seqs; s += 64) {
-    sum += part(seq_work<SHIFT>(a, s, &b).tiles);
-    any |= b;
-  }
-  if (any && blockIdx.x == 0 && threadIdx.x < 64) paged_flag(a.status, kPagedStatusRows);
-  const int total = __builtin_amdgcn_readlane(wave_scan(sum), 63);
-  int c = max(a.chunk_min, ((total + a.chunks - 1) / a.chunks) << a.plan_shift);
-  auto chunks_of = [&](int tiles) { return tiles <= a.whole ? min(tiles, 1) : (tiles + c - 1) / c; };
-  if (a.seqs <= 64) {
-    // few sequences: all their chunks in one round of blocks
-    const int live = __builtin_popcountll(__ballot(w[0].tiles > 0));
-    if (2 * live <= a.round)
-      while (__builtin_amdgcn_readlane(wave_scan(chunks_of(w[0].tiles)), 63) > a.round) c += (c + 7) / 8;
-  }
-  int before = 0, slots = 0;
+  bool b;
+  int c = 0, before = 0, slots = 0;
+  // whether chunk g is one of the 64 sequences' from s0 on, a lane each
   auto find = [&](const SeqWork& w, int s0) {
-    const int n = chunks_of(w.tiles), incl = wave_scan(n), m = n > 1 ? n : 0, sincl = wave_scan(m);
+    const int n = plan_chunks_of(a, c, w.tiles), incl = wave_scan(n), m = n > 1 ? n : 0, sincl = wave_scan(m);
     const unsigned long long hit = __ballot(before + incl > g);
     if (!hit) {
       before += __builtin_amdgcn_readlane(incl, 63);
@@ -402,6 +435,46 @@ __device__ __forceinline__ bool plan(const PagedArgs& a, int g, SeqChunk& r) {
     r.slot = slots + __builtin_amdgcn_readlane(sincl - m, l);
     return true;
   };
+  if (a.plan) {
+    // the last 64 sequences before which there are at most g chunks, by 64 at a time
+    const int groups = plan_groups(a.seqs);
+    int lo = 0, len = groups;
+    while (true) {
+      const int step = (len + 63) / 64, i = lane * step;
+      const int k = __builtin_popcountll(__ballot(i < len && a.plan[1 + lo + min(i, len - 1)] <= g)) - 1;  // the first is
+      lo += k * step;
+      len = min(step, len - k * step);
+      if (step == 1) break;
+    }
+    c = a.plan[0], before = a.plan[1 + lo], slots = a.plan[1 + groups + lo];
+    const int s0 = 64 * lo;
+    return find(s0 + lane < a.seqs ? seq_work<SHIFT>(a, s0 + lane, &b) : none, s0);
+  }
+  // the first kSeqs times 64 sequences stay in registers, a lane each
+  constexpr int kSeqs = 4;
+  SeqWork w[kSeqs];
+  bool bad[kSeqs];
+  int sum = 0;
+#pragma unroll
+  for (int k = 0; k < kSeqs; k++) {
+    w[k] = none, bad[k] = false;
+    if (64 * k < a.seqs && 64 * k + lane < a.seqs) w[k] = seq_work<SHIFT>(a, 64 * k + lane, &bad[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < kSeqs; k++) sum += plan_part(a, w[k].tiles);
+  bool any = bad[0] || bad[1] || bad[2] || bad[3];
+  for (int s = 64 * kSeqs + lane; s < a.seqs; s += 64) {
+    sum += plan_part(a, seq_work<SHIFT>(a, s, &b).tiles);
+    any |= b;
+  }
+  if (any && blockIdx.x == 0 && threadIdx.x < 64) paged_flag(a.status, kPagedStatusRows);
+  c = plan_chunk(a, __builtin_amdgcn_readlane(wave_scan(sum), 63));
+  if (a.seqs <= 64) {
+    // few sequences: all their chunks in one round of blocks
+    const int live = __builtin_popcountll(__ballot(w[0].tiles > 0));
+    if (2 * live <= a.round)
+      while (__builtin_amdgcn_readlane(wave_scan(plan_chunks_of(a, c, w[0].tiles)), 63) > a.round) c += (c + 7) / 8;
+  }
 #pragma unroll
   for (int k = 0; k < kSeqs; k++)
     if (64 * k < a.seqs && find(w[k], 64 * k)) return true;
@@ -820,6 +893,13 @@ void launch_attention_of(PagedArgs a, int cus, size_t part_floats, hipStream_t s
   // A split costs about 3.5 us (counting, joining), a round of the waves' tiles 0.8: up to
   // 32 tiles a sequence stays whole, and chunks have 16 at least.
   const int64_t record = 16 * (DT + 2);
+  a.plan = nullptr;
+  if (a.seqs > kPlanInPlace) {  // the plan lies before the records
+    const size_t ints = (2 * plan_groups(a.seqs) + 1 + 3) & ~3;
+    a.plan = reinterpret_cast<int*>(a.part);
+    a.part += ints;
+    part_floats -= ints;
+  }
   const int64_t fit = std::min<int64_t>((int64_t)part_floats / (2 * a.units * record), kPagedCounters / (2 * a.units));
   a.round = std::max(1, 8 / W * cus / a.units);
   a.chunks = (int)std::max<int64_t>(1, std::min<int64_t>(fit, a.round));
@@ -827,6 +907,7 @@ void launch_attention_of(PagedArgs a, int cus, size_t part_floats, hipStream_t s
   a.whole = 32;
   const int64_t per_seq = fit < 1 || tiles <= a.whole ? 1 : (tiles + a.chunk_min - 1) / a.chunk_min;
   const int64_t blocks = std::min<int64_t>(a.chunks + a.seqs, a.seqs * per_seq) * a.units;
+  if (a.plan) hipLaunchKernelGGL((paged_plan_kernel<T::SHIFT>), dim3(1), dim3(kPlanThreads), 0, st, a);
   hipLaunchKernelGGL((paged_attention_kernel<KT, DT, W, STREAM>), dim3((unsigned)blocks), dim3(64 * W), 0, st, a);
 }
 
