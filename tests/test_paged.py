@@ -125,3 +125,58 @@ def test_null_arguments_refused():
         assert rc == tlm.TLM_ERR_INVALID
         assert L.tlm_last_error().startswith((b"TLMPaged: ", b"TLMVerify: "))
     L.tlm_paged_destroy(None)
+
+
+def buffer(nbytes):
+    b = tlm.Buffer.__new__(tlm.Buffer)  # an address that no call gets as far as
+    b.ctx, b.nbytes, b.ptr = None, nbytes, ctypes.c_void_p(4096)
+    return b
+
+
+def says(part, call, *args, **kw):
+    with pytest.raises(tlm.TlmError) as e:
+        call(*args, **kw)
+    assert e.value.code == tlm.TLM_ERR_INVALID and part in str(e.value), str(e.value)
+
+
+@pytest.mark.parametrize("fmt,size", [(tlm.FMT_F16, 2), (tlm.FMT_F32, 4)])
+def test_rows_that_a_buffer_does_not_hold_are_refused(fmt, size):
+    """A byte too few is refused before the call; enough reaches it, and it has no handle here."""
+    p = tlm.Paged.__new__(tlm.Paged)
+    p.ctx, p.ptr, p.desc = None, None, tlm.paged_desc(6, 2, 64, 100, page_tokens=32)
+    p.sizes = tlm.paged_sizes(p.desc)
+    pool, small = buffer(3 * p.page_bytes()), buffer(1 << 10)
+    b = p.batch(pool, pool, 3, small, 4, small, 5, 7)
+    rows, whole = 35, buffer(35 * 10 * 64 * 4)
+    qkv, q, out = rows * 10 * 64 * 4, rows * 6 * 64 * 4, rows * 6 * 64 * size
+    says("qkv holds", p.append, b, buffer(qkv - 1), whole)
+    says("q holds", p.append, b, whole, buffer(q - 1))
+    says("q holds", p.attention, b, buffer(q - 1), whole, fmt)
+    says("out holds", p.attention, b, whole, buffer(out - 1), fmt)
+    says("null", p.append, b, buffer(qkv), buffer(q))
+    says("null", p.append, b, buffer(qkv))
+    says("null", p.attention, b, buffer(q), buffer(out), fmt)
+    # a batch of another handle, whose pages are smaller
+    p.sizes = tlm.paged_sizes(tlm.paged_desc(6, 2, 64, 100, page_tokens=64))
+    says("k_pages holds", p.append, b, whole, whole)
+    says("k_pages holds", p.attention, b, whole, whole, fmt)
+
+
+def test_verification_buffers_that_are_too_small_are_refused():
+    s, t, v = 3, 4, 100
+    need = dict(logits_buf=4 * s * t * v, accepted=4 * s, out_tokens=4 * s * t, drafts=4 * s * (t - 1),
+                draft_logits=4 * s * (t - 1) * v, counts=4 * s, uniforms=4 * s * t)
+
+    class Ctx:
+        ptr = None
+
+    def call(temperature, **sizes):
+        b = {k: buffer(n) for k, n in {**need, **sizes}.items()}
+        tlm.verify_drafts(Ctx, b.pop("logits_buf"), s, t, v, b.pop("accepted"), b.pop("out_tokens"),
+                          temperature=temperature, **b)
+
+    for temperature in (0.0, 0.7):
+        says("invalid argument", call, temperature)
+        for name, n in need.items():
+            read = temperature > 0 or name not in ("draft_logits", "uniforms")
+            says("holds" if read else "invalid argument", call, temperature, **{name: n - 1})

@@ -404,6 +404,12 @@ def paged_locate(desc: PagedDesc, num_pages: int, table, position: int, kv_head:
     return k.value, v.value
 
 
+def paged_sizes(d: PagedDesc):
+    """(bytes of a page in one pool, elements of a row of queries, of a row of q|k|v)."""
+    return (d.kv_heads * d.page_tokens * d.head_dim * (4 if d.kv_fmt == FMT_F32 else 2), d.heads * d.head_dim,
+            (d.heads + 2 * d.kv_heads) * d.head_dim)
+
+
 def _addr(b):
     return None if b is None else b.ptr
 
@@ -415,14 +421,14 @@ class Paged:
     def __init__(self, ctx: Context, heads, kv_heads, head_dim, max_tokens, page_tokens=64, **options):
         self.ctx = ctx
         self.desc = paged_desc(heads, kv_heads, head_dim, max_tokens, page_tokens, **options)
+        self.sizes = paged_sizes(self.desc)
         p = VP()
         check(lib().tlm_paged_create(ctx.ptr, ctypes.byref(self.desc), ctypes.byref(p)))
         self.ptr = p
 
     def page_bytes(self) -> int:
         """Bytes of one page in the K pool, and again in the V pool."""
-        d = self.desc
-        return d.kv_heads * d.page_tokens * d.head_dim * (4 if d.kv_fmt == FMT_F32 else 2)
+        return self.sizes[0]
 
     def batch(self, k_pages: Buffer, v_pages: Buffer, num_pages: int, tables: Buffer, table_width: int, starts: Buffer,
               seqs: int, tokens: int = 1, counts: Optional[Buffer] = None) -> PagedBatch:
@@ -435,17 +441,47 @@ class Paged:
                 raise TlmError(TLM_ERR_INVALID, f"TLMPaged: {name} holds {b.nbytes} bytes of {need}")
         b = PagedBatch(k_pages.ptr, v_pages.ptr, tables.ptr, starts.ptr, _addr(counts), num_pages, table_width, seqs,
                        tokens)
-        b.keep = (k_pages, v_pages, tables, starts, counts)
+        b.keep, b.page = (k_pages, v_pages, tables, starts, counts), self.sizes[0]
         return b
+
+    def _short(self, batch: PagedBatch, name: str, b, need: int):
+        """Raises for a buffer smaller than what the kernels read or write of it, unless the call refuses by itself."""
+        if batch.seqs * batch.tokens * self.desc.heads <= 1 << 22:
+            raise TlmError(TLM_ERR_INVALID, f"TLMPaged: {name} holds {b.nbytes} bytes of {need}")
+
+    def _pools(self, batch: PagedBatch):
+        for name, b in zip(("k_pages", "v_pages"), getattr(batch, "keep", ())):
+            need = batch.num_pages * self.sizes[0]
+            if getattr(b, "nbytes", need) < need:
+                self._short(batch, name, b, need)
 
     def append(self, batch: PagedBatch, qkv: Buffer, q: Optional[Buffer] = None) -> Optional[Buffer]:
         """qkv fp32 [seqs][tokens][(H+2Hkv)D]: K and V to their pages, the rotated queries to q fp32 [..][H D]."""
-        check(lib().tlm_op_paged_append(self.ptr, ctypes.byref(batch), qkv.ptr, _addr(q)))
+        page, n, width = self.sizes
+        rows = batch.seqs * batch.tokens
+        if isinstance(qkv, Buffer) and qkv.nbytes < 4 * rows * width:
+            self._short(batch, "qkv", qkv, 4 * rows * width)
+        if isinstance(q, Buffer) and q.nbytes < 4 * rows * n:
+            self._short(batch, "q", q, 4 * rows * n)
+        if getattr(batch, "page", 0) != page:  # of another handle
+            self._pools(batch)
+        rc = lib().tlm_op_paged_append(self.ptr, batch, qkv.ptr, None if q is None else q.ptr)
+        if rc:
+            check(rc)
         return q
 
     def attention(self, batch: PagedBatch, q: Buffer, out: Buffer, out_fmt: int = FMT_F16) -> Buffer:
         """Rotated queries fp32 [seqs][tokens][H D] over the pages -> out in out_fmt."""
-        check(lib().tlm_op_paged_attention(self.ptr, ctypes.byref(batch), q.ptr, out_fmt, out.ptr))
+        n = batch.seqs * batch.tokens * self.sizes[1]
+        if isinstance(q, Buffer) and q.nbytes < 4 * n:
+            self._short(batch, "q", q, 4 * n)
+        if isinstance(out, Buffer) and out.nbytes < (4 * n if out_fmt == FMT_F32 else 2 * n):
+            self._short(batch, "out", out, 4 * n if out_fmt == FMT_F32 else 2 * n)
+        if getattr(batch, "page", 0) != self.sizes[0]:  # of another handle
+            self._pools(batch)
+        rc = lib().tlm_op_paged_attention(self.ptr, batch, q.ptr, out_fmt, out.ptr)
+        if rc:
+            check(rc)
         return out
 
     def status(self):
@@ -497,6 +533,17 @@ def verify_drafts(ctx: Context, logits_buf: Buffer, seqs: int, tokens: int, voca
                   out_tokens: Buffer, drafts: Optional[Buffer] = None, draft_logits: Optional[Buffer] = None,
                   counts: Optional[Buffer] = None, uniforms: Optional[Buffer] = None, temperature: float = 1.0):
     """Which drafts stand and the token after them (tlm_op_verify_drafts); (accepted, out_tokens)."""
+    # a buffer smaller than what the kernels read or write, unless the call refuses by itself: 12 bytes of 32 MiB for
+    # every 2048 entries of the rows of 4096 sequences
+    rows, drafted, drawn = seqs * tokens, seqs * (tokens - 1), int(temperature > 0)
+    cells = min(seqs, 4096) * (2 * tokens - 1 if draft_logits is not None and drawn else tokens) * -(-vocab // 2048)
+    if tokens <= 64 and vocab <= 524288 and rows <= 1 << 20 and 12 * cells <= 32 << 20:
+        for name, b, need in (("logits", logits_buf, 4 * rows * vocab), ("drafts", drafts, 4 * drafted),
+                              ("draft_logits", draft_logits, 4 * drawn * drafted * vocab), ("counts", counts, 4 * seqs),
+                              ("uniforms", uniforms, 4 * drawn * rows), ("accepted", accepted, 4 * seqs),
+                              ("out_tokens", out_tokens, 4 * rows)):
+            if isinstance(b, Buffer) and b.nbytes < need:
+                raise TlmError(TLM_ERR_INVALID, f"TLMVerify: {name} holds {b.nbytes} bytes of {need}")
     check(lib().tlm_op_verify_drafts(ctx.ptr, logits_buf.ptr, _addr(draft_logits), _addr(drafts), _addr(counts),
                                      _addr(uniforms), seqs, tokens, vocab, float(temperature), accepted.ptr,
                                      out_tokens.ptr))
