@@ -203,13 +203,14 @@ int tlm_paged_create(tlm_ctx* ctx, const tlm_paged_desc* desc, tlm_paged** out);
 void tlm_paged_destroy(tlm_paged* paged);
 /* qkv: fp32 [seqs][tokens][(heads + 2 kv_heads) * head_dim] (Q|K|V, bias
  * included, pre-RoPE).  The rotated K and the V rows go to their pages; q, when
- * not NULL: fp32 [seqs][tokens][heads * head_dim], the rotated queries, apart
- * from qkv.  Any number of tokens.  Enqueue only. */
+ * not NULL: fp32 [seqs][tokens][heads * head_dim], the rotated queries.  qkv, q,
+ * the pools and the batch's tables and lengths are apart.  Any number of tokens.
+ * Enqueue only. */
 int tlm_op_paged_append(tlm_paged* paged, const tlm_paged_batch* batch, const float* qkv, float* q);
 /* Attention of every row over positions [max(0, pos - W + 1), pos] of its
  * sequence, which the pages hold (append first).  q: fp32 [seqs][tokens]
  * [heads * head_dim], rotated; out: the same shape in out_fmt, TLM_FMT_F16 or
- * TLM_FMT_F32, apart from q.  Scores and the weighted sum to 32 bits: an fp16
+ * TLM_FMT_F32, apart from q and all that the batch names.  Scores and the weighted sum to 32 bits: an fp16
  * cache's products take q and the probabilities as pairs of fp16 values, each to
  * 2^-22 of itself or 2^-39 of its row's largest.  What masked positions hold does
  * not matter; attended K and V are finite.  Enqueue only. */

@@ -697,6 +697,40 @@ def test_refusals(ctx):
     sv.close()
 
 
+@pytest.mark.parametrize("name", ["k_pages", "v_pages", "tables", "starts", "counts"])
+def test_results_over_what_the_batch_names_are_refused(ctx, name):
+    """Every block reads the lengths and its pages for itself, while others write."""
+    sv = Serving(ctx, 4, 2, 64, [5, 40], 2, 32, counts=[2, 1])
+    b = sv.upload(*sv.pools([7, 41]))
+    x, q, out = ctx.buffer(4 * 8 * 64 * 4), ctx.buffer(4 * 4 * 64 * 4), ctx.buffer(4 * 4 * 64 * 4)
+    last = {"k_pages": sv.kb.nbytes, "v_pages": sv.vb.nbytes, "tables": 8 * sv.width, "starts": 8, "counts": 8}[name] - 4
+
+    class At:
+        def __init__(self, base, offset):
+            self.ptr = ctypes.c_void_p(base + offset)
+
+    def refuse(call, *args):
+        with pytest.raises(tlm.TlmError) as e:
+            call(*args)
+        assert e.value.code == tlm.TLM_ERR_INVALID and "overlap" in str(e.value)
+
+    at = At(getattr(b, name), last)
+    refuse(sv.paged.append, b, x, at)
+    for fmt in (tlm.FMT_F16, tlm.FMT_F32):
+        refuse(sv.paged.attention, b, q, at, fmt)
+    if name.endswith("pages"):
+        refuse(sv.paged.append, b, at, q)
+        for other in ("tables", "starts", "counts"):
+            keep = getattr(b, other)
+            setattr(b, other, getattr(b, name))
+            refuse(sv.paged.append, b, x, q)
+            setattr(b, other, keep)
+    sv.paged.append(b, x, q)
+    sv.paged.attention(b, q, out)
+    sv.paged.status()
+    sv.close()
+
+
 def test_calls_allocate_nothing(ctx):
     sv = Serving(ctx, 8, 2, 64, [5000, 90, -1], 4, 32)
     sv.upload(*sv.pools([5004, 94, 0]))

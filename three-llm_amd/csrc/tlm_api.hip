@@ -1214,6 +1214,22 @@ void tlm_paged_destroy(tlm_paged* P) {
   delete P;
 }
 
+static size_t paged_pool_words(const tlm_paged* P, const tlm_paged_batch* b) {  // 4 bytes each
+  const size_t page = (size_t)P->d.kv_heads * P->d.page_tokens * P->d.head_dim;
+  return b->num_pages * (P->d.kv_fmt == TLM_FMT_F32 ? page : page / 2);
+}
+
+// Whether words [p, p + n) share an address with the batch's tables or lengths, which
+// every block reads for itself, or with its pools.
+static bool over_lengths(const tlm_paged_batch* b, const void* p, size_t n) {
+  return overlap(p, n, b->tables, (size_t)b->seqs * b->table_width) || overlap(p, n, b->starts, b->seqs) ||
+         (b->counts && overlap(p, n, b->counts, b->seqs));
+}
+static bool over_pools(const tlm_paged* P, const tlm_paged_batch* b, const void* p, size_t n) {
+  const size_t pool = paged_pool_words(P, b);
+  return overlap(p, n, b->k_pages, pool) || overlap(p, n, b->v_pages, pool);
+}
+
 static int paged_args(const tlm_paged* P, const tlm_paged_batch* b, PagedArgs& a) {
   if (!P || !b) return fail(TLM_ERR_INVALID, "TLMPaged: null argument");
   if (!b->k_pages || !b->v_pages || !b->tables || !b->starts)
@@ -1226,8 +1242,7 @@ static int paged_args(const tlm_paged* P, const tlm_paged_batch* b, PagedArgs& a
                 P->d.heads);
   if ((reinterpret_cast<uintptr_t>(b->k_pages) | reinterpret_cast<uintptr_t>(b->v_pages)) % 16)
     return fail(TLM_ERR_INVALID, "TLMPaged: a pool is not 16-byte aligned");
-  const size_t page = (size_t)P->d.kv_heads * P->d.page_tokens * P->d.head_dim;
-  const size_t pool = b->num_pages * (P->d.kv_fmt == TLM_FMT_F32 ? page : page / 2);
+  const size_t pool = paged_pool_words(P, b);
   if (overlap(b->k_pages, pool, b->v_pages, pool)) return fail(TLM_ERR_INVALID, "TLMPaged: the pools overlap");
   memset(&a, 0, sizeof a);
   a.kc = b->k_pages;
@@ -1261,6 +1276,12 @@ int tlm_op_paged_append(tlm_paged* P, const tlm_paged_batch* b, const float* qkv
   const size_t rows = (size_t)a.seqs * a.tokens;
   if (q && overlap(qkv, rows * (a.Hq + 2 * a.Hkv) * a.D, q, rows * a.Hq * a.D))
     return fail(TLM_ERR_INVALID, "TLMPaged: the rotated queries overlap qkv");
+  if (q && (over_pools(P, b, q, rows * a.Hq * a.D) || over_lengths(b, q, rows * a.Hq * a.D)))
+    return fail(TLM_ERR_INVALID, "TLMPaged: the rotated queries overlap the pools, the tables or the lengths");
+  const size_t pool = paged_pool_words(P, b);
+  if (over_pools(P, b, qkv, rows * (a.Hq + 2 * a.Hkv) * a.D) || over_lengths(b, b->k_pages, pool) ||
+      over_lengths(b, b->v_pages, pool))
+    return fail(TLM_ERR_INVALID, "TLMPaged: the pools overlap qkv, the tables or the lengths");
   a.x = qkv;
   a.q = q;
   const DeviceScope on(P->ctx->device);
@@ -1277,8 +1298,10 @@ int tlm_op_paged_attention(tlm_paged* P, const tlm_paged_batch* b, const float* 
   if (out_fmt != TLM_FMT_F16 && out_fmt != TLM_FMT_F32)
     return fail(TLM_ERR_INVALID, "TLMPaged: output format %d is not fp16 or fp32", out_fmt);
   const size_t n = (size_t)a.seqs * a.tokens * a.Hq * a.D;  // a multiple of 32
-  if (overlap(q, n, out, out_fmt == TLM_FMT_F32 ? n : n / 2))
-    return fail(TLM_ERR_INVALID, "TLMPaged: out overlaps q");
+  const size_t words = out_fmt == TLM_FMT_F32 ? n : n / 2;
+  if (overlap(q, n, out, words)) return fail(TLM_ERR_INVALID, "TLMPaged: out overlaps q");
+  if (over_pools(P, b, out, words) || over_lengths(b, out, words))
+    return fail(TLM_ERR_INVALID, "TLMPaged: out overlaps the pools, the tables or the lengths");
   a.x = q;
   a.out = out;
   a.out_f32 = out_fmt == TLM_FMT_F32;
