@@ -697,6 +697,16 @@ def test_refusals(ctx):
     sv.close()
 
 
+def test_rope_tables_past_the_memory_are_refused(ctx):
+    """512 GB of tables: refused before any is computed.  Without RoPE there are none."""
+    free = ctx.memory()[0]
+    with pytest.raises(tlm.TlmError) as e:
+        tlm.Paged(ctx, 32, 8, 128, 1 << 30, inv_freq=np.ones(64, np.float32))
+    assert e.value.code == tlm.TLM_ERR_OOM and "RoPE" in str(e.value)
+    assert ctx.memory()[0] == free
+    tlm.Paged(ctx, 32, 8, 128, 1 << 30).close()
+
+
 @pytest.mark.parametrize("name", ["k_pages", "v_pages", "tables", "starts", "counts"])
 def test_results_over_what_the_batch_names_are_refused(ctx, name):
     """Every block reads the lengths and its pages for itself, while others write."""

@@ -10,6 +10,7 @@
 #include <exception>
 #include <map>
 #include <mutex>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -818,14 +819,15 @@ int tlm_op_gated_mlp(tlm_linear* gu, tlm_linear* down, const float* x, float* y)
 
 // cos/sin of pos * inv_freq[j] in double, times the attention factor, rounded
 // to fp32 (the CPU reference evaluates the angle in double, math.ts:144-146).
-static void rope_tables(int max_tokens, int rd, const float* inv_freq, double af, std::vector<float>& cs,
-                        std::vector<float>& sn) {
+// Positions first .. first + count - 1.
+static void rope_tables(int count, int rd, const float* inv_freq, double af, std::vector<float>& cs,
+                        std::vector<float>& sn, int first = 0) {
   const int half = rd / 2;
-  cs.assign((size_t)max_tokens * half, 0.f);
-  sn.assign((size_t)max_tokens * half, 0.f);
-  for (int p = 0; p < max_tokens; p++)
+  cs.assign((size_t)count * half, 0.f);
+  sn.assign((size_t)count * half, 0.f);
+  for (int p = 0; p < count; p++)
     for (int j = 0; j < half; j++) {
-      const double angle = (double)p * (double)inv_freq[j];
+      const double angle = (double)(first + p) * (double)inv_freq[j];
       cs[(size_t)p * half + j] = (float)(cos(angle) * af);
       sn[(size_t)p * half + j] = (float)(sin(angle) * af);
     }
@@ -1173,27 +1175,39 @@ int tlm_paged_create(tlm_ctx* ctx, const tlm_paged_desc* desc, tlm_paged** out) 
   if (!ctx || !desc || !out) return fail(TLM_ERR_INVALID, "TLMPaged: null argument");
   if (const int rc = paged_check(desc)) return rc;
   const DeviceScope on(ctx->device);
-  std::vector<float> cs, sn;
-  tlm_paged* P = nullptr;
-  try {
-    P = new tlm_paged();
-    if (desc->rotary_dim > 0)
-      rope_tables(desc->max_tokens, desc->rotary_dim, desc->inv_freq, desc->attention_factor, cs, sn);
-  } catch (const std::exception&) {
-    delete P;
-    return fail(TLM_ERR_OOM, "TLMPaged: no host memory for %d positions", desc->max_tokens);
-  }
+  // Tables that the device has no room for (1 KB a position at 128 dims) are refused
+  // before any of them is computed; the others go up in parts of kRopePart floats.
+  constexpr int kRopePart = 1 << 22;
+  const int half = desc->rotary_dim / 2;
+  const size_t bytes = (size_t)desc->max_tokens * half * sizeof(float);
+  size_t room = 0, all = 0;
+  HIP_TRY(hipMemGetInfo(&room, &all));
+  if (2 * bytes > room)
+    return fail(TLM_ERR_OOM, "TLMPaged: RoPE tables of %d positions take %zu bytes, and %zu are free", desc->max_tokens,
+                2 * bytes, room);
+  tlm_paged* P = new (std::nothrow) tlm_paged();
+  if (!P) return fail(TLM_ERR_OOM, "TLMPaged: no host memory");
   P->ctx = ctx;
   P->d = *desc;
   P->d.inv_freq = nullptr;  // the caller's
   P->scale = (float)(desc->attn_scale > 0 ? desc->attn_scale : 1.0 / sqrt((double)desc->head_dim));
   hipError_t e = hipMalloc(&P->status, sizeof(int));
   if (e == hipSuccess) e = hipMemset(P->status, 0, sizeof(int));
-  const size_t bytes = cs.size() * sizeof(float);
   if (e == hipSuccess && bytes) e = hipMalloc(&P->rope_cos, bytes);
   if (e == hipSuccess && bytes) e = hipMalloc(&P->rope_sin, bytes);
-  if (e == hipSuccess && bytes) e = hipMemcpy(P->rope_cos, cs.data(), bytes, hipMemcpyHostToDevice);
-  if (e == hipSuccess && bytes) e = hipMemcpy(P->rope_sin, sn.data(), bytes, hipMemcpyHostToDevice);
+  try {
+    std::vector<float> cs, sn;
+    for (int p = 0; e == hipSuccess && bytes && p < desc->max_tokens;) {
+      const int count = std::min(desc->max_tokens - p, kRopePart / half);
+      const size_t at = (size_t)p * half, n = (size_t)count * half * sizeof(float);
+      rope_tables(count, desc->rotary_dim, desc->inv_freq, desc->attention_factor, cs, sn, p);
+      e = hipMemcpy(P->rope_cos + at, cs.data(), n, hipMemcpyHostToDevice);
+      if (e == hipSuccess) e = hipMemcpy(P->rope_sin + at, sn.data(), n, hipMemcpyHostToDevice);
+      p += count;
+    }
+  } catch (const std::exception&) {
+    e = hipErrorOutOfMemory;
+  }
   if (e == hipSuccess) e = hipStreamSynchronize(nullptr);  // the fill is on another stream than the context's
   if (e != hipSuccess) {
     tlm_paged_destroy(P);
