@@ -278,7 +278,7 @@ typedef _Float16 ph8_t __attribute__((ext_vector_type(8)));
 // of its group) are the columns of 16-column matrix-core tiles, so that K and V are
 // read once for 16 of them; a block has one column tile (a unit is a kv head and a
 // row group).  Several tiles a block were slower everywhere, as their outputs leave
-// room for fewer waves (16 x 16 Llama-3.2-3B at 2000 positions 31.9 us with four, 22.1 so;
+// room for fewer waves (16 x 16 Llama-3.2-3B up to 2000 positions 31.9 us with four, 22.1 so;
 // Qwen2.5-0.5B 16 x 5 20.5 and 10.2; a 2048-token prompt of Llama-3.2-1B 112 and 65).  The W
 // waves take the position tiles of one chunk of the sequence in turn:
 //   * scores S^T (positions x rows) = K Q^T, K the A operand, q the B operand;
@@ -745,8 +745,8 @@ __global__ __launch_bounds__(64 * W, DT <= 64 ? 4 : 2) void paged_attention_kern
 
   // The next tile's K goes out when this one's has been read, its V likewise: half a
   // tile or more in flight a wave, and the registers of one (with two, 8 waves a CU
-  // instead of 16 at head_dim 64 and less in flight: 128 x 1 Llama-3.2-1B at 1000
-  // positions 31.8 instead of 28.1 us).
+  // instead of 16 at head_dim 64 and less in flight: 128 x 1 Llama-3.2-1B up to
+  // 1000 positions 31.8 instead of 28.1 us).
   while (tb < t1) {
     for (int i = 0; i < n; i++) {
       const bool more = i + 1 < n;
@@ -912,14 +912,15 @@ void launch_attention_of(PagedArgs a, int cus, size_t part_floats, hipStream_t s
 }
 
 // Waves a block: four where the sequences' kv heads and row groups alone give a
-// block a CU (a short sequence then leaves no waves idle), else eight.  us a call,
-// 8 / 4 waves: 128 x 1 Llama-3.2-1B at 1000 positions 25.1 / 22.7, 256 x 1 44.6 / 36.3, 64 x 1
-// Llama-3.2-3B 28.9 / 26.7, 16 x 8 at 2000 20.3 / 18.4; 16 x 5 at 2500 17.0 / 19.7, Qwen2.5-0.5B
-// 1 x 1 at 300 5.6 / 6.2, 16 x 5 at 2000 10.2 / 11.5.
+// block a CU (a short sequence then leaves no waves idle), else eight.  us a call over
+// four sets of inputs in turn, sequences of a 16th of the positions named to all of
+// them, 8 / 4 waves: 128 x 1 Llama-3.2-1B up to 1000 positions 26.6 / 25.0, 256 x 1 45.6 /
+// 41.3, 64 x 1 Llama-3.2-3B 30.0 / 28.6, 16 x 8 up to 2000 20.8 / 18.8; 16 x 5 up to 2500 17.5 /
+// 21.9, Qwen2.5-0.5B 1 x 1 at 300 5.6 / 6.4, 16 x 5 up to 2000 10.2 / 11.7.
 // Past the last-level cache (256 MB), streaming loads where K and V may exceed it and
 // are read once, as nothing of them is still there for the next call: 256 x 1
-// Llama-3.2-1B at 1000 40.3 -> 36.3, 64 x 1 at 8192 76.4 -> 70.9; what fits it is faster kept
-// (64 x 1 at 1000 13.5, streaming 15.4).
+// Llama-3.2-1B up to 1000 41.3 -> 36.1, 64 x 1 up to 8192 77.9 -> 71.1; what fits it is faster
+// kept (64 x 1 up to 1000 13.6, streaming 15.6).
 template <typename KT, int DT>
 void launch_attention_rows(PagedArgs a, int cus, size_t part_floats, hipStream_t st) {
   const int groups = (a.tokens * a.G + 15) / 16;
