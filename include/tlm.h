@@ -47,6 +47,10 @@ enum {
  *                w = f32(scale[n][k/32]) * q.  K must be a multiple of 32.
  *   TLM_FMT_F32: float [N][K] (embedding tables only). */
 enum { TLM_FMT_F16 = 1, TLM_FMT_Q4 = 2, TLM_FMT_F32 = 3 };
+/*   TLM_FMT_F8: 8-bit floating point (e4m3: sign, 4 bits of exponent, 3 of
+ *                mantissa; up to 448, no infinities) with an fp32 scale, a power of
+ *                two, for each 32 tokens and kv head (paged caches only). */
+enum { TLM_FMT_F8 = 4 };
 
 typedef struct tlm_ctx tlm_ctx;
 typedef struct tlm_linear tlm_linear;
@@ -173,7 +177,7 @@ typedef struct tlm_paged_desc {
                                                     max_tokens: positions a sequence can have */
   int32_t rotary_dim;       /* 0 disables RoPE */
   int32_t sliding_window;   /* 0 = full causal */
-  int32_t kv_fmt;           /* TLM_FMT_F16 or TLM_FMT_F32 */
+  int32_t kv_fmt;           /* TLM_FMT_F16, TLM_FMT_F32 or TLM_FMT_F8 */
   int32_t page_tokens;      /* a power of two from 32 to 1024 */
   const float* inv_freq;    /* host, rotary_dim/2 entries (ropeParameters) */
   double attention_factor;  /* ropeParameters().attentionFactor */
@@ -191,8 +195,9 @@ typedef struct tlm_paged_desc {
  * All pointers are device memory; the struct itself is the host's and is read
  * during the call.  seqs * tokens * heads is at most 2^22. */
 typedef struct tlm_paged_batch {
-  void* k_pages;            /* pools of num_pages * kv_heads * page_tokens * head_dim kv_fmt elements, 16-byte */
-  void* v_pages;            /* aligned and apart, in the order that tlm_paged_locate tells */
+  void* k_pages;            /* pools of num_pages * kv_heads * page_tokens * head_dim kv_fmt elements (TLM_FMT_F8: */
+  void* v_pages;            /* and scales; tlm_paged_page_bytes a page), 16-byte aligned and apart, in the order */
+                            /* that tlm_paged_locate tells */
   const int32_t* tables;    /* [seqs][table_width] */
   const int32_t* starts;    /* [seqs] */
   const int32_t* counts;    /* [seqs] or NULL */
@@ -201,18 +206,64 @@ typedef struct tlm_paged_batch {
 
 int tlm_paged_create(tlm_ctx* ctx, const tlm_paged_desc* desc, tlm_paged** out);
 void tlm_paged_destroy(tlm_paged* paged);
+/* Bytes of a page in one pool.  Host only: needs no device. */
+int tlm_paged_page_bytes(const tlm_paged_desc* desc, size_t* bytes);
+/* Positions [0, sinks) stay visible behind a sliding window (attention sinks, a
+ * system prompt): a row at position p attends to them and to (p - W, p].  For the
+ * calls on the handle from here on; 0 at first.  Positions stay what they are. */
+int tlm_paged_set_sinks(tlm_paged* paged, int32_t sinks);
+/* One step's page tables from the lengths of its sequences.  Sequence s has
+ * lengths[s] positions (< 0: it has ended) and wants min(counts[s], tokens) rows
+ * more (counts NULL: tokens; < 1: none now).  It needs the pages of its new rows
+ * and of what its next row sees: all before it, or its window and its sinks.
+ * Pages that its table holds besides are given back: refs - 1.  Then the
+ * sequences get the pages that they lack, in their order, the free ones (refs 0)
+ * lowest first, refs 1, for as long as what they have lacked so far is no more than
+ * what is free; one that it is not enough for keeps what it holds.  An entry
+ * that is no page of the pool is none.  refs counts the tables that a page is in,
+ * and holds of the caller's own (a prefix that is kept); pages may be shared,
+ * each table counted.
+ * starts: lengths[s] where the sequence's rows are served, else -1 (no rows
+ * wanted, no pages left, or a page with positions that it needs below its length is
+ * not held: tlm_paged_status reports that, and rows past max_tokens or
+ * the table, which are left out).  slots (or NULL): page * page_tokens + token of
+ * each row, -1 of those that are not there.  Entries that hold no page are -1.
+ * tables, starts and counts are then a batch's.  All pointers are device memory;
+ * the struct is the host's and read during the call. */
+typedef struct tlm_paged_request {
+  const int32_t* lengths;   /* [seqs] */
+  const int32_t* counts;    /* [seqs] or NULL */
+  const int32_t* tables;    /* [seqs][table_width], as they are */
+  const int32_t* refs;      /* [num_pages] */
+  int32_t* out_tables;      /* as they become: tables and refs themselves, or apart */
+  int32_t* out_refs;        /* (what would be given, without giving it) */
+  int32_t* starts;          /* [seqs] */
+  int64_t* slots;           /* [seqs][tokens] or NULL */
+  int32_t num_pages, table_width, seqs, tokens;
+} tlm_paged_request;
+/* seqs * tokens * heads is at most 2^22, seqs 2^20.  The results are apart from each
+ * other and from the inputs, but for tables and refs in place.  Enqueue only. */
+int tlm_op_paged_reserve(tlm_paged* paged, const tlm_paged_request* request);
 /* qkv: fp32 [seqs][tokens][(heads + 2 kv_heads) * head_dim] (Q|K|V, bias
  * included, pre-RoPE).  The rotated K and the V rows go to their pages; q, when
  * not NULL: fp32 [seqs][tokens][heads * head_dim], the rotated queries.  qkv, q,
  * the pools and the batch's tables and lengths are apart.  Any number of tokens.
- * Enqueue only. */
+ * Enqueue only.
+ * TLM_FMT_F8: a value is its code times the scale of its 32 aligned positions and kv
+ * head, 2^e from 2^-32 to 2^31, the least that takes the largest magnitude to at
+ * most 448.  Rows that start within 32 positions keep the scale that these have or, if
+ * they need it, raise it; the positions before them are then rounded again (exact but
+ * for magnitudes below 2^-14 of the largest).  Positions behind the appended rows, to
+ * the end of their 32, are lost; 32 positions that two sequences append to in one
+ * call are lost.  Values that are not finite become NaN. */
 int tlm_op_paged_append(tlm_paged* paged, const tlm_paged_batch* batch, const float* qkv, float* q);
 /* Attention of every row over positions [max(0, pos - W + 1), pos] of its
  * sequence, which the pages hold (append first).  q: fp32 [seqs][tokens]
  * [heads * head_dim], rotated; out: the same shape in out_fmt, TLM_FMT_F16 or
  * TLM_FMT_F32, apart from q and all that the batch names.  Scores and the weighted sum to 32 bits: an fp16
  * cache's products take q and the probabilities as pairs of fp16 values, each to
- * 2^-22 of itself or 2^-39 of its row's largest.  What masked positions hold does
+ * 2^-22 of itself or 2^-39 of its row's largest (an 8-bit cache's too, whose codes
+ * are exact in fp16; there the probabilities times V's scales).  What masked positions hold does
  * not matter; attended K and V are finite.  Enqueue only. */
 int tlm_op_paged_attention(tlm_paged* paged, const tlm_paged_batch* batch, const float* q, int out_fmt, void* out);
 /* Waits for the stream and tells of what the calls since the last status met on
@@ -225,6 +276,10 @@ int tlm_paged_status(tlm_paged* paged);
  * a host copy of the sequence's table.  Host only: needs no device. */
 int tlm_paged_locate(const tlm_paged_desc* desc, int32_t num_pages, const int32_t* table, int32_t table_width,
                      int32_t position, int32_t kv_head, int32_t dim, int64_t* k_index, int64_t* v_index);
+/* TLM_FMT_F8: where the fp32 scale of `position` lies, in bytes from the start of a K
+ * or a V pool.  Host only: needs no device. */
+int tlm_paged_scale_at(const tlm_paged_desc* desc, int32_t num_pages, const int32_t* table, int32_t table_width,
+                       int32_t position, int32_t kv_head, int64_t* byte);
 
 /* ------------------------------------------------------------------ logits
  * TSLLogits chunk layers + greedy sampler (tsl/TSLLogits.ts:40-69, :201-274):
@@ -238,6 +293,35 @@ int tlm_op_argmax(tlm_ctx* ctx, const float* logits, int n, int32_t* token);
  * take part; missing slots are (0, LOWEST_FLOAT).  1 <= k <= 16; device
  * tokens[k], scores[k].  Enqueue only. */
 int tlm_op_topk(tlm_ctx* ctx, const float* logits, int n, int k, double softcap, int32_t* tokens, float* scores);
+/* Penalties for repeated tokens, biases and masks on logits, for many sequences'
+ * rows at once, before a token is picked (tlm_op_argmax, tlm_op_topk,
+ * tlm_op_verify_drafts).  No counterpart in the reference, whose sampler takes the
+ * logits as they are (TSLLogits.ts:185-191: but for a softcap).
+ * Row j of sequence s follows its history and its drafts 0 .. j - 1; with c(v) the
+ * times that token v is in these, in this order:
+ *   c(v) > 0:  x = (x > 0 ? x / repetition : x * repetition) - presence - frequency * c(v)
+ *   x = x + the biases of v (one listed twice: both, in the list's order)
+ *   x = -inf where bit v % 32 of word v / 32 of the row's mask is 0.
+ * -inf never takes part in picking; where a mask leaves nothing, no token does.
+ * Token ids outside the vocabulary are nobody's. */
+typedef struct tlm_logit_rules {
+  const float* logits;           /* [seqs][tokens][vocab] */
+  float* out;                    /* the same shape: logits itself, or apart from all inputs */
+  const int32_t* counts;         /* [seqs] rows that are there (NULL: tokens); the others' results stay */
+  const int32_t* history;        /* [seqs][history_width] */
+  const int32_t* history_counts; /* [seqs] tokens of it that are there (NULL: all) */
+  const int32_t* drafts;         /* [seqs][tokens - 1], or NULL: none counts */
+  const float* repetition;       /* [seqs], above 0 (NULL: 1) */
+  const float* frequency;        /* [seqs] (NULL: 0) */
+  const float* presence;         /* [seqs] (NULL: 0) */
+  const int32_t* bias_ids;       /* [seqs][bias_width] */
+  const float* biases;           /* [seqs][bias_width] */
+  const uint32_t* masks;         /* [seqs][tokens][(vocab + 31) / 32] (NULL: nothing is masked) */
+  int32_t seqs, tokens, vocab, history_width, bias_width;
+} tlm_logit_rules;
+/* tokens <= 64, vocab <= 524288, seqs * tokens <= 2^20, bias_width <= 4096.
+ * Enqueue only. */
+int tlm_op_adjust_logits(tlm_ctx* ctx, const tlm_logit_rules* rules);
 /* Verification of drafted tokens, for many sequences at once: which of a
  * sequence's drafts the target's distribution lets stand, and the token after
  * them.  No counterpart in the reference (it samples one token at a time,

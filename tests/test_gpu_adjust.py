@@ -1,0 +1,187 @@
+"""Penalties, biases and masks on logits against their plain form (more_oracle.py).
+
+Tolerance: a division or product, a product and two differences, a sum for each bias of the token: each rounding is
+2^-24 of the largest of what it adds, so (4 + biases of the token) 2^-24 of the sum of the magnitudes.  Entries that no
+rule names are the logits' bits."""
+import numpy as np
+import pytest
+
+import more_oracle as mo
+import three_llm_amd.tlm as tlm
+
+pytestmark = pytest.mark.gpu
+
+EPS = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    c = tlm.Context(0)
+    yield c
+    c.close()
+
+
+def rules(n, t, v, seed=0, history=0, biases=0, masked=False, drafts=True, counts=None, penalties=True, said=True):
+    rng = np.random.default_rng([seed, n, t, v, history, biases])
+    ids = lambda *shape: np.where(rng.random(shape) < 0.05, rng.integers(-3, v + 3, shape),  # noqa: E731
+                                  rng.random(shape) ** 3 * v).astype(np.int32)
+    d = dict(logits=(rng.standard_normal((n, t, v)) * 4).astype(np.float32), counts=counts, history=None, said=None,
+             drafts=ids(n, t - 1) if drafts and t > 1 else None, repetition=None, frequency=None, presence=None,
+             bias_ids=None, biases=None, masks=None)
+    if history:
+        d["history"] = ids(n, history)
+        d["said"] = rng.integers(0, history + 2, n).astype(np.int32) if said else None
+    if penalties:
+        d["repetition"] = rng.uniform(0.7, 1.8, n).astype(np.float32)
+        d["frequency"], d["presence"] = (rng.uniform(-1, 1, n).astype(np.float32) for _ in range(2))
+    if biases:
+        d["bias_ids"], d["biases"] = ids(n, biases), (rng.standard_normal((n, biases)) * 5).astype(np.float32)
+        d["bias_ids"][:, -1] = d["bias_ids"][:, 0]
+    if masked:
+        d["masks"] = rng.integers(0, 2 ** 32, (n, t, -(-v // 32)), dtype=np.uint64).astype(np.uint32)
+        d["masks"][0, 0] = 0
+        d["masks"][-1, -1] = 0xFFFFFFFF
+    return d
+
+
+def run(ctx, d, in_place=False):
+    n, t, v = d["logits"].shape
+    put = lambda x: None if x is None else ctx.array(x)  # noqa: E731
+    b = {k: put(x) for k, x in d.items()}
+    out = b["logits"] if in_place else ctx.array(np.full((n, t, v), 77, np.float32))
+    r = tlm.logit_rules(b["logits"], n, t, v, out=out, counts=b["counts"], history=b["history"],
+                        history_width=0 if d["history"] is None else d["history"].shape[1], history_counts=b["said"],
+                        drafts=b["drafts"], repetition=b["repetition"], frequency=b["frequency"],
+                        presence=b["presence"], bias_ids=b["bias_ids"], biases=b["biases"],
+                        bias_width=0 if d["biases"] is None else d["biases"].shape[1], masks=b["masks"])
+    tlm.adjust_logits(ctx, r)
+    got = out.read().reshape(n, t, v)
+    if not in_place:
+        assert np.array_equal(b["logits"].read().reshape(n, t, v), d["logits"], equal_nan=True)
+    for x in {id(x): x for x in [*b.values(), out] if x is not None}.values():
+        x.free()
+    return got
+
+
+def check(ctx, d, in_place=False):
+    got = run(ctx, d, in_place)
+    n, t, v = got.shape
+    out = d["logits"] if in_place else np.full(got.shape, 77, np.float32)
+    want, size = mo.adjust(out=out, **d)
+    fine = np.isfinite(want)
+    assert np.array_equal(got[~fine], want[~fine].astype(np.float32), equal_nan=True)
+    most = 4 + (0 if d["bias_ids"] is None else d["bias_ids"].shape[1])
+    with np.errstate(invalid="ignore"):
+        assert np.all(np.abs(got[fine] - want[fine]) <= most * EPS * size[fine])
+    same = fine & (want == d["logits"])
+    assert np.array_equal(got[same], d["logits"][same])
+    return got
+
+
+@pytest.mark.parametrize("v", [1, 3, 31, 32, 33, 1000, 4095, 4096, 4097, 32000, 50257])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_vocabularies(ctx, v, in_place):
+    check(ctx, rules(3, 2, v, history=100, biases=7, masked=True), in_place)
+
+
+@pytest.mark.parametrize("history", [0, 1, 255, 257, 5000, 40000])
+@pytest.mark.parametrize("n,t", [(1, 1), (1, 5), (9, 3)])
+def test_histories(ctx, history, n, t):
+    check(ctx, rules(n, t, 9000, history=history))
+    check(ctx, rules(n, t, 9000, history=history, said=False), True)
+
+
+@pytest.mark.parametrize("biases", [1, 2, 300, 4096])
+def test_biases(ctx, biases):
+    check(ctx, rules(2, 2, 20000, biases=biases))
+    d = rules(2, 1, 5000, biases=biases, penalties=False)
+    d["bias_ids"][1] = 77  # all on one token, in order: a sum of that many
+    check(ctx, d)
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_each_rule_alone(ctx, in_place):
+    for kw in (dict(), dict(history=50), dict(drafts=True, history=0), dict(biases=4), dict(masked=True)):
+        d = rules(4, 3, 5003, **{"drafts": False, "penalties": False, **kw})
+        got = check(ctx, d, in_place)
+        if not kw:
+            assert np.array_equal(got, d["logits"])
+        for name in ("repetition", "frequency", "presence"):
+            d = rules(4, 3, 5003, **{"drafts": False, **kw})
+            for other in ("repetition", "frequency", "presence"):
+                if other != name:
+                    d[other] = None
+            check(ctx, d, in_place)
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_rows_that_are_not_there(ctx, in_place):
+    check(ctx, rules(6, 4, 3001, history=40, biases=3, masked=True, counts=np.array([4, 0, 1, -1, 3, 9], np.int32)), in_place)
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_values_that_are_not_finite(ctx, in_place):
+    """-inf stays; what a mask takes out may be anything; a row that it takes out whole is -inf."""
+    d = rules(2, 2, 4000, history=300, biases=5, masked=True)
+    x = d["logits"]
+    x[0, 0, ::3], x[0, 1, 5:9], x[1, 0, 100:200] = np.nan, np.inf, -np.inf
+    x[1, 1, 7] = -3.4e38
+    d["masks"][0, 0] = 0
+    got = check(ctx, d, in_place)
+    assert np.all(got[0, 0] == -np.inf)
+
+
+def test_the_same_twice(ctx):
+    """No order of counting changes a bit."""
+    d = rules(5, 3, 30000, history=3000, biases=200, masked=True)
+    d["history"] = d["history"] % 50
+    a = run(ctx, d)
+    for _ in range(3):
+        assert np.array_equal(run(ctx, d).view(np.uint32), a.view(np.uint32))
+
+
+def test_most_rows_and_the_largest_vocabulary(ctx):
+    check(ctx, rules(1, 64, 524288, history=64, masked=True))
+    check(ctx, rules(2000, 2, 40, history=3))
+
+
+def test_picking_after(ctx):
+    """A masked row's argmax is the best that is left, of one with nothing left there is none."""
+    d = rules(1, 2, 10000, masked=True)
+    d["masks"][0, 1] = 0x00010000
+    got = run(ctx, d)
+    out, acc, ids = ctx.array(got), ctx.buffer(4), ctx.buffer(8)
+    tlm.verify_drafts(ctx, out, 1, 2, 10000, acc, ids, drafts=ctx.array(np.array([[3]], np.int32)), temperature=0.0)
+    assert ids.read(np.int32)[0] == -1  # nothing is left of the first row
+    tok = ctx.buffer(4)
+    row = ctx.array(got[0, 1])
+    tlm.argmax(ctx, row, 10000, tok)
+    best = int(np.argmax(got[0, 1]))
+    assert tok.read(np.int32)[0] == best and best % 32 == 16
+
+
+def test_refused(ctx):
+    x, y = ctx.buffer(4 * 6 * 100), ctx.buffer(4 * 6 * 100)
+    ints = ctx.array(np.zeros(64, np.int32))
+
+    def call(**kw):
+        a = dict(seqs=3, tokens=2, vocab=100, out=y)
+        a.update(kw)
+        r = tlm.logit_rules(x, 1, 1, 1, out=a.pop("out"))
+        for k, v in a.items():
+            setattr(r, k, v)
+        tlm.adjust_logits(ctx, r)
+
+    call()
+    ctx.sync()
+    at = lambda b, by: b.ptr.value + by  # noqa: E731
+    for kw, code in ((dict(seqs=0), -1), (dict(tokens=0), -1), (dict(vocab=0), -1), (dict(tokens=65), -1),
+                     (dict(vocab=524289), -1), (dict(seqs=1 << 20), -5), (dict(history_width=5), -1),
+                     (dict(history_width=-1), -1), (dict(bias_width=2), -1), (dict(bias_width=-1), -1),
+                     (dict(bias_width=4097, bias_ids=ints.ptr, biases=ints.ptr), -1),
+                     (dict(logits=at(y, 4)), -1), (dict(masks=at(y, 0)), -1), (dict(counts=at(y, 2396)), -1),
+                     (dict(history=at(y, 8), history_width=1), -1), (dict(drafts=at(y, 0)), -1),
+                     (dict(repetition=at(y, 0)), -1), (dict(logits=None), -1)):
+        with pytest.raises(tlm.TlmError) as e:
+            call(**kw)
+        assert e.value.code == code, kw

@@ -161,6 +161,7 @@ struct tlm_paged {
   float* rope_cos = nullptr;
   float* rope_sin = nullptr;
   int* status = nullptr;  // kPagedStatus* bits since the last tlm_paged_status
+  int sinks = 0;          // tlm_paged_set_sinks
 };
 
 // The device of a context, current for a call's launches; the caller's after it.
@@ -1160,8 +1161,8 @@ static int paged_check(const tlm_paged_desc* d) {
     return fail(TLM_ERR_INVALID, "TLMPaged: invalid rotary dimension %d", d->rotary_dim);
   if (d->rotary_dim > 0 && !d->inv_freq) return fail(TLM_ERR_INVALID, "TLMPaged: missing inv_freq");
   if (d->sliding_window < 0) return fail(TLM_ERR_INVALID, "TLMPaged: negative sliding window");
-  if (d->kv_fmt != TLM_FMT_F16 && d->kv_fmt != TLM_FMT_F32)
-    return fail(TLM_ERR_INVALID, "TLMPaged: cache format %d is not fp16 or fp32", d->kv_fmt);
+  if (d->kv_fmt != TLM_FMT_F16 && d->kv_fmt != TLM_FMT_F32 && d->kv_fmt != TLM_FMT_F8)
+    return fail(TLM_ERR_INVALID, "TLMPaged: cache format %d is not fp16, fp32 or 8-bit", d->kv_fmt);
   if (d->page_tokens < 32 || d->page_tokens > 1024 || (d->page_tokens & (d->page_tokens - 1)))
     return fail(TLM_ERR_INVALID, "TLMPaged: page of %d tokens is not a power of two from 32 to 1024", d->page_tokens);
   if (d->max_tokens <= 0 || d->max_tokens > (1 << 30))
@@ -1170,6 +1171,11 @@ static int paged_check(const tlm_paged_desc* d) {
 }
 
 static int page_shift(const tlm_paged_desc& d) { return __builtin_ctz((unsigned)d.page_tokens); }
+static int kv_size(const tlm_paged_desc& d) { return d.kv_fmt == TLM_FMT_F32 ? 4 : d.kv_fmt == TLM_FMT_F16 ? 2 : 1; }
+static size_t page_bytes(const tlm_paged_desc& d) {
+  return d.kv_fmt == TLM_FMT_F8 ? paged8_page(d.kv_heads, page_shift(d), d.head_dim)
+                                : (size_t)d.kv_heads * d.page_tokens * d.head_dim * kv_size(d);
+}
 
 int tlm_paged_create(tlm_ctx* ctx, const tlm_paged_desc* desc, tlm_paged** out) {
   if (!ctx || !desc || !out) return fail(TLM_ERR_INVALID, "TLMPaged: null argument");
@@ -1229,8 +1235,7 @@ void tlm_paged_destroy(tlm_paged* P) {
 }
 
 static size_t paged_pool_words(const tlm_paged* P, const tlm_paged_batch* b) {  // 4 bytes each
-  const size_t page = (size_t)P->d.kv_heads * P->d.page_tokens * P->d.head_dim;
-  return b->num_pages * (P->d.kv_fmt == TLM_FMT_F32 ? page : page / 2);
+  return b->num_pages * (page_bytes(P->d) / 4);
 }
 
 // Whether words [p, p + n) share an address with the batch's tables or lengths, which
@@ -1279,7 +1284,25 @@ static int paged_args(const tlm_paged* P, const tlm_paged_batch* b, PagedArgs& a
   a.G = P->d.heads / P->d.kv_heads;
   a.rd = P->d.rotary_dim;
   a.window = P->d.sliding_window;
+  a.sinks = a.window > 0 ? P->sinks : 0;
+  a.page_bytes = page_bytes(P->d);
   a.scale = P->scale;
+  return TLM_OK;
+}
+
+int tlm_paged_set_sinks(tlm_paged* P, int32_t sinks) {
+  if (!P) return fail(TLM_ERR_INVALID, "TLMPaged: null argument");
+  if (sinks < 0 || sinks > (1 << 30)) return fail(TLM_ERR_INVALID, "TLMPaged: %d sinks outside [0, 2^30]", sinks);
+  if (sinks > 0 && P->d.sliding_window == 0)
+    return fail(TLM_ERR_INVALID, "TLMPaged: %d sinks without a sliding window", sinks);
+  P->sinks = sinks;
+  return TLM_OK;
+}
+
+int tlm_paged_page_bytes(const tlm_paged_desc* d, size_t* bytes) {
+  if (!d || !bytes) return fail(TLM_ERR_INVALID, "TLMPaged: null argument");
+  if (const int rc = paged_check(d)) return rc;
+  *bytes = page_bytes(*d);
   return TLM_OK;
 }
 
@@ -1299,7 +1322,7 @@ int tlm_op_paged_append(tlm_paged* P, const tlm_paged_batch* b, const float* qkv
   a.x = qkv;
   a.q = q;
   const DeviceScope on(P->ctx->device);
-  if (!launch_paged_append(P->d.kv_fmt == TLM_FMT_F32, a, P->ctx->stream))
+  if (!launch_paged_append(kv_size(P->d), a, P->ctx->stream))
     return fail(TLM_ERR_STATE, "TLMPaged: no append kernel for this shape");
   CHECK_LAUNCH("TLMPaged");
   return TLM_OK;
@@ -1324,7 +1347,7 @@ int tlm_op_paged_attention(tlm_paged* P, const tlm_paged_batch* b, const float* 
   std::lock_guard<std::mutex> lock(P->ctx->part_mu);
   a.part = P->ctx->part;
   a.arrived = P->ctx->paged_arrived;
-  if (!launch_paged_attention(P->d.kv_fmt == TLM_FMT_F32, a, P->ctx->cus, kPartFloats, P->ctx->stream))
+  if (!launch_paged_attention(kv_size(P->d), a, P->ctx->cus, kPartFloats, P->ctx->stream))
     return fail(TLM_ERR_STATE, "TLMPaged: no attention kernel for this shape");
   CHECK_LAUNCH("TLMPaged");
   return TLM_OK;
@@ -1344,9 +1367,70 @@ int tlm_paged_status(tlm_paged* P) {
               bits & kPagedStatusPage ? "a table entry in use is no page of the pool" : "");
 }
 
-int tlm_paged_locate(const tlm_paged_desc* d, int32_t num_pages, const int32_t* table, int32_t table_width,
-                     int32_t position, int32_t kv_head, int32_t dim, int64_t* k_index, int64_t* v_index) {
-  if (!d || !table || !k_index || !v_index) return fail(TLM_ERR_INVALID, "TLMPaged: null argument");
+int tlm_op_paged_reserve(tlm_paged* P, const tlm_paged_request* r) {
+  if (!P || !r) return fail(TLM_ERR_INVALID, "TLMPaged: null argument");
+  if (!r->lengths || !r->tables || !r->refs || !r->out_tables || !r->out_refs || !r->starts)
+    return fail(TLM_ERR_INVALID, "TLMPaged: the request lacks lengths, tables, page counts or starts");
+  if (r->num_pages < 1 || r->table_width < 1 || r->seqs < 1 || r->tokens < 1)
+    return fail(TLM_ERR_INVALID, "TLMPaged: %d pages, tables of %d, %d sequences of %d rows", r->num_pages,
+                r->table_width, r->seqs, r->tokens);
+  if ((int64_t)r->seqs * r->tokens > (1 << 22) / P->d.heads)
+    return fail(TLM_ERR_RANGE, "TLMPaged: %d sequences of %d rows of %d heads are more than 2^22", r->seqs, r->tokens,
+                P->d.heads);
+  if (r->seqs > kReserveMaxSeqs)
+    return fail(TLM_ERR_RANGE, "TLMPaged: %d sequences, at most %d reserve at once", r->seqs, kReserveMaxSeqs);
+  if (reinterpret_cast<uintptr_t>(r->slots) % 8) return fail(TLM_ERR_INVALID, "TLMPaged: the slots are not 8-byte aligned");
+  ReserveArgs a;
+  memset(&a, 0, sizeof a);
+  a.lengths = r->lengths;
+  a.counts = r->counts;
+  a.tables = r->tables;
+  a.refs = r->refs;
+  a.out_tables = r->out_tables;
+  a.out_refs = r->out_refs;
+  a.starts = r->starts;
+  a.slots = r->slots;
+  a.status = P->status;
+  a.num_pages = r->num_pages;
+  a.width = r->table_width;
+  a.page_shift = page_shift(P->d);
+  a.seqs = r->seqs;
+  a.tokens = r->tokens;
+  a.limit = paged_limit(P->d.max_tokens, r->table_width, a.page_shift);
+  a.window = P->d.sliding_window;
+  a.sinks = a.window > 0 ? P->sinks : 0;
+  const size_t need = reserve_work(a);
+  if (need > kPartFloats)
+    return fail(TLM_ERR_RANGE, "TLMPaged: %d sequences of %d rows and %d pages need %zu bytes of workspace, of %zu",
+                r->seqs, r->tokens, r->num_pages, 4 * need, kPartFloats * sizeof(float));
+  // tables and page counts may be brought up to date in place; nothing else is shared
+  const size_t seqs = r->seqs, cells = seqs * r->table_width, slots = 2 * seqs * r->tokens;
+  const struct {
+    const void* p;
+    size_t n;
+  } in[] = {{r->lengths, seqs}, {r->counts, seqs}, {r->tables, cells}, {r->refs, (size_t)r->num_pages}},
+    out[] = {{r->out_tables, cells}, {r->out_refs, (size_t)r->num_pages}, {r->starts, seqs}, {r->slots, slots}};
+  for (int i = 0; i < 4; i++) {
+    for (const auto& x : in)
+      if (x.p && out[i].p && overlap(x.p, x.n, out[i].p, out[i].n) &&
+          !(x.p == out[i].p && (out[i].p == r->tables || out[i].p == r->refs) && x.n == out[i].n && i < 2))
+        return fail(TLM_ERR_INVALID, "TLMPaged: a result of the reservation overlaps an input");
+    for (int k = 0; k < i; k++)
+      if (out[i].p && overlap(out[i].p, out[i].n, out[k].p, out[k].n))
+        return fail(TLM_ERR_INVALID, "TLMPaged: results of the reservation overlap each other");
+  }
+  const DeviceScope on(P->ctx->device);
+  std::lock_guard<std::mutex> lock(P->ctx->part_mu);
+  a.work = reinterpret_cast<int32_t*>(P->ctx->part);
+  a.arrived = P->ctx->paged_arrived;
+  launch_reserve(a, P->ctx->stream);
+  CHECK_LAUNCH("TLMPaged");
+  return TLM_OK;
+}
+
+// The checks of a position that the two calls below share.
+static int locate_check(const tlm_paged_desc* d, int32_t num_pages, const int32_t* table, int32_t table_width,
+                        int32_t position, int32_t kv_head, int32_t dim) {
   if (const int rc = paged_check(d)) return rc;
   if (num_pages < 1 || table_width < 1 || kv_head < 0 || kv_head >= d->kv_heads || dim < 0 || dim >= d->head_dim)
     return fail(TLM_ERR_INVALID, "TLMPaged: no kv head %d or dim %d", kv_head, dim);
@@ -1357,10 +1441,36 @@ int tlm_paged_locate(const tlm_paged_desc* d, int32_t num_pages, const int32_t* 
   if (page < 0)
     return fail(TLM_ERR_RANGE, "TLMPaged: entry %d of position %d is none of %d pages", table[position >> shift],
                 position, num_pages);
+  return TLM_OK;
+}
+
+int tlm_paged_locate(const tlm_paged_desc* d, int32_t num_pages, const int32_t* table, int32_t table_width,
+                     int32_t position, int32_t kv_head, int32_t dim, int64_t* k_index, int64_t* v_index) {
+  if (!d || !table || !k_index || !v_index) return fail(TLM_ERR_INVALID, "TLMPaged: null argument");
+  if (const int rc = locate_check(d, num_pages, table, table_width, position, kv_head, dim)) return rc;
+  const int shift = page_shift(*d), page = paged_page(table, position, shift, num_pages);
+  if (d->kv_fmt == TLM_FMT_F8) {
+    const int token = position & (d->page_tokens - 1);
+    const size_t head = page * page_bytes(*d) + (size_t)kv_head * d->page_tokens * d->head_dim;
+    *k_index = (int64_t)(head + paged8_k_at(token, dim, d->head_dim));
+    *v_index = (int64_t)(head + paged8_v_at(token, dim, d->head_dim));
+    return TLM_OK;
+  }
   const int E = d->kv_fmt == TLM_FMT_F32 ? 4 : 8, token = position & (d->page_tokens - 1);
   const size_t head = paged_head_at(page, kv_head, d->kv_heads, shift, d->head_dim);
   *k_index = (int64_t)(head + paged_k_at(token, dim, d->head_dim, E));
   *v_index = (int64_t)(head + paged_v_at(token, dim, d->head_dim, E));
+  return TLM_OK;
+}
+
+int tlm_paged_scale_at(const tlm_paged_desc* d, int32_t num_pages, const int32_t* table, int32_t table_width,
+                       int32_t position, int32_t kv_head, int64_t* byte) {
+  if (!d || !table || !byte) return fail(TLM_ERR_INVALID, "TLMPaged: null argument");
+  if (const int rc = locate_check(d, num_pages, table, table_width, position, kv_head, 0)) return rc;
+  if (d->kv_fmt != TLM_FMT_F8) return fail(TLM_ERR_INVALID, "TLMPaged: cache format %d has no scales", d->kv_fmt);
+  const int shift = page_shift(*d), page = paged_page(table, position, shift, num_pages);
+  *byte = (int64_t)(page * page_bytes(*d) + paged8_scale_at(kv_head, d->kv_heads, position & (d->page_tokens - 1), shift,
+                                                            d->head_dim));
   return TLM_OK;
 }
 
@@ -1481,6 +1591,64 @@ int tlm_op_verify_drafts(tlm_ctx* ctx, const float* logits, const float* draft_l
   a.work = ctx->part;
   launch_verify(a, ctx->cus, ctx->stream);
   CHECK_LAUNCH("TLMVerify");
+  return TLM_OK;
+}
+
+int tlm_op_adjust_logits(tlm_ctx* ctx, const tlm_logit_rules* r) {
+  if (!ctx || !r || !r->logits || !r->out || r->seqs < 1 || r->tokens < 1 || r->vocab < 1 || r->history_width < 0 ||
+      r->bias_width < 0)
+    return fail(TLM_ERR_INVALID, "TLMLogitRules: invalid argument");
+  if (r->tokens > kVerifyMaxTokens)
+    return fail(TLM_ERR_INVALID, "TLMLogitRules: %d rows per sequence, at most %d", r->tokens, kVerifyMaxTokens);
+  if (r->vocab > kVerifyMaxVocab)
+    return fail(TLM_ERR_INVALID, "TLMLogitRules: a vocabulary of %d, at most %d", r->vocab, kVerifyMaxVocab);
+  if ((int64_t)r->seqs * r->tokens > (1 << 20))
+    return fail(TLM_ERR_RANGE, "TLMLogitRules: %d sequences of %d rows are more than 2^20 rows", r->seqs, r->tokens);
+  if (r->bias_width > kAdjustMaxBiases)
+    return fail(TLM_ERR_INVALID, "TLMLogitRules: %d biases, at most %d", r->bias_width, kAdjustMaxBiases);
+  if (r->history_width > 0 && !r->history) return fail(TLM_ERR_INVALID, "TLMLogitRules: no history of %d", r->history_width);
+  if (r->bias_width > 0 && (!r->bias_ids || !r->biases))
+    return fail(TLM_ERR_INVALID, "TLMLogitRules: %d biases without their tokens or values", r->bias_width);
+  AdjustArgs a;
+  memset(&a, 0, sizeof a);
+  a.logits = r->logits;
+  a.out = r->out;
+  a.counts = r->counts;
+  a.history = r->history_width > 0 ? r->history : nullptr;
+  a.history_counts = r->history_counts;
+  a.drafts = r->tokens > 1 ? r->drafts : nullptr;
+  a.repetition = r->repetition;
+  a.frequency = r->frequency;
+  a.presence = r->presence;
+  a.bias_ids = r->bias_width > 0 ? r->bias_ids : nullptr;
+  a.biases = r->biases;
+  a.masks = r->masks;
+  a.seqs = r->seqs;
+  a.tokens = r->tokens;
+  a.vocab = r->vocab;
+  a.history_width = r->history_width;
+  a.bias_width = r->bias_width;
+  const size_t seqs = r->seqs, rows = seqs * r->tokens, n = rows * r->vocab;
+  const struct {
+    const void* p;
+    size_t n;
+  } in[] = {{r->out == r->logits ? nullptr : r->logits, n},
+            {r->counts, seqs},
+            {a.history, seqs * r->history_width},
+            {a.history ? r->history_counts : nullptr, seqs},
+            {a.drafts, rows - seqs},
+            {r->repetition, seqs},
+            {r->frequency, seqs},
+            {r->presence, seqs},
+            {a.bias_ids, seqs * r->bias_width},
+            {a.bias_ids ? r->biases : nullptr, seqs * r->bias_width},
+            {r->masks, rows * ((r->vocab + 31) / 32)}};
+  for (const auto& x : in)
+    if (x.p && x.n && overlap(x.p, x.n, r->out, n))
+      return fail(TLM_ERR_INVALID, "TLMLogitRules: the results overlap an input");
+  const DeviceScope on(ctx->device);
+  launch_adjust(a, ctx->cus, ctx->stream);
+  CHECK_LAUNCH("TLMLogitRules");
   return TLM_OK;
 }
 

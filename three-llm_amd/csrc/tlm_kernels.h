@@ -485,6 +485,8 @@ struct PagedArgs {
   int* status;            // or'ed with kPagedStatus*
   int num_pages, width, page_shift, seqs, tokens, limit;
   int Hq, Hkv, D, G, rd, window;
+  int sinks;           // first positions that stay visible behind a window (0 without one)
+  size_t page_bytes;   // 8-bit caches: a page's
   int out_f32;
   float scale;
   // attention: how the sequences' position tiles are shared out (launch_paged_attention)
@@ -494,9 +496,49 @@ struct PagedArgs {
   int units, chunks, round, chunk_min, whole, plan_shift;
 };
 constexpr int kPagedCounters = 16384;
-bool launch_paged_append(bool kv_f32, const PagedArgs& a, hipStream_t st);
+// kv_size: bytes of an element of the cache
+bool launch_paged_append(int kv_size, const PagedArgs& a, hipStream_t st);
+void launch_paged_append8(const PagedArgs& a, hipStream_t st);
 // part_floats: what a.part holds
-bool launch_paged_attention(bool kv_f32, const PagedArgs& a, int cus, size_t part_floats, hipStream_t st);
+bool launch_paged_attention(int kv_size, const PagedArgs& a, int cus, size_t part_floats, hipStream_t st);
+
+// Page tables from the sequences' lengths (tlm_op_paged_reserve).
+struct ReserveArgs {
+  const int32_t* lengths;  // [seqs]; < 0: the sequence's pages are given back
+  const int32_t* counts;   // [seqs], or null: tokens each
+  const int32_t* tables;   // [seqs][width]
+  const int32_t* refs;     // [num_pages]
+  int32_t* out_tables;
+  int32_t* out_refs;
+  int32_t* starts;         // [seqs]
+  int64_t* slots;          // [seqs][tokens], or null
+  int* status;
+  int num_pages, width, page_shift, seqs, tokens, limit, window, sinks;
+  int32_t* work;           // reserve_work's ints
+  unsigned* arrived;       // one, zero between launches
+};
+constexpr int kReserveMaxSeqs = 1 << 20;
+size_t reserve_work(const ReserveArgs& a);  // ints that a.work has to hold
+void launch_reserve(const ReserveArgs& a, hipStream_t st);
+
+// Penalties, biases and masks on logits (tlm_op_adjust_logits).
+struct AdjustArgs {
+  const float* logits;  // [seqs][tokens][vocab]
+  float* out;
+  const int32_t* counts;          // [seqs] rows, or null: tokens each
+  const int32_t* history;         // [seqs][history_width], or null
+  const int32_t* history_counts;  // [seqs], or null: history_width each
+  const int32_t* drafts;          // [seqs][tokens - 1], or null
+  const float* repetition;        // [seqs], or null: 1
+  const float* frequency;         // [seqs], or null: 0
+  const float* presence;
+  const int32_t* bias_ids;        // [seqs][bias_width], or null
+  const float* biases;
+  const uint32_t* masks;          // [seqs][tokens][(vocab + 31) / 32], or null
+  int seqs, tokens, vocab, history_width, bias_width;
+};
+constexpr int kAdjustMaxBiases = 4096;
+void launch_adjust(const AdjustArgs& a, int cus, hipStream_t st);
 
 struct VerifyArgs {
   const float* logits;        // [seqs][tokens][vocab]

@@ -295,17 +295,23 @@ typedef _Float16 ph8_t __attribute__((ext_vector_type(8)));
 // 2^-25, and many small weights beside one large are lost while the sum has them.  q's
 // factor is taken out of the scores, P's is in L and O alike.
 // fp32 caches: 16 positions a tile, v_mfma_f32_16x16x4_f32.
+// 8-bit caches: 32 positions a tile, those of one scale of K and one of V; codes are
+// made fp16 values (exactly) on their way to the same products.  K's scale goes into
+// the scores' factor.  V's goes into P: P 2^(lv - d), d the row's largest lv + the
+// tile's maximum - the running maximum so far, so that P stays in fp16's range and is
+// exact to the same share of the row's largest weight times scale; O is under 2^d.
 template <typename KT>
 struct PagedTile {
-  static constexpr int SUB = 4 / sizeof(KT);  // 16-position score tiles
+  static constexpr int SUB = sizeof(KT) == 4 ? 1 : 2;  // 16-position score tiles
   static constexpr int TS = 16 * SUB;         // positions
   static constexpr int SHIFT = SUB == 2 ? 5 : 4;
   static constexpr float kLift = SUB == 2 ? 15.f : 0.f;  // log2 of q's and P's factor
 };
 
-// A sequence's part in a call: its rows and the position tiles that they attend to.
+// A sequence's part in a call: its rows and the position tiles that they attend to:
+// `sunk` tiles of sinks from 0 on that lie before the window's, then those from `first` on.
 struct SeqWork {
-  int start, rows, first, tiles;
+  int start, rows, first, tiles, sunk;
 };
 template <int SHIFT>
 __device__ __forceinline__ SeqWork seq_work(const PagedArgs& a, int s, bool* bad) {
@@ -314,7 +320,8 @@ __device__ __forceinline__ SeqWork seq_work(const PagedArgs& a, int s, bool* bad
   w.rows = paged_rows(w.start, a.counts ? a.counts[s] : a.tokens, a.tokens, a.limit, bad);
   const int first = a.window > 0 ? max(0, w.start - a.window + 1) : 0;
   w.first = first >> SHIFT;
-  w.tiles = w.rows > 0 ? ((w.start + w.rows - 1) >> SHIFT) - w.first + 1 : 0;
+  w.sunk = w.rows > 0 ? min((a.sinks + (1 << SHIFT) - 1) >> SHIFT, w.first) : 0;
+  w.tiles = w.rows > 0 ? ((w.start + w.rows - 1) >> SHIFT) - w.first + 1 + w.sunk : 0;
   return w;
 }
 
@@ -412,7 +419,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedArgs a) {
 template <int SHIFT>
 __device__ __forceinline__ bool plan(const PagedArgs& a, int g, SeqChunk& r) {
   const int lane = threadIdx.x & 63;
-  const SeqWork none{0, 0, 0, 0};
+  const SeqWork none{0, 0, 0, 0, 0};
   bool b;
   int c = 0, before = 0, slots = 0;
   // whether chunk g is one of the 64 sequences' from s0 on, a lane each
@@ -430,6 +437,7 @@ __device__ __forceinline__ bool plan(const PagedArgs& a, int g, SeqChunk& r) {
     r.w.rows = __builtin_amdgcn_readlane(w.rows, l);
     r.w.first = __builtin_amdgcn_readlane(w.first, l);
     r.w.tiles = __builtin_amdgcn_readlane(w.tiles, l);
+    r.w.sunk = __builtin_amdgcn_readlane(w.sunk, l);
     r.n = __builtin_amdgcn_readlane(n, l);
     r.chunk = g - before - __builtin_amdgcn_readlane(incl - n, l);
     r.slot = slots + __builtin_amdgcn_readlane(sincl - m, l);
@@ -491,11 +499,22 @@ __device__ __forceinline__ float* part_row(const PagedArgs& a, int slot, int uni
   return a.part + (((size_t)slot * a.units + unit) * 16 + row) * (DT + 2);
 }
 
+// Eight codes (two dwords of four) as fp16 values, which hold every code.
+__device__ __forceinline__ u32x4 codes_f16(uint32_t a, uint32_t b) {
+  u32x4 y;
+  y[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.f, false));
+  y[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.f, true));
+  y[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.f, false));
+  y[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.f, true));
+  return y;
+}
+
 template <typename KT, int DT, int W, bool STREAM>
 __global__ __launch_bounds__(64 * W, DT <= 64 ? 4 : 2) void paged_attention_kernel(PagedArgs a) {
   using T = PagedTile<KT>;
-  constexpr int SUB = T::SUB, TS = T::TS, NF = DT / 16;  // 1 KB operand pieces of a tile's K, of its V
-  constexpr bool F16 = sizeof(KT) == 2;
+  constexpr int SUB = T::SUB, TS = T::TS, NF = DT / 16;  // 16-dim slabs of the output
+  constexpr bool F8 = sizeof(KT) == 1, F16 = sizeof(KT) <= 2;  // F16: fp16 products
+  constexpr int NL = F8 ? NF / 2 : NF;                   // 1 KB operand pieces of a tile's K, of its V
   constexpr int RS = DT + 2;  // floats of a row's record: maximum, sum, output
   constexpr int LDSF = W * 16 * RS;
   __shared__ __align__(16) float lds[LDSF];
@@ -512,34 +531,46 @@ __global__ __launch_bounds__(64 * W, DT <= 64 ? 4 : 2) void paged_attention_kern
   const int ja = r0 / a.G, jb = (min(r0 + 16, R) - 1) / a.G, start = sc.w.start;
   const int lo_any = a.window > 0 ? max(0, start + ja - a.window + 1) : 0, hi_any = start + jb;
   const int lo_all = a.window > 0 ? max(0, start + jb - a.window + 1) : 0, hi_all = start + ja;
-  const int per = (sc.w.tiles + sc.n - 1) / sc.n;
-  const int t0 = max(sc.w.first + ci * per, lo_any >> T::SHIFT);
-  const int t1 = min(min(sc.w.first + (ci + 1) * per, sc.w.first + sc.w.tiles), (hi_any >> T::SHIFT) + 1);
+  // the chunk's tiles: of the sinks from c0 on, then those of the block's windows [t0, t1)
+  const int per = (sc.w.tiles + sc.n - 1) / sc.n, c0 = ci * per, c1 = min(c0 + per, sc.w.tiles);
+  const int past = (hi_any >> T::SHIFT) + 1, sinks = min((a.sinks + TS - 1) >> T::SHIFT, past);
+  const int sunk = max(0, min(sinks, c1) - c0), base = sc.w.first - sc.w.sunk;
+  const int t0 = max(base + max(c0, sinks), lo_any >> T::SHIFT), t1 = min(base + c1, past);
+  const int tiles = sunk + max(0, t1 - t0);
+  auto tile_of = [&](int i) { return i < sunk ? c0 + i : t0 + i - sunk; };
   const int32_t* const table = a.tables + (size_t)sc.s * a.width;
   const int tpp = a.page_shift - T::SHIFT;  // log2 of the tiles of a page
 
   struct Tile {
-    u32x4 k[NF], v[NF];
+    u32x4 k[NL], v[NL];
   };
   auto load = [&](u32x4* x, const void* pool, int t, int page) {
-    const size_t at = paged_head_at(max(page, 0), hk, a.Hkv, a.page_shift, DT) +
-                      (size_t)(t & ((1 << tpp) - 1)) * (TS * DT) + lane * (16 / sizeof(KT));
+    const size_t head = F8 ? (size_t)max(page, 0) * a.page_bytes + (size_t)hk * ((size_t)DT << a.page_shift)
+                           : paged_head_at(max(page, 0), hk, a.Hkv, a.page_shift, DT);
+    const size_t at = head + (size_t)(t & ((1 << tpp) - 1)) * (TS * DT) + lane * (16 / sizeof(KT));
     const TLM_GLOBAL u32x4* p = gl(reinterpret_cast<const u32x4*>(static_cast<const KT*>(pool) + at));
 #pragma unroll
-    for (int f = 0; f < NF; f++) x[f] = STREAM ? __builtin_nontemporal_load(p + 64 * f) : p[64 * f];
+    for (int f = 0; f < NL; f++) x[f] = STREAM ? __builtin_nontemporal_load(p + 64 * f) : p[64 * f];
   };
-  // The wave's tiles t0 + w, t0 + w + W, ...  Their pages, 64 at a time, a lane each;
-  // the first tile is on its way while q is prepared.
-  int tb = t0 + w, n = 0, page = -1;
+  // The wave's tiles w, w + W, ... of the chunk's.  Their pages (8-bit: and scales), 64 at
+  // a time, a lane each; the first tile is on its way while q is prepared.
+  int tb = w, n = 0, page = -1;
+  uint32_t kscale = 0, vscale = 0;
   auto pages = [&] {
-    const int tl = tb + lane * W;
-    n = min(64, (t1 - tb + W - 1) / W);
-    page = paged_page(table, min(tl, t1 - 1) << T::SHIFT, a.page_shift, a.num_pages);
-    if (page < 0 && tl < t1) paged_flag(a.status, kPagedStatusPage);
+    const int tl = tb + lane * W, t = tile_of(min(tl, tiles - 1));
+    n = min(64, (tiles - tb + W - 1) / W);
+    page = paged_page(table, t << T::SHIFT, a.page_shift, a.num_pages);
+    if (page < 0 && tl < tiles) paged_flag(a.status, kPagedStatusPage);
+    if (F8) {
+      const size_t at = (size_t)max(page, 0) * a.page_bytes +
+                        paged8_scale_at(hk, a.Hkv, (t & ((1 << tpp) - 1)) * TS, a.page_shift, DT);
+      kscale = *gl(reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.kc) + at));
+      vscale = *gl(reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.vc) + at));
+    }
   };
   auto page_of = [&](int i) { return __builtin_amdgcn_readlane(page, i); };
-  auto load_k = [&](Tile& x, int i) { load(x.k, a.kc, tb + i * W, page_of(i)); };
-  auto load_v = [&](Tile& x, int i) { load(x.v, a.vc, tb + i * W, page_of(i)); };
+  auto load_k = [&](Tile& x, int i) { load(x.k, a.kc, tile_of(tb + i * W), page_of(i)); };
+  auto load_v = [&](Tile& x, int i) { load(x.v, a.vc, tile_of(tb + i * W), page_of(i)); };
   // This lane's row (its column of the tiles): its positions' bounds, and q scaled by
   // a power of two to at most 1, or 2^15 as fp16.  q is requested before the first
   // tile: loads return in order.
@@ -553,7 +584,7 @@ __global__ __launch_bounds__(64 * W, DT <= 64 ? 4 : 2) void paged_attention_kern
     qx[f] = *(const TLM_GLOBAL f32x4u*)(q + (F16 ? 32 * (f / 2) + 8 * qd + 4 * (f & 1) : 16 * f + 4 * qd));
   __builtin_amdgcn_sched_barrier(0);
   Tile x;
-  if (tb < t1) {
+  if (tb < tiles) {
     pages();
     load_k(x, 0);
     load_v(x, 0);
@@ -573,7 +604,7 @@ __global__ __launch_bounds__(64 * W, DT <= 64 ? 4 : 2) void paged_attention_kern
 #pragma unroll
     for (int e = 0; e < 4; e++) qx[f][e] = row < R ? ldexpf(qx[f][e], -ex) : 0.f;
   // log2 e: the softmax runs in base 2; above 0, as masked scores are -inf before it
-  const float mult = fmaxf(ldexpf(a.scale * 1.4426950408889634f, ex), FLT_TRUE_MIN);
+  const float qmult = fmaxf(ldexpf(a.scale * 1.4426950408889634f, ex), FLT_TRUE_MIN);
 #pragma unroll
   for (int f = 0; f < NF; f++) {
     if (!F16) {
@@ -593,37 +624,56 @@ __global__ __launch_bounds__(64 * W, DT <= 64 ? 4 : 2) void paged_attention_kern
 
   f32x4 o[NF];
   float mrun = -FLT_MAX, lrun = 0.f;  // running maximum, this lane's share of the sum
+  float drun = kPagedScaleMin;        // 8-bit: O is under 2^drun
 #pragma unroll
   for (int f = 0; f < NF; f++) o[f] = (f32x4){0.f, 0.f, 0.f, 0.f};
 
-  // V with positions outside [first, last] taken out (0 times what they hold may be NaN)
+  // whether a row that sees [first, last] and sinks sees position x
+  auto in = [&](int x, int first, int last) { return (x >= first || x < a.sinks) && x <= last; };
+  // V with positions outside [first, last] and the sinks taken out (0 times what they hold may be NaN)
   auto keep = [&](const u32x4& v, int p, int first, int last) {
     u32x4 y;
 #pragma unroll
     for (int d = 0; d < 4; d++) {
-      if (F16) {  // dword d: positions 16 (d / 2) + 4 qd + 2 (d % 2) + {0, 1}
+      if (F8) {  // dword d: positions 16 (d % 2) + 4 qd + byte
+        const int x = p + 16 * (d & 1) + 4 * qd;
+        unsigned m = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) m |= in(x + e, first, last) ? 0xFFu << 8 * e : 0u;
+        y[d] = v[d] & m;
+      } else if (F16) {  // dword d: positions 16 (d / 2) + 4 qd + 2 (d % 2) + {0, 1}
         const int x = p + 16 * (d / 2) + 4 * qd + 2 * (d & 1);
-        y[d] = v[d] & ((x >= first && x <= last ? 0xFFFFu : 0u) | (x + 1 >= first && x + 1 <= last ? 0xFFFF0000u : 0u));
+        y[d] = v[d] & ((in(x, first, last) ? 0xFFFFu : 0u) | (in(x + 1, first, last) ? 0xFFFF0000u : 0u));
       } else {
         const int x = p + 4 * qd + d;
-        y[d] = x >= first && x <= last ? v[d] : 0u;
+        y[d] = in(x, first, last) ? v[d] : 0u;
       }
     }
     return y;
   };
   auto not_finite = [](unsigned v) -> unsigned {  // the sign bits' places of values that are not finite
-    return F16 ? ((v & 0x7C007C00u) + 0x04000400u) & 0x80008000u : ((v & 0x7F800000u) + 0x00800000u) & 0x80000000u;
+    return F8 ? ((v & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u : F16 ? ((v & 0x7C007C00u) + 0x04000400u) & 0x80008000u : ((v & 0x7F800000u) + 0x00800000u) & 0x80000000u;
   };
-  // tile t; k_read() and v_read() run once x.k and x.v have been read
-  auto process = [&](Tile& x, int t, auto k_read, auto v_read) {
+  // the operand of 16 dims (V: slab f) or of 16 positions (K: piece f / 2's sixteen f % 2)
+  auto operand = [](const u32x4* x, int f) {
+    return F8 ? codes_f16(x[f / 2][2 * (f & 1)], x[f / 2][2 * (f & 1) + 1]) : x[f];
+  };
+  // tile t, the i-th of the 64; k_read() and v_read() run once x.k and x.v have been read
+  auto process = [&](Tile& x, int t, int i64, auto k_read, auto v_read) {
     const int p = t << T::SHIFT;
-    const bool edge = p < lo_all || p + TS - 1 > hi_all;  // some row does not see all of it (wave-uniform)
+    // some row does not see all of it (wave-uniform)
+    const bool edge = (p < lo_all && p + TS > a.sinks) || p + TS - 1 > hi_all;
+    float mult = qmult, lv = 0.f;
+    if (F8) {
+      mult = fmaxf(ldexpf(qmult, paged8_exponent_of(__builtin_amdgcn_readlane(kscale, i64))), FLT_TRUE_MIN);
+      lv = (float)paged8_exponent_of(__builtin_amdgcn_readlane(vscale, i64));
+    }
     bool apart = false;
     if (edge) {
       // only a value that is not finite could reach a row that masks its position
       unsigned nf = 0;
 #pragma unroll
-      for (int f = 0; f < NF; f++) {
+      for (int f = 0; f < NL; f++) {
         x.v[f] = keep(x.v[f], p, lo_any, hi_any);
 #pragma unroll
         for (int d = 0; d < 4; d++) nf |= not_finite(x.v[f][d]);
@@ -637,7 +687,7 @@ __global__ __launch_bounds__(64 * W, DT <= 64 ? 4 : 2) void paged_attention_kern
         const ph8_t qh = __builtin_bit_cast(ph8_t, qreg[2 * jj]), ql = __builtin_bit_cast(ph8_t, qreg[2 * jj + 1]);
 #pragma unroll
         for (int st = 0; st < SUB; st++) {
-          const ph8_t k = __builtin_bit_cast(ph8_t, x.k[st * (NF / SUB) + jj]);
+          const ph8_t k = __builtin_bit_cast(ph8_t, operand(x.k, F8 ? 2 * jj + st : st * (NF / SUB) + jj));
           acc[st] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh, acc[st], 0, 0, 0);
           acc[st] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql, acc[st], 0, 0, 0);
         }
@@ -661,7 +711,7 @@ __global__ __launch_bounds__(64 * W, DT <= 64 ? 4 : 2) void paged_attention_kern
 #pragma unroll
       for (int i = 0; i < 4 * SUB; i++) {
         const int y = p + 16 * (i / 4) + 4 * qd + (i & 3);
-        if (y < lo || y > hi) sv[i] = -INFINITY;
+        if (!in(y, lo, hi)) sv[i] = -INFINITY;
       }
     }
     float mx = sv[0];
@@ -669,7 +719,8 @@ __global__ __launch_bounds__(64 * W, DT <= 64 ? 4 : 2) void paged_attention_kern
     for (int i = 1; i < 4 * SUB; i++) mx = fmaxf(mx, sv[i]);
     mx = fmaxf(mx, lane_swap16(mx));
     mx = fmaxf(mx, lane_swap32(mx));
-    const float mn = fmaxf(mrun, ceilf(mx * mult));  // finite: it starts at -FLT_MAX
+    const float mt = ceilf(mx * mult);
+    const float mn = fmaxf(mrun, mt);  // finite: it starts at -FLT_MAX
     if (__ballot(fabsf(mn) >= 0x1p22f)) {
       // kLift - mn is rounded there, and an unrounded product passes the maximum by as much
 #pragma clang fp contract(off)
@@ -681,14 +732,23 @@ __global__ __launch_bounds__(64 * W, DT <= 64 ? 4 : 2) void paged_attention_kern
       for (int i = 0; i < 4 * SUB; i++) sv[i] = fmaf(sv[i], mult, lift);
     }
     const float corr = __builtin_amdgcn_exp2f(mrun - mn);
+    float ocorr = corr, pf = 1.f;
+    if (F8) {
+      // d: at least the least scale (the maximum's own tile is in it), at most the largest
+      const float dn = fmaxf(drun - (mn - mrun), lv + (mt - mn));
+      ocorr = __builtin_amdgcn_exp2f((mrun - mn) + (drun - dn));
+      pf = __builtin_amdgcn_exp2f(lv - dn);
+      drun = dn;
+    }
     float ps = 0.f;
     u32x4 ph, pl;  // fp16: high and low parts
     if (F16) {
       ph8_t h, l;
 #pragma unroll
       for (int i = 0; i < 4 * SUB; i++) {
-        const float v = __builtin_amdgcn_exp2f(sv[i]);
+        float v = __builtin_amdgcn_exp2f(sv[i]);
         ps += v;
+        if (F8) v *= pf;
         h[i % 8] = (_Float16)v;
         l[i % 8] = (_Float16)(v - (float)h[i % 8]);
       }
@@ -704,9 +764,9 @@ __global__ __launch_bounds__(64 * W, DT <= 64 ? 4 : 2) void paged_attention_kern
     }
     lrun = fmaf(lrun, corr, ps);
     mrun = mn;
-    if (__ballot(corr != 1.f)) {
+    if (__ballot(ocorr != 1.f)) {
 #pragma unroll
-      for (int f = 0; f < NF; f++) o[f] *= corr;
+      for (int f = 0; f < NF; f++) o[f] *= ocorr;
     }
     k_read();
     auto weigh = [&](const u32x4& v, f32x4 y) -> f32x4 {
@@ -724,22 +784,25 @@ __global__ __launch_bounds__(64 * W, DT <= 64 ? 4 : 2) void paged_attention_kern
       // a row that does give such a value a weight becomes NaN there; the others get 0
       // times 0
 #pragma unroll
-      for (int f = 0; f < NF; f++) {
+      for (int f = 0; f < NL; f++) {
         u32x4 one;
 #pragma unroll
         for (int d = 0; d < 4; d++) {
           const unsigned t = not_finite(x.v[f][d]);  // a bit per value, its highest
-          one[d] = F16 ? (t >> 15) * 0x3C00u : (t >> 31) * 0x3F800000u;
-          x.v[f][d] &= ~(F16 ? (t >> 15) * 0xFFFFu : (t >> 31) * 0xFFFFFFFFu);
+          one[d] = F8 ? (t >> 7) * 0x38u : F16 ? (t >> 15) * 0x3C00u : (t >> 31) * 0x3F800000u;
+          x.v[f][d] &= ~(F8 ? (t >> 7) * 0xFFu : F16 ? (t >> 15) * 0xFFFFu : (t >> 31) * 0xFFFFFFFFu);
         }
-        const f32x4 y = weigh(one, (f32x4){0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-        for (int e = 0; e < 4; e++)
-          if (y[e] > 0.f) o[f][e] = __uint_as_float(0x7FC00000u);
+        for (int b = 0; b < NF / NL; b++) {
+          const f32x4 y = weigh(F8 ? operand(&one, b) : one, (f32x4){0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            if (y[e] > 0.f) o[f * (NF / NL) + b][e] = __uint_as_float(0x7FC00000u);
+        }
       }
     }
 #pragma unroll
-    for (int f = 0; f < NF; f++) o[f] = weigh(x.v[f], o[f]);
+    for (int f = 0; f < NF; f++) o[f] = weigh(operand(x.v, f), o[f]);
     v_read();
   };
 
@@ -747,18 +810,18 @@ __global__ __launch_bounds__(64 * W, DT <= 64 ? 4 : 2) void paged_attention_kern
   // tile or more in flight a wave, and the registers of one (with two, 8 waves a CU
   // instead of 16 at head_dim 64 and less in flight: 128 x 1 Llama-3.2-1B up to
   // 1000 positions 31.8 instead of 28.1 us).
-  while (tb < t1) {
+  while (tb < tiles) {
     for (int i = 0; i < n; i++) {
       const bool more = i + 1 < n;
       if (page_of(i) >= 0) {
-        process(x, tb + i * W, [&] { if (more) load_k(x, i + 1); }, [&] { if (more) load_v(x, i + 1); });
+        process(x, tile_of(tb + i * W), i, [&] { if (more) load_k(x, i + 1); }, [&] { if (more) load_v(x, i + 1); });
       } else if (more) {
         load_k(x, i + 1);
         load_v(x, i + 1);
       }
     }
     tb += 64 * W;
-    if (tb < t1) {
+    if (tb < tiles) {
       pages();
       load_k(x, 0);
       load_v(x, 0);
@@ -777,6 +840,11 @@ __global__ __launch_bounds__(64 * W, DT <= 64 ? 4 : 2) void paged_attention_kern
       static_cast<uint16_t*>(a.out)[at + 1] = kv_store<uint16_t>(y1);
     }
   };
+  if (F8) {
+    const float by = __builtin_amdgcn_exp2f(drun);
+#pragma unroll
+    for (int f = 0; f < NF; f++) o[f] *= by;
+  }
   lrun += lane_swap16(lrun);
   lrun += lane_swap32(lrun);
   float* const rec = lds + (w * 16 + i16) * RS;
@@ -885,8 +953,8 @@ void launch_attention_of(PagedArgs a, int cus, size_t part_floats, hipStream_t s
   using T = PagedTile<KT>;
   // tiles that a sequence may have, as far as the host knows
   int64_t most = a.limit;
-  if (a.window > 0) most = std::min<int64_t>(most, (int64_t)a.window + a.tokens);
-  const int64_t tiles = most / T::TS + 2;
+  if (a.window > 0) most = std::min<int64_t>(most, (int64_t)a.window + a.tokens + a.sinks);
+  const int64_t tiles = most / T::TS + (a.sinks > 0 ? 3 : 2);
   a.plan_shift = 0;
   while (a.seqs * ((tiles >> a.plan_shift) + 1) >= ((int64_t)1 << 30)) a.plan_shift++;
   // Sequences of two chunks or more have 2 * chunks at most, each a record and a count.
@@ -925,7 +993,7 @@ template <typename KT, int DT>
 void launch_attention_rows(PagedArgs a, int cus, size_t part_floats, hipStream_t st) {
   const int groups = (a.tokens * a.G + 15) / 16;
   a.units = a.Hkv * groups;
-  const int64_t held = std::min<int64_t>(a.limit, a.window > 0 ? (int64_t)a.window + a.tokens : INT_MAX);
+  const int64_t held = std::min<int64_t>(a.limit, a.window > 0 ? (int64_t)a.window + a.tokens + a.sinks : INT_MAX);
   if ((int64_t)a.seqs * a.units < cus)
     launch_attention_of<KT, DT, 8, false>(a, cus, part_floats, st);
   else if (groups > 1 || a.seqs * held * 2 * a.Hkv * DT * (int64_t)sizeof(KT) <= (int64_t)256 << 20)
@@ -956,17 +1024,19 @@ static void launch_append_of(const PagedArgs& a, hipStream_t st) {
   }
 }
 
-bool launch_paged_append(bool kv_f32, const PagedArgs& a, hipStream_t st) {
-  if (kv_f32) launch_append_of<float>(a, st);
-  else launch_append_of<uint16_t>(a, st);
+bool launch_paged_append(int kv_size, const PagedArgs& a, hipStream_t st) {
+  if (kv_size == 4) launch_append_of<float>(a, st);
+  else if (kv_size == 2) launch_append_of<uint16_t>(a, st);
+  else launch_paged_append8(a, st);
   return true;
 }
 
-bool launch_paged_attention(bool kv_f32, const PagedArgs& a, int cus, size_t part_floats, hipStream_t st) {
+bool launch_paged_attention(int kv_size, const PagedArgs& a, int cus, size_t part_floats, hipStream_t st) {
 #define PAGED_D(DT)                                                                \
   case DT:                                                                         \
-    if (kv_f32) launch_attention_rows<float, DT>(a, cus, part_floats, st);         \
-    else launch_attention_rows<uint16_t, DT>(a, cus, part_floats, st);             \
+    if (kv_size == 4) launch_attention_rows<float, DT>(a, cus, part_floats, st);   \
+    else if (kv_size == 2) launch_attention_rows<uint16_t, DT>(a, cus, part_floats, st); \
+    else launch_attention_rows<uint8_t, DT>(a, cus, part_floats, st);              \
     return true;
   switch (a.D) { PAGED_D(32) PAGED_D(64) PAGED_D(96) PAGED_D(128) }
 #undef PAGED_D

@@ -14,7 +14,7 @@ import numpy as np
 HERE = Path(__file__).resolve().parent
 LIB_PATH = HERE / "libtlm.so"
 
-FMT_F16, FMT_Q4, FMT_F32 = 1, 2, 3
+FMT_F16, FMT_Q4, FMT_F32, FMT_F8 = 1, 2, 3, 4
 (T_EMBED, T_LM_HEAD, T_LM_HEAD_SCALES, T_FINAL_NORM, T_ATTN_NORM, T_FFN_NORM, T_WQKV, T_WQKV_SCALES, T_BQKV, T_WO,
  T_WO_SCALES, T_WGATE, T_WGATE_SCALES, T_WUP, T_WUP_SCALES, T_WDOWN, T_WDOWN_SCALES) = range(17)
 LOGITS = 1
@@ -30,7 +30,8 @@ EXPORTS = [
     "tlm_op_attention", "tlm_op_attention_rows", "tlm_op_attention_rows_noalloc", "tlm_attn_reset", "tlm_attn_read_cache", "tlm_op_logits", "tlm_op_argmax",
     "tlm_op_topk", "tlm_read_candidates",
     "tlm_paged_create", "tlm_paged_destroy", "tlm_op_paged_append", "tlm_op_paged_attention", "tlm_paged_status",
-    "tlm_paged_locate", "tlm_op_verify_drafts",
+    "tlm_paged_locate", "tlm_paged_page_bytes", "tlm_paged_set_sinks", "tlm_paged_scale_at", "tlm_op_paged_reserve",
+    "tlm_op_adjust_logits", "tlm_op_verify_drafts",
     "tlm_model_create", "tlm_model_destroy", "tlm_model_upload", "tlm_model_finalize", "tlm_model_set_prefill",
     "tlm_compute_token",
     "tlm_prefill", "tlm_read_logits", "tlm_read_token", "tlm_decode_greedy", "tlm_reset_cache", "tlm_kv_write",
@@ -65,6 +66,22 @@ class PagedBatch(ctypes.Structure):
     _fields_ = [("k_pages", ctypes.c_void_p), ("v_pages", ctypes.c_void_p), ("tables", ctypes.c_void_p),
                 ("starts", ctypes.c_void_p), ("counts", ctypes.c_void_p), ("num_pages", ctypes.c_int32),
                 ("table_width", ctypes.c_int32), ("seqs", ctypes.c_int32), ("tokens", ctypes.c_int32)]
+
+
+class PagedRequest(ctypes.Structure):
+    _fields_ = [("lengths", ctypes.c_void_p), ("counts", ctypes.c_void_p), ("tables", ctypes.c_void_p),
+                ("refs", ctypes.c_void_p), ("out_tables", ctypes.c_void_p), ("out_refs", ctypes.c_void_p),
+                ("starts", ctypes.c_void_p), ("slots", ctypes.c_void_p), ("num_pages", ctypes.c_int32),
+                ("table_width", ctypes.c_int32), ("seqs", ctypes.c_int32), ("tokens", ctypes.c_int32)]
+
+
+class LogitRules(ctypes.Structure):
+    _fields_ = [("logits", ctypes.c_void_p), ("out", ctypes.c_void_p), ("counts", ctypes.c_void_p),
+                ("history", ctypes.c_void_p), ("history_counts", ctypes.c_void_p), ("drafts", ctypes.c_void_p),
+                ("repetition", ctypes.c_void_p), ("frequency", ctypes.c_void_p), ("presence", ctypes.c_void_p),
+                ("bias_ids", ctypes.c_void_p), ("biases", ctypes.c_void_p), ("masks", ctypes.c_void_p),
+                ("seqs", ctypes.c_int32), ("tokens", ctypes.c_int32), ("vocab", ctypes.c_int32),
+                ("history_width", ctypes.c_int32), ("bias_width", ctypes.c_int32)]
 
 
 class ModelDesc(ctypes.Structure):
@@ -137,6 +154,12 @@ def lib():
             "tlm_paged_status": ([VP], ctypes.c_int),
             "tlm_paged_locate": ([ctypes.POINTER(PagedDesc), i32, VP, i32, i32, i32, i32,
                                   ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_int64)], ctypes.c_int),
+            "tlm_paged_page_bytes": ([ctypes.POINTER(PagedDesc), ctypes.POINTER(sz)], ctypes.c_int),
+            "tlm_paged_set_sinks": ([VP, i32], ctypes.c_int),
+            "tlm_paged_scale_at": ([ctypes.POINTER(PagedDesc), i32, VP, i32, i32, i32, ctypes.POINTER(ctypes.c_int64)],
+                                   ctypes.c_int),
+            "tlm_op_paged_reserve": ([VP, ctypes.POINTER(PagedRequest)], ctypes.c_int),
+            "tlm_op_adjust_logits": ([VP, ctypes.POINTER(LogitRules)], ctypes.c_int),
             "tlm_op_verify_drafts": ([VP, VP, VP, VP, VP, VP, i32, i32, i32, dbl, VP, VP], ctypes.c_int),
             "tlm_read_candidates": ([VP, ctypes.c_int, dbl, VP, VP], ctypes.c_int),
             "tlm_model_create": ([VP, ctypes.POINTER(ModelDesc), ctypes.POINTER(VP)], ctypes.c_int),
@@ -404,10 +427,24 @@ def paged_locate(desc: PagedDesc, num_pages: int, table, position: int, kv_head:
     return k.value, v.value
 
 
+def paged_scale_at(desc: PagedDesc, num_pages: int, table, position: int, kv_head: int) -> int:
+    """The byte in a K and in a V pool of 8-bit values where the fp32 scale of a position lies (no device)."""
+    t = np.ascontiguousarray(table, np.int32).reshape(-1)
+    at = ctypes.c_int64()
+    check(lib().tlm_paged_scale_at(ctypes.byref(desc), num_pages, _ptr(t), t.size, position, kv_head, ctypes.byref(at)))
+    return at.value
+
+
+def paged_page_bytes(desc: PagedDesc) -> int:
+    """Bytes of one page in a pool, its scales among them (no device)."""
+    n = ctypes.c_size_t()
+    check(lib().tlm_paged_page_bytes(ctypes.byref(desc), ctypes.byref(n)))
+    return n.value
+
+
 def paged_sizes(d: PagedDesc):
     """(bytes of a page in one pool, elements of a row of queries, of a row of q|k|v)."""
-    return (d.kv_heads * d.page_tokens * d.head_dim * (4 if d.kv_fmt == FMT_F32 else 2), d.heads * d.head_dim,
-            (d.heads + 2 * d.kv_heads) * d.head_dim)
+    return paged_page_bytes(d), d.heads * d.head_dim, (d.heads + 2 * d.kv_heads) * d.head_dim
 
 
 def _addr(b):
@@ -484,6 +521,35 @@ class Paged:
             check(rc)
         return out
 
+    def set_sinks(self, sinks: int):
+        """The first positions that stay visible behind the sliding window, from the next call on."""
+        check(lib().tlm_paged_set_sinks(self.ptr, int(sinks)))
+
+    def request(self, lengths: Buffer, tables: Buffer, table_width: int, refs: Buffer, num_pages: int, starts: Buffer,
+                seqs: int, tokens: int = 1, counts: Optional[Buffer] = None, slots: Optional[Buffer] = None,
+                out_tables: Optional[Buffer] = None, out_refs: Optional[Buffer] = None) -> PagedRequest:
+        """What a step wants of the pool: lengths, starts (and counts) int32 [seqs], tables int32 [seqs][table_width],
+        refs int32 [num_pages], slots int64 [seqs][tokens]; tables and refs change in place without out_*."""
+        out_tables, out_refs = out_tables or tables, out_refs or refs
+        for name, b, need in (("lengths", lengths, 4 * seqs), ("counts", counts, 4 * seqs),
+                              ("tables", tables, 4 * seqs * table_width), ("refs", refs, 4 * num_pages),
+                              ("out_tables", out_tables, 4 * seqs * table_width),
+                              ("out_refs", out_refs, 4 * num_pages), ("starts", starts, 4 * seqs),
+                              ("slots", slots, 8 * seqs * tokens)):
+            if getattr(b, "nbytes", need) < need:  # the kernels read or write that much
+                raise TlmError(TLM_ERR_INVALID, f"TLMPaged: {name} holds {b.nbytes} bytes of {need}")
+        r = PagedRequest(lengths.ptr, _addr(counts), tables.ptr, refs.ptr, out_tables.ptr, out_refs.ptr, starts.ptr,
+                         _addr(slots), num_pages, table_width, seqs, tokens)
+        r.keep = (lengths, counts, tables, refs, out_tables, out_refs, starts, slots)
+        return r
+
+    def reserve(self, request: PagedRequest) -> PagedRequest:
+        """The step's page tables, first positions and slots from the sequences' lengths (tlm_op_paged_reserve)."""
+        rc = lib().tlm_op_paged_reserve(self.ptr, request)
+        if rc:
+            check(rc)
+        return request
+
     def status(self):
         """Waits; raises where a call since the last status met a row or a page out of range."""
         check(lib().tlm_paged_status(self.ptr))
@@ -527,6 +593,39 @@ def topk(ctx: Context, logits_buf: Buffer, n: int, k: int, softcap: float = 0.0)
     tok.free()
     sc.free()
     return [(int(a), float(b)) for a, b in zip(t, v)]
+
+
+def logit_rules(logits_buf: Buffer, seqs: int, tokens: int, vocab: int, out: Optional[Buffer] = None,
+                counts: Optional[Buffer] = None, history: Optional[Buffer] = None, history_width: int = 0,
+                history_counts: Optional[Buffer] = None, drafts: Optional[Buffer] = None,
+                repetition: Optional[Buffer] = None, frequency: Optional[Buffer] = None,
+                presence: Optional[Buffer] = None, bias_ids: Optional[Buffer] = None,
+                biases: Optional[Buffer] = None, bias_width: int = 0, masks: Optional[Buffer] = None) -> LogitRules:
+    """A step's penalties, biases and masks (tlm_logit_rules); without `out` the logits change in place."""
+    out = out or logits_buf
+    rows = seqs * tokens
+    for name, b, need in (("logits", logits_buf, 4 * rows * vocab), ("out", out, 4 * rows * vocab),
+                          ("counts", counts, 4 * seqs), ("history", history, 4 * seqs * history_width),
+                          ("history_counts", history_counts, 4 * seqs), ("drafts", drafts, 4 * seqs * (tokens - 1)),
+                          ("repetition", repetition, 4 * seqs), ("frequency", frequency, 4 * seqs),
+                          ("presence", presence, 4 * seqs), ("bias_ids", bias_ids, 4 * seqs * bias_width),
+                          ("biases", biases, 4 * seqs * bias_width), ("masks", masks, 4 * rows * (-(-vocab // 32)))):
+        if getattr(b, "nbytes", need) < need:  # the kernels read or write that much
+            raise TlmError(TLM_ERR_INVALID, f"TLMLogitRules: {name} holds {b.nbytes} bytes of {need}")
+    r = LogitRules(logits_buf.ptr, out.ptr, _addr(counts), _addr(history), _addr(history_counts), _addr(drafts),
+                   _addr(repetition), _addr(frequency), _addr(presence), _addr(bias_ids), _addr(biases), _addr(masks),
+                   seqs, tokens, vocab, history_width, bias_width)
+    r.keep = (logits_buf, out, counts, history, history_counts, drafts, repetition, frequency, presence, bias_ids,
+              biases, masks)
+    return r
+
+
+def adjust_logits(ctx: Context, rules: LogitRules) -> LogitRules:
+    """Penalties, biases and masks on logits, before a token is picked (tlm_op_adjust_logits)."""
+    rc = lib().tlm_op_adjust_logits(ctx.ptr, rules)
+    if rc:
+        check(rc)
+    return rules
 
 
 def verify_drafts(ctx: Context, logits_buf: Buffer, seqs: int, tokens: int, vocab: int, accepted: Buffer,
