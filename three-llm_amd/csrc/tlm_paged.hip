@@ -313,14 +313,14 @@ struct PagedTile {
 struct SeqWork {
   int start, rows, first, tiles, sunk;
 };
-template <int SHIFT>
+template <int SHIFT, bool SINK>
 __device__ __forceinline__ SeqWork seq_work(const PagedArgs& a, int s, bool* bad) {
   SeqWork w;
   w.start = a.starts[s];
   w.rows = paged_rows(w.start, a.counts ? a.counts[s] : a.tokens, a.tokens, a.limit, bad);
   const int first = a.window > 0 ? max(0, w.start - a.window + 1) : 0;
   w.first = first >> SHIFT;
-  w.sunk = w.rows > 0 ? min((a.sinks + (1 << SHIFT) - 1) >> SHIFT, w.first) : 0;
+  w.sunk = SINK && w.rows > 0 ? min((a.sinks + (1 << SHIFT) - 1) >> SHIFT, w.first) : 0;
   w.tiles = w.rows > 0 ? ((w.start + w.rows - 1) >> SHIFT) - w.first + 1 + w.sunk : 0;
   return w;
 }
@@ -376,7 +376,7 @@ __device__ __forceinline__ int plan_chunks_of(const PagedArgs& a, int c, int til
   return tiles <= a.whole ? min(tiles, 1) : (tiles + c - 1) / c;
 }
 
-template <int SHIFT>
+template <int SHIFT, bool SINK>
 __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedArgs a) {
   constexpr int W = kPlanThreads / 64;
   __shared__ int sh[2][W];
@@ -385,7 +385,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedArgs a) {
   bool any = false, bad;
   int sum = 0;
   for (int s = tid; s < a.seqs; s += kPlanThreads) {
-    sum += plan_part(a, seq_work<SHIFT>(a, s, &bad).tiles);
+    sum += plan_part(a, seq_work<SHIFT, SINK>(a, s, &bad).tiles);
     any |= bad;
   }
   if (any) paged_flag(a.status, kPagedStatusRows);
@@ -399,7 +399,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedArgs a) {
   int before = 0, slots = 0;
   for (int g0 = 0; g0 < groups; g0 += W) {  // a wave per 64 sequences
     const int s = 64 * (g0 + w) + lane;
-    const int n = s < a.seqs ? plan_chunks_of(a, c, seq_work<SHIFT>(a, s, &bad).tiles) : 0;
+    const int n = s < a.seqs ? plan_chunks_of(a, c, seq_work<SHIFT, SINK>(a, s, &bad).tiles) : 0;
     const int chunks = __builtin_amdgcn_readlane(wave_scan(n), 63);
     const int parts = __builtin_amdgcn_readlane(wave_scan(n > 1 ? n : 0), 63);
     __syncthreads();  // sh of the round before has been read
@@ -416,7 +416,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedArgs a) {
   }
 }
 
-template <int SHIFT>
+template <int SHIFT, bool SINK>
 __device__ __forceinline__ bool plan(const PagedArgs& a, int g, SeqChunk& r) {
   const int lane = threadIdx.x & 63;
   const SeqWork none{0, 0, 0, 0, 0};
@@ -437,7 +437,7 @@ __device__ __forceinline__ bool plan(const PagedArgs& a, int g, SeqChunk& r) {
     r.w.rows = __builtin_amdgcn_readlane(w.rows, l);
     r.w.first = __builtin_amdgcn_readlane(w.first, l);
     r.w.tiles = __builtin_amdgcn_readlane(w.tiles, l);
-    r.w.sunk = __builtin_amdgcn_readlane(w.sunk, l);
+    r.w.sunk = SINK ? __builtin_amdgcn_readlane(w.sunk, l) : 0;
     r.n = __builtin_amdgcn_readlane(n, l);
     r.chunk = g - before - __builtin_amdgcn_readlane(incl - n, l);
     r.slot = slots + __builtin_amdgcn_readlane(sincl - m, l);
@@ -456,7 +456,7 @@ __device__ __forceinline__ bool plan(const PagedArgs& a, int g, SeqChunk& r) {
     }
     c = a.plan[0], before = a.plan[1 + lo], slots = a.plan[1 + groups + lo];
     const int s0 = 64 * lo;
-    return find(s0 + lane < a.seqs ? seq_work<SHIFT>(a, s0 + lane, &b) : none, s0);
+    return find(s0 + lane < a.seqs ? seq_work<SHIFT, SINK>(a, s0 + lane, &b) : none, s0);
   }
   // the first kSeqs times 64 sequences stay in registers, a lane each
   constexpr int kSeqs = 4;
@@ -466,13 +466,13 @@ __device__ __forceinline__ bool plan(const PagedArgs& a, int g, SeqChunk& r) {
 #pragma unroll
   for (int k = 0; k < kSeqs; k++) {
     w[k] = none, bad[k] = false;
-    if (64 * k < a.seqs && 64 * k + lane < a.seqs) w[k] = seq_work<SHIFT>(a, 64 * k + lane, &bad[k]);
+    if (64 * k < a.seqs && 64 * k + lane < a.seqs) w[k] = seq_work<SHIFT, SINK>(a, 64 * k + lane, &bad[k]);
   }
 #pragma unroll
   for (int k = 0; k < kSeqs; k++) sum += plan_part(a, w[k].tiles);
   bool any = bad[0] || bad[1] || bad[2] || bad[3];
   for (int s = 64 * kSeqs + lane; s < a.seqs; s += 64) {
-    sum += plan_part(a, seq_work<SHIFT>(a, s, &b).tiles);
+    sum += plan_part(a, seq_work<SHIFT, SINK>(a, s, &b).tiles);
     any |= b;
   }
   if (any && blockIdx.x == 0 && threadIdx.x < 64) paged_flag(a.status, kPagedStatusRows);
@@ -487,7 +487,7 @@ __device__ __forceinline__ bool plan(const PagedArgs& a, int g, SeqChunk& r) {
   for (int k = 0; k < kSeqs; k++)
     if (64 * k < a.seqs && find(w[k], 64 * k)) return true;
   for (int s0 = 64 * kSeqs; s0 < a.seqs; s0 += 64) {
-    const SeqWork v = s0 + lane < a.seqs ? seq_work<SHIFT>(a, s0 + lane, &b) : none;
+    const SeqWork v = s0 + lane < a.seqs ? seq_work<SHIFT, SINK>(a, s0 + lane, &b) : none;
     if (find(v, s0)) return true;
   }
   return false;
@@ -509,7 +509,7 @@ __device__ __forceinline__ u32x4 codes_f16(uint32_t a, uint32_t b) {
   return y;
 }
 
-template <typename KT, int DT, int W, bool STREAM>
+template <typename KT, int DT, int W, bool STREAM, bool SINK>
 __global__ __launch_bounds__(64 * W, DT <= 64 ? 4 : 2) void paged_attention_kernel(PagedArgs a) {
   using T = PagedTile<KT>;
   constexpr int SUB = T::SUB, TS = T::TS, NF = DT / 16;  // 16-dim slabs of the output
@@ -522,7 +522,7 @@ __global__ __launch_bounds__(64 * W, DT <= 64 ? 4 : 2) void paged_attention_kern
   const int unit = blockIdx.x % a.units, hk = unit % a.Hkv, r0 = (a.units - 1 - unit) / a.Hkv * 16;
   const int g = blockIdx.x / a.units;
   SeqChunk sc;
-  if (!plan<T::SHIFT>(a, g, sc)) return;
+  if (!plan<T::SHIFT, SINK>(a, g, sc)) return;
   const int ci = sc.chunk, tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int R = sc.w.rows * a.G;  // rows of the kv head
   if (r0 >= R) return;
@@ -533,8 +533,8 @@ __global__ __launch_bounds__(64 * W, DT <= 64 ? 4 : 2) void paged_attention_kern
   const int lo_all = a.window > 0 ? max(0, start + jb - a.window + 1) : 0, hi_all = start + ja;
   // the chunk's tiles: of the sinks from c0 on, then those of the block's windows [t0, t1)
   const int per = (sc.w.tiles + sc.n - 1) / sc.n, c0 = ci * per, c1 = min(c0 + per, sc.w.tiles);
-  const int past = (hi_any >> T::SHIFT) + 1, sinks = min((a.sinks + TS - 1) >> T::SHIFT, past);
-  const int sunk = max(0, min(sinks, c1) - c0), base = sc.w.first - sc.w.sunk;
+  const int past = (hi_any >> T::SHIFT) + 1, sinks = SINK ? min((a.sinks + TS - 1) >> T::SHIFT, past) : 0;
+  const int sunk = SINK ? max(0, min(sinks, c1) - c0) : 0, base = sc.w.first - sc.w.sunk;
   const int t0 = max(base + max(c0, sinks), lo_any >> T::SHIFT), t1 = min(base + c1, past);
   const int tiles = sunk + max(0, t1 - t0);
   auto tile_of = [&](int i) { return i < sunk ? c0 + i : t0 + i - sunk; };
@@ -629,7 +629,7 @@ __global__ __launch_bounds__(64 * W, DT <= 64 ? 4 : 2) void paged_attention_kern
   for (int f = 0; f < NF; f++) o[f] = (f32x4){0.f, 0.f, 0.f, 0.f};
 
   // whether a row that sees [first, last] and sinks sees position x
-  auto in = [&](int x, int first, int last) { return (x >= first || x < a.sinks) && x <= last; };
+  auto in = [&](int x, int first, int last) { return (x >= first || (SINK && x < a.sinks)) && x <= last; };
   // V with positions outside [first, last] and the sinks taken out (0 times what they hold may be NaN)
   auto keep = [&](const u32x4& v, int p, int first, int last) {
     u32x4 y;
@@ -662,7 +662,7 @@ __global__ __launch_bounds__(64 * W, DT <= 64 ? 4 : 2) void paged_attention_kern
   auto process = [&](Tile& x, int t, int i64, auto k_read, auto v_read) {
     const int p = t << T::SHIFT;
     // some row does not see all of it (wave-uniform)
-    const bool edge = (p < lo_all && p + TS > a.sinks) || p + TS - 1 > hi_all;
+    const bool edge = (p < lo_all && !(SINK && p + TS <= a.sinks)) || p + TS - 1 > hi_all;
     float mult = qmult, lv = 0.f;
     if (F8) {
       mult = fmaxf(ldexpf(qmult, paged8_exponent_of(__builtin_amdgcn_readlane(kscale, i64))), FLT_TRUE_MIN);
@@ -948,8 +948,8 @@ __global__ __launch_bounds__(64 * W, DT <= 64 ? 4 : 2) void paged_attention_kern
   }
 }
 
-template <typename KT, int DT, int W, bool STREAM>
-void launch_attention_of(PagedArgs a, int cus, size_t part_floats, hipStream_t st) {
+template <typename KT, int DT, int W, bool STREAM, bool SINK>
+void launch_attention_as(PagedArgs a, int cus, size_t part_floats, hipStream_t st) {
   using T = PagedTile<KT>;
   // tiles that a sequence may have, as far as the host knows
   int64_t most = a.limit;
@@ -975,8 +975,16 @@ void launch_attention_of(PagedArgs a, int cus, size_t part_floats, hipStream_t s
   a.whole = 32;
   const int64_t per_seq = fit < 1 || tiles <= a.whole ? 1 : (tiles + a.chunk_min - 1) / a.chunk_min;
   const int64_t blocks = std::min<int64_t>(a.chunks + a.seqs, a.seqs * per_seq) * a.units;
-  if (a.plan) hipLaunchKernelGGL((paged_plan_kernel<T::SHIFT>), dim3(1), dim3(kPlanThreads), 0, st, a);
-  hipLaunchKernelGGL((paged_attention_kernel<KT, DT, W, STREAM>), dim3((unsigned)blocks), dim3(64 * W), 0, st, a);
+  if (a.plan) hipLaunchKernelGGL((paged_plan_kernel<T::SHIFT, SINK>), dim3(1), dim3(kPlanThreads), 0, st, a);
+  hipLaunchKernelGGL((paged_attention_kernel<KT, DT, W, STREAM, SINK>), dim3((unsigned)blocks), dim3(64 * W), 0, st, a);
+}
+
+template <typename KT, int DT, int W, bool STREAM>
+void launch_attention_of(const PagedArgs& a, int cus, size_t part_floats, hipStream_t st) {
+  if (a.sinks > 0)
+    launch_attention_as<KT, DT, W, STREAM, true>(a, cus, part_floats, st);
+  else
+    launch_attention_as<KT, DT, W, STREAM, false>(a, cus, part_floats, st);
 }
 
 // Waves a block: four where the sequences' kv heads and row groups alone give a
