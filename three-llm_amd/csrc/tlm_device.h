@@ -70,6 +70,17 @@ __device__ __forceinline__ float sum8(float v) {
   return v + dpp<kDppHalfMirror>(v);
 }
 
+// Sum over the wave's lanes up to each, over integers.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr:1, within 16 lanes
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
+  return v;
+}
+
 // v of lane l ^ 16 / l ^ 32, through gfx950's VALU lane swaps
 // (v_permlane16_swap / v_permlane32_swap) rather than an LDS round trip.
 __device__ __forceinline__ float lane_swap16(float v) {

@@ -12,28 +12,58 @@ namespace {
 // of those past L is taken: the sequences in their order, the free pages (refs 0)
 // lowest first, as long as the sum of what has been asked for so far is no more than
 // the free pages.  A sequence that lacks one that holds positions below L gets nothing.
-constexpr int kSegment = 4096;  // pages whose free ones a block counts
+constexpr int kSegment = 4096;  // pages whose free ones are counted together
+constexpr int kPiece = 512;     // entries of a table that a wave looks at at a time
+constexpr int kLost = 1 << 30;  // in want: positions are lost
 
-// a.work: want[seqs] (pages that a sequence lacks, -1 where positions are lost), then
-// base[seqs] (before it, or -1: it gets none), the free pages before each segment, the
-// number taken, and the pages taken in order.
+// Waves that share a sequence's table: enough of them to fill the chip.
+__host__ __device__ inline int waves_of(const ReserveArgs& a) {
+  int n = 1;
+  while (2 * n <= 16 && 2 * n * a.seqs <= 4096 && n * kPiece < a.width) n *= 2;
+  return n;
+}
+
+// a.work: want[seqs][waves] (pages that a sequence lacks), base[seqs] (those before it, or
+// -1: it gets none), the free pages of each segment (then: before each), the number
+// taken, and the pages taken in order.
 struct Work {
   int32_t *want, *base, *segment, *taken, *pages;
-  int segments;
+  int segments, waves;
 };
 __host__ __device__ inline Work work_of(const ReserveArgs& a) {
   Work w;
   w.segments = (a.num_pages + kSegment - 1) / kSegment;
+  w.waves = waves_of(a);
   w.want = a.work;
-  w.base = w.want + a.seqs;
+  w.base = w.want + (size_t)a.seqs * w.waves;
   w.segment = w.base + a.seqs;
   w.taken = w.segment + w.segments;
   w.pages = w.taken + 1;
   return w;
 }
 
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4u __attribute__((ext_vector_type(4), aligned(4)));  // from any 4-byte address
+__device__ __forceinline__ i32x4u four(const int32_t* p, int i, int n, int none) {
+  i32x4u v = {none, none, none, none};
+  if (i + 4 <= n) return *(const TLM_GLOBAL i32x4u*)(p + i);
+#pragma unroll
+  for (int e = 0; e < 3; e++)
+    if (i + e < n) v[e] = p[i + e];
+  return v;
+}
+__device__ __forceinline__ void put_four(int32_t* p, int i, int n, i32x4u v) {
+  if (i + 4 <= n) {
+    *(TLM_GLOBAL i32x4u*)(p + i) = v;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 3; e++)
+      if (i + e < n) p[i + e] = v[e];
+  }
+}
+
 struct Seq {
-  int length, rows;
+  int length, rows, past;  // past: the first page that begins at its length or later
   PagedUse use;
   bool bad;
   __device__ __forceinline__ bool used(int i) const { return i < use.sink || (i >= use.first && i < use.end); }
@@ -43,6 +73,7 @@ __device__ __forceinline__ Seq seq_of(const ReserveArgs& a, int s) {
   q.length = a.lengths[s];
   q.rows = paged_rows(q.length, a.counts ? a.counts[s] : a.tokens, a.tokens, a.limit, &q.bad);
   q.use = PagedUse{0, 0, 0};
+  q.past = (int)(((int64_t)q.length + (1 << a.page_shift) - 1) >> a.page_shift);
   if (q.length >= 0) {
     // a length past the limit keeps what the table can hold of it
     q.use = paged_use(min(q.length, a.limit), q.rows, a.window, a.sinks, a.page_shift);
@@ -50,39 +81,64 @@ __device__ __forceinline__ Seq seq_of(const ReserveArgs& a, int s) {
   return q;
 }
 
-__device__ __forceinline__ int sum64(int v) {
-#pragma unroll
-  for (int w = 1; w < 64; w <<= 1) v += __shfl_xor(v, w);
-  return v;
+__device__ __forceinline__ int sum64(int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
+
+// One entry, `p`, of a sequence's table: what becomes of it; whether the sequence lacks a
+// page there, and whether with positions that it has.
+struct Entry {
+  int becomes;
+  bool back, lacks, lost;
+};
+__device__ __forceinline__ Entry entry_of(const ReserveArgs& a, const Seq& q, int i, int p) {
+  const bool has = p >= 0 && p < a.num_pages, used = q.used(i), old = i < q.past;
+  return Entry{has && used ? p : -1, has && !used, used && !has && !old, used && !has && old};
 }
 
+__device__ __forceinline__ void report(const ReserveArgs& a, bool bad, bool lost) {
+  const int bits = (bad ? kPagedStatusRows : 0) | (lost ? kPagedStatusPage : 0);
+  if (bits) __hip_atomic_fetch_or(a.status, bits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// The counts as they are, where they do not change in place.
 __global__ __launch_bounds__(256) void reserve_copy_kernel(ReserveArgs a) {
-  for (int i = blockIdx.x * 256 + threadIdx.x; i < a.num_pages; i += gridDim.x * 256) a.out_refs[i] = a.refs[i];
+  const int64_t step = (int64_t)gridDim.x * 1024;
+  for (int64_t i = 4 * ((int64_t)blockIdx.x * 256 + threadIdx.x); i < a.num_pages; i += step)
+    put_four(a.out_refs, (int)i, a.num_pages, four(a.refs, (int)i, a.num_pages, 0));
 }
 
-// What goes back and what is lacking: a wave per sequence.
+// What goes back and what is lacking.
 __global__ __launch_bounds__(256) void reserve_rows_kernel(ReserveArgs a) {
-  const int s = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const Work w = work_of(a);
+  const int item = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, s = item / w.waves;
   if (s >= a.seqs) return;
-  const Seq q = seq_of(a, s);
   const int32_t* const from = a.tables + (size_t)s * a.width;
   int32_t* const to = a.out_tables + (size_t)s * a.width;
+  const Seq q = seq_of(a, s);
   int want = 0, lost = 0;
-  for (int i = lane; i < a.width; i += 64) {
-    const int p = from[i];
-    const bool has = p >= 0 && p < a.num_pages, used = q.used(i);
-    if (has && !used) atomicSub(a.out_refs + p, 1);
-    const bool lacks = used && !has, old = ((int64_t)i << a.page_shift) < q.length;
-    want += lacks && !old;
-    lost += lacks && old;
-    to[i] = has && used ? p : -1;
+  for (int64_t i0 = item % w.waves * kPiece; i0 < a.width; i0 += w.waves * kPiece) {
+    i32x4u v[kPiece / 256];
+#pragma unroll
+    for (int k = 0; k < kPiece / 256; k++) v[k] = four(from, (int)i0 + 256 * k + 4 * lane, a.width, -1);
+#pragma unroll
+    for (int k = 0; k < kPiece / 256; k++) {
+      const int i = (int)i0 + 256 * k + 4 * lane;
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        if (i + e >= a.width) continue;
+        const Entry x = entry_of(a, q, i + e, v[k][e]);
+        if (x.back) atomicSub(a.out_refs + v[k][e], 1);
+        want += x.lacks;
+        lost |= x.lost;
+        v[k][e] = x.becomes;
+      }
+      put_four(to, i, a.width, v[k]);
+    }
   }
   want = sum64(want);
-  lost = sum64(lost);
+  lost = __ballot(lost) != 0;
   if (lane == 0) {
-    work_of(a).want[s] = lost ? -1 : want;
-    const int bits = (q.bad ? kPagedStatusRows : 0) | (lost ? kPagedStatusPage : 0);
-    if (bits) __hip_atomic_fetch_or(a.status, bits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    w.want[item] = lost ? kLost : want;
+    report(a, q.bad && item % w.waves == 0, lost);
   }
 }
 
@@ -92,12 +148,7 @@ struct Scan {
 };
 __device__ __forceinline__ int64_t scan1024(int v, Scan& sc, int64_t* all) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  int incl = v;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int x = __shfl_up(incl, d);
-    if (lane >= d) incl += x;
-  }
+  const int incl = wave_scan(v);
   __syncthreads();
   if (lane == 63) sc.sh[w] = incl;
   __syncthreads();
@@ -110,106 +161,228 @@ __device__ __forceinline__ int64_t scan1024(int v, Scan& sc, int64_t* all) {
   return before;
 }
 
-// Free pages of each segment; the last block turns them into running sums and shares
-// them out.
+// The free pages of each segment, a block each; the last block turns the sums into
+// running ones and shares the pages out.
 __global__ __launch_bounds__(1024) void reserve_count_kernel(ReserveArgs a) {
   __shared__ Scan sc;
   __shared__ int last;
   const Work w = work_of(a);
-  const int tid = threadIdx.x;
-  int n = 0;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int64_t i0 = (int64_t)blockIdx.x * kSegment;
+  const int n = (int)min((int64_t)kSegment, a.num_pages - i0);
+  const i32x4u v = four(a.out_refs + i0, 4 * tid, n, 1);
+  // what a sequence lacks in all; the first 1024 sequences' is on its way meanwhile
+  auto want_of = [&](int s) {
+    int x[16], want = 0, lost = 0;
 #pragma unroll
-  for (int k = 0; k < kSegment / 1024; k++) {
-    const int64_t i = (int64_t)blockIdx.x * kSegment + k * 1024 + tid;
-    n += i < a.num_pages && a.out_refs[i] == 0;
-  }
+    for (int k = 0; k < 16; k++) x[k] = k < w.waves ? w.want[(size_t)s * w.waves + k] : 0;
+#pragma unroll
+    for (int k = 0; k < 16; k++) want += x[k] & ~kLost, lost |= x[k] & kLost;
+    return lost ? kLost : want;
+  };
+  const int first = tid < a.seqs ? want_of(tid) : kLost;
   int64_t all;
-  scan1024(n, sc, &all);
+  scan1024((v[0] == 0) + (v[1] == 0) + (v[2] == 0) + (v[3] == 0), sc, &all);
   if (tid == 0) {
     __hip_atomic_store(w.segment + blockIdx.x, (int)all, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // it is performed
     last = __hip_atomic_fetch_add(a.arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
   }
   __syncthreads();
   if (!last) return;
   if (tid == 0) __hip_atomic_store(a.arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  // what other blocks stored: past this CU's cache
+  auto left_at = [](const int32_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
   int64_t free = 0;
   for (int b = 0; b < w.segments; b += 1024) {
-    const int v = b + tid < w.segments
-                      ? __hip_atomic_load(w.segment + b + tid, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
-                      : 0;
-    const int64_t before = scan1024(v, sc, &all) + free;
+    const int64_t before = scan1024(b + tid < w.segments ? left_at(w.segment + b + tid) : 0, sc, &all) + free;
     if (b + tid < w.segments) w.segment[b + tid] = (int)before;
     free += all;
   }
-  int64_t asked = 0, taken = 0;
+  int64_t asked = 0;
+  int taken = 0;
   for (int s0 = 0; s0 < a.seqs; s0 += 1024) {
-    const int s = s0 + tid, want = s < a.seqs ? w.want[s] : -1;
-    const int64_t before = scan1024(max(want, 0), sc, &all) + asked;
-    const bool gets = want == 0 || (want > 0 && before + want <= free);
+    const int s = s0 + tid;
+    const int want = s0 == 0 ? first : s < a.seqs ? want_of(s) : kLost;
+    const bool lost = want == kLost;
+    const int64_t before = scan1024(lost ? 0 : want, sc, &all) + asked;
+    const bool gets = !lost && (want == 0 || before + want <= free);
     if (s < a.seqs) w.base[s] = gets ? (int)before : -1;
-    taken = max(taken, gets ? before + want : 0);
+    if (gets && want) taken = max(taken, (int)before + want);
     asked += all;
   }
   // the sequences that get some are the first that ask: the largest end is the number
-  for (int d = 1; d < 64; d <<= 1) taken = max(taken, (int64_t)__shfl_xor((int)taken, d));
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) taken = max(taken, __shfl_xor(taken, d));
   __syncthreads();
-  if ((tid & 63) == 0) sc.sh[tid >> 6] = (int)taken;
+  if (lane == 0) sc.sh[tid >> 6] = taken;
   __syncthreads();
   if (tid == 0) {
-    int most = 0;
-    for (int i = 0; i < 16; i++) most = max(most, sc.sh[i]);
-    *w.taken = most;
+    for (int i = 0; i < 16; i++) taken = max(taken, sc.sh[i]);
+    *w.taken = taken;
   }
 }
 
-// The free pages in order, those taken.
+// The free pages in order, those taken: a block a segment.
 __global__ __launch_bounds__(1024) void reserve_take_kernel(ReserveArgs a) {
   __shared__ Scan sc;
   const Work w = work_of(a);
+  const int64_t i0 = (int64_t)blockIdx.x * kSegment;
+  const int n = (int)min((int64_t)kSegment, a.num_pages - i0);
+  i32x4u v = four(a.out_refs + i0, 4 * threadIdx.x, n, 1);
   const int taken = *w.taken;
   int64_t before = w.segment[blockIdx.x], all;
   if (before >= taken) return;
-  for (int k = 0; k < kSegment / 1024; k++) {
-    const int64_t i = (int64_t)blockIdx.x * kSegment + k * 1024 + threadIdx.x;
-    const int free = i < a.num_pages && a.out_refs[i] == 0;
-    const int64_t rank = scan1024(free, sc, &all) + before;
-    if (free && rank < taken) {
-      w.pages[rank] = (int)i;
-      a.out_refs[i] = 1;
+  const int free = (v[0] == 0) + (v[1] == 0) + (v[2] == 0) + (v[3] == 0);
+  int64_t rank = scan1024(free, sc, &all) + before;
+  if (!free || rank >= taken) return;
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    if (v[e] == 0) {
+      if (rank < taken) {
+        w.pages[rank] = (int)i0 + 4 * threadIdx.x + e;
+        a.out_refs[i0 + 4 * threadIdx.x + e] = 1;
+      }
+      rank++;
     }
-    before += all;
   }
 }
 
-// The pages into the tables, the first positions and the slots: a wave per sequence.
-__global__ __launch_bounds__(256) void reserve_fill_kernel(ReserveArgs a) {
-  const int s = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (s >= a.seqs) return;
-  const Work w = work_of(a);
-  const Seq q = seq_of(a, s);
-  const int want = w.want[s], base = w.base[s];
+// The pages that a sequence gets into its table, its first position and its slots: a wave.
+template <typename P>
+__device__ __forceinline__ void fill(const ReserveArgs& a, const Seq& q, int s, int base, int lane, P page_at) {
   int32_t* const to = a.out_tables + (size_t)s * a.width;
   const int page = 1 << a.page_shift;
   const bool served = q.rows > 0 && base >= 0;
   // what is lacking is all past the length
-  const int i0 = max((int)(((int64_t)q.length + page - 1) >> a.page_shift), 0);
+  const int i0 = max(q.past, 0);
   int at = base;
-  for (int b = i0; served && want > 0 && b < q.use.end; b += 64) {
+  for (int b = i0; served && b < q.use.end; b += 64) {
     const int i = b + lane;
     const bool lacks = i < q.use.end && to[i] < 0;
     const uint64_t m = __ballot(lacks);
-    if (lacks) to[i] = w.pages[at + __popcll(m & ((1ull << lane) - 1))];
+    if (lacks) to[i] = page_at(at + __popcll(m & ((1ull << lane) - 1)));
     at += __popcll(m);
   }
   if (lane == 0) a.starts[s] = served ? q.length : -1;
   if (!a.slots) return;
   __threadfence_block();
   for (int j = lane; j < a.tokens; j += 64) {
-    const int p = q.length + j;
     int64_t slot = -1;
-    if (served && j < q.rows) slot = ((int64_t)to[p >> a.page_shift] << a.page_shift) + (p & (page - 1));
+    if (served && j < q.rows) {
+      const int p = q.length + j;
+      slot = ((int64_t)to[p >> a.page_shift] << a.page_shift) + (p & (page - 1));
+    }
     a.slots[(size_t)s * a.tokens + j] = slot;
+  }
+}
+
+__global__ __launch_bounds__(256) void reserve_fill_kernel(ReserveArgs a) {
+  const int s = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (s >= a.seqs) return;
+  const Work w = work_of(a);
+  fill(a, seq_of(a, s), s, w.base[s], threadIdx.x & 63, [&](int rank) { return w.pages[rank]; });
+}
+
+// Few sequences over a small pool: all of it by one block, with the counts, what is
+// shared out and the pages of the new rows in LDS, in place of four or five launches.
+constexpr int kOnePages = 16384, kOneSeqs = 1024, kOneEntries = 32768, kOneRows = 4096, kOneSlots = 65536;
+__host__ __device__ inline int span_of(const ReserveArgs& a) {  // pages that a sequence's new rows may touch
+  return ((a.tokens - 1) >> a.page_shift) + 2;
+}
+// n / d for n * d below 2^32, by = by_of(d).
+__host__ __device__ inline uint32_t by_of(int d) { return (uint32_t)((((uint64_t)1 << 32) + d - 1) / d); }
+__device__ __forceinline__ int over(int n, int d, uint32_t by) { return d == 1 ? n : (int)__umulhi((uint32_t)n, by); }
+
+__global__ __launch_bounds__(1024) void reserve_one_kernel(ReserveArgs a, uint32_t by_width, uint32_t by_tokens) {
+  constexpr int A = 8;  // entries in flight a thread
+  __shared__ __align__(16) int refs[kOnePages];
+  __shared__ uint16_t pages[kOnePages];
+  __shared__ Seq seqs[kOneSeqs];
+  __shared__ int want[kOneSeqs];
+  __shared__ bool served[kOneSeqs];
+  __shared__ int rowpage[kOneRows];  // of the pages from the one of position `length` on
+  __shared__ Scan sc;
+  const int tid = threadIdx.x, cells = a.seqs * a.width, span = span_of(a);
+  int entry[A];
+#pragma unroll
+  for (int k = 0; k < A; k++) entry[k] = tid + 1024 * k < cells ? a.tables[tid + 1024 * k] : -1;
+  for (int i = 4 * tid; i < a.num_pages; i += 4096)
+    *reinterpret_cast<i32x4*>(refs + i) = four(a.refs, i, a.num_pages, 1);
+  if (tid < a.seqs) {
+    const Seq q = seq_of(a, tid);
+    seqs[tid] = q;
+    want[tid] = 0;
+    report(a, q.bad, false);
+  }
+  __syncthreads();
+  // what goes back and what is lacking
+  for (int c0 = tid; c0 < cells; c0 += A * 1024) {
+#pragma unroll
+    for (int k = 0; k < A; k++) {
+      const int c = c0 + 1024 * k, p = entry[k];
+      if (c >= cells) continue;
+      const int s = over(c, a.width, by_width), i = c - s * a.width;
+      const Seq q = seqs[s];
+      const Entry x = entry_of(a, q, i, p);
+      if (x.back) atomicSub(refs + p, 1);
+      if (x.lacks) atomicAdd(want + s, 1);
+      if (x.lost) atomicOr(want + s, kLost);
+      const int at = i - (q.length >> a.page_shift);
+      if (at >= 0 && at < span) rowpage[s * span + at] = x.lacks ? -2 : x.becomes;
+      a.out_tables[c] = x.becomes;
+      entry[k] = c + A * 1024 < cells ? a.tables[c + A * 1024] : -1;
+    }
+  }
+  __syncthreads();
+  // the free pages that are asked for, lowest first; a sequence gets what it lacks while
+  // it is no more than these
+  const int mine = tid < a.seqs ? want[tid] : kLost;
+  const bool lost = mine & kLost;
+  int64_t asked, free = 0;
+  const int64_t before = scan1024(lost ? 0 : mine, sc, &asked);
+  for (int b = 0; b < a.num_pages && free < asked; b += 4096) {
+    const int i = b + 4 * tid;
+    i32x4 v = {1, 1, 1, 1};
+    if (i < a.num_pages) v = *reinterpret_cast<const i32x4*>(refs + i);
+    int64_t all;
+    int64_t rank = free + scan1024((v[0] == 0) + (v[1] == 0) + (v[2] == 0) + (v[3] == 0), sc, &all);
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+      if (v[e] == 0 && rank < asked) pages[rank++] = (uint16_t)(i + e);
+    free += all;
+  }
+  __syncthreads();
+  if (tid < a.seqs) {
+    const bool gets = !lost && (mine == 0 || before + mine <= free);
+    const Seq q = seqs[tid];
+    const bool serve = q.rows > 0 && gets;
+    report(a, false, lost);
+    a.starts[tid] = serve ? q.length : -1;
+    served[tid] = serve;
+    const int first = q.length >> a.page_shift;
+    int at = (int)before;
+    for (int k = 0; serve && k < span && first + k < q.use.end; k++)
+      if (rowpage[tid * span + k] == -2) {
+        const int p = pages[at++];
+        rowpage[tid * span + k] = p;
+        refs[p] = 1;
+        a.out_tables[tid * a.width + first + k] = p;
+      }
+  }
+  __syncthreads();
+  for (int i = 4 * tid; i < a.num_pages; i += 4096)
+    put_four(a.out_refs, i, a.num_pages, *reinterpret_cast<const i32x4*>(refs + i));
+  if (!a.slots) return;
+  for (int c = tid; c < a.seqs * a.tokens; c += 1024) {
+    const int s = over(c, a.tokens, by_tokens), j = c - s * a.tokens;
+    const Seq& q = seqs[s];
+    int64_t slot = -1;
+    if (served[s] && j < q.rows) {
+      const int p = q.length + j, k = (p >> a.page_shift) - (q.length >> a.page_shift);
+      slot = ((int64_t)rowpage[s * span + k] << a.page_shift) + (p & ((1 << a.page_shift) - 1));
+    }
+    a.slots[c] = slot;
   }
 }
 
@@ -219,18 +392,23 @@ size_t reserve_work(const ReserveArgs& a) {
   const Work w = work_of(a);
   // a sequence's new rows lie in at most tokens / page pages that begin past its length, rounded up
   const int64_t most = (int64_t)a.seqs * (((int64_t)a.tokens + (1 << a.page_shift) - 1) >> a.page_shift);
-  return (size_t)2 * a.seqs + w.segments + 1 + (size_t)std::min<int64_t>(most, a.num_pages);
+  return (size_t)a.seqs * (w.waves + 1) + w.segments + 1 + (size_t)std::min<int64_t>(most, a.num_pages);
 }
 
 void launch_reserve(const ReserveArgs& a, hipStream_t st) {
+  if (a.num_pages <= kOnePages && a.seqs <= kOneSeqs && (int64_t)a.seqs * a.width <= kOneEntries &&
+      (int64_t)a.seqs * span_of(a) <= kOneRows && (int64_t)a.seqs * a.tokens <= kOneSlots) {
+    hipLaunchKernelGGL(reserve_one_kernel, dim3(1), dim3(1024), 0, st, a, by_of(a.width), by_of(a.tokens));
+    return;
+  }
   const Work w = work_of(a);
-  const dim3 rows((unsigned)((a.seqs + 3) / 4));
+  const dim3 segments((unsigned)w.segments);
   if (a.refs != a.out_refs)
-    hipLaunchKernelGGL(reserve_copy_kernel, dim3((unsigned)std::min(1024, (a.num_pages + 255) / 256)), dim3(256), 0, st, a);
-  hipLaunchKernelGGL(reserve_rows_kernel, rows, dim3(256), 0, st, a);
-  hipLaunchKernelGGL(reserve_count_kernel, dim3((unsigned)w.segments), dim3(1024), 0, st, a);
-  hipLaunchKernelGGL(reserve_take_kernel, dim3((unsigned)w.segments), dim3(1024), 0, st, a);
-  hipLaunchKernelGGL(reserve_fill_kernel, rows, dim3(256), 0, st, a);
+    hipLaunchKernelGGL(reserve_copy_kernel, dim3((unsigned)std::min(1024, a.num_pages / 1024 + 1)), dim3(256), 0, st, a);
+  hipLaunchKernelGGL(reserve_rows_kernel, dim3((unsigned)((a.seqs * w.waves + 3) / 4)), dim3(256), 0, st, a);
+  hipLaunchKernelGGL(reserve_count_kernel, segments, dim3(1024), 0, st, a);
+  hipLaunchKernelGGL(reserve_take_kernel, segments, dim3(1024), 0, st, a);
+  hipLaunchKernelGGL(reserve_fill_kernel, dim3((unsigned)((a.seqs + 3) / 4)), dim3(256), 0, st, a);
 }
 
 }  // namespace tlm
