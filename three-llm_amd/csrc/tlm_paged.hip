@@ -8,16 +8,10 @@
 #include <algorithm>
 
 #include "tlm_device.h"
-#include "tlm_paged.h"
+#include "tlm_paged_rows.h"
 
 namespace tlm {
 namespace {
-
-typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // a row from any 4-byte address
-
-__device__ __forceinline__ void paged_flag(int* status, int bit) {
-  __hip_atomic_fetch_or(status, bit, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
 
 // The append: q' = R(p) q, k' = R(p) k (rotate-half over the first rd dims) and v,
 // k' and v rounded to the cache's type.  Three kernels.
@@ -57,29 +51,6 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedArgs a) {
     }
   }
 }
-
-// Eight consecutive dims of a row.
-struct Oct {
-  f32x4 a, b;
-  __device__ __forceinline__ void load(const float* x) {
-    a = *(const TLM_GLOBAL f32x4u*)(x);
-    b = *(const TLM_GLOBAL f32x4u*)(x + 4);
-  }
-  __device__ __forceinline__ void store(float* x) const {
-    *(TLM_GLOBAL f32x4u*)(x) = a;
-    *(TLM_GLOBAL f32x4u*)(x + 4) = b;
-  }
-};
-__device__ __forceinline__ f32x4 rotated(f32x4 x, f32x4 partner, f32x4 c, f32x4 s) { return x * c + partner * s; }
-
-// Octs of a head that a thread takes: the first `half / 8` with their partners half
-// dims further on, and those past the rotary dims alone.
-struct Octs {
-  int n, half, rd;
-  __device__ __forceinline__ Octs(int D, int rotary) : n((D - rotary) / 8 + rotary / 16), half(rotary / 2), rd(rotary) {}
-  __device__ __forceinline__ bool pair(int o) const { return 8 * o < half; }
-  __device__ __forceinline__ int dim(int o) const { return pair(o) ? 8 * o : rd + 8 * o - half; }
-};
 
 // Dims d .. d + 7 of a token's K: one 16-byte piece of fp16, two of fp32.
 template <typename KT>
@@ -200,25 +171,7 @@ __global__ __launch_bounds__(256) void paged_append_group_kernel(PagedArgs a, in
   const size_t at = paged_head_at(max(page, 0), hk, a.Hkv, a.page_shift, D);
   const size_t row0 = (size_t)s * a.tokens - start;  // + position: the row
   if (item < n.q) {
-    const int quads = n.q / 32, f = item % quads, pos = p0 + item / quads, d = 4 * f < half ? 4 * f : 4 * f + half;
-    if (pos < start || pos > last) return;
-    const bool pair = d < half;
-    const float* x = a.x + (row0 + pos) * N + (size_t)hk * a.G * D + d;
-    float* q = a.q + ((row0 + pos) * a.Hq + hk * a.G) * D + d;
-    f32x4 c = {1.f, 1.f, 1.f, 1.f}, w = {0.f, 0.f, 0.f, 0.f};
-    if (pair) {
-      c = *(const TLM_GLOBAL f32x4*)(a.rope_cos + (size_t)pos * half + d);
-      w = *(const TLM_GLOBAL f32x4*)(a.rope_sin + (size_t)pos * half + d);
-    }
-    const int to = pair ? half : 0;
-    f32x4 lo = *(const TLM_GLOBAL f32x4u*)(x), hi = *(const TLM_GLOBAL f32x4u*)(x + to);
-    for (int g = 0; g < a.G; g++) {
-      const float* y = x + (size_t)min(g + 1, a.G - 1) * D;  // the next head's, in flight meanwhile
-      const f32x4 nlo = *(const TLM_GLOBAL f32x4u*)(y), nhi = *(const TLM_GLOBAL f32x4u*)(y + to);
-      *(TLM_GLOBAL f32x4u*)(q + g * D) = pair ? rotated(lo, -hi, c, w) : lo;
-      if (pair) *(TLM_GLOBAL f32x4u*)(q + g * D + half) = rotated(hi, lo, c, w);
-      lo = nlo, hi = nhi;
-    }
+    append_quad(a, hk, p0, start, last, row0, item, n.q / 32);
     return;
   }
   if (page < 0) return;

@@ -4,19 +4,12 @@
 
 #include <algorithm>
 
-#include "tlm_device.h"
-#include "tlm_paged.h"
+#include "tlm_paged_rows.h"
 
 namespace tlm {
 namespace {
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
-typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // a row from any 4-byte address
-
-__device__ __forceinline__ void flag(int* status, int bit) {
-  __hip_atomic_fetch_or(status, bit, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-
 // The magnitude of a value as far as it counts for its block's scale: values that are
 // not finite become NaN codes and leave the others' precision alone.
 __device__ __forceinline__ float magnitude(float v) { return fabsf(v) < INFINITY ? fabsf(v) : 0.f; }
@@ -29,6 +22,10 @@ __device__ __forceinline__ float coded(float v, int e) {
 }
 __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false), true);
+}
+__device__ __forceinline__ u32x2 codes8(const Oct& x, int e) {
+  return (u32x2){codes4(coded(x.a[0], e), coded(x.a[1], e), coded(x.a[2], e), coded(x.a[3], e)),
+                 codes4(coded(x.b[0], e), coded(x.b[1], e), coded(x.b[2], e), coded(x.b[3], e))};
 }
 // Four codes under a scale 2^by times theirs (by >= 0): exact but for what falls below
 // 2^-6 of the code's range.
@@ -70,44 +67,158 @@ __device__ __forceinline__ void rotated_oct(const float* x, const float* cs, con
   }
 }
 
-// Per sequence, kv head and aligned block of 32 positions: q' = R(p) q of the head's
-// group; k' = R(p) k and v as codes under the block's scale, the larger of what its
-// new rows need and, where it has rows before them, of its old one.  Rows before them
-// are then coded again.  A block of threads has K and V in registers between the
-// maximum and the codes (slice 0); queries are further blocks' (slices 1 ..).
+// The rows of a sequence that lie in one aligned block of 32 positions.
+struct Rows {
+  int p0, from, n, held;  // the block, its first new position, how many, those before them in the block
+};
+__device__ __forceinline__ Rows rows_of(const PagedArgs& a, int s, int g, int start, int count, bool* bad) {
+  const int rows = paged_rows(start, count, a.tokens, a.limit, bad);
+  Rows r;
+  r.p0 = ((start >> 5) + g) << 5;
+  r.from = max(start, r.p0);
+  r.n = rows < 1 ? 0 : max(0, min(start + rows, r.p0 + 32) - r.from);
+  r.held = r.from - r.p0;
+  return r;
+}
+
+// q' = R(p) q of the block's new rows, items `first`, `first` + `step`, ... of n * Hq * D / 8.
 template <bool WHOLE>
+__device__ __forceinline__ void append8_queries(const PagedArgs& a, size_t row, const Rows& r, int heads, int h0,
+                                                int first, int step) {
+  const int D = a.D, octs = D / 8, half = a.rd / 2, N = (a.Hq + 2 * a.Hkv) * D, items = r.n * heads * octs;
+  for (int i = first; i < items; i += step) {
+    const int o = i % octs, h = h0 + i / octs % heads, j = i / octs / heads;
+    float y[8];
+    rotated_oct<WHOLE>(a.x + (row + j) * N + h * D, a.rope_cos + (size_t)(r.from + j) * half,
+                       a.rope_sin + (size_t)(r.from + j) * half, 8 * o, a.rd, y);
+    float* q = a.q + ((row + j) * a.Hq + h) * D + 8 * o;
+    *(TLM_GLOBAL f32x4u*)(q) = (f32x4){y[0], y[1], y[2], y[3]};
+    *(TLM_GLOBAL f32x4u*)(q + 4) = (f32x4){y[4], y[5], y[6], y[7]};
+  }
+}
+
+// Two kernels.  Both: k' = R(p) k and v as codes under the scale of the block of 32
+// positions, the larger of what its new rows need and, where it has rows before them,
+// of its old one; those rows are then coded again.
+//
+// Few rows: 16 lanes per kv head and K or V, a lane per eight dims, which goes over the
+// rows twice (for the maximum, then from the caches for the codes); the queries are
+// further blocks' (slices 1 ..).  Latency: a load of the start, the table and the old
+// scales, then the stores.
+template <bool WHOLE>
+__global__ __launch_bounds__(256) void paged_append8_few_kernel(PagedArgs a, int groups, int slices) {
+  const int slice = blockIdx.x % slices, block = blockIdx.x / slices, g = block % groups, s = block / groups;
+  const int tid = threadIdx.x, D = a.D, octs = D / 8, half = a.rd / 2, N = (a.Hq + 2 * a.Hkv) * D;
+  const int start = a.starts[s];
+  bool bad;
+  const Rows r = rows_of(a, s, g, start, a.counts ? a.counts[s] : a.tokens, &bad);
+  if (bad && g == 0 && slice == 0 && tid == 0) paged_flag(a.status, kPagedStatusRows);
+  if (r.n == 0) return;
+  const size_t row = (size_t)s * a.tokens + r.from - start;
+  if (slice > 0) {
+    append8_queries<WHOLE>(a, row, r, a.Hq, 0, (slice - 1) * 256 + tid, (slices - 1) * 256);
+    return;
+  }
+  const int page = paged_page(a.tables + (size_t)s * a.width, r.p0, a.page_shift, a.num_pages);
+  if (page < 0) {
+    if (tid == 0) paged_flag(a.status, kPagedStatusPage);
+    return;
+  }
+  const int tok0 = r.p0 & ((1 << a.page_shift) - 1), o = tid & 15, d = 8 * o;
+  const float* const cs = a.rope_cos + (size_t)r.from * half;
+  const float* const sn = a.rope_sin + (size_t)r.from * half;
+  for (int u = tid >> 4; u < 2 * a.Hkv; u += 16) {
+    const bool is_v = u >= a.Hkv, here = o < octs;
+    const int hk = is_v ? u - a.Hkv : u;
+    uint8_t* const p = static_cast<uint8_t*>(is_v ? a.vc : a.kc) + (size_t)page * a.page_bytes;
+    uint8_t* const head = p + (size_t)hk * ((size_t)D << a.page_shift);
+    uint32_t* const scale = reinterpret_cast<uint32_t*>(p + paged8_scale_at(hk, a.Hkv, tok0, a.page_shift, D));
+    const uint32_t old = r.held ? *scale : 0;
+    const float* const x = a.x + row * N + (a.Hq + u) * D;
+    auto oct = [&](int j, float* y) {
+      if (!is_v) {
+        rotated_oct<WHOLE>(x + (size_t)j * N, cs + j * half, sn + j * half, d, a.rd, y);
+      } else {
+        const f32x4 b = *(const TLM_GLOBAL f32x4u*)(x + (size_t)j * N + d);
+        const f32x4 c = *(const TLM_GLOBAL f32x4u*)(x + (size_t)j * N + d + 4);
+#pragma unroll
+        for (int e = 0; e < 4; e++) y[e] = b[e], y[4 + e] = c[e];
+      }
+    };
+    float y[8] = {}, top = 0.f;
+    for (int j = r.n - 1; j >= 0; j--) {  // the first row last: it stays in y
+      if (here) oct(j, y);
+#pragma unroll
+      for (int e = 0; e < 8; e++) top = fmaxf(top, magnitude(y[e]));
+    }
+    top = fmaxf(top, dpp<kDppXor1>(top));
+    top = fmaxf(top, dpp<kDppXor2>(top));
+    top = fmaxf(top, dpp<kDppHalfMirror>(top));
+    top = fmaxf(top, dpp<kDppMirror>(top));
+    if (!here) continue;
+    int ex = paged8_exponent(__float_as_uint(top)), by = 0;
+    if (r.held) {
+      const int was = paged8_exponent_of(old);
+      ex = max(ex, was), by = ex - was;
+    }
+    if (o == 0) *scale = (uint32_t)(ex + 127) << 23;  // its lanes have read the old one
+    if (by && !is_v)
+      for (int t = 0; t < r.held; t++) {
+        TLM_GLOBAL u32x2* c = (TLM_GLOBAL u32x2*)(head + paged8_k_at(tok0 + t, d, D));
+        const u32x2 v = *c;
+        *c = (u32x2){recoded(v[0], by), recoded(v[1], by)};
+      }
+    if (by && is_v)
+      for (int t = 0; t < min(r.held, 16); t += 4)  // tokens t .. t + 3 and 16 further on
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          TLM_GLOBAL u32x2* c = (TLM_GLOBAL u32x2*)(head + paged8_v_at(tok0 + t, d + e, D));
+          const u32x2 v = *c;
+          *c = (u32x2){recoded(v[0], by), recoded(v[1], by)};
+        }
+    for (int j = 0; j < r.n; j++) {
+      if (j) oct(j, y);
+      u32x2 c;
+#pragma unroll
+      for (int e = 0; e < 2; e++)
+        c[e] = codes4(coded(y[4 * e], ex), coded(y[4 * e + 1], ex), coded(y[4 * e + 2], ex), coded(y[4 * e + 3], ex));
+      const int t = tok0 + r.held + j;
+      if (!is_v) {
+        *(TLM_GLOBAL u32x2*)(head + paged8_k_at(t, d, D)) = c;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) head[paged8_v_at(t, d + e, D)] = (uint8_t)(c[e >> 2] >> 8 * (e & 3));
+      }
+    }
+  }
+}
+
+// Many rows: a block of threads per kv head, which has K and V in registers between the
+// maximum and the codes (slice 0); the queries of the head's group are further blocks'.
+// Half the rotary dims are a multiple of 8 here.
 __global__ __launch_bounds__(256) void paged_append8_kernel(PagedArgs a, int groups, int slices) {
   __shared__ float top[2][4];
   const int slice = blockIdx.x % slices, block = blockIdx.x / slices, hk = block % a.Hkv;
   const int g = block / a.Hkv % groups, s = block / a.Hkv / groups, tid = threadIdx.x;
   const int start = a.starts[s];
   bool bad;
-  const int rows = paged_rows(start, a.counts ? a.counts[s] : a.tokens, a.tokens, a.limit, &bad);
-  if (bad && g == 0 && hk == 0 && slice == 0 && tid == 0) flag(a.status, kPagedStatusRows);
-  if (rows < 1) return;
-  const int p0 = ((start >> 5) + g) << 5, end = min(start + rows, p0 + 32);  // positions from max(start, p0) on
-  if (p0 >= end) return;
-  const int from = max(start, p0), n = end - from, D = a.D, octs = D / 8, half = a.rd / 2;
+  const Rows r = rows_of(a, s, g, start, a.counts ? a.counts[s] : a.tokens, &bad);
+  if (bad && g == 0 && hk == 0 && slice == 0 && tid == 0) paged_flag(a.status, kPagedStatusRows);
+  if (r.n == 0) return;
+  const int p0 = r.p0, from = r.from, n = r.n, held = r.held, D = a.D, octs = D / 8, half = a.rd / 2;
   const int N = (a.Hq + 2 * a.Hkv) * D;
-  const size_t row0 = (size_t)s * a.tokens - start;  // + position: the row
+  const size_t row = (size_t)s * a.tokens + from - start;
   const float* const cs = a.rope_cos + (size_t)from * half;
   const float* const sn = a.rope_sin + (size_t)from * half;
-  const float* const x0 = a.x + (row0 + from) * N;
+  const float* const x0 = a.x + row * N;
   if (slice > 0) {
-    const int items = n * a.G * octs;
-    for (int i = (slice - 1) * 256 + tid; i < items; i += (slices - 1) * 256) {
-      const int o = i % octs, h = i / octs % a.G, j = i / octs / a.G;
-      float y[8];
-      rotated_oct<WHOLE>(x0 + (size_t)j * N + (hk * a.G + h) * D, cs + j * half, sn + j * half, 8 * o, a.rd, y);
-      float* q = a.q + ((row0 + from + j) * a.Hq + hk * a.G + h) * D + 8 * o;
-      *(TLM_GLOBAL f32x4u*)(q) = (f32x4){y[0], y[1], y[2], y[3]};
-      *(TLM_GLOBAL f32x4u*)(q + 4) = (f32x4){y[4], y[5], y[6], y[7]};
-    }
+    const int quads = D / 4 - a.rd / 8, item = (slice - 1) * 256 + tid;
+    if (item < 32 * quads) append_quad(a, hk, p0, start, from + n - 1, row - from, item, quads);
     return;
   }
   const int page = paged_page(a.tables + (size_t)s * a.width, p0, a.page_shift, a.num_pages);
   if (page < 0) {
-    if (tid == 0) flag(a.status, kPagedStatusPage);
+    if (tid == 0) paged_flag(a.status, kPagedStatusPage);
     return;
   }
   const int tok0 = p0 & ((1 << a.page_shift) - 1);
@@ -117,19 +228,33 @@ __global__ __launch_bounds__(256) void paged_append8_kernel(PagedArgs a, int gro
   const size_t scale_at = paged8_scale_at(hk, a.Hkv, tok0, a.page_shift, D);
   uint32_t* const ks = reinterpret_cast<uint32_t*>(kp + scale_at);
   uint32_t* const vs = reinterpret_cast<uint32_t*>(vp + scale_at);
-  const int held = from - p0;  // tokens of the block that it has already
   const uint32_t kold = held ? *ks : 0, vold = held ? *vs : 0;
-  // at most 32 * 16 octs of K, and 4 * 128 dims of eight tokens of V (4 q .. of each sixteen)
+  // at most 32 * 16 octs of K (with their partners 32 * 8), and 4 * 128 dims of eight
+  // tokens of V (4 q .. of each sixteen)
   constexpr int NI = 2;
-  float k[NI][8], v[NI][8];
+  const Octs oc(D, a.rd);
+  Oct k[NI][2];
+  float v[NI][8];
   float kt = 0.f, vt = 0.f;
 #pragma unroll
   for (int m = 0; m < NI; m++) {
-    const int i = tid + 256 * m, o = i % octs, j = i / octs;
+    const int i = tid + 256 * m, o = i % oc.n, j = i / oc.n, d = oc.dim(o);
     if (j >= n) continue;
-    rotated_oct<WHOLE>(x0 + (size_t)j * N + (a.Hq + hk) * D, cs + j * half, sn + j * half, 8 * o, a.rd, k[m]);
+    const float* x = x0 + (size_t)j * N + (a.Hq + hk) * D + d;
+    k[m][0].load(x);
+    if (oc.pair(o)) {
+      Oct c, w;
+      k[m][1].load(x + half);
+      c.load(cs + (size_t)j * half + d);
+      w.load(sn + (size_t)j * half + d);
+      const Oct y = k[m][0];
+      k[m][0].a = rotated(y.a, -k[m][1].a, c.a, w.a), k[m][0].b = rotated(y.b, -k[m][1].b, c.b, w.b);
+      k[m][1].a = rotated(k[m][1].a, y.a, c.a, w.a), k[m][1].b = rotated(k[m][1].b, y.b, c.b, w.b);
 #pragma unroll
-    for (int e = 0; e < 8; e++) kt = fmaxf(kt, magnitude(k[m][e]));
+      for (int e = 0; e < 4; e++) kt = fmaxf(kt, fmaxf(magnitude(k[m][1].a[e]), magnitude(k[m][1].b[e])));
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) kt = fmaxf(kt, fmaxf(magnitude(k[m][0].a[e]), magnitude(k[m][0].b[e])));
   }
 #pragma unroll
   for (int m = 0; m < NI; m++) {
@@ -141,11 +266,8 @@ __global__ __launch_bounds__(256) void paged_append8_kernel(PagedArgs a, int gro
       vt = fmaxf(vt, magnitude(v[m][e]));
     }
   }
-#pragma unroll
-  for (int w = 1; w < 64; w <<= 1) {
-    kt = fmaxf(kt, __shfl_xor(kt, w));
-    vt = fmaxf(vt, __shfl_xor(vt, w));
-  }
+  kt = wave_max(kt);
+  vt = wave_max(vt);
   if ((tid & 63) == 0) top[0][tid >> 6] = kt, top[1][tid >> 6] = vt;
   __syncthreads();  // also: the old scales have been read
   kt = fmaxf(fmaxf(top[0][0], top[0][1]), fmaxf(top[0][2], top[0][3]));
@@ -162,14 +284,10 @@ __global__ __launch_bounds__(256) void paged_append8_kernel(PagedArgs a, int gro
   }
 #pragma unroll
   for (int m = 0; m < NI; m++) {
-    const int i = tid + 256 * m, o = i % octs, j = i / octs;
+    const int i = tid + 256 * m, o = i % oc.n, j = i / oc.n, d = oc.dim(o);
     if (j >= n) continue;
-    u32x2 c;
-#pragma unroll
-    for (int e = 0; e < 2; e++)
-      c[e] = codes4(coded(k[m][4 * e], ke), coded(k[m][4 * e + 1], ke), coded(k[m][4 * e + 2], ke),
-                    coded(k[m][4 * e + 3], ke));
-    *(TLM_GLOBAL u32x2*)(kp + head + paged8_k_at(tok0 + held + j, 8 * o, D)) = c;
+    *(TLM_GLOBAL u32x2*)(kp + head + paged8_k_at(tok0 + held + j, d, D)) = codes8(k[m][0], ke);
+    if (oc.pair(o)) *(TLM_GLOBAL u32x2*)(kp + head + paged8_k_at(tok0 + held + j, d + half, D)) = codes8(k[m][1], ke);
   }
   for (int i = tid; kby && i < held * octs; i += 256) {
     TLM_GLOBAL u32x2* p = (TLM_GLOBAL u32x2*)(kp + head + paged8_k_at(tok0 + i / octs, 8 * (i % octs), D));
@@ -207,13 +325,19 @@ __global__ __launch_bounds__(256) void paged_append8_kernel(PagedArgs a, int gro
 
 void launch_paged_append8(const PagedArgs& a, hipStream_t st) {
   const int groups = (a.tokens + 30) / 32 + 1;  // aligned blocks that `tokens` positions may touch
-  const int items = std::min(a.tokens, 32) * a.G * (a.D / 8);
-  const int slices = 1 + (a.q ? (items + 255) / 256 : 0);
-  const dim3 grid((unsigned)((int64_t)a.seqs * groups * a.Hkv * slices)), block(256);
-  if (a.rd % 16)
-    hipLaunchKernelGGL(paged_append8_kernel<false>, grid, block, 0, st, a, groups, slices);
-  else
-    hipLaunchKernelGGL(paged_append8_kernel<true>, grid, block, 0, st, a, groups, slices);
+  const dim3 block(256);
+  if (a.tokens < 12 || a.rd % 16) {
+    const int slices = 1 + (a.q ? (std::min(a.tokens, 32) * a.Hq * (a.D / 8) + 255) / 256 : 0);
+    const dim3 grid((unsigned)((int64_t)a.seqs * groups * slices));
+    if (a.rd % 16)
+      hipLaunchKernelGGL(paged_append8_few_kernel<false>, grid, block, 0, st, a, groups, slices);
+    else
+      hipLaunchKernelGGL(paged_append8_few_kernel<true>, grid, block, 0, st, a, groups, slices);
+    return;
+  }
+  const int slices = 1 + (a.q ? (32 * (a.D / 4 - a.rd / 8) + 255) / 256 : 0);
+  hipLaunchKernelGGL(paged_append8_kernel, dim3((unsigned)((int64_t)a.seqs * groups * a.Hkv * slices)), block, 0, st, a,
+                     groups, slices);
 }
 
 }  // namespace tlm
