@@ -614,6 +614,8 @@ def _bind(s):
         return
     s["batch"] = s["paged"].batch(d["k"], d["v"], s["k"].shape[0], d["tables"], s["tables"].shape[1], d["starts"],
                                   s["seqs"], s["tokens"], counts=d["counts"])
+    if s["op"] == "append":
+        s["views"] = _appended(s)  # of its own buffers
 
 
 def _own(s):
@@ -626,7 +628,7 @@ def _own(s):
         return _reserved(s)
     if s["op"] == "append":
         s["paged"].append(s["batch"], d["x"], d["y"])
-        return _appended(s)
+        return s["views"]
     if s["op"] == "attention":
         s["paged"].attention(s["batch"], d["x"], d["y"], {"f16": tlm.FMT_F16, "f32": tlm.FMT_F32}[s["out"]])
         return s["y"]
