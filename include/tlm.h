@@ -241,7 +241,7 @@ typedef struct tlm_paged_request {
   int64_t* slots;           /* [seqs][tokens] or NULL */
   int32_t num_pages, table_width, seqs, tokens;
 } tlm_paged_request;
-/* seqs * tokens * heads is at most 2^22, seqs 2^20.  The results are apart from each
+/* seqs * tokens * heads is at most 2^22, seqs 2^20, num_pages 2^30, table_width 2^26.  The results are apart from each
  * other and from the inputs, but for tables and refs in place.  Enqueue only. */
 int tlm_op_paged_reserve(tlm_paged* paged, const tlm_paged_request* request);
 /* qkv: fp32 [seqs][tokens][(heads + 2 kv_heads) * head_dim] (Q|K|V, bias
@@ -253,7 +253,8 @@ int tlm_op_paged_reserve(tlm_paged* paged, const tlm_paged_request* request);
  * head, 2^e from 2^-32 to 2^31, the least that takes the largest magnitude to at
  * most 448.  Rows that start within 32 positions keep the scale that these have or, if
  * they need it, raise it; the positions before them are then rounded again (exact but
- * for magnitudes below 2^-14 of the largest).  Positions behind the appended rows, to
+ * for magnitudes below 2^-14 of the largest).  Of rows that start within 32 positions
+ * the earlier ones have been appended (or their page is all zeros).  Positions behind the appended rows, to
  * the end of their 32, are lost; 32 positions that two sequences append to in one
  * call are lost.  Values that are not finite become NaN. */
 int tlm_op_paged_append(tlm_paged* paged, const tlm_paged_batch* batch, const float* qkv, float* q);
@@ -319,7 +320,8 @@ typedef struct tlm_logit_rules {
   const uint32_t* masks;         /* [seqs][tokens][(vocab + 31) / 32] (NULL: nothing is masked) */
   int32_t seqs, tokens, vocab, history_width, bias_width;
 } tlm_logit_rules;
-/* tokens <= 64, vocab <= 524288, seqs * tokens <= 2^20, bias_width <= 4096.
+/* tokens <= 64, vocab <= 524288, seqs * tokens <= 2^20, bias_width <= 4096;
+ * seqs * tokens * vocab, vocab rounded up to a multiple of 4096, below 2^35.
  * Enqueue only. */
 int tlm_op_adjust_logits(tlm_ctx* ctx, const tlm_logit_rules* rules);
 /* Verification of drafted tokens, for many sequences at once: which of a

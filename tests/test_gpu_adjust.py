@@ -176,7 +176,8 @@ def test_refused(ctx):
     ctx.sync()
     at = lambda b, by: b.ptr.value + by  # noqa: E731
     for kw, code in ((dict(seqs=0), -1), (dict(tokens=0), -1), (dict(vocab=0), -1), (dict(tokens=65), -1),
-                     (dict(vocab=524289), -1), (dict(seqs=1 << 20), -5), (dict(history_width=5), -1),
+                     (dict(vocab=524289), -1), (dict(seqs=1 << 20), -5),
+                     (dict(seqs=1 << 17, tokens=1, vocab=1 << 18), -5), (dict(history_width=5), -1),
                      (dict(history_width=-1), -1), (dict(bias_width=2), -1), (dict(bias_width=-1), -1),
                      (dict(bias_width=4097, bias_ids=ints.ptr, biases=ints.ptr), -1),
                      (dict(logits=at(y, 4)), -1), (dict(masks=at(y, 0)), -1), (dict(counts=at(y, 2396)), -1),

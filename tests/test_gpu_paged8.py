@@ -548,3 +548,13 @@ def test_results_over_the_scales_are_refused(ctx):
             call()
         assert e.value.code == tlm.TLM_ERR_INVALID and "overlap" in str(e.value)
     p.close()
+
+
+def test_other_caches_are_not_of_8_bits(ctx):
+    with pytest.raises(tlm.TlmError) as e:
+        tlm.Attention(ctx, 4, 2, 64, 100, inv_freq=np.ones(32, np.float32), kv_fmt=F8)
+    assert e.value.code == tlm.TLM_ERR_INVALID and "paged" in str(e.value)
+    d = tlm.ModelDesc(256, 512, 1, 4, 2, 64, 1000, 64, 64, 0, tlm.FMT_F16, tlm.FMT_F16, tlm.FMT_F16, F8)
+    with pytest.raises(tlm.TlmError) as e:
+        tlm.Model(ctx, d, np.ones(32, np.float32))
+    assert e.value.code == tlm.TLM_ERR_INVALID and "paged" in str(e.value)

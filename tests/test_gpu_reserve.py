@@ -153,29 +153,27 @@ def test_refused(ctx):
         x.ctx, x.nbytes, x.ptr = ctx, 1 << 20, type(b.ptr)(b.ptr.value + by)
         return x
 
+    wide = at(t, 0)  # a table as large as the counts: still not one for the other
     for change, code in ((dict(num_pages=0), tlm.TLM_ERR_INVALID), (dict(table_width=0), tlm.TLM_ERR_INVALID),
                          (dict(seqs=0), tlm.TLM_ERR_INVALID), (dict(tokens=0), tlm.TLM_ERR_INVALID),
                          (dict(out_tables=at(t, 4)), tlm.TLM_ERR_INVALID), (dict(out_refs=at(r, 4)), tlm.TLM_ERR_INVALID),
-                         (dict(out_tables=r), tlm.TLM_ERR_INVALID), (dict(starts=l), tlm.TLM_ERR_INVALID),
+                         (dict(out_tables=at(r, 0)), tlm.TLM_ERR_INVALID), (dict(starts=at(l, 0)), tlm.TLM_ERR_INVALID),
+                         (dict(out_refs=at(t, 0)), tlm.TLM_ERR_INVALID),
+                         (dict(refs=wide, num_pages=16, out_refs=at(r, 0)), tlm.TLM_ERR_INVALID),
+                         (dict(refs=at(r, 0), num_pages=16, out_tables=at(r, 0)), tlm.TLM_ERR_INVALID),
                          (dict(starts=at(t, 60)), tlm.TLM_ERR_INVALID), (dict(starts=at(r, 32)), tlm.TLM_ERR_INVALID),
-                         (dict(slots=at(slots, 4)), tlm.TLM_ERR_INVALID), (dict(out_refs=at(t, 0)), tlm.TLM_ERR_INVALID)):
-        kw = {**ok, **change}
-        for name in ("out_tables", "out_refs", "slots", "starts"):
-            if name in change:
-                change[name].nbytes = 1 << 20
-        if "out_tables" in change and change["out_tables"] is r:
-            t2 = ctx.buffer(64)
+                         (dict(slots=at(slots, 4)), tlm.TLM_ERR_INVALID), (dict(slots=at(t, 0)), tlm.TLM_ERR_INVALID)):
         with pytest.raises(tlm.TlmError) as e:
-            p.reserve(p.request(**kw))
+            p.reserve(p.request(**{**ok, **change}))
         assert e.value.code == code, change
-    big = dict(ok, lengths=at(l, 0), tables=at(t, 0), refs=at(r, 0), starts=at(s, 0))
+    big = {k: at(ok[k], 0) for k in ("lengths", "tables", "refs", "starts")}
     for b in big.values():
-        if isinstance(b, tlm.Buffer):
-            b.nbytes = 1 << 40
-    for seqs, tokens in ((1 << 21, 2), ((1 << 20) + 1, 1)):
+        b.nbytes = 1 << 60
+    for kw in (dict(seqs=1 << 20, tokens=5), dict(seqs=(1 << 20) + 1, tokens=1), dict(num_pages=(1 << 30) + 1),
+               dict(table_width=(1 << 26) + 1)):
         with pytest.raises(tlm.TlmError) as e:
-            p.reserve(p.request(**{**big, "seqs": seqs, "tokens": 4 if tokens > 1 else 1, "out_tables": None}))
-        assert e.value.code == tlm.TLM_ERR_RANGE
+            p.reserve(p.request(**{**ok, **big, **kw}))
+        assert e.value.code == tlm.TLM_ERR_RANGE, kw
     p.close()
 
 

@@ -843,6 +843,7 @@ static int attn_init(tlm_ctx* ctx, const tlm_attn_desc* d, tlm_attn* A, bool own
     return fail(TLM_ERR_INVALID, "TLMAttention: invalid rotary dimension %d", d->rotary_dim);
   if (d->rotary_dim > 0 && !d->inv_freq) return fail(TLM_ERR_INVALID, "TLMAttention: missing inv_freq");
   if (d->max_tokens <= 0) return fail(TLM_ERR_INVALID, "TLMAttention: max_tokens must be positive");
+  if (d->kv_fmt == TLM_FMT_F8) return fail(TLM_ERR_INVALID, "TLMAttention: a cache of 8-bit values is a paged one");
   A->ctx = ctx;
   A->d = *d;
   A->G = d->heads / d->kv_heads;
@@ -1377,8 +1378,9 @@ int tlm_op_paged_reserve(tlm_paged* P, const tlm_paged_request* r) {
   if ((int64_t)r->seqs * r->tokens > (1 << 22) / P->d.heads)
     return fail(TLM_ERR_RANGE, "TLMPaged: %d sequences of %d rows of %d heads are more than 2^22", r->seqs, r->tokens,
                 P->d.heads);
-  if (r->seqs > kReserveMaxSeqs)
-    return fail(TLM_ERR_RANGE, "TLMPaged: %d sequences, at most %d reserve at once", r->seqs, kReserveMaxSeqs);
+  if (r->seqs > kReserveMaxSeqs || r->num_pages > kReserveMaxPages || r->table_width > kReserveMaxWidth)
+    return fail(TLM_ERR_RANGE, "TLMPaged: %d sequences, %d pages, tables of %d; at most %d, %d, %d reserve at once",
+                r->seqs, r->num_pages, r->table_width, kReserveMaxSeqs, kReserveMaxPages, kReserveMaxWidth);
   if (reinterpret_cast<uintptr_t>(r->slots) % 8) return fail(TLM_ERR_INVALID, "TLMPaged: the slots are not 8-byte aligned");
   ReserveArgs a;
   memset(&a, 0, sizeof a);
@@ -1411,9 +1413,8 @@ int tlm_op_paged_reserve(tlm_paged* P, const tlm_paged_request* r) {
   } in[] = {{r->lengths, seqs}, {r->counts, seqs}, {r->tables, cells}, {r->refs, (size_t)r->num_pages}},
     out[] = {{r->out_tables, cells}, {r->out_refs, (size_t)r->num_pages}, {r->starts, seqs}, {r->slots, slots}};
   for (int i = 0; i < 4; i++) {
-    for (const auto& x : in)
-      if (x.p && out[i].p && overlap(x.p, x.n, out[i].p, out[i].n) &&
-          !(x.p == out[i].p && (out[i].p == r->tables || out[i].p == r->refs) && x.n == out[i].n && i < 2))
+    for (int k = 0; k < 4; k++)
+      if (in[k].p && out[i].p && overlap(in[k].p, in[k].n, out[i].p, out[i].n) && !(k == i + 2 && in[k].p == out[i].p))
         return fail(TLM_ERR_INVALID, "TLMPaged: a result of the reservation overlaps an input");
     for (int k = 0; k < i; k++)
       if (out[i].p && overlap(out[i].p, out[i].n, out[k].p, out[k].n))
@@ -1422,7 +1423,6 @@ int tlm_op_paged_reserve(tlm_paged* P, const tlm_paged_request* r) {
   const DeviceScope on(P->ctx->device);
   std::lock_guard<std::mutex> lock(P->ctx->part_mu);
   a.work = reinterpret_cast<int32_t*>(P->ctx->part);
-  a.arrived = P->ctx->paged_arrived;
   launch_reserve(a, P->ctx->stream);
   CHECK_LAUNCH("TLMPaged");
   return TLM_OK;
@@ -1604,6 +1604,9 @@ int tlm_op_adjust_logits(tlm_ctx* ctx, const tlm_logit_rules* r) {
     return fail(TLM_ERR_INVALID, "TLMLogitRules: a vocabulary of %d, at most %d", r->vocab, kVerifyMaxVocab);
   if ((int64_t)r->seqs * r->tokens > (1 << 20))
     return fail(TLM_ERR_RANGE, "TLMLogitRules: %d sequences of %d rows are more than 2^20 rows", r->seqs, r->tokens);
+  if ((int64_t)r->seqs * r->tokens * ((r->vocab + 4095) / 4096) >= 1 << 23)
+    return fail(TLM_ERR_RANGE, "TLMLogitRules: %d sequences of %d rows of %d logits are more than 2^35", r->seqs, r->tokens,
+                r->vocab);
   if (r->bias_width > kAdjustMaxBiases)
     return fail(TLM_ERR_INVALID, "TLMLogitRules: %d biases, at most %d", r->bias_width, kAdjustMaxBiases);
   if (r->history_width > 0 && !r->history) return fail(TLM_ERR_INVALID, "TLMLogitRules: no history of %d", r->history_width);
@@ -1829,6 +1832,7 @@ int tlm_model_create(tlm_ctx* ctx, const tlm_model_desc* d, tlm_model** out) {
   if (d->hidden_size % 4 != 0)
     return fail(TLM_ERR_INVALID, "TLMModel: hidden_size %d must be a multiple of 4", d->hidden_size);
   if (d->sliding_window < 0) return fail(TLM_ERR_INVALID, "TLMModel: negative sliding window");
+  if (d->kv_fmt == TLM_FMT_F8) return fail(TLM_ERR_INVALID, "TLMModel: a cache of 8-bit values is a paged one");
   for (int l = 0; d->layer_windows && l < d->num_layers; l++)
     if (d->layer_windows[l] < 0) return fail(TLM_ERR_INVALID, "TLMModel: negative sliding window of layer %d", l);
   tlm_model* m = new tlm_model();

@@ -515,9 +515,8 @@ struct ReserveArgs {
   int* status;
   int num_pages, width, page_shift, seqs, tokens, limit, window, sinks;
   int32_t* work;           // reserve_work's ints
-  unsigned* arrived;       // one, zero between launches
 };
-constexpr int kReserveMaxSeqs = 1 << 20;
+constexpr int kReserveMaxSeqs = 1 << 20, kReserveMaxPages = 1 << 30, kReserveMaxWidth = 1 << 26;
 size_t reserve_work(const ReserveArgs& a);  // ints that a.work has to hold
 void launch_reserve(const ReserveArgs& a, hipStream_t st);
 

@@ -23,12 +23,13 @@ __host__ __device__ inline int waves_of(const ReserveArgs& a) {
   return n;
 }
 
-// a.work: want[seqs][waves] (pages that a sequence lacks), base[seqs] (those before it, or
-// -1: it gets none), the free pages of each segment (then: before each), the number
-// taken, and the pages taken in order.
+// a.work: want[seqs][waves] (pages that a sequence lacks), the free pages of each segment,
+// the free pages in order as far as they may be asked for; of many sequences or segments
+// (reserve_share_kernel) also all free pages and base[seqs] (what the sequences before one
+// lack, or -1: it gets none), and of each segment the free pages before it.
 struct Work {
-  int32_t *want, *base, *segment, *taken, *pages;
-  int segments, waves;
+  int32_t *want, *base, *segment, *free, *pages;
+  int segments, waves, most;  // most: pages that are asked for
 };
 __host__ __device__ inline Work work_of(const ReserveArgs& a) {
   Work w;
@@ -37,8 +38,11 @@ __host__ __device__ inline Work work_of(const ReserveArgs& a) {
   w.want = a.work;
   w.base = w.want + (size_t)a.seqs * w.waves;
   w.segment = w.base + a.seqs;
-  w.taken = w.segment + w.segments;
-  w.pages = w.taken + 1;
+  w.free = w.segment + w.segments;
+  w.pages = w.free + 1;
+  // a sequence's new rows lie in at most tokens / page pages that begin past its length, rounded up
+  const int64_t most = (int64_t)a.seqs * (((int64_t)a.tokens + (1 << a.page_shift) - 1) >> a.page_shift);
+  w.most = (int)(most < a.num_pages ? most : a.num_pages);
   return w;
 }
 
@@ -161,96 +165,80 @@ __device__ __forceinline__ int64_t scan1024(int v, Scan& sc, int64_t* all) {
   return before;
 }
 
-// The free pages of each segment, a block each; the last block turns the sums into
-// running ones and shares the pages out.
+// The free pages of each segment, a block each.
 __global__ __launch_bounds__(1024) void reserve_count_kernel(ReserveArgs a) {
-  __shared__ Scan sc;
-  __shared__ int last;
-  const Work w = work_of(a);
-  const int tid = threadIdx.x, lane = tid & 63;
+  __shared__ int sh[16];
+  const int tid = threadIdx.x;
   const int64_t i0 = (int64_t)blockIdx.x * kSegment;
-  const int n = (int)min((int64_t)kSegment, a.num_pages - i0);
-  const i32x4u v = four(a.out_refs + i0, 4 * tid, n, 1);
-  // what a sequence lacks in all; the first 1024 sequences' is on its way meanwhile
-  auto want_of = [&](int s) {
-    int x[16], want = 0, lost = 0;
-#pragma unroll
-    for (int k = 0; k < 16; k++) x[k] = k < w.waves ? w.want[(size_t)s * w.waves + k] : 0;
-#pragma unroll
-    for (int k = 0; k < 16; k++) want += x[k] & ~kLost, lost |= x[k] & kLost;
-    return lost ? kLost : want;
-  };
-  const int first = tid < a.seqs ? want_of(tid) : kLost;
-  int64_t all;
-  scan1024((v[0] == 0) + (v[1] == 0) + (v[2] == 0) + (v[3] == 0), sc, &all);
-  if (tid == 0) {
-    __hip_atomic_store(w.segment + blockIdx.x, (int)all, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // it is performed
-    last = __hip_atomic_fetch_add(a.arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
-  }
+  const i32x4u v = four(a.out_refs + i0, 4 * tid, (int)min((int64_t)kSegment, a.num_pages - i0), 1);
+  const int free = sum64((v[0] == 0) + (v[1] == 0) + (v[2] == 0) + (v[3] == 0));
+  if ((tid & 63) == 0) sh[tid >> 6] = free;
   __syncthreads();
-  if (!last) return;
-  if (tid == 0) __hip_atomic_store(a.arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  // what other blocks stored: past this CU's cache
-  auto left_at = [](const int32_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
-  int64_t free = 0;
+  int all = 0;
+  for (int i = 0; i < 16; i++) all += sh[i];
+  if (tid == 0) work_of(a).segment[blockIdx.x] = all;
+}
+
+// What sequence s lacks in all (kLost: positions).
+__device__ __forceinline__ int want_of(const Work& w, int s) {
+  int x[16], want = 0, lost = 0;
+#pragma unroll
+  for (int k = 0; k < 16; k++) x[k] = k < w.waves ? w.want[(size_t)s * w.waves + k] : 0;
+#pragma unroll
+  for (int k = 0; k < 16; k++) want += x[k] & ~kLost, lost |= x[k] & kLost;
+  return lost ? kLost : want;
+}
+// Where its pages begin among the free ones, or -1: none are left for it.
+__device__ __forceinline__ int base_of(int want, int64_t before, int64_t free) {
+  return want != kLost && (want == 0 || before + want <= free) ? (int)before : -1;
+}
+
+// Running sums over many sequences or segments, by one block; up to 1024 of each the
+// kernels below work them out for themselves.
+constexpr int kInPlace = 1024;
+__global__ __launch_bounds__(1024) void reserve_share_kernel(ReserveArgs a) {
+  __shared__ Scan sc;
+  const Work w = work_of(a);
+  const int tid = threadIdx.x;
+  int64_t free = 0, asked = 0, all;
   for (int b = 0; b < w.segments; b += 1024) {
-    const int64_t before = scan1024(b + tid < w.segments ? left_at(w.segment + b + tid) : 0, sc, &all) + free;
+    const int64_t before = scan1024(b + tid < w.segments ? w.segment[b + tid] : 0, sc, &all) + free;
     if (b + tid < w.segments) w.segment[b + tid] = (int)before;
     free += all;
   }
-  int64_t asked = 0;
-  int taken = 0;
   for (int s0 = 0; s0 < a.seqs; s0 += 1024) {
-    const int s = s0 + tid;
-    const int want = s0 == 0 ? first : s < a.seqs ? want_of(s) : kLost;
-    const bool lost = want == kLost;
-    const int64_t before = scan1024(lost ? 0 : want, sc, &all) + asked;
-    const bool gets = !lost && (want == 0 || before + want <= free);
-    if (s < a.seqs) w.base[s] = gets ? (int)before : -1;
-    if (gets && want) taken = max(taken, (int)before + want);
+    const int s = s0 + tid, want = s < a.seqs ? want_of(w, s) : kLost;
+    const int64_t before = scan1024(want == kLost ? 0 : want, sc, &all) + asked;
+    if (s < a.seqs) w.base[s] = base_of(want, before, free);
     asked += all;
   }
-  // the sequences that get some are the first that ask: the largest end is the number
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) taken = max(taken, __shfl_xor(taken, d));
-  __syncthreads();
-  if (lane == 0) sc.sh[tid >> 6] = taken;
-  __syncthreads();
-  if (tid == 0) {
-    for (int i = 0; i < 16; i++) taken = max(taken, sc.sh[i]);
-    *w.taken = taken;
-  }
+  if (tid == 0) *w.free = (int)free;
 }
 
-// The free pages in order, those taken: a block a segment.
-__global__ __launch_bounds__(1024) void reserve_take_kernel(ReserveArgs a) {
+// The free pages in order, a block a segment.
+template <bool SHARED>
+__global__ __launch_bounds__(1024) void reserve_list_kernel(ReserveArgs a) {
   __shared__ Scan sc;
   const Work w = work_of(a);
+  const int tid = threadIdx.x;
   const int64_t i0 = (int64_t)blockIdx.x * kSegment;
-  const int n = (int)min((int64_t)kSegment, a.num_pages - i0);
-  i32x4u v = four(a.out_refs + i0, 4 * threadIdx.x, n, 1);
-  const int taken = *w.taken;
-  int64_t before = w.segment[blockIdx.x], all;
-  if (before >= taken) return;
-  const int free = (v[0] == 0) + (v[1] == 0) + (v[2] == 0) + (v[3] == 0);
-  int64_t rank = scan1024(free, sc, &all) + before;
-  if (!free || rank >= taken) return;
+  const i32x4u v = four(a.out_refs + i0, 4 * tid, (int)min((int64_t)kSegment, a.num_pages - i0), 1);
+  int64_t before, all;
+  if (SHARED)
+    before = w.segment[blockIdx.x];
+  else
+    scan1024(tid < (int)blockIdx.x ? w.segment[tid] : 0, sc, &before);
+  if (before >= w.most) return;
+  int64_t rank = scan1024((v[0] == 0) + (v[1] == 0) + (v[2] == 0) + (v[3] == 0), sc, &all) + before;
 #pragma unroll
-  for (int e = 0; e < 4; e++) {
-    if (v[e] == 0) {
-      if (rank < taken) {
-        w.pages[rank] = (int)i0 + 4 * threadIdx.x + e;
-        a.out_refs[i0 + 4 * threadIdx.x + e] = 1;
-      }
-      rank++;
-    }
-  }
+  for (int e = 0; e < 4; e++)
+    if (v[e] == 0 && rank < w.most) w.pages[rank++] = (int)i0 + 4 * tid + e;
 }
 
 // The pages that a sequence gets into its table, its first position and its slots: a wave.
-template <typename P>
-__device__ __forceinline__ void fill(const ReserveArgs& a, const Seq& q, int s, int base, int lane, P page_at) {
+// `entry`: its table's at the first of the pages past its length + lane.
+__device__ __forceinline__ void fill(const ReserveArgs& a, const Work& w, const Seq& q, int s, int base, int lane,
+                                     int entry) {
   int32_t* const to = a.out_tables + (size_t)s * a.width;
   const int page = 1 << a.page_shift;
   const bool served = q.rows > 0 && base >= 0;
@@ -259,9 +247,13 @@ __device__ __forceinline__ void fill(const ReserveArgs& a, const Seq& q, int s, 
   int at = base;
   for (int b = i0; served && b < q.use.end; b += 64) {
     const int i = b + lane;
-    const bool lacks = i < q.use.end && to[i] < 0;
+    const bool lacks = i < q.use.end && (b == i0 ? entry : to[i]) < 0;
     const uint64_t m = __ballot(lacks);
-    if (lacks) to[i] = page_at(at + __popcll(m & ((1ull << lane) - 1)));
+    if (lacks) {
+      const int p = w.pages[at + __popcll(m & ((1ull << lane) - 1))];
+      to[i] = p;
+      a.out_refs[p] = 1;
+    }
     at += __popcll(m);
   }
   if (lane == 0) a.starts[s] = served ? q.length : -1;
@@ -277,11 +269,28 @@ __device__ __forceinline__ void fill(const ReserveArgs& a, const Seq& q, int s, 
   }
 }
 
-__global__ __launch_bounds__(256) void reserve_fill_kernel(ReserveArgs a) {
-  const int s = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (s >= a.seqs) return;
+template <bool SHARED>
+__global__ __launch_bounds__(1024) void reserve_fill_kernel(ReserveArgs a) {
+  __shared__ Scan sc;
+  __shared__ int base[kInPlace];
   const Work w = work_of(a);
-  fill(a, seq_of(a, s), s, w.base[s], threadIdx.x & 63, [&](int rank) { return w.pages[rank]; });
+  const int tid = threadIdx.x, s = blockIdx.x * 16 + (tid >> 6);
+  Seq q;
+  int entry = 0;  // on its way while the sums are made
+  if (s < a.seqs) {
+    q = seq_of(a, s);
+    const int i = max(q.past, 0) + (tid & 63);
+    if (i < q.use.end) entry = a.out_tables[(size_t)s * a.width + i];
+  }
+  if (!SHARED) {
+    const int want = tid < a.seqs ? want_of(w, tid) : kLost, segment = tid < w.segments ? w.segment[tid] : 0;
+    int64_t free, all;
+    scan1024(segment, sc, &free);
+    const int64_t before = scan1024(want == kLost ? 0 : want, sc, &all);
+    base[tid] = base_of(want, before, free);
+    __syncthreads();
+  }
+  if (s < a.seqs) fill(a, w, q, s, SHARED ? w.base[s] : base[s], tid & 63, entry);
 }
 
 // Few sequences over a small pool: all of it by one block, with the counts, what is
@@ -390,9 +399,7 @@ __global__ __launch_bounds__(1024) void reserve_one_kernel(ReserveArgs a, uint32
 
 size_t reserve_work(const ReserveArgs& a) {
   const Work w = work_of(a);
-  // a sequence's new rows lie in at most tokens / page pages that begin past its length, rounded up
-  const int64_t most = (int64_t)a.seqs * (((int64_t)a.tokens + (1 << a.page_shift) - 1) >> a.page_shift);
-  return (size_t)a.seqs * (w.waves + 1) + w.segments + 1 + (size_t)std::min<int64_t>(most, a.num_pages);
+  return (size_t)(w.pages - w.want) + w.most;
 }
 
 void launch_reserve(const ReserveArgs& a, hipStream_t st) {
@@ -407,8 +414,15 @@ void launch_reserve(const ReserveArgs& a, hipStream_t st) {
     hipLaunchKernelGGL(reserve_copy_kernel, dim3((unsigned)std::min(1024, a.num_pages / 1024 + 1)), dim3(256), 0, st, a);
   hipLaunchKernelGGL(reserve_rows_kernel, dim3((unsigned)((a.seqs * w.waves + 3) / 4)), dim3(256), 0, st, a);
   hipLaunchKernelGGL(reserve_count_kernel, segments, dim3(1024), 0, st, a);
-  hipLaunchKernelGGL(reserve_take_kernel, segments, dim3(1024), 0, st, a);
-  hipLaunchKernelGGL(reserve_fill_kernel, dim3((unsigned)((a.seqs + 3) / 4)), dim3(256), 0, st, a);
+  const dim3 rows((unsigned)((a.seqs + 15) / 16));
+  if (a.seqs > kInPlace || w.segments > kInPlace) {
+    hipLaunchKernelGGL(reserve_share_kernel, dim3(1), dim3(1024), 0, st, a);
+    hipLaunchKernelGGL(reserve_list_kernel<true>, segments, dim3(1024), 0, st, a);
+    hipLaunchKernelGGL(reserve_fill_kernel<true>, rows, dim3(1024), 0, st, a);
+  } else {
+    hipLaunchKernelGGL(reserve_list_kernel<false>, segments, dim3(1024), 0, st, a);
+    hipLaunchKernelGGL(reserve_fill_kernel<false>, rows, dim3(1024), 0, st, a);
+  }
 }
 
 }  // namespace tlm
