@@ -255,7 +255,7 @@ int tlm_op_paged_reserve(tlm_paged* paged, const tlm_paged_request* request);
  * they need it, raise it; the positions before them are then rounded again (exact but
  * for magnitudes below 2^-14 of the largest).  Of rows that start within 32 positions
  * the earlier ones have been appended (or their page is all zeros).  Positions behind the appended rows, to
- * the end of their 32, are lost; 32 positions that two sequences append to in one
+ * the end of their 32, keep their codes, not their values; 32 positions that two sequences append to in one
  * call are lost.  Values that are not finite become NaN. */
 int tlm_op_paged_append(tlm_paged* paged, const tlm_paged_batch* batch, const float* qkv, float* q);
 /* Attention of every row over positions [max(0, pos - W + 1), pos] of its

@@ -225,9 +225,6 @@ def append(sv, x=None, want_q=True):
             touched[name][at] = True
             for i in range(4):
                 touched[name][4 * sat + i] = True
-            behind = np.arange(p0 + r, ((p0 + r - 1) // 32 + 1) * 32)
-            if behind.size:
-                touched[name][mo.places8(sv.tables[s], behind, hkv, sv.page, sv.d, where)] = True
     for name, was in (("k", kp), ("v", vp)):
         assert np.array_equal(got[name][~touched[name]], was[~touched[name]]), f"bytes of no new position in {name}"
     sv.close()

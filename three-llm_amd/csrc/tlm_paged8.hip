@@ -34,6 +34,9 @@ __device__ __forceinline__ uint32_t recoded(uint32_t c, int by) {
   return codes4(ldexpf(lo[0], -by), ldexpf(lo[1], -by), ldexpf(hi[0], -by), ldexpf(hi[1], -by));
 }
 
+// The bytes of four tokens of which the first n are there.
+__device__ __forceinline__ uint32_t held_bytes(int n) { return n >= 4 ? ~0u : n > 0 ? (1u << 8 * n) - 1 : 0u; }
+
 // Eight dims from 8 o on of a rotated head's row x at a position (cs and sn: its cos and
 // sin).  WHOLE: half the rotary dims are a multiple of 8, rows are read 16 bytes at a time.
 template <bool WHOLE>
@@ -169,13 +172,15 @@ __global__ __launch_bounds__(256) void paged_append8_few_kernel(PagedArgs a, int
         *c = (u32x2){recoded(v[0], by), recoded(v[1], by)};
       }
     if (by && is_v)
-      for (int t = 0; t < min(r.held, 16); t += 4)  // tokens t .. t + 3 and 16 further on
+      for (int t = 0; t < min(r.held, 16); t += 4) {  // tokens t .. t + 3 and 16 further on
+        const uint32_t lo = held_bytes(r.held - t), hi = held_bytes(r.held - t - 16);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
           TLM_GLOBAL u32x2* c = (TLM_GLOBAL u32x2*)(head + paged8_v_at(tok0 + t, d + e, D));
           const u32x2 v = *c;
-          *c = (u32x2){recoded(v[0], by), recoded(v[1], by)};
+          *c = (u32x2){(recoded(v[0], by) & lo) | (v[0] & ~lo), (recoded(v[1], by) & hi) | (v[1] & ~hi)};
         }
+      }
     for (int j = 0; j < r.n; j++) {
       if (j) oct(j, y);
       u32x2 c;
