@@ -446,6 +446,15 @@ def test_nan_reaches_only_the_rows_that_see_it(ctx):
     sv.close()
 
 
+@pytest.mark.parametrize("kv,window,sinks", [(F8, 0, 0), (F8, 1060, 40), (tlm.FMT_F16, 1060, 40)])
+@pytest.mark.parametrize("n,hkv", [(100, 4), (400, 1)])
+def test_attention_of_many_sequences_of_one_length(ctx, n, hkv, kv, window, sinks):
+    """So many that they stay whole, whatever their length; a few idle ones and a short one among them."""
+    lengths = [1090 + s % 40 for s in range(n)]
+    lengths[3], lengths[n - 1] = -1, 2
+    attend(Serving(ctx, hkv, hkv, 32, lengths, 1, 64, kv, window=window, sinks=sinks))
+
+
 # -------------------------------------------------------------------- sinks --
 
 @pytest.mark.parametrize("sinks", [1, 4, 31, 32, 33, 100, 700])

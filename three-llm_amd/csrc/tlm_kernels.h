@@ -485,8 +485,6 @@ struct PagedArgs {
   int* status;            // or'ed with kPagedStatus*
   int num_pages, width, page_shift, seqs, tokens, limit;
   int Hq, Hkv, D, G, rd, window;
-  int sinks;           // first positions that stay visible behind a window (0 without one)
-  size_t page_bytes;   // 8-bit caches: a page's
   int out_f32;
   float scale;
   // attention: how the sequences' position tiles are shared out (launch_paged_attention)
@@ -494,6 +492,9 @@ struct PagedArgs {
   unsigned* arrived;  // [kPagedCounters], zero between launches
   int* plan;          // of many sequences (paged_plan_kernel), or null
   int units, chunks, round, chunk_min, whole, plan_shift;
+  int sinks;          // first positions that stay visible behind a window (0 without one)
+  size_t page_bytes;  // 8-bit caches: a page's
+  int enough;         // sequences that may stay whole (plan_even)
 };
 constexpr int kPagedCounters = 16384;
 // kv_size: bytes of an element of the cache

@@ -318,25 +318,52 @@ __device__ __forceinline__ int plan_chunks_of(const PagedArgs& a, int c, int til
   return tiles <= a.whole ? min(tiles, 1) : (tiles + c - 1) / c;
 }
 
-template <int SHIFT, bool SINK>
+// Sequences of about one length that fill the chip as they are stay whole (8-bit caches
+// and sinks): splits would only cost their joins and blocks of a second round.  us a call,
+// split / whole, 8-bit: 64 x 1 Llama-3.2-1B with a window of 1024 and 100 sinks 19.0 / 18.0, 64 x 4
+// with one of 1300 21.4 / 19.9, 64 x 2 Llama-3.2-3B with one of 1500 49.0 / 39.2.  Up to twice the
+// mean (128 x 1 Llama-3.2-3B up to 3000 with a window of 1500) 45.9 / 47.7.
+__device__ __forceinline__ bool plan_even(const PagedArgs& a, int total, int most, int live) {
+  return live >= a.enough && (int64_t)most * live <= total + (int64_t)total / 4;
+}
+__device__ __forceinline__ int wave_most(int v) {
+  v = max(v, dpp<kDppXor1>(v));
+  v = max(v, dpp<kDppXor2>(v));
+  v = max(v, dpp<kDppHalfMirror>(v));
+  v = max(v, dpp<kDppMirror>(v));
+  return max(max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+             max(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
+}
+
+template <int SHIFT, bool SINK, bool EVEN>
 __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedArgs a) {
   constexpr int W = kPlanThreads / 64;
-  __shared__ int sh[2][W];
+  __shared__ int sh[3][W];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int groups = plan_groups(a.seqs);
   bool any = false, bad;
-  int sum = 0;
+  int sum = 0, most = 0, live = 0;
   for (int s = tid; s < a.seqs; s += kPlanThreads) {
-    sum += plan_part(a, seq_work<SHIFT, SINK>(a, s, &bad).tiles);
+    const int tiles = seq_work<SHIFT, SINK>(a, s, &bad).tiles;
+    sum += plan_part(a, tiles);
     any |= bad;
+    if (EVEN) most = max(most, tiles), live += tiles > 0;
   }
   if (any) paged_flag(a.status, kPagedStatusRows);
   sum = __builtin_amdgcn_readlane(wave_scan(sum), 63);
-  if (lane == 0) sh[0][w] = sum;
+  if (EVEN) most = wave_most(most), live = __builtin_amdgcn_readlane(wave_scan(live), 63);
+  if (lane == 0) {
+    sh[0][w] = sum;
+    if (EVEN) sh[1][w] = most, sh[2][w] = live;
+  }
   __syncthreads();
   int total = 0;
-  for (int i = 0; i < W; i++) total += sh[0][i];
-  const int c = plan_chunk(a, total);
+  most = live = 0;
+  for (int i = 0; i < W; i++) {
+    total += sh[0][i];
+    if (EVEN) most = max(most, sh[1][i]), live += sh[2][i];
+  }
+  const int c = EVEN && a.plan_shift == 0 && plan_even(a, total, most, live) ? max(most, 1) : plan_chunk(a, total);
   if (tid == 0) a.plan[0] = c;
   int before = 0, slots = 0;
   for (int g0 = 0; g0 < groups; g0 += W) {  // a wave per 64 sequences
@@ -358,7 +385,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedArgs a) {
   }
 }
 
-template <int SHIFT, bool SINK>
+template <int SHIFT, bool SINK, bool EVEN>
 __device__ __forceinline__ bool plan(const PagedArgs& a, int g, SeqChunk& r) {
   const int lane = threadIdx.x & 63;
   const SeqWork none{0, 0, 0, 0, 0};
@@ -412,17 +439,28 @@ __device__ __forceinline__ bool plan(const PagedArgs& a, int g, SeqChunk& r) {
   }
 #pragma unroll
   for (int k = 0; k < kSeqs; k++) sum += plan_part(a, w[k].tiles);
+  int most = max(max(w[0].tiles, w[1].tiles), max(w[2].tiles, w[3].tiles)), live = 0;
+#pragma unroll
+  for (int k = 0; k < kSeqs && EVEN; k++) live += w[k].tiles > 0;
   bool any = bad[0] || bad[1] || bad[2] || bad[3];
   for (int s = 64 * kSeqs + lane; s < a.seqs; s += 64) {
-    sum += plan_part(a, seq_work<SHIFT, SINK>(a, s, &b).tiles);
+    const int tiles = seq_work<SHIFT, SINK>(a, s, &b).tiles;
+    sum += plan_part(a, tiles);
     any |= b;
+    if (EVEN) most = max(most, tiles), live += tiles > 0;
   }
   if (any && blockIdx.x == 0 && threadIdx.x < 64) paged_flag(a.status, kPagedStatusRows);
-  c = plan_chunk(a, __builtin_amdgcn_readlane(wave_scan(sum), 63));
-  if (a.seqs <= 64) {
+  const int total = __builtin_amdgcn_readlane(wave_scan(sum), 63);
+  bool even = false;
+  if (EVEN && a.plan_shift == 0 && a.seqs >= a.enough) {
+    most = wave_most(most);
+    even = plan_even(a, total, most, __builtin_amdgcn_readlane(wave_scan(live), 63));
+  }
+  c = even ? max(most, 1) : plan_chunk(a, total);
+  if (a.seqs <= 64 && !even) {
     // few sequences: all their chunks in one round of blocks
-    const int live = __builtin_popcountll(__ballot(w[0].tiles > 0));
-    if (2 * live <= a.round)
+    const int here = __builtin_popcountll(__ballot(w[0].tiles > 0));
+    if (2 * here <= a.round)
       while (__builtin_amdgcn_readlane(wave_scan(plan_chunks_of(a, c, w[0].tiles)), 63) > a.round) c += (c + 7) / 8;
   }
 #pragma unroll
@@ -464,7 +502,7 @@ __global__ __launch_bounds__(64 * W, DT <= 64 ? 4 : 2) void paged_attention_kern
   const int unit = blockIdx.x % a.units, hk = unit % a.Hkv, r0 = (a.units - 1 - unit) / a.Hkv * 16;
   const int g = blockIdx.x / a.units;
   SeqChunk sc;
-  if (!plan<T::SHIFT, SINK>(a, g, sc)) return;
+  if (!plan<T::SHIFT, SINK, F8 || SINK>(a, g, sc)) return;
   const int ci = sc.chunk, tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int R = sc.w.rows * a.G;  // rows of the kv head
   if (r0 >= R) return;
@@ -917,9 +955,10 @@ void launch_attention_as(PagedArgs a, int cus, size_t part_floats, hipStream_t s
   a.chunks = (int)std::max<int64_t>(1, std::min<int64_t>(fit, a.round));
   a.chunk_min = fit < 1 ? INT_MAX / 2 : 16;
   a.whole = 32;
+  a.enough = (3 * cus / 2 + a.units - 1) / a.units;  // sequences whose blocks fill the chip
   const int64_t per_seq = fit < 1 || tiles <= a.whole ? 1 : (tiles + a.chunk_min - 1) / a.chunk_min;
   const int64_t blocks = std::min<int64_t>(a.chunks + a.seqs, a.seqs * per_seq) * a.units;
-  if (a.plan) hipLaunchKernelGGL((paged_plan_kernel<T::SHIFT, SINK>), dim3(1), dim3(kPlanThreads), 0, st, a);
+  if (a.plan) hipLaunchKernelGGL((paged_plan_kernel<T::SHIFT, SINK, sizeof(KT) == 1 || SINK>), dim3(1), dim3(kPlanThreads), 0, st, a);
   hipLaunchKernelGGL((paged_attention_kernel<KT, DT, W, STREAM, SINK>), dim3((unsigned)blocks), dim3(64 * W), 0, st, a);
 }
 
