@@ -250,6 +250,18 @@ def test_append_partial_rotary_and_no_q(ctx, rotary, tokens):
     append(Serving(ctx, 3, 1, 64, [9, 40], tokens, 64, rotary=rotary), want_q=False)
 
 
+@pytest.mark.parametrize("rotary", [0, 16, 64, 112, 128])
+@pytest.mark.parametrize("tokens", [3, 40])
+def test_append_partial_rotary_of_wide_heads(ctx, rotary, tokens):
+    append(Serving(ctx, 4, 2, 128, [9, 40], tokens, 64, rotary=rotary))
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(40, 40, 32), (48, 3, 64), (33, 33, 128)])
+@pytest.mark.parametrize("tokens", [1, 5, 33])
+def test_append_many_heads(ctx, hq, hkv, d, tokens):
+    append(Serving(ctx, hq, hkv, d, [30, 5], tokens, 32))
+
+
 def test_append_far_positions(ctx):
     append(Serving(ctx, 2, 1, 128, [100000, 99999, 65535, 131071], 2, 128, window=40, max_tokens=1 << 18))
 
@@ -432,6 +444,41 @@ def test_attention_over_what_append_wrote(ctx):
             keep[s] = mo.CODES[pool[mo.places8(sv.tables[s], pos, 2, 32, 64, where)]] * scale[..., None]
     sv.check(qh, got, tlm.FMT_F32)
     sv.close()
+
+
+@pytest.mark.parametrize("tokens", [5, 40])
+def test_pools_past_32_bits(ctx, tokens):
+    """Pages that begin past 2^32 bytes of the pools: appended, attended to, read back."""
+    hq, hkv, d, page, pages = 8, 8, 128, 1024, 4200
+    p = tlm.Paged(ctx, hq, hkv, d, 4 * page, page_tokens=page, kv_fmt=F8)
+    size = p.page_bytes()
+    assert 4100 * size > 1 << 32
+    kb, vb = ctx.buffer(pages * size), ctx.buffer(pages * size)
+    tables, starts = np.array([[4199, -1], [4101, 4150]], np.int32), np.array([0, 0], np.int32)
+    rng = np.random.default_rng(tokens)
+    x = rng.standard_normal((2, tokens, hq + 2 * hkv, d)).astype(np.float32)
+    b = p.batch(kb, vb, pages, ctx.array(tables), 2, ctx.array(starts), 2, tokens)
+    q, out = ctx.buffer(4 * 2 * tokens * hq * d), ctx.buffer(4 * 2 * tokens * hq * d)
+    p.append(b, ctx.array(x), q)
+    p.attention(b, q, out, tlm.FMT_F32)
+    p.status()
+    got, rows = out.read().reshape(2, tokens, hq, d).astype(np.float64), {}
+    assert np.array_equal(q.read().reshape(2, tokens, hq, d), x[:, :, :hq])  # no rotation here
+    for s in range(2):
+        for name, buf, new, where in (("k", kb, x[s, :, hq:2 * hq], mo.k8_at), ("v", vb, x[s, :, 2 * hq:], mo.v8_at)):
+            at = tlm.Buffer.__new__(tlm.Buffer)  # the sequence's page
+            at.ctx, at.nbytes, at.ptr = ctx, size, type(buf.ptr)(buf.ptr.value + int(tables[s, 0]) * size)
+            one, pos = at.read(np.uint8), np.arange(tokens)
+            scale = one.view(np.float32)[mo.scales_at([0], pos, hkv, page, d)].astype(np.float64)
+            code = one[mo.places8([0], pos, hkv, page, d, where)]
+            assert np.array_equal(code, mo.encode(new / scale[..., None]))
+            rows[name] = mo.CODES[code] * scale[..., None]
+        for j in range(tokens):
+            ref = mo.attend(x[s, j, :hq], rows["k"], rows["v"], np.arange(j + 1), d ** -0.5)
+            assert np.all(np.abs(got[s, j] - ref) <= 2.0 ** -16 * np.abs(rows["v"]).max())
+    kb.free()
+    vb.free()
+    p.close()
 
 
 def test_nan_reaches_only_the_rows_that_see_it(ctx):

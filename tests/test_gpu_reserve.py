@@ -86,6 +86,22 @@ def test_steps_of_a_server(ctx, n, width, pages, tokens, window, sinks, in_place
     p.paged.close()
 
 
+@pytest.mark.parametrize("n,width,pages,tokens", [(1024, 32, 16384, 64), (1024, 32, 16385, 64), (1025, 31, 16384, 64),
+                                                  (1024, 33, 16384, 64), (40, 100, 300, 3200), (2, 2100, 2300, 65537),
+                                                  (3, 40, 5000000, 700)])
+def test_sizes_where_the_kernels_change(ctx, n, width, pages, tokens):
+    """The last size that one block takes and the first that it does not; more pages than 1024 blocks count."""
+    rng = np.random.default_rng([n, width, pages])
+    p = Pool(ctx, n, width, pages, tokens)
+    p.refs[rng.random(pages) < 0.5] = 1
+    lengths = np.zeros(n, np.int64)
+    for _ in range(3):
+        counts = rng.integers(0, tokens + 1, n)
+        starts = p.step(lengths, counts, True)
+        lengths = np.minimum(np.where(starts >= 0, lengths + counts, lengths), width * 32)
+    p.paged.close()
+
+
 @pytest.mark.parametrize("page", [64, 1024])
 def test_page_sizes(ctx, page):
     p = Pool(ctx, 6, 3, 20, 1500, page, 0, 0)
