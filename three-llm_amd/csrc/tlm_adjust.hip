@@ -18,11 +18,12 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 // of a row's vocabulary in LDS, where it also has their biases, while its logits are on
 // their way to registers, and makes one pass over the chunk; what a mask takes out four
 // at a time is not read.  In place it reads and writes the fours that a rule changes.
-constexpr int kThreads = 512, kAhead = 8;  // tokens of the history in flight a thread
+constexpr int kThreads = 512, kFours = 2, kChunk = 4 * kFours * kThreads;
+constexpr int kAhead = 8;  // tokens of the history in flight a thread
 
-template <int Q, bool MASKED, bool BIASED, bool PLACE>
+template <bool MASKED, bool BIASED, bool PLACE>
 __global__ __launch_bounds__(kThreads) void adjust_kernel(AdjustArgs a, int chunks) {
-  constexpr int C = 4 * Q * kThreads;
+  constexpr int Q = kFours, C = kChunk;
   __shared__ __align__(16) int times[C];
   __shared__ __align__(16) float bias[BIASED ? C : 4];
   const int row = blockIdx.x / chunks, v0 = blockIdx.x % chunks * C, tid = threadIdx.x;
@@ -138,28 +139,28 @@ __global__ __launch_bounds__(kThreads) void adjust_kernel(AdjustArgs a, int chun
   }
 }
 
-template <int Q, bool PLACE>
+template <bool PLACE>
 void launch_of(const AdjustArgs& a, hipStream_t st) {
-  const int chunks = (a.vocab + 4 * Q * kThreads - 1) / (4 * Q * kThreads);
+  const int chunks = (a.vocab + kChunk - 1) / kChunk;
   const dim3 grid((unsigned)(a.seqs * a.tokens * chunks)), block(kThreads);
-  if (a.masks && a.bias_ids) hipLaunchKernelGGL((adjust_kernel<Q, true, true, PLACE>), grid, block, 0, st, a, chunks);
-  else if (a.masks) hipLaunchKernelGGL((adjust_kernel<Q, true, false, PLACE>), grid, block, 0, st, a, chunks);
-  else if (a.bias_ids) hipLaunchKernelGGL((adjust_kernel<Q, false, true, PLACE>), grid, block, 0, st, a, chunks);
-  else hipLaunchKernelGGL((adjust_kernel<Q, false, false, PLACE>), grid, block, 0, st, a, chunks);
+  if (a.masks && a.bias_ids) hipLaunchKernelGGL((adjust_kernel<true, true, PLACE>), grid, block, 0, st, a, chunks);
+  else if (a.masks) hipLaunchKernelGGL((adjust_kernel<true, false, PLACE>), grid, block, 0, st, a, chunks);
+  else if (a.bias_ids) hipLaunchKernelGGL((adjust_kernel<false, true, PLACE>), grid, block, 0, st, a, chunks);
+  else hipLaunchKernelGGL((adjust_kernel<false, false, PLACE>), grid, block, 0, st, a, chunks);
 }
 
 }  // namespace
 
-// Chunks of 4096 where they make a block for every CU, else of 2048.  Each block reads
-// the whole history, so that larger chunks read less of it, but fewer of them fit a CU
-// (16 KB of LDS each, 32 with biases): 62 rows of 128256 with everything and histories of
-// 4096, chunks of 4096 / 6144 / 8192: 14.7 / 16.3 / 18.6 us (4.5 TB/s of logits).
-void launch_adjust(const AdjustArgs& a, int cus, hipStream_t st) {
-  const bool large = (int64_t)a.seqs * a.tokens * ((a.vocab + 4095) / 4096) >= cus, place = a.out == a.logits;
-  if (large && place) launch_of<2, true>(a, st);
-  else if (large) launch_of<2, false>(a, st);
-  else if (place) launch_of<1, true>(a, st);
-  else launch_of<1, false>(a, st);
+// Chunks of 4096.  Each block reads the whole history, so that larger chunks read less of
+// it, but fewer of them fit a CU (16 KB of LDS each, 32 with biases): 62 rows of 128256 with
+// everything and histories of 4096, chunks of 4096 / 6144 / 8192: 14.7 / 16.3 / 18.6 us (4.5 TB/s of
+// logits); of 2048, 64 x 32000 5.8 against 5.6 and 1 x 5 x 151936 3.7 either way.  64 x 128256 without
+// masks 14.7, in place 11.1.
+void launch_adjust(const AdjustArgs& a, hipStream_t st) {
+  if (a.out == a.logits)
+    launch_of<true>(a, st);
+  else
+    launch_of<false>(a, st);
 }
 
 }  // namespace tlm

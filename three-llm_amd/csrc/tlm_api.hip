@@ -1650,7 +1650,7 @@ int tlm_op_adjust_logits(tlm_ctx* ctx, const tlm_logit_rules* r) {
     if (x.p && x.n && overlap(x.p, x.n, r->out, n))
       return fail(TLM_ERR_INVALID, "TLMLogitRules: the results overlap an input");
   const DeviceScope on(ctx->device);
-  launch_adjust(a, ctx->cus, ctx->stream);
+  launch_adjust(a, ctx->stream);
   CHECK_LAUNCH("TLMLogitRules");
   return TLM_OK;
 }

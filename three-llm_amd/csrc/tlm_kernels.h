@@ -538,7 +538,7 @@ struct AdjustArgs {
   int seqs, tokens, vocab, history_width, bias_width;
 };
 constexpr int kAdjustMaxBiases = 4096;
-void launch_adjust(const AdjustArgs& a, int cus, hipStream_t st);
+void launch_adjust(const AdjustArgs& a, hipStream_t st);
 
 struct VerifyArgs {
   const float* logits;        // [seqs][tokens][vocab]

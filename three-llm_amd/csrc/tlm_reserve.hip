@@ -295,7 +295,7 @@ __global__ __launch_bounds__(1024) void reserve_fill_kernel(ReserveArgs a) {
 
 // Few sequences over a small pool: all of it by one block, with the counts, what is
 // shared out and the pages of the new rows in LDS, in place of four or five launches.
-constexpr int kOnePages = 16384, kOneSeqs = 1024, kOneEntries = 32768, kOneRows = 4096, kOneSlots = 65536;
+constexpr int kOnePages = 16384, kOneSeqs = 1024, kOneEntries = 20480, kOneRows = 4096, kOneSlots = 65536;
 __host__ __device__ inline int span_of(const ReserveArgs& a) {  // pages that a sequence's new rows may touch
   return ((a.tokens - 1) >> a.page_shift) + 2;
 }
