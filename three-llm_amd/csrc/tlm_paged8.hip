@@ -108,15 +108,15 @@ __device__ __forceinline__ void append8_queries(const PagedArgs& a, size_t row, 
 // as there are lanes, so that a store's bytes lie together), in registers between the
 // maximum and the codes; a block has the rows of `heads` kv heads, the queries are further
 // blocks' (slices from `parts` on).  Latency: loads of the start, then of the table, the old
-// scales and the rows, then the stores (64 x 1 Llama-3.2-1B %1 us, 0.9 MB read and written).
-constexpr int kFewRows = 8;  // a block has room for a head's 16
+// scales and the rows, then the stores (64 x 1 Llama-3.2-1B 4.1 us, 0.9 MB read and as much written).
+constexpr int kFewHeads = 8;  // that a block has, of one row each
 template <bool WHOLE>
 __global__ __launch_bounds__(256) void paged_append8_few_kernel(PagedArgs a, int groups, int heads, int parts, int slices) {
   constexpr int NI = 4;  // 2 * 32 rows of one head, where rotations of an odd width bring so many here
-  __shared__ unsigned top[2][kFewRows];
+  __shared__ unsigned top[2][kFewHeads];
   const int slice = blockIdx.x % slices, block = blockIdx.x / slices, g = block % groups, s = block / groups;
   const int tid = threadIdx.x, D = a.D, octs = D / 8, half = a.rd / 2, N = (a.Hq + 2 * a.Hkv) * D;
-  if (tid < 2 * kFewRows) top[tid / kFewRows][tid % kFewRows] = 0;
+  if (tid < 2 * kFewHeads) top[tid / kFewHeads][tid % kFewHeads] = 0;
   const int start = a.starts[s];
   bool bad;
   const Rows r = rows_of(a, s, g, start, a.counts ? a.counts[s] : a.tokens, &bad);
@@ -362,8 +362,11 @@ __global__ __launch_bounds__(256) void paged_append8_kernel(PagedArgs a, int gro
 void launch_paged_append8(const PagedArgs& a, hipStream_t st) {
   const int groups = (a.tokens + 30) / 32 + 1;  // aligned blocks that `tokens` positions may touch
   const dim3 block(256);
-  if (a.tokens <= kFewRows || a.rd % 16) {
-    const int heads = std::max(1, kFewRows / a.tokens), parts = (a.Hkv + heads - 1) / heads;
+  // us a call, few-rows / many-rows kernel, 64 sequences of 4, 8, 12 and 16 tokens: Llama-3.2-1B heads
+  // 6.1 / 11.7, 9.9 / 12.1, 9.7 / 12.9, 11.8 / 13.0; Llama-3.2-3B 6.0 / 11.4, 8.5 / 12.7, 11.1 / 14.1,
+  // 17.1 / 14.7.  2 x up to 2048 (3B, 122 MB) 28.5 us, 4.3 TB/s.
+  if (a.tokens <= 12 || a.rd % 16) {
+    const int heads = std::max(1, kFewHeads / a.tokens), parts = (a.Hkv + heads - 1) / heads;
     const int slices = parts + (a.q ? (std::min(a.tokens, 32) * a.Hq * (a.D / 8) + 255) / 256 : 0);
     const dim3 grid((unsigned)((int64_t)a.seqs * groups * slices));
     if (a.rd % 16)
