@@ -221,8 +221,8 @@ int tlm_paged_set_sinks(tlm_paged* paged, int32_t sinks);
  * lowest first, refs 1, for as long as what they have lacked so far is no more than
  * what is free; one that it is not enough for keeps what it holds.  An entry
  * that is no page of the pool is none.  refs counts the tables that a page is in,
- * and holds of the caller's own (a prefix that is kept); pages may be shared,
- * each table counted.
+ * and holds of the caller's own (a prefix that is kept); pages may be shared, each
+ * table counted, but for those that a sequence appends to.
  * starts: lengths[s] where the sequence's rows are served, else -1 (no rows
  * wanted, no pages left, or a page with positions that it needs below its length is
  * not held: tlm_paged_status reports that, and rows past max_tokens or
@@ -241,8 +241,9 @@ typedef struct tlm_paged_request {
   int64_t* slots;           /* [seqs][tokens] or NULL */
   int32_t num_pages, table_width, seqs, tokens;
 } tlm_paged_request;
-/* seqs * tokens * heads is at most 2^22, seqs 2^20, num_pages 2^30, table_width 2^26.  The results are apart from each
- * other and from the inputs, but for tables and refs in place.  Enqueue only. */
+/* seqs * tokens * heads is at most 2^22, seqs 2^20, num_pages 2^30, table_width
+ * 2^26.  The results are apart from each other and from the inputs, but for tables
+ * and refs in place.  Enqueue only. */
 int tlm_op_paged_reserve(tlm_paged* paged, const tlm_paged_request* request);
 /* qkv: fp32 [seqs][tokens][(heads + 2 kv_heads) * head_dim] (Q|K|V, bias
  * included, pre-RoPE).  The rotated K and the V rows go to their pages; q, when
@@ -254,9 +255,10 @@ int tlm_op_paged_reserve(tlm_paged* paged, const tlm_paged_request* request);
  * most 448.  Rows that start within 32 positions keep the scale that these have or, if
  * they need it, raise it; the positions before them are then rounded again (exact but
  * for magnitudes below 2^-14 of the largest).  Of rows that start within 32 positions
- * the earlier ones have been appended (or their page is all zeros).  Positions behind the appended rows, to
- * the end of their 32, keep their codes, not their values; 32 positions that two sequences append to in one
- * call are lost.  Values that are not finite become NaN. */
+ * the earlier ones have been appended (or their page is all zeros).  Positions behind
+ * the appended rows, to the end of their 32, keep their codes, not their values; 32
+ * positions that two sequences append to in one call are lost.  Values that are not
+ * finite become NaN, magnitudes past 448 * 2^31 become that. */
 int tlm_op_paged_append(tlm_paged* paged, const tlm_paged_batch* batch, const float* qkv, float* q);
 /* Attention of every row over positions [max(0, pos - W + 1), pos] of its
  * sequence, which the pages hold (append first).  q: fp32 [seqs][tokens]
@@ -264,7 +266,8 @@ int tlm_op_paged_append(tlm_paged* paged, const tlm_paged_batch* batch, const fl
  * TLM_FMT_F32, apart from q and all that the batch names.  Scores and the weighted sum to 32 bits: an fp16
  * cache's products take q and the probabilities as pairs of fp16 values, each to
  * 2^-22 of itself or 2^-39 of its row's largest (an 8-bit cache's too, whose codes
- * are exact in fp16; there the probabilities times V's scales).  What masked positions hold does
+ * are exact in fp16; there the probabilities times V's scales).  What masked
+ * positions hold does
  * not matter; attended K and V are finite.  Enqueue only. */
 int tlm_op_paged_attention(tlm_paged* paged, const tlm_paged_batch* batch, const float* q, int out_fmt, void* out);
 /* Waits for the stream and tells of what the calls since the last status met on

@@ -99,6 +99,23 @@ def test_biases(ctx, biases):
     check(ctx, d)
 
 
+@pytest.mark.parametrize("biases", [64, 150, 700])
+def test_biases_of_the_same_tokens(ctx, biases):
+    """Tokens 256 apart, and each several times among 64 of the list: bit for bit the sums in the list's order."""
+    d = rules(3, 1, 9000, biases=biases, penalties=False)
+    rng = np.random.default_rng(biases)
+    d["bias_ids"] = (rng.integers(0, 12, (3, biases)) * 256 + rng.integers(0, 3, (3, biases))).astype(np.int32)
+    got = run(ctx, d)
+    for s in range(3):
+        sums = {}
+        for i, b in zip(d["bias_ids"][s], d["biases"][s]):
+            sums[i] = np.float32(sums[i] + b) if i in sums else b
+        want = d["logits"][s, 0].copy()
+        for i, b in sums.items():
+            want[i] += b
+        assert np.array_equal(got[s, 0], want)
+
+
 @pytest.mark.parametrize("in_place", [False, True])
 def test_each_rule_alone(ctx, in_place):
     for kw in (dict(), dict(history=50), dict(drafts=True, history=0), dict(biases=4), dict(masked=True)):

@@ -21,11 +21,22 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 constexpr int kThreads = 512, kFours = 2, kChunk = 4 * kFours * kThreads;
 constexpr int kAhead = 8;  // tokens of the history in flight a thread
 
+// What other lanes of the wave leave in LDS, in the order of its instructions.
+template <typename T>
+__device__ __forceinline__ T get_lds(const T* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+}
+template <typename T>
+__device__ __forceinline__ void put_lds(T* p, T v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+}
+
 template <bool MASKED, bool BIASED, bool PLACE>
 __global__ __launch_bounds__(kThreads) void adjust_kernel(AdjustArgs a, int chunks) {
   constexpr int Q = kFours, C = kChunk;
   __shared__ __align__(16) int times[C];
   __shared__ __align__(16) float bias[BIASED ? C : 4];
+  __shared__ int turn[BIASED ? 256 : 1];
   const int row = blockIdx.x / chunks, v0 = blockIdx.x % chunks * C, tid = threadIdx.x;
   const int s = row / a.tokens, j = row % a.tokens;
   const int n = min(C, a.vocab - v0);
@@ -81,25 +92,37 @@ __global__ __launch_bounds__(kThreads) void adjust_kernel(AdjustArgs a, int chun
     if (id >= 0 && v < (unsigned)n) atomicAdd(times + v, 1);
   }
   if (BIASED && tid < 64) {
-    // one wave, 64 of the list at a time, so that a token listed more than once gets its
-    // biases in the list's order
+    // One wave, 64 of the list at a time, so that a token listed more than once gets its
+    // biases in the list's order: the first of the lanes that share a place of `turn` add
+    // theirs at once, then the next; what is left after a few turns goes token by token (24
+    // rows of 10198 with 151 biases: 10.7 us so from the start, 5.1 with the turns).
     for (int i = 0; i < a.bias_width; i += 64) {
       const bool here = i + tid < a.bias_width;
       const size_t at = (size_t)s * a.bias_width + i + (here ? tid : 0);
       const int id = here ? a.bias_ids[at] : -1;
       const float b = a.biases[at];
       const unsigned v = (unsigned)id - (unsigned)v0;
-      uint64_t left = __ballot(id >= 0 && v < (unsigned)n);
+      bool todo = id >= 0 && v < (unsigned)n;
+      for (int k = 0; k < 4 && __ballot(todo); k++) {
+        int* const place = turn + (v & 255);
+        if (todo) put_lds(place, 64);
+        if (todo) __hip_atomic_fetch_min(place, tid, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        if (todo && get_lds(place) == tid) {
+          put_lds(bias + v, get_lds(bias + v) + b);
+          todo = false;
+        }
+      }
+      uint64_t left = __ballot(todo);
       while (left) {
         const int first = __builtin_ctzll(left), at_v = __builtin_amdgcn_readlane((int)v, first);
         uint64_t same = __ballot((int)v == at_v) & left;
         left &= ~same;
-        float sum = bias[at_v];
+        float sum = get_lds(bias + at_v);
         while (same) {
           sum += __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(b), __builtin_ctzll(same)));
           same &= same - 1;
         }
-        bias[at_v] = sum;
+        put_lds(bias + at_v, sum);
       }
     }
   }
