@@ -126,3 +126,78 @@ def test_steps(kv, window, sinks):
     paged.close()
     head.close()
     ctx.close()
+
+
+def test_two_contexts_at_once():
+    """Two programs' calls in turn, nothing waits between them: each one's results are what it gets alone."""
+    rng = np.random.default_rng(3)
+    n, hq, hkv, d, page, width, pages, vocab = 3, 8, 2, 64, 32, 64, 200, 3000
+    x = rng.standard_normal((2, n, 40, hq + 2 * hkv, d)).astype(np.float32)
+    logits = rng.standard_normal((2, n, vocab)).astype(np.float32)
+    ids = rng.integers(0, vocab, (2, n, 50)).astype(np.int32)
+
+    def begin(ctx, k):
+        p = tlm.Paged(ctx, hq, hkv, d, width * page, page_tokens=page, sliding_window=1500, kv_fmt=tlm.FMT_F8)
+        p.set_sinks(5)
+        z = lambda *shape: ctx.array(np.zeros(shape, np.int32))  # noqa: E731
+        b = dict(tables=ctx.array(np.full((n, width), -1, np.int32)), refs=z(pages), starts=z(n), q=ctx.buffer(4 * n * 40 * hq * d),
+                 out=ctx.array(np.zeros((n, 40, hq * d), np.float32)), x=ctx.array(x[k]), logits=ctx.array(logits[k]),
+                 kp=ctx.array(np.zeros(pages * p.page_bytes(), np.uint8)), vp=ctx.array(np.zeros(pages * p.page_bytes(), np.uint8)))
+        lengths = [ctx.array(np.array([40 * i, 40 * i - 3 if i else 0, 40 * i], np.int32)) for i in range(46)]
+        rules = tlm.logit_rules(b["logits"], n, 1, vocab, history=ctx.array(ids[k]), history_width=50,
+                                frequency=ctx.array(np.full(n, 0.5, np.float32)))
+        return p, b, lengths, rules
+
+    def step(ctx, state, i):
+        p, b, lengths, rules = state
+        p.reserve(p.request(lengths[i], b["tables"], width, b["refs"], pages, b["starts"], n, 40))
+        batch = p.batch(b["kp"], b["vp"], pages, b["tables"], width, b["starts"], n, 40)
+        p.append(batch, b["x"], b["q"])
+        p.attention(batch, b["q"], b["out"], tlm.FMT_F32)
+        tlm.adjust_logits(ctx, rules)
+
+    def end(state):
+        p, b, _, _ = state
+        p.status()
+        r = [b["tables"].read(np.int32), b["refs"].read(np.int32), b["kp"].read(np.uint8), b["vp"].read(np.uint8),
+             b["out"].read(), b["logits"].read()]
+        p.close()
+        return r
+
+    alone = []
+    for k in range(2):
+        ctx = tlm.Context(0)
+        s = begin(ctx, k)
+        for i in range(46):
+            step(ctx, s, i)
+        alone.append(end(s))
+        ctx.close()
+    both = [tlm.Context(0), tlm.Context(0)]
+    states = [begin(c, k) for k, c in enumerate(both)]
+    for i in range(46):
+        for c, s in zip(both, states):
+            step(c, s, i)
+    for s, want in zip(states, alone):
+        for got, w in zip(end(s), want):
+            assert np.array_equal(got.view(np.uint8), w.view(np.uint8))
+    for c in both:
+        c.close()
+
+
+def test_a_step_of_idle_slots():
+    """No sequence has rows: nothing is written, nothing reported."""
+    ctx = tlm.Context(0)
+    for kv in (tlm.FMT_F8, tlm.FMT_F16):
+        p = tlm.Paged(ctx, 4, 2, 64, 256, page_tokens=32, sliding_window=40, kv_fmt=kv)
+        p.set_sinks(3)
+        kp = ctx.array(np.full(4 * p.page_bytes(), 7, np.uint8))
+        vp = ctx.array(np.full(4 * p.page_bytes(), 7, np.uint8))
+        b = p.batch(kp, vp, 4, ctx.array(np.full((70, 8), -1, np.int32)), 8, ctx.array(np.full(70, -1, np.int32)), 70, 2)
+        q, out = ctx.array(np.full((70, 2, 256), 5, np.float32)), ctx.array(np.full((70, 2, 256), 6, np.float32))
+        p.append(b, ctx.array(np.full((70, 2, 512), 1, np.float32)), q)
+        p.attention(b, q, out, tlm.FMT_F32)
+        p.status()
+        assert np.all(kp.read(np.uint8) == 7) and np.all(vp.read(np.uint8) == 7)
+        assert np.all(q.read() == 5) and np.all(out.read() == 6)
+        p.close()
+    ctx.close()

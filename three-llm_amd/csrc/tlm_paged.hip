@@ -516,8 +516,9 @@ __global__ __launch_bounds__(64 * W, DT <= 64 ? 4 : 2) void paged_attention_kern
   const int past = (hi_any >> T::SHIFT) + 1, sinks = SINK ? min((a.sinks + TS - 1) >> T::SHIFT, past) : 0;
   const int sunk = SINK ? max(0, min(sinks, c1) - c0) : 0, base = sc.w.first - sc.w.sunk;
   const int t0 = max(base + max(c0, sinks), lo_any >> T::SHIFT), t1 = min(base + c1, past);
-  const int tiles = sunk + max(0, t1 - t0);
-  auto tile_of = [&](int i) { return i < sunk ? c0 + i : t0 + i - sunk; };
+  // numbered from `lead` to `tiles`; without sinks by their own numbers
+  const int lead = SINK ? 0 : t0, tiles = SINK ? sunk + max(0, t1 - t0) : t1;
+  auto tile_of = [&](int i) { return !SINK ? i : i < sunk ? c0 + i : t0 + i - sunk; };
   const int32_t* const table = a.tables + (size_t)sc.s * a.width;
   const int tpp = a.page_shift - T::SHIFT;  // log2 of the tiles of a page
 
@@ -532,9 +533,9 @@ __global__ __launch_bounds__(64 * W, DT <= 64 ? 4 : 2) void paged_attention_kern
 #pragma unroll
     for (int f = 0; f < NL; f++) x[f] = STREAM ? __builtin_nontemporal_load(p + 64 * f) : p[64 * f];
   };
-  // The wave's tiles w, w + W, ... of the chunk's.  Their pages (8-bit: and scales), 64 at
+  // The wave's tiles lead + w, lead + w + W, ...  Their pages (8-bit: and scales), 64 at
   // a time, a lane each; the first tile is on its way while q is prepared.
-  int tb = w, n = 0, page = -1;
+  int tb = lead + w, n = 0, page = -1;
   uint32_t kscale = 0, vscale = 0;
   auto pages = [&] {
     const int tl = tb + lane * W, t = tile_of(min(tl, tiles - 1));
