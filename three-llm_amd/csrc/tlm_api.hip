@@ -92,6 +92,7 @@ struct tlm_ctx {
   unsigned long long* arg_key = nullptr;
   unsigned* arg_arrived = nullptr;
   unsigned* paged_arrived = nullptr;  // tlm_op_paged_attention's chunks done (zero between launches)
+  int32_t* reserve_back = nullptr;    // tlm_op_paged_reserve's pages that go back (zero between launches)
   unsigned* verify_arrived = nullptr;  // tlm_op_verify_drafts' blocks done, per sequence (zero between launches)
   unsigned* topk_arrived = nullptr;  // tlm_op_topk's blocks done (zero between launches)
   // top-k levels: two levels of kTopkWork (score, id) pairs
@@ -542,6 +543,8 @@ int tlm_open(int device, tlm_ctx** out) {
   if (e == hipSuccess) e = hipMalloc(&c->topk_arrived, sizeof(unsigned));
   if (e == hipSuccess) e = hipMalloc(&c->paged_arrived, kPagedCounters * sizeof(unsigned));
   if (e == hipSuccess) e = hipMemset(c->paged_arrived, 0, kPagedCounters * sizeof(unsigned));
+  if (e == hipSuccess) e = hipMalloc(&c->reserve_back, kReserveBack * sizeof(int32_t));
+  if (e == hipSuccess) e = hipMemset(c->reserve_back, 0, kReserveBack * sizeof(int32_t));
   if (e == hipSuccess) e = hipMalloc(&c->verify_arrived, kVerifyCounters * sizeof(unsigned));
   if (e == hipSuccess) e = hipMemset(c->verify_arrived, 0, kVerifyCounters * sizeof(unsigned));
   if (e == hipSuccess) e = hipMemset(c->topk_arrived, 0, sizeof(unsigned));
@@ -573,6 +576,7 @@ void tlm_close(tlm_ctx* ctx) {
   hipFree(ctx->arg_arrived);
   hipFree(ctx->topk_arrived);
   hipFree(ctx->paged_arrived);
+  hipFree(ctx->reserve_back);
   hipFree(ctx->verify_arrived);
   if (ctx->stream) hipStreamDestroy(ctx->stream);
   delete ctx;
@@ -1423,6 +1427,7 @@ int tlm_op_paged_reserve(tlm_paged* P, const tlm_paged_request* r) {
   const DeviceScope on(P->ctx->device);
   std::lock_guard<std::mutex> lock(P->ctx->part_mu);
   a.work = reinterpret_cast<int32_t*>(P->ctx->part);
+  a.back = a.num_pages <= kReserveBack ? P->ctx->reserve_back : nullptr;
   launch_reserve(a, P->ctx->stream);
   CHECK_LAUNCH("TLMPaged");
   return TLM_OK;

@@ -516,7 +516,9 @@ struct ReserveArgs {
   int* status;
   int num_pages, width, page_shift, seqs, tokens, limit, window, sinks;
   int32_t* work;           // reserve_work's ints
+  int32_t* back;           // times that a page goes back [num_pages], zero between launches; null past kReserveBack pages
 };
+constexpr int kReserveBack = 1 << 20;
 constexpr int kReserveMaxSeqs = 1 << 20, kReserveMaxPages = 1 << 30, kReserveMaxWidth = 1 << 26;
 size_t reserve_work(const ReserveArgs& a);  // ints that a.work has to hold
 void launch_reserve(const ReserveArgs& a, hipStream_t st);

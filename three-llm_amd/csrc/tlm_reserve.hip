@@ -105,7 +105,7 @@ __device__ __forceinline__ void report(const ReserveArgs& a, bool bad, bool lost
   if (bits) __hip_atomic_fetch_or(a.status, bits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// The counts as they are, where they do not change in place.
+// The counts as they are, where they do not change in place and the pool is past kReserveBack pages.
 __global__ __launch_bounds__(256) void reserve_copy_kernel(ReserveArgs a) {
   const int64_t step = (int64_t)gridDim.x * 1024;
   for (int64_t i = 4 * ((int64_t)blockIdx.x * 256 + threadIdx.x); i < a.num_pages; i += step)
@@ -132,7 +132,8 @@ __global__ __launch_bounds__(256) void reserve_rows_kernel(ReserveArgs a) {
       for (int e = 0; e < 4; e++) {
         if (i + e >= a.width) continue;
         const Entry x = entry_of(a, q, i + e, v[k][e]);
-        if (x.back) atomicSub(a.out_refs + v[k][e], 1);
+        if (x.back && a.back) atomicAdd(a.back + v[k][e], 1);
+        if (x.back && !a.back) atomicSub(a.out_refs + v[k][e], 1);
         want += x.lacks;
         lost |= x.lost;
         v[k][e] = x.becomes;
@@ -167,12 +168,21 @@ __device__ __forceinline__ int64_t scan1024(int v, Scan& sc, int64_t* all) {
   return before;
 }
 
-// The free pages of each segment, a block each.
+// The counts without what goes back (a.back: cleared again), and the free pages of each
+// segment, a block each.
 __global__ __launch_bounds__(1024) void reserve_count_kernel(ReserveArgs a) {
   __shared__ int sh[16];
   const int tid = threadIdx.x;
   const int64_t i0 = (int64_t)blockIdx.x * kSegment;
-  const i32x4u v = four(a.out_refs + i0, 4 * tid, (int)min((int64_t)kSegment, a.num_pages - i0), 1);
+  const int n = (int)min((int64_t)kSegment, a.num_pages - i0);
+  i32x4u v = four((a.back ? a.refs : a.out_refs) + i0, 4 * tid, n, 1);
+  if (a.back) {
+    const i32x4u b = four(a.back + i0, 4 * tid, n, 0), none = {0, 0, 0, 0};
+    const bool some = (b[0] | b[1] | b[2] | b[3]) != 0;
+    v -= b;
+    if (some || a.refs != a.out_refs) put_four(a.out_refs + i0, 4 * tid, n, v);
+    if (some) put_four(a.back + i0, 4 * tid, n, none);
+  }
   const int free = sum64((v[0] == 0) + (v[1] == 0) + (v[2] == 0) + (v[3] == 0));
   if ((tid & 63) == 0) sh[tid >> 6] = free;
   __syncthreads();
@@ -414,7 +424,7 @@ void launch_reserve(const ReserveArgs& a, hipStream_t st) {
   }
   const Work w = work_of(a);
   const dim3 segments((unsigned)w.segments);
-  if (a.refs != a.out_refs)
+  if (!a.back && a.refs != a.out_refs)
     hipLaunchKernelGGL(reserve_copy_kernel, dim3((unsigned)std::min(1024, a.num_pages / 1024 + 1)), dim3(256), 0, st, a);
   hipLaunchKernelGGL(reserve_rows_kernel, dim3((unsigned)((a.seqs * w.waves + 3) / 4)), dim3(256), 0, st, a);
   hipLaunchKernelGGL(reserve_count_kernel, segments, dim3(1024), 0, st, a);
