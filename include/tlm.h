@@ -241,7 +241,7 @@ typedef struct tlm_paged_request {
   int64_t* slots;           /* [seqs][tokens] or NULL */
   int32_t num_pages, table_width, seqs, tokens;
 } tlm_paged_request;
-/* seqs * tokens * heads is at most 2^22, seqs 2^20, num_pages 2^30, table_width
+/* seqs * tokens * heads is at most 2^22, seqs 2^20, num_pages 2^27, table_width
  * 2^26.  The results are apart from each other and from the inputs, but for tables
  * and refs in place.  Enqueue only. */
 int tlm_op_paged_reserve(tlm_paged* paged, const tlm_paged_request* request);
@@ -267,8 +267,7 @@ int tlm_op_paged_append(tlm_paged* paged, const tlm_paged_batch* batch, const fl
  * cache's products take q and the probabilities as pairs of fp16 values, each to
  * 2^-22 of itself or 2^-39 of its row's largest (an 8-bit cache's too, whose codes
  * are exact in fp16; there the probabilities times V's scales).  What masked
- * positions hold does
- * not matter; attended K and V are finite.  Enqueue only. */
+ * positions hold does not matter; attended K and V are finite.  Enqueue only. */
 int tlm_op_paged_attention(tlm_paged* paged, const tlm_paged_batch* batch, const float* q, int out_fmt, void* out);
 /* Waits for the stream and tells of what the calls since the last status met on
  * the device: TLM_ERR_RANGE where counts[s] was above `tokens`, a row's position

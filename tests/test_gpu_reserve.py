@@ -88,16 +88,19 @@ def test_steps_of_a_server(ctx, n, width, pages, tokens, window, sinks, in_place
 
 @pytest.mark.parametrize("n,width,pages,tokens", [(1024, 32, 16384, 64), (1024, 32, 16385, 64), (1025, 31, 16384, 64),
                                                   (1024, 33, 16384, 64), (40, 100, 300, 3200), (2, 2100, 2300, 65537),
+                                                  (3, 40, 1 << 20, 700), (3, 40, (1 << 20) + 5, 700),
                                                   (3, 40, 5000000, 700)])
-def test_sizes_where_the_kernels_change(ctx, n, width, pages, tokens):
-    """The last size that one block takes and the first that it does not; more pages than 1024 blocks count."""
+@pytest.mark.parametrize("in_place", [True, False])
+def test_sizes_where_the_kernels_change(ctx, n, width, pages, tokens, in_place):
+    """The last size that one block takes and the first that it does not; the most pages whose returns are counted
+    apart; more pages than 1024 blocks count."""
     rng = np.random.default_rng([n, width, pages])
     p = Pool(ctx, n, width, pages, tokens)
     p.refs[rng.random(pages) < 0.5] = 1
     lengths = np.zeros(n, np.int64)
     for _ in range(3):
         counts = rng.integers(0, tokens + 1, n)
-        starts = p.step(lengths, counts, True)
+        starts = p.step(lengths, counts, in_place)
         lengths = np.minimum(np.where(starts >= 0, lengths + counts, lengths), width * 32)
     p.paged.close()
 
@@ -185,7 +188,7 @@ def test_refused(ctx):
     big = {k: at(ok[k], 0) for k in ("lengths", "tables", "refs", "starts")}
     for b in big.values():
         b.nbytes = 1 << 60
-    for kw in (dict(seqs=1 << 20, tokens=5), dict(seqs=(1 << 20) + 1, tokens=1), dict(num_pages=(1 << 30) + 1),
+    for kw in (dict(seqs=1 << 20, tokens=5), dict(seqs=(1 << 20) + 1, tokens=1), dict(num_pages=(1 << 27) + 1),
                dict(table_width=(1 << 26) + 1)):
         with pytest.raises(tlm.TlmError) as e:
             p.reserve(p.request(**{**ok, **big, **kw}))

@@ -519,7 +519,9 @@ struct ReserveArgs {
   int32_t* back;           // times that a page goes back [num_pages], zero between launches; null past kReserveBack pages
 };
 constexpr int kReserveBack = 1 << 20;
-constexpr int kReserveMaxSeqs = 1 << 20, kReserveMaxPages = 1 << 30, kReserveMaxWidth = 1 << 26;
+// Pages: 2^27 of the smallest (one 8-bit kv head of 32, K and V) are 288 GiB, all that the card
+// has, and a bit for each of 2^28 would no longer fit in the workspace.
+constexpr int kReserveMaxSeqs = 1 << 20, kReserveMaxPages = 1 << 27, kReserveMaxWidth = 1 << 26;
 size_t reserve_work(const ReserveArgs& a);  // ints that a.work has to hold
 void launch_reserve(const ReserveArgs& a, hipStream_t st);
 

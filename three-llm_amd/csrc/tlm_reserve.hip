@@ -25,26 +25,23 @@ __host__ __device__ inline int waves_of(const ReserveArgs& a) {
   return n;
 }
 
-// a.work: want[seqs][waves] (pages that a sequence lacks), the free pages of each segment,
-// the free pages in order as far as they may be asked for; of many sequences or segments
-// (reserve_share_kernel) also all free pages and base[seqs] (what the sequences before one
-// lack, or -1: it gets none), and of each segment the free pages before it.
+// a.work: a bit per page, set where it is free; want[seqs][waves] (pages that a sequence
+// lacks); the free pages of each segment; of many sequences or segments
+// (reserve_share_kernel) also base[seqs] (what the sequences before one lack, or -1: it
+// gets none), and of each segment the free pages before it.
 struct Work {
-  int32_t *want, *base, *segment, *free, *pages;
-  int segments, waves, most;  // most: pages that are asked for
+  uint64_t* mask;
+  int32_t *want, *base, *segment;
+  int segments, waves;
 };
 __host__ __device__ inline Work work_of(const ReserveArgs& a) {
   Work w;
   w.segments = (a.num_pages + kSegment - 1) / kSegment;
   w.waves = waves_of(a);
-  w.want = a.work;
+  w.mask = reinterpret_cast<uint64_t*>(a.work);
+  w.want = a.work + (size_t)w.segments * (kSegment / 32);
   w.base = w.want + (size_t)a.seqs * w.waves;
   w.segment = w.base + a.seqs;
-  w.free = w.segment + w.segments;
-  w.pages = w.free + 1;
-  // a sequence's new rows lie in at most tokens / page pages that begin past its length, rounded up
-  const int64_t most = (int64_t)a.seqs * (((int64_t)a.tokens + (1 << a.page_shift) - 1) >> a.page_shift);
-  w.most = (int)(most < a.num_pages ? most : a.num_pages);
   return w;
 }
 
@@ -168,27 +165,35 @@ __device__ __forceinline__ int64_t scan1024(int v, Scan& sc, int64_t* all) {
   return before;
 }
 
-// The counts without what goes back (a.back: cleared again), and the free pages of each
-// segment, a block each.
+// The counts without what goes back (a.back: cleared again), which pages are free and how
+// many of each segment, a block each.
 __global__ __launch_bounds__(1024) void reserve_count_kernel(ReserveArgs a) {
   __shared__ int sh[16];
-  const int tid = threadIdx.x;
-  const int64_t i0 = (int64_t)blockIdx.x * kSegment;
-  const int n = (int)min((int64_t)kSegment, a.num_pages - i0);
-  i32x4u v = four((a.back ? a.refs : a.out_refs) + i0, 4 * tid, n, 1);
-  if (a.back) {
-    const i32x4u b = four(a.back + i0, 4 * tid, n, 0), none = {0, 0, 0, 0};
-    const bool some = (b[0] | b[1] | b[2] | b[3]) != 0;
-    v -= b;
-    if (some || a.refs != a.out_refs) put_four(a.out_refs + i0, 4 * tid, n, v);
-    if (some) put_four(a.back + i0, 4 * tid, n, none);
+  const Work w = work_of(a);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int32_t* const from = a.back ? a.refs : a.out_refs;
+  int c[kSegment / 1024], b[kSegment / 1024], free = 0;
+#pragma unroll
+  for (int k = 0; k < kSegment / 1024; k++) {
+    const int64_t i = (int64_t)blockIdx.x * kSegment + 1024 * k + tid;
+    c[k] = i < a.num_pages ? from[i] : 1;
+    b[k] = i < a.num_pages && a.back ? a.back[i] : 0;
   }
-  const int free = sum64((v[0] == 0) + (v[1] == 0) + (v[2] == 0) + (v[3] == 0));
-  if ((tid & 63) == 0) sh[tid >> 6] = free;
+#pragma unroll
+  for (int k = 0; k < kSegment / 1024; k++) {
+    const int64_t i = (int64_t)blockIdx.x * kSegment + 1024 * k + tid;
+    c[k] -= b[k];
+    if (b[k]) a.back[i] = 0;
+    if (i < a.num_pages && a.back && (b[k] || a.refs != a.out_refs)) a.out_refs[i] = c[k];
+    const uint64_t m = __ballot(c[k] == 0);
+    if (lane == 0) w.mask[(size_t)blockIdx.x * (kSegment / 64) + 16 * k + wave] = m;
+    free += __popcll(m);
+  }
+  if (lane == 0) sh[wave] = free;
   __syncthreads();
   int all = 0;
   for (int i = 0; i < 16; i++) all += sh[i];
-  if (tid == 0) work_of(a).segment[blockIdx.x] = all;
+  if (tid == 0) w.segment[blockIdx.x] = all;
 }
 
 // What sequence s lacks in all (kLost: positions).
@@ -224,33 +229,48 @@ __global__ __launch_bounds__(1024) void reserve_share_kernel(ReserveArgs a) {
     if (s < a.seqs) w.base[s] = base_of(want, before, free);
     asked += all;
   }
-  if (tid == 0) *w.free = (int)free;
 }
 
-// The free pages in order, a block a segment.
-template <bool SHARED>
-__global__ __launch_bounds__(1024) void reserve_list_kernel(ReserveArgs a) {
-  __shared__ Scan sc;
-  const Work w = work_of(a);
-  const int tid = threadIdx.x;
-  const int64_t i0 = (int64_t)blockIdx.x * kSegment;
-  const i32x4u v = four(a.out_refs + i0, 4 * tid, (int)min((int64_t)kSegment, a.num_pages - i0), 1);
-  int64_t before, all;
-  if (SHARED)
-    before = w.segment[blockIdx.x];
-  else
-    scan1024(tid < (int)blockIdx.x ? w.segment[tid] : 0, sc, &before);
-  if (before >= w.most) return;
-  int64_t rank = scan1024((v[0] == 0) + (v[1] == 0) + (v[2] == 0) + (v[3] == 0), sc, &all) + before;
-#pragma unroll
-  for (int e = 0; e < 4; e++)
-    if (v[e] == 0 && rank < w.most) w.pages[rank++] = (int)i0 + 4 * tid + e;
+// The last segment before which there are at most `rank` free pages (which holds that
+// one), 64 at a time.
+template <typename B>
+__device__ __forceinline__ int segment_of(int rank, int segments, int lane, B before) {
+  int lo = 0, len = segments;
+  while (true) {
+    const int step = (len + 63) / 64, i = lane * step;
+    const int k = __popcll(__ballot(i < len && before(lo + min(i, len - 1)) <= rank)) - 1;  // the first is
+    lo += k * step;
+    len = min(step, len - k * step);
+    if (step == 1) return lo;
+  }
+}
+
+// The free pages of ranks at .. at + n - 1, n <= 64, a lane each (`pick`: the wave's 64 words of LDS);
+// -1 where none is, which is so only if the inputs change during the call.
+template <typename B>
+__device__ __forceinline__ int pages_at(const Work& w, int at, int n, int lane, int* pick, B before) {
+  __hip_atomic_store(pick + lane, -1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+  for (int r = at; r < at + n;) {
+    const int g = segment_of(r, w.segments, lane, before);
+    uint64_t word = w.mask[(size_t)g * (kSegment / 64) + lane];
+    const int c = __popcll(word), incl = wave_scan(c);
+    int rank = before(g) + incl - c;
+    if (rank + c <= r) word = 0;
+    for (; word && rank < at + n; word &= word - 1, rank++)
+      if (rank >= r)
+        __hip_atomic_store(pick + rank - at, g * kSegment + 64 * lane + __builtin_ctzll(word), __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_WORKGROUP);
+    r = max(r + 1, before(g) + __builtin_amdgcn_readlane(incl, 63));
+  }
+  // a wave's LDS instructions are done in their order
+  return __hip_atomic_load(pick + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
 }
 
 // The pages that a sequence gets into its table, its first position and its slots: a wave.
 // `entry`: its table's at the first of the pages past its length + lane.
+template <typename B>
 __device__ __forceinline__ void fill(const ReserveArgs& a, const Work& w, const Seq& q, int s, int base, int lane,
-                                     int entry) {
+                                     int entry, int* pick, B before) {
   int32_t* const to = a.out_tables + (size_t)s * a.width;
   const int page = 1 << a.page_shift;
   const bool served = q.rows > 0 && base >= 0;
@@ -261,12 +281,16 @@ __device__ __forceinline__ void fill(const ReserveArgs& a, const Work& w, const 
     const int i = b + lane;
     const bool lacks = i < q.use.end && (b == i0 ? entry : to[i]) < 0;
     const uint64_t m = __ballot(lacks);
-    if (lacks) {
-      const int p = w.pages[at + __popcll(m & ((1ull << lane) - 1))];
-      to[i] = p;
-      a.out_refs[p] = 1;
+    const int n = __popcll(m);
+    if (n) {
+      const int got = pages_at(w, at, n, lane, pick, before);
+      const int p = __shfl(got, __popcll(m & ((1ull << lane) - 1)));
+      if (lacks && p >= 0) {
+        to[i] = p;
+        a.out_refs[p] = 1;
+      }
     }
-    at += __popcll(m);
+    at += n;
   }
   if (lane == 0) a.starts[s] = served ? q.length : -1;
   if (!a.slots) return;
@@ -284,9 +308,10 @@ __device__ __forceinline__ void fill(const ReserveArgs& a, const Work& w, const 
 template <bool SHARED>
 __global__ __launch_bounds__(1024) void reserve_fill_kernel(ReserveArgs a) {
   __shared__ Scan sc;
-  __shared__ int base[kInPlace];
+  __shared__ int base[kInPlace], segment[kInPlace], picks[1024];
   const Work w = work_of(a);
   const int tid = threadIdx.x, s = blockIdx.x * 16 + (tid >> 6);
+  int* const pick = picks + (tid & ~63);
   Seq q;
   int entry = 0;  // on its way while the sums are made
   if (s < a.seqs) {
@@ -295,18 +320,22 @@ __global__ __launch_bounds__(1024) void reserve_fill_kernel(ReserveArgs a) {
     if (i < q.use.end) entry = a.out_tables[(size_t)s * a.width + i];
   }
   if (!SHARED) {
-    const int want = tid < a.seqs ? want_of(w, tid) : kLost, segment = tid < w.segments ? w.segment[tid] : 0;
+    const int want = tid < a.seqs ? want_of(w, tid) : kLost, mine = tid < w.segments ? w.segment[tid] : 0;
     int64_t free, all;
-    scan1024(segment, sc, &free);
+    segment[tid] = (int)scan1024(mine, sc, &free);
     const int64_t before = scan1024(want == kLost ? 0 : want, sc, &all);
     base[tid] = base_of(want, before, free);
     __syncthreads();
   }
-  if (s < a.seqs) fill(a, w, q, s, SHARED ? w.base[s] : base[s], tid & 63, entry);
+  if (s >= a.seqs) return;
+  if (SHARED)
+    fill(a, w, q, s, w.base[s], tid & 63, entry, pick, [&](int g) { return w.segment[g]; });
+  else
+    fill(a, w, q, s, base[s], tid & 63, entry, pick, [&](int g) { return segment[g]; });
 }
 
 // Few sequences over a small pool: all of it by one block, with the counts, what is
-// shared out and the pages of the new rows in LDS, in place of four or five launches.
+// shared out and the pages of the new rows in LDS, in place of three launches or four.
 // us a call, so / by launches: 16 sequences of 32 pages 4.1 / 13.0, 64 of 129 7.8 / 14.3, 60 of 469
 // 15.5 / 14.5, 256 of 126 17.6 / 15.5.  It is the instructions of one CU, about 40 an entry.
 constexpr int kOnePages = 16384, kOneSeqs = 1024, kOneEntries = 20480, kOneRows = 4096, kOneSlots = 65536;
@@ -413,7 +442,7 @@ __global__ __launch_bounds__(1024) void reserve_one_kernel(ReserveArgs a, uint32
 
 size_t reserve_work(const ReserveArgs& a) {
   const Work w = work_of(a);
-  return (size_t)(w.pages - w.want) + w.most;
+  return (size_t)(w.segment - a.work) + w.segments;
 }
 
 void launch_reserve(const ReserveArgs& a, hipStream_t st) {
@@ -431,10 +460,8 @@ void launch_reserve(const ReserveArgs& a, hipStream_t st) {
   const dim3 rows((unsigned)((a.seqs + 15) / 16));
   if (a.seqs > kInPlace || w.segments > kInPlace) {
     hipLaunchKernelGGL(reserve_share_kernel, dim3(1), dim3(1024), 0, st, a);
-    hipLaunchKernelGGL(reserve_list_kernel<true>, segments, dim3(1024), 0, st, a);
     hipLaunchKernelGGL(reserve_fill_kernel<true>, rows, dim3(1024), 0, st, a);
   } else {
-    hipLaunchKernelGGL(reserve_list_kernel<false>, segments, dim3(1024), 0, st, a);
     hipLaunchKernelGGL(reserve_fill_kernel<false>, rows, dim3(1024), 0, st, a);
   }
 }
