@@ -17,8 +17,8 @@ constexpr int kPiece = 512;     // entries of a table that a wave looks at at a 
 constexpr int kLost = 1 << 30;  // in want: positions are lost
 
 // Waves that share a sequence's table: enough of them to fill the chip (1024 sequences of
-// 1025 entries, pieces of 256 / 512 / 1024 a wave: 23.6 / 19.8 / 19.4 us in all; bound by the
-// launches, of which this one moves 9 MB in 6.0 us, 1.4 of it the counts' atomics).
+// 1025 entries, pieces of 256 / 512 / 1024 a wave: 14.9 / 15.3 / 15.3 us in all; bound by the
+// three launches, of which this one moves 9 MB in 6.4 us, 1.4 of it the counts' atomics).
 __host__ __device__ inline int waves_of(const ReserveArgs& a) {
   int n = 1;
   while (2 * n <= 16 && 2 * n * a.seqs <= 4096 && n * kPiece < a.width) n *= 2;
@@ -336,8 +336,8 @@ __global__ __launch_bounds__(1024) void reserve_fill_kernel(ReserveArgs a) {
 
 // Few sequences over a small pool: all of it by one block, with the counts, what is
 // shared out and the pages of the new rows in LDS, in place of three launches or four.
-// us a call, so / by launches: 16 sequences of 32 pages 4.1 / 13.0, 64 of 129 7.8 / 14.3, 60 of 469
-// 15.5 / 14.5, 256 of 126 17.6 / 15.5.  It is the instructions of one CU, about 40 an entry.
+// us a call, so / by launches: 16 sequences of 32 pages 4.3 / 10.2, 64 of 128 7.8 / 11.5, 60 of 313
+// 11.9 / 12.2, 60 of 469 15.6 / 12.1, 256 of 125 17.6 / 12.5.  It is the instructions of one CU, about 40 an entry.
 constexpr int kOnePages = 16384, kOneSeqs = 1024, kOneEntries = 20480, kOneRows = 4096, kOneSlots = 65536;
 __host__ __device__ inline int span_of(const ReserveArgs& a) {  // pages that a sequence's new rows may touch
   return ((a.tokens - 1) >> a.page_shift) + 2;
