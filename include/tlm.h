@@ -322,8 +322,8 @@ typedef struct tlm_logit_rules {
   const uint32_t* masks;         /* [seqs][tokens][(vocab + 31) / 32] (NULL: nothing is masked) */
   int32_t seqs, tokens, vocab, history_width, bias_width;
 } tlm_logit_rules;
-/* tokens <= 64, vocab <= 524288, seqs * tokens <= 2^20, bias_width <= 4096;
- * seqs * tokens * vocab, vocab rounded up to a multiple of 4096, below 2^35.
+/* tokens <= 64, vocab <= 524288, seqs * tokens <= 2^20, bias_width <= 4096,
+ * history_width <= 2^30; seqs * tokens * vocab, vocab rounded up to a multiple of 4096, below 2^35.
  * Enqueue only. */
 int tlm_op_adjust_logits(tlm_ctx* ctx, const tlm_logit_rules* rules);
 /* Verification of drafted tokens, for many sequences at once: which of a

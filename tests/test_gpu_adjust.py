@@ -162,6 +162,39 @@ def test_most_rows_and_the_largest_vocabulary(ctx):
     check(ctx, rules(2000, 2, 40, history=3))
 
 
+def test_the_longest_history(ctx):
+    """2^30 tokens: those at both ends count, as many as the sequence says; one token more is refused."""
+    width = 1 << 30
+    ids = ctx.buffer(4 * width)
+
+    def part(first):
+        b = tlm.Buffer.__new__(tlm.Buffer)
+        b.ctx, b.nbytes, b.ptr = ctx, ids.nbytes - 4 * first, type(ids.ptr)(ids.ptr.value + 4 * first)
+        return b
+
+    n = 1 << 20
+    part(0).write(np.full(n, -1, np.int32))  # nobody's
+    while n < width:
+        part(n).copy_from(ids, 4 * n)
+        n *= 2
+    part(0).write(np.array([3, 4, 3], np.int32))
+    part(width - 3).write(np.array([3, 5, 6], np.int32))
+    x = np.arange(1, 11, dtype=np.float32)
+    for said, times in ((width, [0, 0, 0, 3, 1, 1, 1, 0, 0, 0]), (width - 1, [0, 0, 0, 3, 1, 1, 0, 0, 0, 0]),
+                        (2, [0, 0, 0, 1, 1, 0, 0, 0, 0, 0])):
+        logits = ctx.array(x)
+        r = tlm.logit_rules(logits, 1, 1, 10, history=ids, history_width=width,
+                            history_counts=ctx.array(np.array([said], np.int32)),
+                            frequency=ctx.array(np.array([0.25], np.float32)))
+        tlm.adjust_logits(ctx, r)
+        assert np.array_equal(logits.read(), x - np.float32(0.25) * np.array(times, np.float32))
+    r.history_width = width + 1
+    with pytest.raises(tlm.TlmError) as e:
+        tlm.adjust_logits(ctx, r)
+    assert e.value.code == tlm.TLM_ERR_INVALID
+    ids.free()
+
+
 def test_picking_after(ctx):
     """A masked row's argmax is the best that is left, of one with nothing left there is none."""
     d = rules(1, 2, 10000, masked=True)

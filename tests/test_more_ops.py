@@ -147,6 +147,16 @@ def test_null_arguments_refused():
         assert L.tlm_last_error().startswith((b"TLMPaged: ", b"TLMLogitRules: "))
 
 
+def test_histories_longer_than_a_sequence_are_refused():
+    """A sequence has at most 2^30 positions; indexes into a longer history would pass 31 bits."""
+    some = (ctypes.c_uint8 * 4096)()  # a context that the refusal does not look at, and buffers that nothing reads
+    at = ctypes.addressof(some)
+    for width in ((1 << 30) + 1, (1 << 31) - 4096, (1 << 31) - 1):
+        r = tlm.LogitRules(logits=at, out=at, history=1 << 40, seqs=1, tokens=1, vocab=10, history_width=width)
+        assert tlm.lib().tlm_op_adjust_logits(at, r) == tlm.TLM_ERR_INVALID
+        assert tlm.lib().tlm_last_error() == b"TLMLogitRules: a history of %d, at most %d" % (width, 1 << 30)
+
+
 def test_buffers_that_are_too_small_are_refused():
     """A byte too few is refused when the arguments are put together."""
     p = tlm.Paged.__new__(tlm.Paged)

@@ -76,7 +76,7 @@ __global__ __launch_bounds__(kThreads) void adjust_kernel(AdjustArgs a, int chun
   for (int q = 0; q < Q && !PLACE; q++) fetch(q);
   __syncthreads();
   const bool said = h > 0 || (a.drafts && j > 0);
-  for (int i0 = tid; i0 < h; i0 += kAhead * kThreads) {
+  for (int i0 = tid; i0 < h; i0 += kAhead * kThreads) {  // h <= kAdjustMaxHistory: no index passes 31 bits
     int id[kAhead];
 #pragma unroll
     for (int k = 0; k < kAhead; k++) id[k] = i0 + k * kThreads < h ? ids[i0 + k * kThreads] : -1;

@@ -1614,6 +1614,8 @@ int tlm_op_adjust_logits(tlm_ctx* ctx, const tlm_logit_rules* r) {
                 r->vocab);
   if (r->bias_width > kAdjustMaxBiases)
     return fail(TLM_ERR_INVALID, "TLMLogitRules: %d biases, at most %d", r->bias_width, kAdjustMaxBiases);
+  if (r->history_width > kAdjustMaxHistory)
+    return fail(TLM_ERR_INVALID, "TLMLogitRules: a history of %d, at most %d", r->history_width, kAdjustMaxHistory);
   if (r->history_width > 0 && !r->history) return fail(TLM_ERR_INVALID, "TLMLogitRules: no history of %d", r->history_width);
   if (r->bias_width > 0 && (!r->bias_ids || !r->biases))
     return fail(TLM_ERR_INVALID, "TLMLogitRules: %d biases without their tokens or values", r->bias_width);

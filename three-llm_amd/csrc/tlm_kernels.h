@@ -542,6 +542,7 @@ struct AdjustArgs {
   int seqs, tokens, vocab, history_width, bias_width;
 };
 constexpr int kAdjustMaxBiases = 4096;
+constexpr int kAdjustMaxHistory = 1 << 30;  // positions of a sequence; indexes past it stay in 31 bits
 void launch_adjust(const AdjustArgs& a, hipStream_t st);
 
 struct VerifyArgs {
