@@ -253,8 +253,10 @@ int tlm_op_paged_reserve(tlm_paged* paged, const tlm_paged_request* request);
  * TLM_FMT_F8: a value is its code times the scale of its 32 aligned positions and kv
  * head, 2^e from 2^-32 to 2^31, the least that takes the largest magnitude to at
  * most 448.  Rows that start within 32 positions keep the scale that these have or, if
- * they need it, raise it; the positions before them are then rounded again (exact but
- * for magnitudes below 2^-14 of the largest).  Of rows that start within 32 positions
+ * they need it, raise it; it never falls again, also where the rows that raised it are
+ * dropped (drafts that fell).  The positions before them are then rounded again, exact
+ * but for magnitudes below 2^-6 of the new scale: at most 2^-13.8 of the largest that it
+ * was raised for.  Of rows that start within 32 positions
  * the earlier ones have been appended (or their page is all zeros).  Positions behind
  * the appended rows, to the end of their 32, keep their codes, not their values; 32
  * positions that two sequences append to in one call are lost.  Values that are not

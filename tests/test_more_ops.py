@@ -53,6 +53,21 @@ def test_codes():
         assert mo.encode(mid * (1 - 1e-9)) == c and mo.encode(mid * (1 + 1e-9)) == c + 1
 
 
+def test_codes_under_a_larger_scale():
+    """Coded again, values from 2^-6 of the new scale on are exact; below it some are not, up to 2^-13.8 of a largest
+    magnitude that the scale is the least for."""
+    whole = mo.CODES[[c for c in range(256) if c & 127 != 127]]
+    largest = np.nextafter(np.float32(224), np.float32(225))
+    assert mo.exponent(float(largest)) == 0 and mo.exponent(224.0) == -1
+    inexact = 0.0
+    for by in range(1, 64):
+        v = whole * 2.0 ** -by
+        again = mo.CODES[mo.encode(v)]
+        assert np.array_equal(again[np.abs(v) >= 2.0 ** -6], v[np.abs(v) >= 2.0 ** -6])
+        inexact = max(inexact, np.abs(v[again != v]).max(initial=0))
+    assert 2.0 ** -14 < inexact / largest < 2.0 ** -13.8
+
+
 def test_exponents(host):
     """The least power of two that takes a magnitude to at most 448, at its borders and at the range's ends."""
     f = np.array([448.0, np.nextafter(np.float32(448), np.float32(1e9)), 1.0, 1.75, 1.7500001, 3.5, 3.6, 0.0, 1e-45,

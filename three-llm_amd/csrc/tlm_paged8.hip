@@ -27,8 +27,8 @@ __device__ __forceinline__ u32x2 codes8(const Oct& x, int e) {
   return (u32x2){codes4(coded(x.a[0], e), coded(x.a[1], e), coded(x.a[2], e), coded(x.a[3], e)),
                  codes4(coded(x.b[0], e), coded(x.b[1], e), coded(x.b[2], e), coded(x.b[3], e))};
 }
-// Four codes under a scale 2^by times theirs (by >= 0): exact but for what falls below
-// 2^-6 of the code's range.
+// Four codes under a scale 2^by times theirs (by >= 0): exact but for magnitudes below 2^-6
+// of the new scale, the least normal code.
 __device__ __forceinline__ uint32_t recoded(uint32_t c, int by) {
   const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
   return codes4(ldexpf(lo[0], -by), ldexpf(lo[1], -by), ldexpf(hi[0], -by), ldexpf(hi[1], -by));
