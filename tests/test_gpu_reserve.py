@@ -105,6 +105,45 @@ def test_sizes_where_the_kernels_change(ctx, n, width, pages, tokens, in_place):
     p.paged.close()
 
 
+@pytest.mark.parametrize("n,width,tokens", [(2, 5000, 4800), (3, 8193, 4800), (2, 20001, 4800), (2500, 1100, 1600)])
+@pytest.mark.parametrize("quarter", [0, 1])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_wide_tables(ctx, n, width, tokens, quarter, in_place):
+    """Tables that sixteen waves share, and ones that their waves look at in several parts (widths that are no multiple
+    of four, few waves for many sequences): pages held, lacking, given back and lost up to the last entry."""
+    rng = np.random.default_rng([n, width, quarter])
+    window, sinks = quarter * 8 * width, quarter * 70
+    most = min(n, 12)  # with long tables; the others hold a few pages here and there
+    pages = most * width + 8 * n + 17000
+    ends = [((width - tokens // 32) * 32, tokens), (100, 5), (width * 32 - 20, 7), ((width - 1) * 32, 32)]
+    for shift in range(4) if n < 4 else [0]:
+        p = Pool(ctx, n, width, pages, tokens, 32, window, sinks)
+        free = rng.permutation(pages)
+        lengths, counts = rng.integers(-1, 60, n), rng.integers(0, 40, n)
+        for s in range(n):
+            where = np.arange(width) if s < most else np.concatenate([np.arange(2), rng.integers(2, width, 5), [width - 1]])
+            p.tables[s, where], free = free[:where.size], free[where.size:]
+        for s in range(most):
+            kind = (s + shift) % 4
+            lengths[s], counts[s] = ends[kind]
+            if kind == 0:
+                p.tables[s, width - tokens // 32:] = -1  # lacking, and some in between held
+                p.tables[s, width - 7:width - 4], free = free[:3], free[3:]
+            elif kind == 2:
+                p.tables[s, width - 1] = -1  # holds positions
+            elif kind == 3:
+                p.tables[s, width - 1] = pages  # no page: lacking
+        p.refs[:] = rng.random(pages) < 0.2  # others'
+        np.add.at(p.refs, p.tables[(p.tables >= 0) & (p.tables < pages)], 1)
+        starts = p.step(lengths, counts, in_place)
+        for s in range(most):
+            assert (starts[s] >= 0) == ((s + shift) % 4 != 2)
+        lengths = np.where(starts >= 0, lengths + counts, lengths)
+        lengths[(np.arange(n) + shift) % 4 == 3] = -1  # it ends
+        p.step(np.minimum(lengths, width * 32), np.minimum(counts, 3), in_place)
+        p.paged.close()
+
+
 @pytest.mark.parametrize("page", [64, 1024])
 def test_page_sizes(ctx, page):
     p = Pool(ctx, 6, 3, 20, 1500, page, 0, 0)
