@@ -308,6 +308,9 @@ int tlm_op_topk(tlm_ctx* ctx, const float* logits, int n, int k, double softcap,
  *   x = x + the biases of v (one listed twice: both, in the list's order)
  *   x = -inf where bit v % 32 of word v / 32 of the row's mask is 0.
  * -inf never takes part in picking; where a mask leaves nothing, no token does.
+ * All three penalties count the same history.  Repetition over prompt and reply with
+ * frequency and presence over the reply alone are two calls: the first with the whole
+ * history and repetition only, the second with the reply's and all the rest.
  * Token ids outside the vocabulary are nobody's. */
 typedef struct tlm_logit_rules {
   const float* logits;           /* [seqs][tokens][vocab] */

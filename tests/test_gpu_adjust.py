@@ -99,6 +99,47 @@ def test_biases(ctx, biases):
     check(ctx, d)
 
 
+@pytest.mark.parametrize("n,t,v,history,biases,masked", [(3, 2, 9000, 2000, 7, False), (2, 2, 20000, 300, 300, True),
+                                                         (2, 1, 5000, 5000, 4096, False), (1, 5, 4097, 0, 151, False)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_each_token_to_its_own_roundings(ctx, n, t, v, history, biases, masked, in_place):
+    """(4 + biases of that very token) 2^-24: with 4096 of them listed, a token that none names gets no more."""
+    d = rules(n, t, v, history=history, biases=biases, masked=masked)
+    got = run(ctx, d, in_place)
+    want, size = mo.adjust(out=d["logits"], **d)
+    named = np.zeros((n, v))
+    for s in range(n):
+        np.add.at(named[s], d["bias_ids"][s][(d["bias_ids"][s] >= 0) & (d["bias_ids"][s] < v)], 1)
+    assert (named == 0).any() and named.max() < biases
+    fine = np.isfinite(want)
+    assert np.array_equal(got[~fine], want[~fine].astype(np.float32))
+    assert np.all(np.abs(got[fine] - want[fine]) <= ((4 + named[:, None]) * EPS * size)[fine])
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_one_history_for_repetition_and_another_for_the_rest(ctx, in_place):
+    """Two calls: repetition over prompt and reply, then frequency and presence over the reply, biases and masks."""
+    n, t, v = 3, 4, 9001
+    d = rules(n, t, v, history=700, biases=9, masked=True)
+    d["drafts"][:, 1] = d["drafts"][:, 0]
+    empty = dict(history=None, said=None, repetition=None, frequency=None, presence=None, bias_ids=None, biases=None,
+                 masks=None)
+    first = {**d, **empty, "history": d["history"], "said": d["said"], "repetition": d["repetition"]}
+    second = {**d, "history": np.ascontiguousarray(d["history"][:, 500:]), "said": np.array([200, 0, 77], np.int32),
+              "repetition": None}
+    got = run(ctx, {**second, "logits": run(ctx, first, in_place)}, in_place)
+    want, _ = mo.adjust(out=d["logits"], **first)
+    want, more = mo.adjust(out=want, **{**second, "logits": want})
+    named = np.zeros((n, v))
+    for s in range(n):
+        np.add.at(named[s], d["bias_ids"][s][(d["bias_ids"][s] >= 0) & (d["bias_ids"][s] < v)], 1)
+    fine = np.isfinite(want)
+    assert np.array_equal(got[~fine], want[~fine].astype(np.float32))
+    # one rounding of the first call's, of its result, where the second one's magnitudes start; three of frequency and
+    # presence, one for each bias
+    assert np.all(np.abs(got[fine] - want[fine]) <= ((4 + named[:, None]) * EPS * more)[fine])
+
+
 @pytest.mark.parametrize("biases", [64, 150, 700])
 def test_biases_of_the_same_tokens(ctx, biases):
     """Tokens 256 apart, and each several times among 64 of the list: bit for bit the sums in the list's order."""
