@@ -178,7 +178,7 @@ void launch_of(const AdjustArgs& a, hipStream_t st) {
 // it, but fewer of them fit a CU (16 KB of LDS each, 32 with biases): 62 rows of 128256 with
 // everything and histories of 4096, chunks of 4096 / 6144 / 8192: 14.7 / 16.3 / 18.6 us (4.5 TB/s of
 // logits); of 2048, 64 x 32000 5.8 against 5.6 and 1 x 5 x 151936 3.7 either way.  64 x 128256 without
-// masks 14.7, in place 11.1.
+// masks 14.7, in place 11.1 (histories of 300: 9.8, the blocks').
 void launch_adjust(const AdjustArgs& a, hipStream_t st) {
   if (a.out == a.logits)
     launch_of<true>(a, st);

@@ -364,7 +364,8 @@ void launch_paged_append8(const PagedArgs& a, hipStream_t st) {
   const dim3 block(256);
   // us a call, few-rows / many-rows kernel, 64 sequences of 4, 8, 12 and 16 tokens: Llama-3.2-1B heads
   // 6.1 / 11.7, 9.9 / 12.1, 9.7 / 12.9, 11.8 / 13.0; Llama-3.2-3B 6.0 / 11.4, 8.5 / 12.7, 11.1 / 14.1,
-  // 17.1 / 14.7.  2 x up to 2048 (3B, 122 MB) 28.5 us, 4.3 TB/s.
+  // 17.1 / 14.7.  2 x up to 2048 (3B, 122 MB) 28.5 us, 4.3 TB/s; of Llama-3.2-1B 14.4, with 20
+  // rotated dims, which only the few-rows kernel takes, 43.3.
   if (a.tokens <= 12 || a.rd % 16) {
     const int heads = std::max(1, kFewHeads / a.tokens), parts = (a.Hkv + heads - 1) / heads;
     const int slices = parts + (a.q ? (std::min(a.tokens, 32) * a.Hq * (a.D / 8) + 255) / 256 : 0);

@@ -18,7 +18,8 @@ constexpr int kLost = 1 << 30;  // in want: positions are lost
 
 // Waves that share a sequence's table: enough of them to fill the chip (1024 sequences of
 // 1025 entries, pieces of 256 / 512 / 1024 a wave: 14.9 / 15.3 / 15.3 us in all; bound by the
-// three launches, of which this one moves 9 MB in 6.4 us, 1.4 of it the counts' atomics).
+// three launches, of which this one moves 9 MB in 6.4 us, 1.4 of it the counts' atomics; in
+// place too, as entries that stay are written back: 7.2).
 __host__ __device__ inline int waves_of(const ReserveArgs& a) {
   int n = 1;
   while (2 * n <= 16 && 2 * n * a.seqs <= 4096 && n * kPiece < a.width) n *= 2;
@@ -335,7 +336,7 @@ __global__ __launch_bounds__(1024) void reserve_fill_kernel(ReserveArgs a) {
 }
 
 // Few sequences over a small pool: all of it by one block, with the counts, what is
-// shared out and the pages of the new rows in LDS, in place of three launches or four.
+// shared out and the pages of the new rows in LDS, in place of three launches.
 // us a call, so / by launches: 16 sequences of 32 pages 4.3 / 10.2, 64 of 128 7.8 / 11.5, 60 of 313
 // 11.9 / 12.2, 60 of 469 15.6 / 12.1, 256 of 125 17.6 / 12.5.  It is the instructions of one CU, about 40 an entry.
 constexpr int kOnePages = 16384, kOneSeqs = 1024, kOneEntries = 20480, kOneRows = 4096, kOneSlots = 65536;
@@ -445,6 +446,8 @@ size_t reserve_work(const ReserveArgs& a) {
   return (size_t)(w.segment - a.work) + w.segments;
 }
 
+// Past one block: three launches; the running sums are one more past kInPlace sequences or
+// segments, the counts' copy another past kReserveBack pages where the result is not in place.
 void launch_reserve(const ReserveArgs& a, hipStream_t st) {
   if (a.num_pages <= kOnePages && a.seqs <= kOneSeqs && (int64_t)a.seqs * a.width <= kOneEntries &&
       (int64_t)a.seqs * span_of(a) <= kOneRows && (int64_t)a.seqs * a.tokens <= kOneSlots) {
